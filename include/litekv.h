@@ -50,7 +50,7 @@ extern "C" {
 #define LITEKV_ERR_INVALID_ARGUMENT 1
 #define LITEKV_ERR_LAUNCH 2
 
-#define LITEKV_ABI_VERSION 4
+#define LITEKV_ABI_VERSION 5
 
 /* ABI version of the loaded library (LITEKV_ABI_VERSION at build time). */
 int litekv_abi_version(void);
@@ -761,6 +761,77 @@ int litekv_paged_prefill_int8(const void *q, int64_t q_token_stride,
                              int32_t head_dim, int32_t page_size,
                              int64_t num_pages, int32_t max_q_len,
                              float softmax_scale, void *stream);
+
+/*
+ * 4-bit KV pools (no counterpart in the reference). Every row (token, kv head) is quantised over
+ * its own range, 0 included; nothing has to be calibrated and there is no scales argument:
+ *     lo = min(0, min x)   hi = max(0, max x)
+ *     s  = (hi - lo) / 15, rounded up to 7 significant bits (below 2^-14: to a multiple of 2^-20)
+ *     z  = rint(-lo / s)   c = clamp(rint(x / s) + z, 0, 15)      halves go to the even integer
+ *     value = s * (c - z)
+ * Every value is an fp16 number and at most s / 2 from its element. Elements saturate at +-57344, NaN
+ * counts as 0. The pool is
+ *     kv_pool_int4[num_pages * page_size][2 * num_kv_heads][head_dim / 2 + 2]  bytes
+ * (head_dim 64 or 128), of which 16 consecutive slots, a block, hold
+ *     codes [2 * num_kv_heads][8 * head_dim]  bytes, K heads then V heads
+ *     words [2 * num_kv_heads][16]            uint16: fp16 bits of s (its low 4 bits are 0) | z
+ * K: the 16 rows one after the other; dword w of a row holds elements 8w .. 8w + 7, element 8w + 2i in
+ * nibble i, 8w + 2i + 1 in nibble 4 + i. V: for rows 4r .. 4r + 3 and each of 16 columns of head_dim / 16
+ * elements, head_dim / 32 dwords (p, e), e fastest; the low half of a dword is row 4r + 2p, the high half row
+ * 4r + 2p + 1, and nibble j of a half is element column * head_dim / 16 + (head_dim / 64) * j + e. A page is one
+ * contiguous run of page_size * 2 * num_kv_heads * (head_dim / 2 + 2) bytes, so litekv_page_copy /
+ * litekv_page_gather move 4-bit pages as they are.
+ *
+ * litekv_kv_append_int4, litekv_page_dequant_int4: as their _int8 namesakes, without scales.
+ *
+ * litekv_qk_norm_rope_append_int4: litekv_qk_norm_rope_append into a 4-bit pool. Between the fp16
+ * inputs and the one rounding of q, and to the quantiser, everything is fp32 (the sum of squares fp64):
+ * q is rounded once, where the other pools' variants round the normalised value and its product
+ * with the weight to fp16 as well, and a K row is quantised without being rounded to fp16 first.
+ *
+ * litekv_paged_decode_int4: litekv_paged_decode (splits, both stages; workspace from
+ * litekv_paged_decode_workspace_bytes) over a 4-bit pool, with the step's append fused in where k_new / v_new are not
+ * NULL (see litekv_paged_decode_append).
+ *
+ * litekv_paged_prefill_int4: litekv_paged_prefill_bounded over a 4-bit pool (key_slices 1), or
+ * litekv_paged_prefill_split (key_slices 2 .. 8, with its workspace; max_kv_len is then not read).
+ */
+int litekv_kv_append_int4(const void *k, const void *v, int64_t k_token_stride,
+                          int64_t v_token_stride, const int32_t *slot_mapping,
+                          void *kv_pool_int4, int32_t num_tokens, int32_t num_kv_heads,
+                          int32_t head_dim, int64_t num_slots, void *stream);
+
+int litekv_qk_norm_rope_append_int4(void *q, int64_t q_token_stride, const void *k,
+                                    int64_t k_token_stride, const void *v, int64_t v_token_stride,
+                                    const void *q_norm_weight, const void *k_norm_weight,
+                                    const void *cos_rows, const void *sin_rows,
+                                    int64_t cos_sin_token_stride, const int32_t *slot_mapping,
+                                    void *kv_pool_int4, int32_t num_tokens, int32_t num_q_heads,
+                                    int32_t num_kv_heads, int32_t head_dim, int64_t num_slots,
+                                    float rms_eps, void *stream);
+
+int litekv_page_dequant_int4(const void *kv_pool_int4, void *dst_pool, const int32_t *src_ids,
+                             const int32_t *dst_ids, int32_t n, int32_t num_kv_heads,
+                             int32_t head_dim, int32_t page_size, int64_t num_src_pages,
+                             int64_t num_dst_pages, void *stream);
+
+int litekv_paged_decode_int4(const void *q, int64_t q_batch_stride, void *kv_pool_int4,
+                             const int32_t *block_table, int32_t block_table_stride,
+                             const int32_t *seq_lens, const void *k_new, const void *v_new,
+                             int64_t k_new_stride, int64_t v_new_stride, void *out,
+                             void *workspace, size_t workspace_bytes, int32_t batch,
+                             int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                             int32_t page_size, int64_t num_pages, int32_t max_splits,
+                             int32_t min_pages_per_split, float softmax_scale, void *stream);
+
+int litekv_paged_prefill_int4(const void *q, int64_t q_token_stride, const void *kv_pool_int4,
+                              const int32_t *block_table, int32_t block_table_stride,
+                              const int32_t *cu_q_lens, const int32_t *context_lens, void *out,
+                              int64_t out_token_stride, int32_t batch, int32_t num_q_heads,
+                              int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                              int64_t num_pages, int32_t max_q_len, int64_t max_kv_len,
+                              int64_t num_tokens, int32_t key_slices, void *workspace,
+                              size_t workspace_bytes, float softmax_scale, void *stream);
 
 #ifdef __cplusplus
 }

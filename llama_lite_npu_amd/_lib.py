@@ -19,7 +19,7 @@ import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "csrc" / "liblitekv.so"
 
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 # name -> (restype, argtypes); mirrors include/litekv.h declaration by declaration.
 SIGNATURES = {
@@ -219,6 +219,33 @@ SIGNATURES = {
         c_int32,
         [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int64,
          c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int32, c_float, c_void_p],
+    ),
+    "litekv_kv_append_int4": (
+        c_int32,
+        [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int32, c_int32,
+         c_int64, c_void_p],
+    ),
+    "litekv_qk_norm_rope_append_int4": (
+        c_int32,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_int64, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int64, c_float, c_void_p],
+    ),
+    "litekv_page_dequant_int4": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int64,
+         c_int64, c_void_p],
+    ),
+    "litekv_paged_decode_int4": (
+        c_int32,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+         c_void_p, c_void_p, c_size_t, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int32,
+         c_int32, c_float, c_void_p],
+    ),
+    "litekv_paged_prefill_int4": (
+        c_int32,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int64,
+         c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int32, c_int64, c_int64, c_int32,
+         c_void_p, c_size_t, c_float, c_void_p],
     ),
     "litekv_varlen_prefill": (
         c_int32,

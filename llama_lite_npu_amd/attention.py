@@ -13,7 +13,7 @@ arguments, driven by the same ``AttentionInfo``. Differences:
   chunks), so one kernel serves both branches of the reference;
 * ``qkv_epilogue`` folds the step before the append (QK RMSNorm, rotary embedding,
   qwen3.py:124-129) into the append itself; the forward calls are then made with ``xk=None``;
-* a layer whose pool holds fp8 or int8 codes (``atten_info.kv_scales[layer]`` set) quantises on append
+* a layer whose pool holds fp8 or int8 codes (or 4-bit ones, which need no scales) (``atten_info.kv_scales[layer]`` set) quantises on append
   and attends straight from the codes, in decode and in chunks over cached history; fresh
   prompts attend to their own fp16 K/V.
 
@@ -61,7 +61,7 @@ class Attention:
         (None when ``qkv_epilogue`` already stored them)."""
         pool = atten_info.kv_buffer[layer_index]
         scale = (1.0 / math.sqrt(self.head_dim)) if qk_scale is None else float(qk_scale) / LOG2E
-        if ops.is_quantised_pool(pool):
+        if ops.is_quantised_pool(pool) or ops.is_int4_pool(pool):
             return self._context_forward_fp8(xq, xk, xv, atten_info, pool, atten_info.kv_scales[layer_index], scale)
         if xk is not None:
             ops.kv_append(xk, xv, atten_info.cur_select_index, pool)
@@ -104,7 +104,7 @@ class Attention:
         if plan is not None:
             return ops.decode_step(xq, pool, plan, xk, xv, scale, kv_scales=scales)
         if xk is not None:
-            if scales is not None:
+            if scales is not None or ops.is_int4_pool(pool):
                 ops.kv_append_quantised(xk, xv, atten_info.cur_select_index, pool, scales)
             else:
                 ops.kv_append(xk, xv, atten_info.cur_select_index, pool)

@@ -27,10 +27,12 @@ SOURCES = (
     "status.hip",
     "kv_append.hip",
     "kv_fp8.hip",
+    "kv_int4.hip",
     "qk_rope_append.hip",
     "page_ops.hip",
     "paged_decode.hip",
     "paged_decode_hd64.hip",
+    "paged_decode_int4.hip",
     "decode_advance.hip",
     "copy_segments.hip",
     "paged_prefill.hip",

@@ -107,6 +107,18 @@ struct LineCut {
   }
 };
 
+// 16-token pages of a sequence, and the splits it is cut into (see litekv_paged_decode).
+__host__ __device__ __forceinline__ int pages_of(int len) {
+  return len > 0 ? (len + kPageSize - 1) / kPageSize : 0;
+}
+
+__host__ __device__ __forceinline__ int splits_for_pages(int pages, int max_splits,
+                                                         int min_pages_per_split) {
+  int n = (pages + min_pages_per_split - 1) / min_pages_per_split;
+  n = n < 1 ? 1 : n;
+  return n < max_splits ? n : max_splits;
+}
+
 // One decode call, as the launchers of paged_decode.hip take it.
 struct DecodeArgs {
   const void *q;
@@ -215,6 +227,26 @@ int launch_generic_attention(const char *what, const GenericLaunch &a);
 // 2^x on the transcendental unit (v_exp_f32); exp2(-inf) == 0.
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float fast_log2(float x) { return __builtin_amdgcn_logf(x); }
+
+__device__ __forceinline__ int clamp_page(int pid, int num_pages) {
+  return pid < 0 ? 0 : (pid >= num_pages ? num_pages - 1 : pid);
+}
+
+// Pools whose pages hold 16 << shift tokens: the kernels keep working on 16-token pages, and the
+// 16-token page j of a sequence is part j % (1 << shift) of the sequence's page j >> shift, whose
+// tokens are contiguous in the pool. `entry` is the block-table entry of that page.
+__device__ __forceinline__ int sub_page_id(int entry, int j, int shift, int num_pages) {
+  return (clamp_page(entry, num_pages) << shift) + (j & ((1 << shift) - 1));
+}
+
+// Step metadata that no launch of the decode kernel modifies (plan entries, sequence lengths) is
+// read through the constant address space: with a wavefront-uniform address such a load is
+// always a scalar load, whatever fences and atomics surround it, so it never joins the in-order
+// queue of the vector loads that stream K/V.
+typedef const __attribute__((address_space(4))) int32_t *uniform_i32_ptr;
+__device__ __forceinline__ uniform_i32_ptr as_uniform(const int32_t *p) {
+  return (uniform_i32_ptr)(uintptr_t)p;
+}
 
 // Value held by lane (lane ^ mask) of the same wavefront.
 __device__ __forceinline__ float xor_lane(float v, int mask) { return __shfl_xor(v, mask, kWave); }

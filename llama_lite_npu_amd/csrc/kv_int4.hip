@@ -1,0 +1,257 @@
+// 4-bit pools (kv_int4.h): the append of rows, alone or as the tail of the QKV projection's epilogue, and the
+// read-back of pages as fp16.
+//
+// A row is held by D / 8 lanes, 8 elements each. The epilogue (per-head RMSNorm, rotary embedding; see qk_rope_append.hip) stays
+// in fp32 from the fp16 inputs to the one rounding of q and to the quantiser: a K row is not rounded to fp16 on the way,
+// which would move one element in some hundred over a code's border. The sum of squares is taken in fp64, where the order
+// of its additions does not show, and each product and sum behind it is rounded by itself (no contraction): codes next
+// to a border are then the same however a row's lanes are laid out.
+#include <type_traits>
+
+#include "common.h"
+#include "kv_int4.h"
+
+namespace litekv {
+
+// Rows [0, num_q_heads) of a token are q's, the next num_kv_heads K's, then V's. num_q_heads 0: the append alone. TOK tokens a
+// lane, see qk_norm_rope_append_kernel.
+template <int L, int TOK>
+__global__ __launch_bounds__(256) void int4_append_kernel(
+    half_t *__restrict__ q, int64_t q_stride, const half_t *__restrict__ k, int64_t k_stride,
+    const half_t *__restrict__ v, int64_t v_stride, const half_t *__restrict__ q_weight,
+    const half_t *__restrict__ k_weight, const half_t *__restrict__ cos_rows,
+    const half_t *__restrict__ sin_rows, int64_t cs_stride, const int32_t *__restrict__ slot_mapping,
+    uint8_t *__restrict__ pool, int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads, int64_t num_slots,
+    float eps) {
+#pragma clang fp contract(off)
+  constexpr int kDim = 8 * L;
+  const int l = threadIdx.x & (L - 1);
+  const int r = (int)blockIdx.y * (256 / L) + (int)(threadIdx.x / L);
+  if (r >= num_q_heads + 2 * num_kv_heads) return;  // whole L-lane groups leave together
+  const bool is_v = r >= num_q_heads + num_kv_heads;
+  const bool is_q = r < num_q_heads;
+  const int head = is_q ? r : (is_v ? r - num_q_heads - num_kv_heads : r - num_q_heads);
+  int64_t token[TOK], slot[TOK];
+  bool live[TOK];
+  half8_t x[TOK], c[TOK], sn[TOK];
+#pragma unroll
+  for (int t = 0; t < TOK; ++t) {
+    token[t] = (int64_t)blockIdx.x * TOK + t;
+    live[t] = token[t] < num_tokens;
+    if (!live[t]) token[t] = num_tokens - 1;  // loads repeat the last token; nothing is stored
+    const half_t *src = is_q   ? q + token[t] * q_stride + (int64_t)head * kDim
+                        : is_v ? v + token[t] * v_stride + (int64_t)head * kDim
+                               : k + token[t] * k_stride + (int64_t)head * kDim;
+    x[t] = *(const half8_t *)(src + 8 * l);
+    slot[t] = slot_mapping[token[t]];
+    if (cos_rows != nullptr && !is_v) {
+      const int j = 8 * (l & (L / 2 - 1));  // the first D / 2 entries of a cos / sin row
+      c[t] = *(const half8_t *)(cos_rows + token[t] * cs_stride + j);
+      sn[t] = *(const half8_t *)(sin_rows + token[t] * cs_stride + j);
+    }
+  }
+  const half_t *weight = is_q ? q_weight : k_weight;
+  half8_t w = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+  if (weight != nullptr && !is_v) w = *(const half8_t *)(weight + 8 * l);
+
+#pragma unroll
+  for (int t = 0; t < TOK; ++t) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = (float)x[t][i];
+    if (weight != nullptr && !is_v) {
+      double ss = 0.0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = __builtin_fma((double)y[i], (double)y[i], ss);
+      ss = over_row<L>(ss, [](double a, double b) { return a + b; });
+      const double ms = ss * (1.0 / kDim) + (double)eps;
+      // 1 / sqrt(ms): the hardware's approximation, twice improved (one step leaves about 2^-50 of it)
+      double rs = __builtin_amdgcn_rsq(ms);
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        const double e = __builtin_fma(-ms * rs, rs, 1.0);
+        rs = __builtin_fma(0.5 * rs, e, rs);
+      }
+      const float rrms = (float)rs;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = y[i] * rrms * (float)w[i];
+    }
+    if (cos_rows != nullptr && !is_v) {
+      // partner: element i + D / 2 for the first half of the row, i - D / 2 for the second
+      const float sign = l < L / 2 ? -1.0f : 1.0f;
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = half_a_row_away<L>(y[i]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float own = y[i] * (float)c[t][i], other = p[i] * (float)sn[t][i];
+        y[i] = own + sign * other;
+      }
+    }
+    if (is_q) {
+      half8_t o;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = (half_t)y[i];
+      if (live[t]) *(half8_t *)(q + token[t] * q_stride + (int64_t)head * kDim + 8 * l) = o;
+    } else {
+      const Int4Row row = int4_row<L>(y);
+      if (live[t] && slot[t] >= 0 && slot[t] < num_slots) {
+        int4_store<kDim>(pool, slot[t], num_kv_heads, is_v ? num_kv_heads + head : head, l, row);
+      }
+    }
+  }
+}
+
+// Pages as fp16 [slots][2 * Hkv][D]: a lane makes 8 elements of a row, neighbouring lanes neighbouring ones, so that stores
+// are whole lines; a block's codes are read in pieces of 4 (K) and 2 bytes (V) that share lines.
+template <int D>
+__global__ __launch_bounds__(256) void page_dequant_int4_kernel(
+    const uint8_t *__restrict__ src_pool, half_t *__restrict__ dst_pool, const int32_t *__restrict__ src_ids,
+    const int32_t *__restrict__ dst_ids, int32_t kv_heads, int32_t page_size, int64_t num_src_pages,
+    int64_t num_dst_pages, int32_t tiles) {
+  const int64_t i = blockIdx.x / (uint32_t)tiles;
+  const int32_t item = (int32_t)(blockIdx.x - i * tiles) * 256 + (int32_t)threadIdx.x;
+  constexpr int kPieces = D / 8;   // of a row
+  if (item >= page_size * 2 * kv_heads * kPieces) return;
+  const int64_t sp = src_ids[i];
+  const int64_t dp = dst_ids ? (int64_t)dst_ids[i] : i;
+  if (sp < 0 || sp >= num_src_pages || dp < 0 || dp >= num_dst_pages) return;
+  const int w = item % kPieces;
+  const int row = item / kPieces;
+  const int head = row % (2 * kv_heads);
+  const int in_page = row / (2 * kv_heads);
+  const int t = in_page & 15;
+  const uint8_t *block = src_pool + ((sp * page_size + in_page) >> 4) * int4_block_bytes(kv_heads, D);
+  const uint8_t *codes = block + int4_codes_at(head, D);
+  const uint32_t word = *(const uint16_t *)(block + int4_words_at(head, kv_heads, D) + 2 * t);
+  uint32_t x;
+  if (head < kv_heads) {
+    x = *(const uint32_t *)(codes + t * (D / 2) + 4 * w);
+  } else if constexpr (D == 128) {
+    x = *(const uint16_t *)(codes + int4_v_unit<D>(t, w, 0)) |
+        ((uint32_t)*(const uint16_t *)(codes + int4_v_unit<D>(t, w, 1)) << 16);
+  } else {
+    const uint32_t a = *(const uint16_t *)(codes + int4_v_unit<D>(t, 2 * w, 0));
+    const uint32_t b = *(const uint16_t *)(codes + int4_v_unit<D>(t, 2 * w + 1, 0));
+    // even elements down, odd ones up, as in int4_pack
+    x = (a & 0xfu) | ((a >> 4) & 0xf0u) | ((b & 0xfu) << 8) | ((b & 0xf00u) << 4) | ((a & 0xf0u) << 12) |
+        ((a & 0xf000u) << 8) | ((b & 0xf0u) << 20) | ((b & 0xf000u) << 16);
+  }
+  const half8_t y = int4x8_to_half(x, word | (word << 16));
+  *(half8_t *)(dst_pool + ((dp * page_size + in_page) * (int64_t)(2 * kv_heads) + head) * D + 8 * w) = y;
+}
+
+static int launch_int4_append(const char *what, void *q, int64_t q_token_stride, const void *k,
+                              int64_t k_token_stride, const void *v, int64_t v_token_stride,
+                              const void *q_norm_weight, const void *k_norm_weight, const void *cos_rows,
+                              const void *sin_rows, int64_t cos_sin_token_stride, const int32_t *slot_mapping,
+                              void *kv_pool, int32_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                              int32_t head_dim, int64_t num_slots, float rms_eps, void *stream) {
+  LITEKV_REQUIRE(num_tokens >= 0, "%s: num_tokens %d < 0", what, num_tokens);
+  LITEKV_REQUIRE(int4_head_dim(head_dim), "%s: head_dim %d unsupported (64 or 128)", what, head_dim);
+  LITEKV_REQUIRE(num_q_heads >= 0 && num_kv_heads > 0 && num_q_heads <= 65535 && num_kv_heads <= 65535,
+                 "%s: num_q_heads %d / num_kv_heads %d invalid", what, num_q_heads, num_kv_heads);
+  if (num_tokens == 0) {
+    clear_error();
+    return LITEKV_OK;
+  }
+  LITEKV_REQUIRE((q || num_q_heads == 0) && k && v && slot_mapping && kv_pool, "%s: null pointer", what);
+  LITEKV_REQUIRE((q_norm_weight == nullptr) == (k_norm_weight == nullptr),
+                 "%s: q_norm_weight and k_norm_weight go together", what);
+  LITEKV_REQUIRE((cos_rows == nullptr) == (sin_rows == nullptr), "%s: cos and sin go together", what);
+  LITEKV_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(kv_pool) &&
+                     aligned16(q_norm_weight) && aligned16(k_norm_weight) && aligned16(cos_rows) &&
+                     aligned16(sin_rows),
+                 "%s: all tensors must be 16-byte aligned", what);
+  LITEKV_REQUIRE((num_q_heads == 0 || (q_token_stride >= (int64_t)num_q_heads * head_dim && q_token_stride % 8 == 0)) &&
+                     k_token_stride >= (int64_t)num_kv_heads * head_dim && k_token_stride % 8 == 0 &&
+                     v_token_stride >= (int64_t)num_kv_heads * head_dim && v_token_stride % 8 == 0,
+                 "%s: token strides (%lld, %lld, %lld) invalid", what, (long long)q_token_stride,
+                 (long long)k_token_stride, (long long)v_token_stride);
+  LITEKV_REQUIRE(cos_rows == nullptr || (cos_sin_token_stride >= head_dim / 2 && cos_sin_token_stride % 8 == 0),
+                 "%s: cos/sin token stride %lld invalid (>= %d, multiple of 8)", what,
+                 (long long)cos_sin_token_stride, head_dim / 2);
+  LITEKV_REQUIRE(num_slots > 0 && num_slots % kInt4Block == 0, "%s: num_slots %lld is not a positive multiple of 16",
+                 what, (long long)num_slots);
+  LITEKV_REQUIRE(rms_eps >= 0.f, "%s: rms_eps %g < 0", what, (double)rms_eps);
+  const int rows_per_wg = 256 / (head_dim / 8);
+  const int row_blocks = (num_q_heads + 2 * num_kv_heads + rows_per_wg - 1) / rows_per_wg;
+  LITEKV_REQUIRE(row_blocks <= 65535, "%s: too many heads", what);
+  auto launch = [&](auto kernel, int tok) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((num_tokens + tok - 1) / tok), (unsigned)row_blocks), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), static_cast<half_t *>(q), q_token_stride,
+                       static_cast<const half_t *>(k), k_token_stride, static_cast<const half_t *>(v), v_token_stride,
+                       static_cast<const half_t *>(q_norm_weight), static_cast<const half_t *>(k_norm_weight),
+                       static_cast<const half_t *>(cos_rows), static_cast<const half_t *>(sin_rows),
+                       cos_sin_token_stride, slot_mapping, static_cast<uint8_t *>(kv_pool), (int64_t)num_tokens,
+                       num_q_heads, num_kv_heads, num_slots, rms_eps);
+  };
+  if (head_dim == 64) {
+    launch(int4_append_kernel<8, 1>, 1);
+  } else {
+    launch(int4_append_kernel<16, 1>, 1);
+  }
+  return check_launch(what);
+}
+
+}  // namespace litekv
+
+extern "C" int litekv_kv_append_int4(const void *k, const void *v, int64_t k_token_stride, int64_t v_token_stride,
+                                     const int32_t *slot_mapping, void *kv_pool_int4, int32_t num_tokens,
+                                     int32_t num_kv_heads, int32_t head_dim, int64_t num_slots, void *stream) {
+  return litekv::launch_int4_append("kv_append_int4", nullptr, 0, k, k_token_stride, v, v_token_stride, nullptr,
+                                    nullptr, nullptr, nullptr, 0, slot_mapping, kv_pool_int4, num_tokens, 0,
+                                    num_kv_heads, head_dim, num_slots, 0.f, stream);
+}
+
+extern "C" int litekv_qk_norm_rope_append_int4(void *q, int64_t q_token_stride, const void *k, int64_t k_token_stride,
+                                               const void *v, int64_t v_token_stride, const void *q_norm_weight,
+                                               const void *k_norm_weight, const void *cos_rows, const void *sin_rows,
+                                               int64_t cos_sin_token_stride, const int32_t *slot_mapping,
+                                               void *kv_pool_int4, int32_t num_tokens, int32_t num_q_heads,
+                                               int32_t num_kv_heads, int32_t head_dim, int64_t num_slots,
+                                               float rms_eps, void *stream) {
+  if (num_q_heads <= 0) {
+    return litekv::fail(LITEKV_ERR_INVALID_ARGUMENT, "qk_norm_rope_append_int4: num_q_heads %d invalid", num_q_heads);
+  }
+  return litekv::launch_int4_append("qk_norm_rope_append_int4", q, q_token_stride, k, k_token_stride, v,
+                                    v_token_stride, q_norm_weight, k_norm_weight, cos_rows, sin_rows,
+                                    cos_sin_token_stride, slot_mapping, kv_pool_int4, num_tokens, num_q_heads,
+                                    num_kv_heads, head_dim, num_slots, rms_eps, stream);
+}
+
+extern "C" int litekv_page_dequant_int4(const void *kv_pool_int4, void *dst_pool, const int32_t *src_ids,
+                                        const int32_t *dst_ids, int32_t n, int32_t num_kv_heads, int32_t head_dim,
+                                        int32_t page_size, int64_t num_src_pages, int64_t num_dst_pages,
+                                        void *stream) {
+  using namespace litekv;
+  LITEKV_REQUIRE(n >= 0, "page_dequant_int4: n %d < 0", n);
+  if (n == 0) {
+    clear_error();
+    return LITEKV_OK;
+  }
+  LITEKV_REQUIRE(kv_pool_int4 && dst_pool && src_ids, "page_dequant_int4: null pointer");
+  LITEKV_REQUIRE(int4_head_dim(head_dim), "page_dequant_int4: head_dim %d unsupported (64 or 128)", head_dim);
+  LITEKV_REQUIRE(num_kv_heads > 0 && num_kv_heads <= 65535, "page_dequant_int4: num_kv_heads %d invalid", num_kv_heads);
+  LITEKV_REQUIRE(page_shift_of(page_size) >= 0, "page_dequant_int4: page_size %d unsupported (16, 32, 64, 128 or 256)",
+                 page_size);
+  LITEKV_REQUIRE(aligned16(kv_pool_int4) && aligned16(dst_pool), "page_dequant_int4: pools must be 16-byte aligned");
+  LITEKV_REQUIRE(num_src_pages > 0 && num_dst_pages > 0, "page_dequant_int4: empty pool");
+  LITEKV_REQUIRE(dst_ids != nullptr || n <= num_dst_pages,
+                 "page_dequant_int4: %d pages do not fit a destination of %lld", n, (long long)num_dst_pages);
+  const int64_t items = (int64_t)page_size * 2 * num_kv_heads * (head_dim / 8);
+  const int64_t tiles = (items + 255) / 256;
+  LITEKV_REQUIRE(items <= 0x7fffffffLL && tiles * n <= 0x7fffffffLL,
+                 "page_dequant_int4: %d pages are too many for one launch", n);
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * n)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                       static_cast<const uint8_t *>(kv_pool_int4), static_cast<half_t *>(dst_pool), src_ids, dst_ids,
+                       num_kv_heads, page_size, num_src_pages, num_dst_pages, (int32_t)tiles);
+  };
+  if (head_dim == 64) {
+    launch(page_dequant_int4_kernel<64>);
+  } else {
+    launch(page_dequant_int4_kernel<128>);
+  }
+  return check_launch("page_dequant_int4");
+}

@@ -67,17 +67,6 @@ constexpr float kLn2 = 0.6931471805599453f;
 // division by the denominator cancels the choice of max exactly.
 constexpr float kMaxSlack = 8.0f;
 
-__host__ __device__ __forceinline__ int pages_of(int len) {
-  return len > 0 ? (len + kPageSize - 1) / kPageSize : 0;
-}
-
-__host__ __device__ __forceinline__ int splits_for_pages(int pages, int max_splits,
-                                                         int min_pages_per_split) {
-  int n = (pages + min_pages_per_split - 1) / min_pages_per_split;
-  n = n < 1 ? 1 : n;
-  return n < max_splits ? n : max_splits;
-}
-
 // One page of an fp16 pool as this lane requested it. A V row is 16 columns of 16 bytes at head dim 128, so a load of
 // the wavefront covers four rows; at 64 it is 8 columns, and a load covers eight (over codes: all sixteen). With
 // the lanes of 128, the upper half re-reading the lower half's columns, every V byte was loaded, converted and
@@ -539,17 +528,6 @@ __device__ __forceinline__ void unpark_state(const float *park, bool final_row, 
 // branch joins the main path, and would drain the whole prefetch queue on every iteration.
 __device__ __forceinline__ void wait_vector_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
-__device__ __forceinline__ int clamp_page(int pid, int num_pages) {
-  return pid < 0 ? 0 : (pid >= num_pages ? num_pages - 1 : pid);
-}
-
-// Pools whose pages hold 16 << shift tokens: the kernels keep working on 16-token pages, and the
-// 16-token page j of a sequence is part j % (1 << shift) of the sequence's page j >> shift, whose
-// tokens are contiguous in the pool. `entry` is the block-table entry of that page.
-__device__ __forceinline__ int sub_page_id(int entry, int j, int shift, int num_pages) {
-  return (clamp_page(entry, num_pages) << shift) + (j & ((1 << shift) - 1));
-}
-
 // This lane's parts of the step's new K and V rows (fp16, head h of one sequence): the pieces
 // that sit where the lane's page registers hold the token's row (see PageRegs / PageRegsFp8).
 template <bool FP8>
@@ -569,15 +547,6 @@ __device__ __forceinline__ void load_new_rows(uint4_t (&kr)[4], uint4_t (&vr)[2]
     vr[0] = *(const uint4_t *)(vn + v_col_of(n));
     vr[1] = uint4_t{0, 0, 0, 0};  // fp8 only
   }
-}
-
-// Step metadata that no launch of the decode kernel modifies (plan entries, sequence lengths) is
-// read through the constant address space: with a wavefront-uniform address such a load is
-// always a scalar load, whatever fences and atomics surround it, so it never joins the in-order
-// queue of the vector loads that stream K/V.
-typedef const __attribute__((address_space(4))) int32_t *uniform_i32_ptr;
-__device__ __forceinline__ uniform_i32_ptr as_uniform(const int32_t *p) {
-  return (uniform_i32_ptr)(uintptr_t)p;
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -1,0 +1,425 @@
+// Paged flash-decoding over a 4-bit pool (kv_int4.h): one wavefront per (sequence, kv head, split), partial rows
+// merged by litekv_paged_decode_merge.
+//
+// The kernel works on the codes. With q the rows of up to 16 query heads of the kv head as columns, key i's score is
+//     S[i] = s_i * (sum_d c_id q_d - z_i * sum_d q_d)
+// and an output row
+//     O[d] = sum_i (p_i s'_i) (c'_id - z'_i)       p = softmax of S, s', z', c' those of V
+// so a scale and a zero point cost a few instructions per key instead of one per element. Codes reach the matrix cores with
+// nothing but a shift and a mask: c in bits 4 .. 7 of an fp16 number is the subnormal c * 2^-20. The matrix cores take it as it
+// is, but do not normalise it: products are lined up by the exponents of their factors and cut off some 27 bits below the largest of
+// a sum. From bits 4 .. 7 that leaves 24 bits of a code's own size; in bits 0 .. 3, which need two instructions fewer for eight
+// codes, 20 (333 keys with one that carries nearly all of the weight: outputs 1e-5 of sum p |v| off, all to one side).
+// For the same reason the z' are subtracted step by step, by an MFMA of their own per tile, and not at the end from an accumulator
+// that would have grown to some twenty times the result.
+//
+// S^T[key][col] is the accumulator of the first product (16x16x32: 16 keys, 32 of D) and in the same lanes the right operand of the
+// second, O^T[d][col] += V^T[d][key] P^T[key][col], whose 32 keys are two blocks of 16: nothing crosses lanes and no LDS
+// is used. p s' as fp16 would cost the result as much again as its own rounding: up to 8 query heads, which leave half
+// of the columns empty, columns 8..15 carry the same heads and hold what the rounding left; with more
+// a second MFMA does. So a result is as good as with fp32 probabilities.
+//
+// The reference of the exponentials is the largest p s' so far, not the largest p: in fp16 it is p s' that has to fit. It is put
+// at 2^7 and may grow to 2^15 before the accumulators are rescaled.
+#include <type_traits>
+
+#include "common.h"
+#include "kv_int4.h"
+
+namespace litekv {
+
+typedef uint32_t uint2v_t __attribute__((ext_vector_type(2)));
+
+constexpr int kInt4Waves = 4;            // most wavefronts of a workgroup
+constexpr float kInt4Top = 7.0f;         // log2 of where the largest p s' is put
+constexpr float kInt4Grown = 32768.0f;   // and what it may grow to
+constexpr float kLog2eI4 = 1.4426950408889634f, kLn2I4 = 0.6931471805599453f;
+
+// A block of 16 tokens as a lane (n = lane % 16, g = lane / 16) holds it: of K row n the g-th quarter, of V rows 4g .. 4g + 3
+// column n, and the words of rows 4g .. 4g + 3 of both.
+template <int D>
+struct Int4Regs {
+  uint32_t k[D / 32], v[D / 32];
+  uint32_t kw[2], vw[2];
+};
+
+// Eight codes of a dword as fp16 pairs, times 2^-20.
+__device__ __forceinline__ void int4_pairs(uint32_t x, uint32_t (&out)[4]) {
+  out[0] = (x << 4) & 0x00f000f0u;
+  out[1] = x & 0x00f000f0u;
+  out[2] = (x >> 4) & 0x00f000f0u;
+  out[3] = (x >> 8) & 0x00f000f0u;
+}
+__device__ __forceinline__ half8_t as_half8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(half8_t, uint4_t{a, b, c, d});
+}
+
+// TWO: more than 8 query heads, whose second part of p s' has MFMAs of its own.
+template <int D, bool TWO>
+__global__ __launch_bounds__(kInt4Waves *kWave) void paged_decode_int4_kernel(
+    const half_t *__restrict__ q, int64_t q_batch_stride, uint8_t *pool, const int32_t *__restrict__ block_table,
+    int32_t bt_stride, const int32_t *__restrict__ seq_lens, const half_t *__restrict__ k_new,
+    const half_t *__restrict__ v_new, int64_t k_new_stride, int64_t v_new_stride, half_t *__restrict__ out,
+    float *__restrict__ part_o, float *__restrict__ part_lse, int32_t num_q_heads, int32_t num_kv_heads,
+    int32_t group_all, int32_t slices, int32_t max_splits, int32_t min_pages_per_split, int32_t num_pages,
+    int32_t page_shift, float scale_log2) {
+  constexpr int kSteps = D / 32;   // MFMAs of a block's scores; dwords a lane holds of K and of V
+  constexpr int kTiles = D / 16;   // 16-row tiles of O^T
+  constexpr int kUnits = D / 64;   // see int4_v_unit
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int n = lane & 15, g = lane >> 4;
+  const HeadSlice hs = head_slice(blockIdx.x * (blockDim.x >> 6) + wave, slices, group_all);
+  const int h = hs.kv_head, group = hs.q_heads, hq0 = hs.q_head0;
+  const int split = blockIdx.y, b = blockIdx.z;
+  const int len = as_uniform(seq_lens)[b];
+  half_t *out_row = out + ((int64_t)b * num_q_heads + hq0) * D;
+  if (len <= 0) {
+    if (split == 0) {
+      for (int i = lane; i < group * (D / 8); i += kWave) *(half8_t *)(out_row + 8 * i) = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+    return;
+  }
+  const int pages = pages_of(len);
+  const int n_splits = splits_for_pages(pages, max_splits, min_pages_per_split);
+  if (split >= n_splits) return;
+  const int p0 = (int)(((int64_t)split * pages) / n_splits);
+  const int p1 = (int)(((int64_t)(split + 1) * pages) / n_splits);
+
+  const int64_t block_bytes = int4_block_bytes(num_kv_heads, D);
+  const uniform_i32_ptr table = as_uniform(block_table) + (int64_t)b * bt_stride;
+  // A length beyond what a block-table row can name re-reads the row's last entry; pages past the split's re-read its last.
+  auto page_id = [&](int p) {
+    const int pp = p < p1 ? p : p1 - 1;
+    const int at = pp >> page_shift;
+    return sub_page_id(table[at < bt_stride ? at : bt_stride - 1], pp, page_shift, num_pages);
+  };
+
+  // The step's new token goes into the last block before anything of it is read (by this wavefront, the only one that reads it
+  // in this launch; the slices of a wide group all write the same bytes).
+  if (k_new != nullptr && p1 == pages && pages <= (bt_stride << page_shift)) {
+    constexpr int L = D / 8;
+    if (lane < 2 * L) {
+      const bool is_v = lane >= L;
+      const int l = lane & (L - 1);
+      const half_t *src = is_v ? v_new + (int64_t)b * v_new_stride : k_new + (int64_t)b * k_new_stride;
+      const half8_t x16 = *(const half8_t *)(src + (int64_t)h * D + 8 * l);
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = (float)x16[i];
+      const int64_t slot = (int64_t)page_id(pages - 1) * kInt4Block + ((len - 1) & (kInt4Block - 1));
+      int4_store<D>(pool, slot, num_kv_heads, is_v ? num_kv_heads + h : h, l, int4_row<L>(x));
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the stores are done
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  }
+
+  const uint32_t k_off = (uint32_t)(int4_codes_at(h, D) + n * (D / 2) + g * (D / 8));
+  const uint32_t v_off = (uint32_t)(int4_codes_at(num_kv_heads + h, D) + g * (2 * D) + n * (D / 8));
+  const uint32_t kw_off = (uint32_t)(int4_words_at(h, num_kv_heads, D) + 8 * g);
+  const uint32_t vw_off = (uint32_t)(int4_words_at(num_kv_heads + h, num_kv_heads, D) + 8 * g);
+  auto request = [&](int p, Int4Regs<D> &r) {
+    const uint8_t *block = pool + (int64_t)page_id(p) * block_bytes;
+    typedef uint32_t vec __attribute__((ext_vector_type(kSteps)));
+    const vec kk = *(const vec *)(block + k_off), vv = *(const vec *)(block + v_off);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      r.k[i] = kk[i];
+      r.v[i] = vv[i];
+    }
+    const uint2v_t kw = *(const uint2v_t *)(block + kw_off), vw = *(const uint2v_t *)(block + vw_off);
+    r.kw[0] = kw[0];
+    r.kw[1] = kw[1];
+    r.vw[0] = vw[0];
+    r.vw[1] = vw[1];
+  };
+  Int4Regs<D> buf[2][2];
+  request(p0, buf[0][0]);
+  request(p0 + 1, buf[0][1]);
+
+  // q as the right operand: column n, of every dword of K that the lane of the same g holds the eight elements, scaled by a
+  // power of two that puts the row's largest at 2^14 or above.
+  half8_t qf[kSteps];
+  float q_sum = 0.f, k_mul;
+  {
+    const int col = TWO ? n : (n & 7);
+    const half_t *row = q + (int64_t)b * q_batch_stride + (int64_t)(hq0 + (col < group ? col : group - 1)) * D +
+                        (D / 4) * g;
+    float x[kSteps][8], most = 0.f;
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t) {
+      const half8_t y = *(const half8_t *)(row + 8 * t);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[t][i] = (float)y[i];
+        most = __builtin_fmaxf(most, __builtin_fabsf(x[t][i]));
+      }
+    }
+    most = __builtin_fmaxf(most, xor_lane(most, 16));
+    most = __builtin_fmaxf(most, xor_lane(most, 32));
+    const int up = most > 0.f ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const half_t y = (half_t)__builtin_amdgcn_ldexpf(x[t][i], up);
+        q_sum += (float)y;
+        qf[t][i] = y;
+      }
+    }
+    q_sum += xor_lane(q_sum, 16);
+    q_sum += xor_lane(q_sum, 32);
+    k_mul = __builtin_amdgcn_ldexpf(scale_log2, 20 - up);
+  }
+  const uint32_t hi_mask = !TWO && n >= 8 ? ~0u : 0u;   // of the columns that carry the second part
+
+  float4_t acc[kTiles];
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j) acc[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+  float ref = -1e30f, total = 0.f;   // reference of the exponentials; sum of p
+  const int end = len < p1 * kInt4Block ? len : p1 * kInt4Block;
+
+  auto attend = [&](Int4Regs<D> (&r)[2], int p, auto masked_tag) {
+    constexpr bool MASKED = decltype(masked_tag)::value;
+    float4_t st[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      st[u] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t) {
+        uint32_t x[4];
+        int4_pairs(r[u].k[t], x);
+        st[u] = mfma_16x16x32(as_half8(x[0], x[1], x[2], x[3]), qf[t], st[u]);
+      }
+    }
+    half2_t ks[4], kz[4], vs[4];   // of the lane's keys 2i, 2i + 1 (0, 1: the first block's)
+    uint32_t vz[4];                       // -z' of those keys, times 2^-20
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t kw = r[i >> 1].kw[i & 1], vw = r[i >> 1].vw[i & 1];
+      if constexpr (MASKED) {
+        // rows past the end: finite values for zero probabilities to multiply
+        const int left = end - p * kInt4Block - 16 * (i >> 1) - 4 * g - 2 * (i & 1);
+        const uint32_t keep = left >= 2 ? ~0u : left == 1 ? 0xffffu : 0u;
+        kw &= keep;
+        vw &= keep;
+      }
+      ks[i] = int4_scales(kw);
+      kz[i] = __builtin_bit_cast(half2_t, (kw << 4) & 0x00f000f0u);
+      vs[i] = int4_scales(vw);
+      vz[i] = ((vw << 4) & 0x00f000f0u) | 0x80008000u;
+    }
+    float x[8];   // scores in log2 units
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float y = __builtin_fmaf(-(float)kz[i >> 1][i & 1], q_sum, st[i >> 2][i & 3]) * k_mul;
+      x[i] = y * (float)ks[i >> 1][i & 1];
+      if constexpr (MASKED) {
+        if (p * kInt4Block + 16 * (i >> 2) + 4 * g + (i & 3) >= end) x[i] = -INFINITY;
+      }
+    }
+    float pr[8], w[8], sum;
+    auto exponentials = [&]() {
+      sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        pr[i] = fast_exp2(x[i] - ref);
+        sum += pr[i];
+        w[i] = __builtin_fmaf(pr[i], (float)vs[i >> 1][i & 1], 0.0f);
+      }
+    };
+    exponentials();
+    float most = sum * 0x1p-40f;   // (p alone may outgrow fp32 where s' is tiny or 0)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = __builtin_fmaxf(most, w[i]);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > kInt4Grown) != 0, false)) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        top = __builtin_fmaxf(top, x[i] + fast_log2(__builtin_fmaxf((float)vs[i >> 1][i & 1], 0x1p-24f)));
+      }
+      top = __builtin_fmaxf(top, xor_lane(top, 16));
+      top = __builtin_fmaxf(top, xor_lane(top, 32)) - kInt4Top;
+      const float next = __builtin_fmaxf(ref, top);
+      const float alpha = fast_exp2(ref - next);
+      ref = next;
+      total *= alpha;
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) acc[j] *= alpha;
+      exponentials();
+    }
+    total += sum;
+    uint32_t hi[4], lo[4];   // p s' of keys 2i, 2i + 1: what a column carries, and TWO: what that leaves
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      auto toward_zero = [&](float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+      };
+      const uint32_t first = toward_zero(w[2 * i], w[2 * i + 1]);
+      const half2_t off = __builtin_bit_cast(half2_t, TWO ? first : first & hi_mask);
+      const uint32_t rest = toward_zero(w[2 * i] - (float)off[0], w[2 * i + 1] - (float)off[1]);
+      hi[i] = TWO ? first : rest;
+      lo[i] = rest;
+    }
+    const half8_t ph = as_half8(hi[0], hi[1], hi[2], hi[3]), pl = as_half8(lo[0], lo[1], lo[2], lo[3]);
+    const half8_t z = as_half8(vz[0], vz[1], vz[2], vz[3]);
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) acc[j] = mfma_16x16x32(z, ph, acc[j]);
+#pragma unroll
+    for (int e = 0; e < kUnits; ++e) {
+      uint32_t x0[4], x1[4], x2[4], x3[4];   // rows 4g, 4g + 1 of the first block, 4g + 2, 4g + 3, the same of the second
+      int4_pairs(r[0].v[e], x0);
+      int4_pairs(r[0].v[kUnits + e], x1);
+      int4_pairs(r[1].v[e], x2);
+      int4_pairs(r[1].v[kUnits + e], x3);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const half8_t a = as_half8(x0[j], x1[j], x2[j], x3[j]);
+        acc[4 * e + j] = mfma_16x16x32(a, ph, acc[4 * e + j]);
+        if constexpr (TWO) {   // (the small parts only once the large ones have met their zero points)
+          acc[4 * e + j] = mfma_16x16x32(z, pl, acc[4 * e + j]);
+          acc[4 * e + j] = mfma_16x16x32(a, pl, acc[4 * e + j]);
+        }
+      }
+    }
+  };
+
+  // Two blocks a step, the next two in flight.
+  auto step = [&](int p, Int4Regs<D> (&now)[2], Int4Regs<D> (&next)[2]) {
+    if (p + 2 < p1) {
+      request(p + 2, next[0]);
+      request(p + 3, next[1]);
+    }
+    if ((p + 2) * kInt4Block > end) {
+      attend(now, p, std::true_type{});
+    } else {
+      attend(now, p, std::false_type{});
+    }
+  };
+  for (int p = p0; p < p1; p += 4) {
+    step(p, buf[0], buf[1]);
+    if (p + 2 < p1) step(p + 2, buf[1], buf[0]);
+  }
+
+  total += xor_lane(total, 16);
+  total += xor_lane(total, 32);
+  const float inv = 0x1p20f / total;
+  const int head = TWO ? n : (n & 7);
+  const bool whole = n_splits == 1;
+  const int64_t cell = ((int64_t)b * num_q_heads + hq0 + head) * max_splits + split;
+  // O^T tile (e, j): row m is element m * D / 16 + kUnits * j + e of the output row; a lane has rows 4g .. 4g + 3
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float y[kTiles];   // elements (4g + i) * D / 16 ...
+#pragma unroll
+    for (int e = 0; e < kUnits; ++e) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float a = acc[4 * e + j][i];
+        if constexpr (!TWO) a += dpp<kDppRotate8>(a);
+        y[kUnits * j + e] = a * inv;
+      }
+    }
+    // (both halves of the columns have the rows: each stores two of the four)
+    if (head < group && (TWO || (i >> 1) == (n >> 3))) {
+      const int at = (4 * g + i) * kTiles;
+      if (whole) {
+        half_t *o = out_row + (int64_t)head * D + at;
+#pragma unroll
+        for (int j = 0; j < kTiles; j += 4) {
+          *(half4_t *)(o + j) = half4_t{(half_t)y[j], (half_t)y[j + 1], (half_t)y[j + 2], (half_t)y[j + 3]};
+        }
+      } else {
+        float *o = part_o + cell * D + at;
+#pragma unroll
+        for (int j = 0; j < kTiles; j += 4) {
+          __builtin_nontemporal_store(float4_t{y[j], y[j + 1], y[j + 2], y[j + 3]}, (float4_t *)(o + j));
+        }
+      }
+    }
+  }
+  if (!whole && g == 0 && n < group) {
+    __builtin_nontemporal_store((ref + fast_log2(total)) * kLn2I4, part_lse + cell);
+  }
+}
+
+}  // namespace litekv
+
+extern "C" int litekv_paged_decode_int4(const void *q, int64_t q_batch_stride, void *kv_pool_int4,
+                                        const int32_t *block_table, int32_t block_table_stride,
+                                        const int32_t *seq_lens, const void *k_new, const void *v_new,
+                                        int64_t k_new_stride, int64_t v_new_stride, void *out, void *workspace,
+                                        size_t workspace_bytes, int32_t batch, int32_t num_q_heads,
+                                        int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int64_t num_pages,
+                                        int32_t max_splits, int32_t min_pages_per_split, float softmax_scale,
+                                        void *stream) {
+  using namespace litekv;
+  const char *what = "paged_decode_int4";
+  LITEKV_REQUIRE(max_splits >= 1 && max_splits <= 65535, "%s: max_splits %d out of [1, 65535]", what, max_splits);
+  LITEKV_REQUIRE(min_pages_per_split >= 1, "%s: min_pages_per_split %d < 1", what, min_pages_per_split);
+  LITEKV_REQUIRE(batch >= 0 && batch <= 65535, "%s: batch %d out of [0, 65535]", what, batch);
+  LITEKV_REQUIRE(int4_head_dim(head_dim), "%s: head_dim %d unsupported (64 or 128)", what, head_dim);
+  const int page_shift = page_shift_of(page_size);
+  LITEKV_REQUIRE(page_shift >= 0, "%s: page_size %d unsupported (16, 32, 64, 128 or 256)", what, page_size);
+  LITEKV_REQUIRE(num_q_heads > 0 && num_q_heads <= 65535 && num_kv_heads > 0 && num_q_heads % num_kv_heads == 0,
+                 "%s: num_q_heads %d / num_kv_heads %d invalid", what, num_q_heads, num_kv_heads);
+  const int group = num_q_heads / num_kv_heads;
+  LITEKV_REQUIRE(group <= kMaxGroup, "%s: %d query heads per kv head unsupported (max %d)", what, group, kMaxGroup);
+  LITEKV_REQUIRE(num_kv_heads <= 1024, "%s: num_kv_heads %d > 1024", what, num_kv_heads);
+  if (batch == 0) {
+    clear_error();
+    return LITEKV_OK;
+  }
+  LITEKV_REQUIRE(q && kv_pool_int4 && block_table && seq_lens && out, "%s: null pointer", what);
+  LITEKV_REQUIRE((k_new == nullptr) == (v_new == nullptr), "%s: k_new and v_new go together", what);
+  LITEKV_REQUIRE(aligned16(q) && aligned16(kv_pool_int4) && aligned16(out) && aligned16(k_new) && aligned16(v_new),
+                 "%s: q, kv_pool, out, k_new and v_new must be 16-byte aligned", what);
+  LITEKV_REQUIRE(q_batch_stride >= (int64_t)num_q_heads * head_dim && q_batch_stride % 8 == 0,
+                 "%s: q_batch_stride %lld invalid", what, (long long)q_batch_stride);
+  const int64_t row = (int64_t)num_kv_heads * head_dim;
+  LITEKV_REQUIRE(k_new == nullptr || (k_new_stride >= row && v_new_stride >= row && k_new_stride % 8 == 0 &&
+                                      v_new_stride % 8 == 0),
+                 "%s: k_new/v_new strides (%lld, %lld) invalid", what, (long long)k_new_stride, (long long)v_new_stride);
+  LITEKV_REQUIRE(block_table_stride >= 1 &&
+                     (int64_t)block_table_stride * (page_size / kPageSize) <= 0x7fffffffLL / 4,
+                 "%s: block_table_stride %d out of range", what, block_table_stride);
+  LITEKV_REQUIRE(num_pages >= 1 && num_pages <= 0x7fffffffLL / page_size, "%s: num_pages %lld out of range", what,
+                 (long long)num_pages);
+  const size_t need = litekv_paged_decode_workspace_bytes(batch, num_q_heads, head_dim, max_splits);
+  LITEKV_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && aligned16(workspace)),
+                 "%s: 16-byte aligned workspace of %zu bytes needed, got %zu", what, need,
+                 workspace ? workspace_bytes : (size_t)0);
+  // (the kernels count in 16-token pages; saturating)
+  const int64_t min16 = (int64_t)min_pages_per_split * (page_size / kPageSize);
+  const int slices = head_slices(group);
+  const int slice_heads = num_kv_heads * slices;
+  LITEKV_REQUIRE(slice_heads <= 65535, "%s: num_q_heads %d too large", what, num_q_heads);
+  float *part_o = max_splits > 1 ? static_cast<float *>(workspace) : nullptr;
+  float *part_lse = max_splits > 1 ? part_o + (size_t)batch * num_q_heads * max_splits * head_dim : nullptr;
+  // Wavefronts per workgroup: as many kv heads of one (sequence, split), whose codes and words are neighbours in memory, as
+  // leave at least two workgroups per compute unit.
+  const int64_t units = (int64_t)batch * slice_heads * max_splits;
+  int waves = kInt4Waves;
+  while (waves > 1 && (units / waves < 512 || slice_heads % waves != 0)) waves >>= 1;
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(slice_heads / waves), (unsigned)max_splits, (unsigned)batch),
+                       dim3((unsigned)(waves * kWave)), 0, static_cast<hipStream_t>(stream),
+                       static_cast<const half_t *>(q), q_batch_stride, static_cast<uint8_t *>(kv_pool_int4),
+                       block_table, block_table_stride, seq_lens, static_cast<const half_t *>(k_new),
+                       static_cast<const half_t *>(v_new), k_new_stride, v_new_stride, static_cast<half_t *>(out),
+                       part_o, part_lse, num_q_heads, num_kv_heads, group, slices, max_splits,
+                       (int32_t)(min16 < 0x7fffffffLL ? min16 : 0x7fffffffLL), (int32_t)num_pages, page_shift,
+                       softmax_scale * kLog2eI4);
+  };
+  const bool two = (group + slices - 1) / slices > 8;
+  if (head_dim == 64) {
+    two ? launch(paged_decode_int4_kernel<64, true>) : launch(paged_decode_int4_kernel<64, false>);
+  } else {
+    two ? launch(paged_decode_int4_kernel<128, true>) : launch(paged_decode_int4_kernel<128, false>);
+  }
+  const int rc = check_launch(what);
+  if (rc != LITEKV_OK || max_splits == 1) return rc;
+  return litekv_paged_decode_merge(seq_lens, out, workspace, workspace_bytes, batch, num_q_heads, head_dim, page_size,
+                                   max_splits, min_pages_per_split, stream);
+}

@@ -210,7 +210,8 @@ static int launch_paged_prefill(const char *what, const void *q, int64_t q_token
                                 int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
                                 int64_t num_pages, int32_t max_q_len, float softmax_scale,
                                 void *stream, int format, const PrefillKeySplit &split) {
-  const bool fp8 = format != kKvF16;  // a pool of 8-bit codes
+  const bool fp8 = format != kKvF16;  // a pool of codes
+  const bool scaled = fp8 && format != kKvInt4;  // by head (4-bit rows carry their own scales)
   LITEKV_REQUIRE(split.key_slices >= 1 && split.key_slices <= kMaxPrefillKeySlices,
                  "%s: key_slices %d out of [1, %d]", what, split.key_slices, kMaxPrefillKeySlices);
   LITEKV_REQUIRE(split.key_slices == 1 || head_dim == 128 || head_dim == 64,
@@ -231,7 +232,7 @@ static int launch_paged_prefill(const char *what, const void *q, int64_t q_token
     LITEKV_REQUIRE(max_q_len >= 0, "%s: max_q_len %d < 0", what, max_q_len);
     LITEKV_REQUIRE(batch == 0 || max_q_len == 0 || (kv_pool && block_table && cu_q_lens),
                    "%s: null pointer", what);
-    LITEKV_REQUIRE(!fp8 || kv_scales, "%s: null pointer (kv_scales)", what);
+    LITEKV_REQUIRE(!scaled || kv_scales, "%s: null pointer (kv_scales)", what);
     GenericLaunch g;
     g.q = q;
     g.q_row_stride = q_token_stride;
@@ -265,7 +266,7 @@ static int launch_paged_prefill(const char *what, const void *q, int64_t q_token
     return LITEKV_OK;
   }
   LITEKV_REQUIRE(kv_pool && block_table && cu_q_lens, "%s: null pointer", what);
-  LITEKV_REQUIRE(!fp8 || kv_scales, "%s: null pointer (kv_scales)", what);
+  LITEKV_REQUIRE(!scaled || kv_scales, "%s: null pointer (kv_scales)", what);
   LITEKV_REQUIRE(aligned16(kv_pool), "%s: kv_pool must be 16-byte aligned", what);
   LITEKV_REQUIRE(block_table_stride >= 1, "%s: block_table_stride %d < 1", what, block_table_stride);
   LITEKV_REQUIRE(num_pages >= 1 && num_pages <= 0x7fffffffLL / page_size,
@@ -316,7 +317,9 @@ static int launch_paged_prefill(const char *what, const void *q, int64_t q_token
         launch_slices(varlen_prefill_tiled_kernel<MODE>);
       }
     };
-    if (format == kKvInt8) {
+    if (format == kKvInt4) {
+      by_width(std::integral_constant<int, kPagedPrefillSplitInt4>{});
+    } else if (format == kKvInt8) {
       by_width(std::integral_constant<int, kPagedPrefillSplitInt8>{});
     } else if (format == kKvFp8) {
       by_width(std::integral_constant<int, kPagedPrefillSplitFp8>{});
@@ -360,6 +363,12 @@ static int launch_paged_prefill(const char *what, const void *q, int64_t q_token
 #endif
     with(varlen_prefill_tiled_kernel<MODE>, prefill_waves(MODE));
   };
+#if LITEKV_HD != 256
+  if (format == kKvInt4) {
+    launch(std::integral_constant<int, kPagedPrefillInt4>{});
+    return check_launch(what);
+  }
+#endif
   if (format == kKvInt8) {
     launch(std::integral_constant<int, kPagedPrefillInt8>{});
   } else if (format == kKvFp8) {
@@ -597,6 +606,28 @@ extern "C" int litekv_paged_prefill_int8(const void *q, int64_t q_token_stride, 
                                       out_token_stride, batch, num_q_heads, num_kv_heads, head_dim,
                                       page_size, num_pages, max_q_len, softmax_scale, stream,
                                       litekv::kKvInt8, litekv::PrefillKeySplit{});
+}
+
+extern "C" int litekv_paged_prefill_int4(const void *q, int64_t q_token_stride, const void *kv_pool_int4,
+                                         const int32_t *block_table, int32_t block_table_stride,
+                                         const int32_t *cu_q_lens, const int32_t *context_lens,
+                                         void *out, int64_t out_token_stride, int32_t batch,
+                                         int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                         int32_t page_size, int64_t num_pages, int32_t max_q_len,
+                                         int64_t max_kv_len, int64_t num_tokens, int32_t key_slices,
+                                         void *workspace, size_t workspace_bytes, float softmax_scale,
+                                         void *stream) {
+  LITEKV_REQUIRE(litekv::int4_head_dim(head_dim), "paged_prefill_int4: head_dim %d unsupported (64 or 128)", head_dim);
+  litekv::PrefillKeySplit split;
+  split.key_slices = key_slices;
+  split.workspace = workspace;
+  split.workspace_bytes = workspace_bytes;
+  split.num_tokens = num_tokens;
+  split.max_kv_len = max_kv_len;
+  return litekv::launch_paged_prefill("paged_prefill_int4", q, q_token_stride, kv_pool_int4, nullptr, block_table,
+                                      block_table_stride, cu_q_lens, context_lens, out, out_token_stride, batch,
+                                      num_q_heads, num_kv_heads, head_dim, page_size, num_pages, max_q_len,
+                                      softmax_scale, stream, litekv::kKvInt4, split);
 }
 
 extern "C" int litekv_varlen_prefill(const void *q, int64_t q_token_stride, const void *k,

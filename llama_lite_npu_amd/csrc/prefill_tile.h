@@ -69,6 +69,7 @@
 #include "common.h"
 #include "head_dim.h"
 #include "kv_fp8.h"
+#include "kv_int4.h"
 #include "prefill_rows.h"
 
 namespace litekv {
@@ -179,7 +180,8 @@ __device__ __forceinline__ float vmax3(float a, float b, float c) {
 __device__ __forceinline__ float vmax2(float a, float b) { return __builtin_fmaxf(a, b); }
 constexpr int kPagedPrefill = 0, kPackedPrefill = 1, kSharedPrefix = 2, kPagedPrefillFp8 = 3,
               kSharedPrefixFp8 = 4, kPagedPrefillInt8 = 5, kSharedPrefixInt8 = 6,
-              kPagedPrefillSplit = 7, kPagedPrefillSplitFp8 = 8, kPagedPrefillSplitInt8 = 9;
+              kPagedPrefillSplit = 7, kPagedPrefillSplitFp8 = 8, kPagedPrefillSplitInt8 = 9,
+              kPagedPrefillInt4 = 10, kPagedPrefillSplitInt4 = 11;
 // kPagedPrefillSplit: a launch with too few row blocks to fill the device (one request's chunk
 // over a long history) cuts every block's keys into `key_slices` runs of tiles, one workgroup
 // each; a slice leaves a normalised fp32 partial row + log-sum-exp per (query row, head), and a
@@ -258,15 +260,17 @@ __device__ __forceinline__ void prefill_tile_body(
   constexpr bool PAGED = MODE != kPackedPrefill;
   // causal prefill over one slice of the block's keys
   constexpr bool KSPLIT = MODE == kPagedPrefillSplit || MODE == kPagedPrefillSplitFp8 ||
-                          MODE == kPagedPrefillSplitInt8;
+                          MODE == kPagedPrefillSplitInt8 || MODE == kPagedPrefillSplitInt4;
   // An fp8 pool cannot take the direct HBM -> LDS load: its codes go through registers, are
   // converted to fp16 (exactly) and written to LDS in the same swizzled layout, so everything
   // after the staging is shared. The K scale joins the softmax scale, the V scale the final
-  // normalisation, as in the decode kernel.
-  constexpr bool FP8 = MODE == kPagedPrefillFp8 || MODE == kSharedPrefixFp8 ||
+  // normalisation, as in the decode kernel. A 4-bit pool takes the same way; its rows carry their own
+  // scales, and what is written to LDS are the values, which are fp16 numbers.
+  constexpr bool INT4 = MODE == kPagedPrefillInt4 || MODE == kPagedPrefillSplitInt4;
+  constexpr bool FP8 = INT4 || MODE == kPagedPrefillFp8 || MODE == kSharedPrefixFp8 ||
                        MODE == kPagedPrefillInt8 || MODE == kSharedPrefixInt8 ||
                        MODE == kPagedPrefillSplitFp8 || MODE == kPagedPrefillSplitInt8;  // 8-bit codes
-  constexpr int KV = (MODE == kPagedPrefillInt8 || MODE == kSharedPrefixInt8 ||
+  constexpr int KV = INT4 ? kKvInt4 : (MODE == kPagedPrefillInt8 || MODE == kSharedPrefixInt8 ||
                       MODE == kPagedPrefillSplitInt8) ? kKvInt8 : kKvFp8;
   constexpr bool SHARED = MODE == kSharedPrefix || MODE == kSharedPrefixFp8 || MODE == kSharedPrefixInt8;
   // (rows of 64 codes staged by 8 wavefronts would leave a lane 8 codes, half a 16-byte load)
@@ -303,7 +307,7 @@ __device__ __forceinline__ void prefill_tile_body(
   // which rows with a few large channels of q and K (scores tens of log2 units apart) turn into
   // percent-level errors of their probabilities.
   float v_scale = 1.0f, k_mul = scale_log2;
-  if constexpr (FP8) {
+  if constexpr (FP8 && !INT4) {
     k_mul *= paged.scales[h];
     v_scale = paged.scales[paged.num_kv_heads + h];
   }
@@ -444,11 +448,31 @@ __device__ __forceinline__ void prefill_tile_body(
   // of codes per lane and operand
   constexpr int kLanesPerRow = kWave / kRowsPerWave;
   constexpr int kCodesPerLane = kHD / kLanesPerRow;
-  constexpr int kRawVecs = FP8 ? kCodesPerLane / 16 : 1;
+  constexpr int kRawVecs = FP8 && !INT4 ? kCodesPerLane / 16 : 1;
   uint4_t raw_k[kRawVecs], raw_v[kRawVecs];  // this lane's codes of K and of V of the tile requested last
+  // 4-bit pools: a lane takes lane-th D / 8 bytes of the block's K codes, a quarter of row lane / 4, and of its V codes, column
+  // n of rows 4g .. 4g + 3 (see kv_int4.h), and those rows' words
+  uint32_t raw4_k[kHD / 32], raw4_v[kHD / 32], raw4_kw, raw4_vw[2];
   auto issue_tile = [&](int kt) {
     const int row0 = (tile0 + kt) * kKvTile + kRowsPerWave * wave;  // first key of this wavefront's rows
-    if constexpr (FP8) {
+    if constexpr (INT4) {
+      int pidx = (tile0 + kt) * 4 + wave;
+      pidx = pidx < last_page ? pidx : last_page;
+      const uint8_t *block = (const uint8_t *)paged.kv + (int64_t)page_of(pidx) * int4_block_bytes(paged.num_kv_heads, kHD);
+      typedef uint32_t vec __attribute__((ext_vector_type(kHD / 32)));
+      const vec kk = *(const vec *)(block + int4_codes_at(h, kHD) + (kHD / 8) * lane);
+      const vec vv = *(const vec *)(block + int4_codes_at(paged.num_kv_heads + h, kHD) + (kHD / 8) * lane);
+#pragma unroll
+      for (int i = 0; i < kHD / 32; ++i) {
+        raw4_k[i] = kk[i];
+        raw4_v[i] = vv[i];
+      }
+      raw4_kw = *(const uint16_t *)(block + int4_words_at(h, paged.num_kv_heads, kHD) + 2 * (lane >> 2));
+      const uint2_t vw = *(const uint2_t *)(block + int4_words_at(paged.num_kv_heads + h, paged.num_kv_heads, kHD) + 8 * g);
+      raw4_vw[0] = vw[0];
+      raw4_vw[1] = vw[1];
+      return;
+    } else if constexpr (FP8) {
       // lane l: row l / kLanesPerRow of the wavefront's rows, kCodesPerLane codes of the head's row
       int pidx = (tile0 + kt) * 4 + (kRowsPerWave * wave) / 16;
       pidx = pidx < last_page ? pidx : last_page;
@@ -584,7 +608,9 @@ __device__ __forceinline__ void prefill_tile_body(
   }
   if constexpr (!SHARED) {
     // the loads of tile 0 (K and V) were requested after q's
-    if constexpr (FP8) {
+    if constexpr (INT4) {
+      __builtin_amdgcn_s_waitcnt(wait_vm(0));  // (tile 0 is waited for next)
+    } else if constexpr (FP8) {
       __builtin_amdgcn_s_waitcnt(wait_vm(2 * kRawVecs));
     } else {
       __builtin_amdgcn_s_waitcnt(wait_vm(2 * kLoads));
@@ -781,7 +807,51 @@ __device__ __forceinline__ void prefill_tile_body(
 
   // Publishes tile kt (already requested) and requests tile kt + 1 into the other half.
   auto sync_and_prefetch = [&](int kt, bool issue_next = true) {
-    if constexpr (FP8) {
+    if constexpr (INT4) {
+      // Rows past the last key have scale 0: finite values that zero probabilities multiply.
+      const int left = last_key + 1 - ((tile0 + kt) * kKvTile + kRowsPerWave * wave);
+      if (left < 16) {
+        if ((lane >> 2) >= left) raw4_kw = 0;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int mine = left - 4 * g - 2 * p;
+          raw4_vw[p] &= mine >= 2 ? ~0u : mine == 1 ? 0xffffu : 0u;
+        }
+      }
+      const uint32_t tile_at = (uint32_t)((kt & 1) * kTileHalfs + kRowsPerWave * wave * kHD) * 2u;
+      const uint32_t kw = raw4_kw | (raw4_kw << 16);
+      const int kr = lane >> 2;
+#pragma unroll
+      for (int j = 0; j < kHD / 32; ++j) {
+        const int chunk = (kHD / 32) * (lane & 3) + j;
+        *(lds_half8_t *)(uintptr_t)(k_lds + tile_at + (uint32_t)(2 * kHD * kr) + 16u * (uint32_t)(chunk ^ k_swz(kr))) =
+            int4x8_to_half(raw4_k[j], kw);
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        if constexpr (kHD == 128) {
+#pragma unroll
+          for (int b2 = 0; b2 < 2; ++b2) {
+            // row 4g + 2p + b2: its halves of the two units' dwords
+            const uint32_t x = __builtin_amdgcn_perm(raw4_v[2 * p + 1], raw4_v[2 * p], b2 ? 0x07060302u : 0x05040100u);
+            const uint32_t w = __builtin_amdgcn_perm(0u, raw4_vw[p], b2 ? 0x03020302u : 0x01000100u);
+            const int r = 4 * g + 2 * p + b2;
+            *(lds_half8_t *)(uintptr_t)(v_lds + tile_at + (uint32_t)(2 * kHD * r) + 16u * (uint32_t)(n ^ v_swz(r))) =
+                int4x8_to_half(x, w);
+          }
+        } else {
+          // four elements of two rows at once, each row's under its own scale, then row by row
+          const half8_t y = int4x8_to_half(raw4_v[p], raw4_vw[p]);  // element j of rows 4g + 2p, 4g + 2p + 1
+#pragma unroll
+          for (int b2 = 0; b2 < 2; ++b2) {
+            const int r = 4 * g + 2 * p + b2;
+            *(__attribute__((address_space(3))) half4_t *)(uintptr_t)(
+                v_lds + tile_at + (uint32_t)(2 * kHD * r) + 16u * (uint32_t)((n >> 1) ^ v_swz(r)) + 8u * (uint32_t)(n & 1)) =
+                half4_t{y[b2], y[2 + b2], y[4 + b2], y[6 + b2]};
+          }
+        }
+      }
+    } else if constexpr (FP8) {
       // The codes of tile kt (requested a tile ago) become fp16 rows in its LDS half: 16-byte
       // chunk c of row r goes where the direct load of the fp16 path would have put it.
       const int r = sub + lane / kLanesPerRow;   // row inside the page: what the swizzle goes by
@@ -1252,7 +1322,7 @@ __global__ __launch_bounds__(prefill_waves(MODE) * kWave, kWgPerCu *prefill_wave
     int32_t heads_per_wg, int32_t row_tiles, float scale_log2, int32_t key_slices) {
   __shared__ __attribute__((aligned(1024))) half_t lds_all[tile_lds_bytes<prefill_waves(MODE)>() / 2];
   if constexpr (MODE == kPagedPrefillSplit || MODE == kPagedPrefillSplitFp8 ||
-                MODE == kPagedPrefillSplitInt8) {
+                MODE == kPagedPrefillSplitInt8 || MODE == kPagedPrefillSplitInt4) {
     // blockIdx.y = row block * key_slices + slice: the slices of a block are neighbours
     const int by = (int)blockIdx.y / key_slices;
     prefill_tile_body<MODE, prefill_waves(MODE), 1, CT>((uint32_t)(uintptr_t)(lds_half_t *)lds_all, (int)blockIdx.x, by,

@@ -47,9 +47,9 @@ int64_t row_stride(const at::Tensor &t, int64_t tokens, int64_t heads, int64_t d
   return tokens > 1 ? t.stride(0) : std::max(t.stride(0), heads * d);
 }
 
-enum Format { kNone, kF16, kFp8, kInt8 };
+enum Format { kNone, kF16, kFp8, kInt8, kInt4 };
 
-// A [slots, 2 * Hkv, D] pool and its scales (codes only); kNone: not a plain one.
+// A [slots, 2 * Hkv, D] pool and its scales (8-bit codes only); kNone: not a plain one.
 struct Pool {
   Format format = kNone;
   const at::Tensor *t = nullptr;
@@ -69,6 +69,13 @@ Pool pool_of(PyObject *pool, PyObject *scales) {
       if (scales == Py_None) p.format = kF16;
       return p;
     case at::kByte:
+      if (p.d == 34 || p.d == 66) {  // 4-bit codes: rows of head_dim / 2 + 2 bytes, in blocks of 16 slots, no scales
+        if (scales != Py_None || p.slots % 16 != 0) return p;
+        p.d = 2 * (p.d - 2);
+        p.format = kInt4;
+        return p;
+      }
+      [[fallthrough]];
     case at::kFloat8_e4m3fn:
     case at::kChar: {
       const at::Tensor *s = gpu_tensor(scales);
@@ -143,6 +150,9 @@ PyObject *qk_norm_rope_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
         case kF16:
           return litekv_qk_norm_rope_append(qp, qs, kp, ks, vp, vs, qwp, kwp, cp, sp, cs, slp, pp, (int32_t)t, (int32_t)hq,
                                             (int32_t)pool.hkv, (int32_t)d, pool.slots, (float)eps, stream);
+        case kInt4:
+          return litekv_qk_norm_rope_append_int4(qp, qs, kp, ks, vp, vs, qwp, kwp, cp, sp, cs, slp, pp, (int32_t)t,
+                                                 (int32_t)hq, (int32_t)pool.hkv, (int32_t)d, pool.slots, (float)eps, stream);
         case kFp8:
           return litekv_qk_norm_rope_append_fp8(qp, qs, kp, ks, vp, vs, qwp, kwp, cp, sp, cs, slp, pp, scales, (int32_t)t,
                                                 (int32_t)hq, (int32_t)pool.hkv, (int32_t)d, pool.slots, (float)eps, stream);
@@ -216,6 +226,11 @@ PyObject *paged_prefill(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const int64_t pages = pool.slots / page;
     void *wp = slices > 1 ? partials.data_ptr() : nullptr;
     const int rc = unlocked([&] {
+      if (pool.format == kInt4) {
+        return litekv_paged_prefill_int4(qp, qs, pp, tp, ts, cup, ctxp, op, hq * d, (int32_t)b, (int32_t)hq, (int32_t)pool.hkv,
+                                         (int32_t)d, (int32_t)page, pages, (int32_t)max_q, max_kv < 0 ? 0 : max_kv, t,
+                                         slices > 1 ? slices : 1, wp, partial_bytes, (float)scale, stream);
+      }
       if (slices > 1 && pool.format == kF16) {
         return litekv_paged_prefill_split(qp, qs, pp, tp, ts, cup, ctxp, op, hq * d, (int32_t)b, (int32_t)hq, (int32_t)pool.hkv,
                                           (int32_t)d, (int32_t)page, pages, (int32_t)max_q, t, slices, wp, partial_bytes,

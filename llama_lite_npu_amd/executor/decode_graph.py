@@ -89,7 +89,7 @@ class DeviceDecodeBatch:
                                           executor.local_kv_heads, executor.kv_mem_manager.num_pages,
                                           page_size=executor.page_size, shared_pages=self.shared_pages,
                                           token_bytes=getattr(executor, "kv_token_bytes", None),
-                                          kv_dtype=executor.kv_mem_manager.gpu_kv_buffer[0].dtype)
+                                          kv_dtype=ops.pool_dtype(executor.kv_mem_manager.gpu_kv_buffer[0]))
         self.load(request_ids, reserve_tokens, host_ahead)
 
     # ---- host side -------------------------------------------------------------------------

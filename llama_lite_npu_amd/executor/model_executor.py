@@ -55,7 +55,8 @@ class ModelExecutor:
         self.atten_info.page_size = self.page_size
         self.build_decode_plans = build_decode_plans and torch.device(device).type == "cuda"
         # K + V bytes of one token in a layer's pool (what a decode step reads per token attended)
-        self.kv_token_bytes = 2 * self.local_kv_heads * head_dim * torch.empty((), dtype=dtype).element_size()
+        pool = self.kv_mem_manager.gpu_kv_buffer[0]
+        self.kv_token_bytes = 2 * self.local_kv_heads * pool.shape[2] * pool.element_size()
         self.shared_prefix_min_pages = 4  # below that the two extra launches cost more than they save
         self._decode_plan = None
         self._paged_request_ids: tuple[int, ...] = ()
@@ -316,7 +317,7 @@ class ModelExecutor:
                                               shared_pages=self.shared_prefix_pages(ids),
                                               host_seq_lens=[mgr.req_token_count[r] for r in ids],
                                               token_bytes=self.kv_token_bytes,
-                                              kv_dtype=self.kv_mem_manager.gpu_kv_buffer[0].dtype)
+                                              kv_dtype=ops.pool_dtype(self.kv_mem_manager.gpu_kv_buffer[0]))
         self._decode_meta_sig = sig
 
     def common_leading_pages(self, request_ids: Sequence[int], upcoming_tokens: int = 0) -> int:
@@ -340,7 +341,9 @@ class ModelExecutor:
     def shared_prefix_pages(self, request_ids: Sequence[int], upcoming_tokens: int = 0) -> int:
         """Leading pages the decode step attends once for the whole batch (prefix-cache hits map one
         page list into many requests, :547-620). 0 when the batch shares fewer than
-        ``shared_prefix_min_pages`` pages."""
+        ``shared_prefix_min_pages`` pages, and over pools of 4-bit codes, whose step has no form for it."""
+        if self.kv_mem_manager.is_int4:
+            return 0
         n = self.common_leading_pages(request_ids, upcoming_tokens)
         return n if n >= self.shared_prefix_min_pages else 0
 

@@ -39,7 +39,9 @@ class PagedKVCacheManager:
     head_dim]``: K heads first, then V heads (reference :54-62). With ``dtype``
     ``torch.float8_e4m3fn`` (or ``torch.uint8``) the pools hold E4M3 codes and
     ``kv_scales[l]`` (float32 ``[2 * num_kv_heads]``, K heads then V heads, 1.0 until
-    ``set_kv_scales``) the per-head scales; for fp16 pools ``kv_scales[l]`` is None.
+    ``set_kv_scales``) the per-head scales; for fp16 pools ``kv_scales[l]`` is None. ``torch.int8`` pools hold signed
+    codes with such scales; ``torch.uint4`` pools (uint8 ``[..., head_dim / 2 + 2]``, head_dim 64 or 128) 4-bit codes whose
+    rows carry their own scales, so ``kv_scales[l]`` is None there too.
     """
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int,
@@ -53,8 +55,17 @@ class PagedKVCacheManager:
         self.device = device
         self.max_tokens = self.num_pages * self.page_size
         self.max_num_tokens = self.max_tokens
+        self.is_int4 = dtype is torch.uint4
+        if self.is_int4:
+            from .. import ops
+
+            if self.page_size % 16 != 0:
+                raise ValueError("pages of a 4-bit pool are multiples of 16 slots")
+            width, dtype = ops.int4_row_bytes(self.head_dim), None
+        else:
+            width = self.head_dim
         self.gpu_kv_buffer = [
-            torch.empty((self.max_tokens, 2 * self.num_kv_heads, self.head_dim), dtype=dtype, device=device)
+            torch.empty((self.max_tokens, 2 * self.num_kv_heads, width), dtype=dtype or torch.uint8, device=device)
             for _ in range(self.num_layers)
         ]
         # pools of 8-bit codes (fp8 E4M3 or int8) carry one scale per head
@@ -74,7 +85,7 @@ class PagedKVCacheManager:
     def set_kv_scales(self, layer: int, k_scales, v_scales) -> None:
         """Per-head scales of an fp8 or int8 layer (value = code * scale); set them before anything is cached."""
         if not self.is_fp8:
-            raise ValueError("fp16 pools have no scales")
+            raise ValueError("fp16 and 4-bit pools have no scales per head")
         both = torch.cat([torch.as_tensor(k_scales, dtype=torch.float32).reshape(-1),
                           torch.as_tensor(v_scales, dtype=torch.float32).reshape(-1)])
         if both.numel() != 2 * self.num_kv_heads or not bool((both > 0).all()):

@@ -55,9 +55,32 @@ def _dev_pool(name: str, t: torch.Tensor) -> None:
         raise ValueError(f"{name} must be float16, fp8 or int8, got {t.dtype}")
 
 
+# A pool of 4-bit codes is a uint8 tensor as well, known by its rows of head_dim / 2 codes' bytes and two more (no pool of
+# 8-bit codes has such a width): see kv_append_quantised. As an element type it goes by torch.uint4.
+INT4_DTYPE = torch.uint4
+_INT4_HEAD_DIMS = {d // 2 + 2: d for d in (64, 128)}
+
+
+def int4_row_bytes(head_dim: int) -> int:
+    """Bytes a row (slot, kv head) takes in a 4-bit pool: uint8 [slots, 2 * Hkv, head_dim / 2 + 2]."""
+    if head_dim not in _INT4_HEAD_DIMS.values():
+        raise ValueError(f"a 4-bit pool takes head_dim 64 or 128, not {head_dim}")
+    return head_dim // 2 + 2
+
+
+def is_int4_pool(kv_pool: torch.Tensor) -> bool:
+    """A pool of 4-bit codes, every row with its own scale and zero point: uint8 [slots, 2 * Hkv, D / 2 + 2]."""
+    return kv_pool.dtype is torch.uint8 and kv_pool.dim() == 3 and kv_pool.shape[2] in _INT4_HEAD_DIMS
+
+
+def pool_dtype(kv_pool: torch.Tensor) -> torch.dtype:
+    """The element type of a pool, torch.uint4 for one of 4-bit codes."""
+    return INT4_DTYPE if is_int4_pool(kv_pool) else kv_pool.dtype
+
+
 def is_fp8_pool(kv_pool: torch.Tensor) -> bool:
     """An fp8 pool holds one E4M3 code per element (a uint8 or float8_e4m3fn tensor)."""
-    return kv_pool.dtype in FP8_DTYPES
+    return kv_pool.dtype in FP8_DTYPES and not is_int4_pool(kv_pool)
 
 
 def is_int8_pool(kv_pool: torch.Tensor) -> bool:
@@ -67,7 +90,7 @@ def is_int8_pool(kv_pool: torch.Tensor) -> bool:
 
 def is_quantised_pool(kv_pool: torch.Tensor) -> bool:
     """A pool of 8-bit codes (fp8 or int8) with one fp32 scale per kv head: value = code * scale."""
-    return kv_pool.dtype in _Q8_DTYPES
+    return kv_pool.dtype in _Q8_DTYPES and not is_int4_pool(kv_pool)
 
 
 def _q8_entry(lib, stem: str, kv_pool: torch.Tensor):
@@ -83,6 +106,15 @@ def _dev_fp8_pool(kv_pool: torch.Tensor, scales: Optional[torch.Tensor], num_kv_
     if not (scales.is_cuda and scales.dtype is torch.float32 and scales.is_contiguous()
             and scales.numel() == 2 * num_kv_heads):
         raise ValueError("scales must be float32 [2 * Hkv] on the GPU (K heads, then V heads)")
+
+
+def _dev_int4_pool(kv_pool: torch.Tensor, scales: Optional[torch.Tensor]) -> None:
+    if not kv_pool.is_cuda:
+        raise ValueError("kv_pool must live on the GPU")
+    if scales is not None:
+        raise ValueError("a pool of 4-bit codes has no scales per head: its rows carry their own")
+    if kv_pool.shape[0] % 16 != 0:
+        raise ValueError("a pool of 4-bit codes holds its slots in blocks of 16")
 
 
 def _dev_i32(name: str, t: torch.Tensor) -> torch.Tensor:
@@ -117,7 +149,8 @@ def _rows(name: str, t: torch.Tensor) -> int:
 
 
 def pool_geometry(kv_pool: torch.Tensor, page_size: int = PAGE_SIZE):
-    """(num_slots, num_kv_heads, head_dim, num_pages, page_bytes) of a [slots, 2*Hkv, D] pool."""
+    """(num_slots, num_kv_heads, head_dim, num_pages, page_bytes) of a [slots, 2*Hkv, D] pool (a pool of 4-bit codes
+    is [slots, 2*Hkv, D/2 + 2])."""
     shape = kv_pool.shape
     if len(shape) != 3 or not kv_pool.is_contiguous():
         raise ValueError("kv_pool must be contiguous [slots, 2*Hkv, D]")
@@ -126,6 +159,8 @@ def pool_geometry(kv_pool: torch.Tensor, page_size: int = PAGE_SIZE):
         raise ValueError("kv_pool dim 1 must be 2 * num_kv_heads")
     if slots % page_size != 0:
         raise ValueError("kv_pool slots must be a multiple of page_size")
+    if is_int4_pool(kv_pool):
+        return slots, two_h // 2, _INT4_HEAD_DIMS[d], slots // page_size, page_size * two_h * d
     return slots, two_h // 2, d, slots // page_size, page_size * two_h * d * kv_pool.element_size()
 
 
@@ -147,18 +182,30 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, kv_p
 
 
 def kv_append_quantised(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, kv_pool: torch.Tensor,
-                        scales: torch.Tensor) -> None:
+                        scales: Optional[torch.Tensor] = None) -> None:
     """kv_pool[slot_mapping[t]] = code(concat(k[t], v[t]) / scale of the head) for every token t, in the
     pool's format (E4M3 for a uint8 / float8_e4m3fn pool, int8 for a torch.int8 pool);
-    scales is float32 [2 * Hkv]: K-head scales, then V-head scales."""
+    scales is float32 [2 * Hkv]: K-head scales, then V-head scales.
+
+    A pool of 4-bit codes (uint8 [slots, 2 * Hkv, D / 2 + 2], D 64 or 128) takes no scales: every row (token, kv head)
+    is quantised over its own range, 0 included, and keeps its scale s and zero point z beside its codes: a code c
+    stands for s * (c - z), at most s / 2 from the element, s = (max - min) / 15 rounded up to 7 bits."""
     _dev_half("k", k), _dev_half("v", v)
     slots, hkv, d, _, _ = pool_geometry(kv_pool, 1)
-    _dev_fp8_pool(kv_pool, scales, hkv)
+    int4 = is_int4_pool(kv_pool)
+    if int4:
+        _dev_int4_pool(kv_pool, scales)
+    else:
+        _dev_fp8_pool(kv_pool, scales, hkv)
     _need(k.shape == v.shape and k.shape[1] == hkv and k.shape[2] == d, "k / v must be [T, Hkv, D] matching the pool")
     slot_mapping = _dev_i32("slot_mapping", slot_mapping)
     t = k.shape[0]
     _need(slot_mapping.numel() == t, "slot_mapping must hold one slot per token")
     lib = _lib.load()
+    if int4:
+        _lib.check(lib.litekv_kv_append_int4(_ptr(k), _ptr(v), _rows("k", k), _rows("v", v), _ptr(slot_mapping),
+                                             _ptr(kv_pool), t, hkv, d, slots, _stream()))
+        return
     _lib.check(_q8_entry(lib, "kv_append", kv_pool)(_ptr(k), _ptr(v), _rows("k", k), _rows("v", v),
                                                     _ptr(slot_mapping), _ptr(kv_pool), _ptr(scales), t, hkv, d,
                                                     slots, _stream()))
@@ -168,18 +215,27 @@ kv_append_fp8 = kv_append_quantised     # the name from before int8 pools
 
 
 def page_dequant(kv_pool: torch.Tensor, dst_pool: torch.Tensor, src_ids: torch.Tensor,
-                 dst_ids: Optional[torch.Tensor], scales: torch.Tensor, page_size: int = PAGE_SIZE) -> None:
-    """dst_pool[page dst_ids[i]] (fp16) = decoded page src_ids[i] of the fp8 pool; dst_ids None means page i."""
+                 dst_ids: Optional[torch.Tensor], scales: Optional[torch.Tensor], page_size: int = PAGE_SIZE) -> None:
+    """dst_pool[page dst_ids[i]] (fp16) = decoded page src_ids[i] of the fp8, int8 or (scales None) 4-bit pool; dst_ids
+    None means page i."""
     _dev_half("dst_pool", dst_pool)
     _, hkv, d, n_src, _ = pool_geometry(kv_pool, page_size)
     _, hkv_d, d_d, n_dst, _ = pool_geometry(dst_pool, page_size)
-    _dev_fp8_pool(kv_pool, scales, hkv)
+    int4 = is_int4_pool(kv_pool)
+    if int4:
+        _dev_int4_pool(kv_pool, scales)
+    else:
+        _dev_fp8_pool(kv_pool, scales, hkv)
     _need((hkv, d) == (hkv_d, d_d), "pools differ in head geometry")
     src_ids = _dev_i32("src_ids", src_ids)
     if dst_ids is not None:
         dst_ids = _dev_i32("dst_ids", dst_ids)
         _need(dst_ids.numel() == src_ids.numel(), "src_ids and dst_ids differ in length")
     lib = _lib.load()
+    if int4:
+        _lib.check(lib.litekv_page_dequant_int4(_ptr(kv_pool), _ptr(dst_pool), _ptr(src_ids), _ptr(dst_ids),
+                                                src_ids.numel(), hkv, d, page_size, n_src, n_dst, _stream()))
+        return
     fn = lib.litekv_page_dequant_int8 if is_int8_pool(kv_pool) else lib.litekv_page_dequant
     _lib.check(fn(_ptr(kv_pool), _ptr(dst_pool), _ptr(src_ids), _ptr(dst_ids), src_ids.numel(),
                   _ptr(scales), hkv, d, page_size, n_src, n_dst, _stream()))
@@ -193,7 +249,8 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_
     """Per-head RMSNorm (optional) and rotary embedding (optional) of q [T, Hq, D] in place and of
     k [T, Hkv, D] on its way into the pool, plus the append of v: one launch for the reference's
     skip_rmsnorm x2 + rope_emb_forward + cat + update_kv_buffer. cos / sin are [T, >= D/2] rows of
-    each token's position. An fp8 pool (with its ``kv_scales``) receives the quantised rows. Returns q."""
+    each token's position. An fp8 pool (with its ``kv_scales``) receives the quantised rows, and so does a pool of
+    4-bit codes (without any), for which everything up to the quantiser and the one rounding of q is fp32. Returns q."""
     if q.is_cuda:
         done = _lib.calls().qk_norm_rope_append(q, k, v, slot_mapping, kv_pool, q_norm_weight, k_norm_weight, cos, sin,
                                                 rms_eps, kv_scales, _stream())
@@ -204,9 +261,11 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_
     # (not a plain call: found out below)
     _dev_half("q", q), _dev_half("k", k), _dev_half("v", v)
     slots, hkv, d, _, _ = pool_geometry(kv_pool, 1)
-    fp8 = is_quantised_pool(kv_pool)
+    fp8, int4 = is_quantised_pool(kv_pool), is_int4_pool(kv_pool)
     if fp8:
         _dev_fp8_pool(kv_pool, kv_scales, hkv)
+    elif int4:
+        _dev_int4_pool(kv_pool, kv_scales)
     else:
         _dev_half("kv_pool", kv_pool)
     t, hq = q.shape[0], q.shape[1]
@@ -243,7 +302,8 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_
             _ptr(k_norm_weight), _ptr(cos), _ptr(sin), cs_stride, _ptr(slot_mapping), _ptr(kv_pool),
             _ptr(kv_scales), t, hq, hkv, d, slots, float(rms_eps), _stream()))
         return q
-    _lib.check(lib.litekv_qk_norm_rope_append(
+    fn = lib.litekv_qk_norm_rope_append_int4 if int4 else lib.litekv_qk_norm_rope_append
+    _lib.check(fn(
         _ptr(q), _rows("q", q), _ptr(k), _rows("k", k), _ptr(v), _rows("v", v), _ptr(q_norm_weight),
         _ptr(k_norm_weight), _ptr(cos), _ptr(sin), cs_stride, _ptr(slot_mapping), _ptr(kv_pool), t, hq, hkv, d,
         slots, float(rms_eps), _stream()))
@@ -259,6 +319,7 @@ def page_gather(src_pool: torch.Tensor, dst_pool: torch.Tensor, src_ids: torch.T
     _, hs, ds, n_src, page_bytes = pool_geometry(src_pool, page_size)
     _, hd, dd, n_dst, page_bytes_d = pool_geometry(dst_pool, page_size)
     _need((hs, ds) == (hd, dd) and page_bytes == page_bytes_d, "pools differ in page geometry")
+    _need(page_size % 16 == 0 or not is_int4_pool(src_pool), "pages of a 4-bit pool are multiples of 16 slots")
     src_ids = _dev_i32("src_ids", src_ids)
     if dst_ids is not None:
         dst_ids = _dev_i32("dst_ids", dst_ids)
@@ -273,6 +334,7 @@ def page_copy(kv_pool: torch.Tensor, src_ids: torch.Tensor, dst_ids: torch.Tenso
     """kv_pool[page dst_ids[i]] = kv_pool[page src_ids[i]] (copy-on-write move inside one pool, fp16 or fp8)."""
     _dev_pool("kv_pool", kv_pool)
     _, _, _, n_pages, page_bytes = pool_geometry(kv_pool, page_size)
+    _need(page_size % 16 == 0 or not is_int4_pool(kv_pool), "pages of a 4-bit pool are multiples of 16 slots")
     src_ids = _dev_i32("src_ids", src_ids)
     dst_ids = _dev_i32("dst_ids", dst_ids)
     _need(dst_ids.numel() == src_ids.numel(), "src_ids and dst_ids differ in length")
@@ -295,6 +357,26 @@ def decode_split_plan(batch: int, num_kv_heads: int, max_blocks: int,
     target_waves = 4096
     pps = max(8, min(64, (items * max_blocks + target_waves - 1) // target_waves))
     return max(1, (max_blocks + pps - 1) // pps), pps
+
+
+# A split of a decode step over 4-bit codes is at least this many tokens long.
+INT4_SPLIT_TOKENS = 128
+
+
+def int4_decode_splits(batch: int, num_kv_heads: int, max_pages: int, total_pages: Optional[int] = None,
+                       page_size: int = PAGE_SIZE) -> tuple[int, int]:
+    """(max_splits, min_pages_per_split) of a decode step over a 4-bit pool whose longest sequence has ``max_pages`` pages and
+    all of them together ``total_pages`` (None: as many for every sequence)."""
+    min_pages = max(1, INT4_SPLIT_TOKENS // page_size)
+    steps = max(1, page_size // PAGE_SIZE)
+    total = batch * max_pages if total_pages is None else total_pages
+    wavefronts = 2048 / max(1, num_kv_heads)                 # per kv head
+    each = max(1.0, total * steps / wavefronts)              # 16-token pages a wavefront should get
+    want = max_pages * steps / each
+    splits = 1
+    while splits < want and splits * min_pages < max_pages:
+        splits *= 2
+    return splits, min_pages
 
 
 def decode_workspace(batch: int, num_q_heads: int, max_splits: int, device) -> Optional[torch.Tensor]:
@@ -459,16 +541,21 @@ class DecodePlan:
         per-sequence schedule (and its split count) where ``decode_schedule`` says so. ``token_bytes``:
         K + V bytes of one token in the pool (default: fp16). ``kv_dtype``: the pool's element type
         (default fp16); with a shared prefix it decides how the default chunk count is chosen, and
-        with ``token_bytes`` it tells the width of the heads, which the schedule depends on."""
+        with ``token_bytes`` it tells the width of the heads, which the schedule depends on. torch.uint4: a pool of
+        4-bit codes, whose steps are always on the per-sequence schedule (see ``int4_decode_splits``)."""
         lib = _lib.load()
         self.shared_pages = int(shared_pages)
         self.kv_dtype = kv_dtype
         self.per_sequence = False
         self.splits = 1
         self.split_workspace: Optional[torch.Tensor] = None
+        self._outgrown: list = []
         self.token_bytes = int(token_bytes) if token_bytes is not None else 2 * int(num_kv_heads) * HEAD_DIM * 2
         self.head_dim = pool_head_dim(self.token_bytes, int(num_kv_heads), kv_dtype)
+        self.int4 = kv_dtype is INT4_DTYPE
+        self.min_pages_per_split = 1
         _need(0 <= self.shared_pages <= block_table.shape[1], "shared_pages out of range")
+        _need(self.shared_pages == 0 or not self.int4, "a step over 4-bit codes has no shared-prefix form")
         _need(block_table.dim() == 2, "block_table must be [B, max_blocks]")
         self.block_table = _dev_i32("block_table", block_table)
         self.seq_lens = _dev_i32("seq_lens", seq_lens)
@@ -477,6 +564,17 @@ class DecodePlan:
         self.num_q_heads, self.num_kv_heads = int(num_q_heads), int(num_kv_heads)
         self.num_pages, self.page_size = int(num_pages), int(page_size)
         self.block_table, self.bt_stride = _table_rows(self.block_table)
+        if self.int4:
+            _need(self.page_size in (16, 32, 64, 128, 256),
+                  f"page_size {self.page_size} unsupported (16, 32, 64, 128 or 256)")
+            self.chunks, self.plan_bytes, self.workspace_bytes = 1, 0, 0
+            self.buffer = self.workspace = None
+            if host_seq_lens is not None:
+                self.choose_schedule(host_seq_lens)
+            else:
+                self.set_schedule(int4_decode_splits(self.batch, self.num_kv_heads, int(self.block_table.shape[1]),
+                                                     page_size=self.page_size)[0])
+            return
         if chunks is not None:
             self.chunks = int(chunks)
         elif self.shared_pages > 0 and block_table.shape[0] > 0:
@@ -500,13 +598,19 @@ class DecodePlan:
 
     def set_schedule(self, splits: int) -> None:
         """0: balanced; otherwise the per-sequence schedule with that many splits per sequence
-        (the partial-result buffer of several splits is allocated here, not at the launch)."""
+        (the partial-result buffer of several splits is allocated here, not at the launch). A step over 4-bit codes has
+        no balanced form: 0 is one split, and several are at least ``INT4_SPLIT_TOKENS`` long."""
+        if self.int4:
+            splits = max(1, int(splits))
+            self.min_pages_per_split = max(1, INT4_SPLIT_TOKENS // self.page_size)
         self.per_sequence = splits > 0
         self.splits = max(1, int(splits))
         if self.splits > 1:
             need = int(_lib.load().litekv_paged_decode_workspace_bytes(self.batch, self.num_q_heads, HEAD_DIM,
                                                                        self.splits)) // 4
             if self.split_workspace is None or self.split_workspace.numel() < need:
+                if self.split_workspace is not None:
+                    self._outgrown.append(self.split_workspace)   # a captured graph may hold its address
                 self.split_workspace = torch.empty(need, dtype=torch.float32, device=self.block_table.device)
 
     @property
@@ -524,7 +628,14 @@ class DecodePlan:
         pages = [(int(n) + self.page_size - 1) // self.page_size for n in host_seq_lens if n > 0]
         if not pages:
             self.set_schedule(0)
-            return False
+            return self.per_sequence
+        if self.int4:
+            splits = int4_decode_splits(self.batch, self.num_kv_heads, max(pages), sum(pages), self.page_size)[0]
+            # a batch that grows past a power of two does not flip back with the next length
+            if hysteresis > 1.0 and self.per_sequence and splits < self.splits and splits * 4 > self.splits:
+                splits = self.splits
+            self.set_schedule(splits)
+            return True
         # the rule is told what its defaults do not say
         differs = {} if self.head_dim == HEAD_DIM else {"head_dim": self.head_dim}
         if self.chunks != _whole_device_chunks(self.num_kv_heads):
@@ -649,6 +760,7 @@ def decode_step(q: torch.Tensor, kv_pool: torch.Tensor, plan: DecodePlan,
     its per-head ``kv_scales``."""
     if plan.per_sequence:
         return paged_decode(q, kv_pool, plan.block_table, plan.seq_lens, softmax_scale, num_splits=plan.splits,
+                            min_pages_per_split=plan.min_pages_per_split if plan.int4 else None,
                             out=out, workspace=plan.split_workspace if plan.splits > 1 else None,
                             page_size=plan.page_size, schedule="splits", kv_scales=kv_scales,
                             k_new=k_new, v_new=v_new)
@@ -732,12 +844,16 @@ def paged_decode(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tens
     kv head (default: one workgroup per CU); a DecodePlan is built for the call unless one is
     passed. schedule "splits" (chosen when num_splits, max_splits or min_pages_per_split is
     given): every sequence is cut into its own splits; two launches (`stage` selects one).
-    An fp8 pool comes with its ``kv_scales``; either schedule reads it.
+    An fp8 pool comes with its ``kv_scales``; either schedule reads it. A pool of 4-bit codes is read on the "splits"
+    schedule, whatever is left open here (see ``int4_decode_splits``).
     ``k_new`` / ``v_new`` [B, Hkv, D] (splits schedule, both stages): the step's new token of every
     sequence is written at logical position seq_lens[b] - 1 by the same launch and attended.
     """
     _dev_half("q", q)
-    if not is_quantised_pool(kv_pool):
+    int4 = is_int4_pool(kv_pool)
+    if int4:
+        _dev_int4_pool(kv_pool, kv_scales)
+    elif not is_quantised_pool(kv_pool):
         _dev_half("kv_pool", kv_pool)
     if not (q.dim() == 3 and q.stride(2) == 1 and q.stride(1) == q.shape[2]):
         raise ValueError("q must be [B, Hq, D] with contiguous heads")
@@ -747,6 +863,10 @@ def paged_decode(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tens
         raise ValueError("q and kv_pool differ in head_dim")
     if not (stage in _STAGES):
         raise ValueError(f"unknown stage {stage!r}")
+    if int4:
+        if schedule == "balanced" or plan is not None or shared_pages or chunks is not None:
+            raise ValueError("a pool of 4-bit codes has no balanced schedule (and no shared prefix)")
+        schedule = "splits"
     if schedule is None:
         split_args = (num_splits, max_splits, min_pages_per_split)
         schedule = "splits" if any(x is not None for x in split_args) or stage != "both" else "balanced"
@@ -770,6 +890,8 @@ def paged_decode(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tens
         _dev_fp8_pool(kv_pool, kv_scales, hkv)
         if not (stage == "both"):
             raise ValueError("an fp8 pool is read by both stages in one call")
+    if int4 and stage != "both":
+        raise ValueError("a pool of 4-bit codes is read by both stages in one call")
     if not (block_table.dim() == 2 and block_table.shape[0] == b):
         raise ValueError("block_table must be [B, max_blocks]")
     block_table, bt_stride = _table_rows(_dev_i32("block_table", block_table))
@@ -786,13 +908,31 @@ def paged_decode(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tens
             raise ValueError("out must be contiguous [B, Hq, D]")
     lib = _lib.load()
     q_stride = q.stride(0) if b > 1 else max(q.stride(0), hq * d)
-    if max_splits is None or min_pages_per_split is None:
+    if int4 and (max_splits is None or min_pages_per_split is None):
+        s, pps = int4_decode_splits(b, hkv, block_table.shape[1], page_size=page_size)
+        if num_splits is not None:
+            s, pps = max(1, int(num_splits)), 1
+        max_splits = s if max_splits is None else max_splits
+        min_pages_per_split = pps if min_pages_per_split is None else min_pages_per_split
+    elif max_splits is None or min_pages_per_split is None:
         s, pps = decode_split_plan(b, hkv, block_table.shape[1], num_splits)
         max_splits = s if max_splits is None else max_splits
         min_pages_per_split = pps if min_pages_per_split is None else min_pages_per_split
     if workspace is None:
         workspace = decode_workspace(b, hq, max_splits, q.device)
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    if int4:
+        kn_stride = vn_stride = 0
+        if k_new is not None:
+            _dev_half("k_new", k_new), _dev_half("v_new", v_new)
+            if not (k_new.shape == (b, hkv, d) and v_new.shape == (b, hkv, d)):
+                raise ValueError("k_new / v_new must be [B, Hkv, D]")
+            kn_stride, vn_stride = _rows("k_new", k_new), _rows("v_new", v_new)
+        _lib.check(lib.litekv_paged_decode_int4(
+            _ptr(q), q_stride, _ptr(kv_pool), _ptr(block_table), bt_stride, _ptr(seq_lens), _ptr(k_new), _ptr(v_new),
+            kn_stride, vn_stride, _ptr(out), _ptr(workspace), ws_bytes, b, hq, hkv, d, page_size, n_pages,
+            int(max_splits), int(min_pages_per_split), float(softmax_scale), _stream()))
+        return out
     if k_new is not None:
         if not (stage == "both"):
             raise ValueError("the fused append belongs to the call that runs both stages")
@@ -863,7 +1003,7 @@ def paged_prefill(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Ten
                   key_slices: Optional[int] = None, max_kv_len: Optional[int] = None,
                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal varlen attention of packed q [T, Hq, D] over paged KV (history + the chunk itself).
-    An fp8 pool (uint8 / float8_e4m3fn) comes with its per-head ``kv_scales``.
+    An fp8 pool (uint8 / float8_e4m3fn) comes with its per-head ``kv_scales``, a pool of 4-bit codes with none.
 
     A launch with too few query rows to fill the device (one request's chunk over a long history)
     is cut along the keys as well: ``key_slices`` workgroups per row block and a merge launch
@@ -880,8 +1020,10 @@ def paged_prefill(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Ten
             return done
     # (not a plain call)
     _dev_half("q", q)
-    fp8 = is_quantised_pool(kv_pool)
-    if not fp8:
+    fp8, int4 = is_quantised_pool(kv_pool), is_int4_pool(kv_pool)
+    if int4:
+        _dev_int4_pool(kv_pool, kv_scales)
+    elif not fp8:
         _dev_half("kv_pool", kv_pool)
         if not (kv_scales is None):
             raise ValueError("kv_scales belong to an fp8 pool")
@@ -920,6 +1062,14 @@ def paged_prefill(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Ten
         if not (workspace.is_cuda and workspace.dtype == torch.float32
                 and workspace.is_contiguous() and workspace.numel() >= need):
             raise ValueError(f"workspace must be {need} contiguous float32 on the device")
+    if int4:
+        _lib.check(lib.litekv_paged_prefill_int4(
+            _ptr(q), q_stride, _ptr(kv_pool), _ptr(block_table), block_table.stride(0), _ptr(cu_q_lens),
+            _ptr(context_lens), _ptr(out), _rows("out", out), b, hq, hkv, d, page_size, n_pages, int(max_q_len),
+            0 if max_kv_len is None else int(max_kv_len), t, max(1, key_slices),
+            _ptr(workspace) if key_slices > 1 else None, workspace.numel() * 4 if key_slices > 1 else 0,
+            float(softmax_scale), _stream()))
+        return out
     if key_slices <= 1:
         # (max_kv_len 0: not known)
         _lib.check(lib.litekv_paged_prefill_bounded(
