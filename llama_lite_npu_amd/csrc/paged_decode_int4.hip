@@ -56,7 +56,7 @@ __device__ __forceinline__ half8_t as_half8(uint32_t a, uint32_t b, uint32_t c, 
 
 // TWO: more than 8 query heads, whose second part of p s' has MFMAs of its own.
 template <int D, bool TWO>
-__global__ __launch_bounds__(kInt4Waves *kWave) void paged_decode_int4_kernel(
+__global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_eu(3, 3))) void paged_decode_int4_kernel(
     const half_t *__restrict__ q, int64_t q_batch_stride, uint8_t *pool, const int32_t *__restrict__ block_table,
     int32_t bt_stride, const int32_t *__restrict__ seq_lens, const half_t *__restrict__ k_new,
     const half_t *__restrict__ v_new, int64_t k_new_stride, int64_t v_new_stride, half_t *__restrict__ out,
@@ -286,20 +286,25 @@ __global__ __launch_bounds__(kInt4Waves *kWave) void paged_decode_int4_kernel(
   };
 
   // Two blocks a step, the next two in flight.
-  auto step = [&](int p, Int4Regs<D> (&now)[2], Int4Regs<D> (&next)[2]) {
-    if (p + 2 < p1) {
-      request(p + 2, next[0]);
-      request(p + 3, next[1]);
-    }
-    if ((p + 2) * kInt4Block > end) {
-      attend(now, p, std::true_type{});
-    } else {
-      attend(now, p, std::false_type{});
+  auto request_pair = [&](int p, Int4Regs<D> (&r)[2]) {
+    if (p < p1) {
+      request(p, r[0]);
+      request(p + 1, r[1]);
     }
   };
-  for (int p = p0; p < p1; p += 4) {
-    step(p, buf[0], buf[1]);
-    if (p + 2 < p1) step(p + 2, buf[1], buf[0]);
+  int p = p0;
+  for (; (p + 4) * kInt4Block <= end; p += 4) {
+    request_pair(p + 2, buf[1]);
+    attend(buf[0], p, std::false_type{});
+    request_pair(p + 4, buf[0]);
+    attend(buf[1], p + 2, std::false_type{});
+  }
+#pragma unroll 1
+  for (; p < p1; p += 2) {   // less than 64 tokens
+    request_pair(p + 2, buf[1]);
+    attend(buf[0], p, std::true_type{});
+    buf[0][0] = buf[1][0];
+    buf[0][1] = buf[1][1];
   }
 
   total += xor_lane(total, 16);
