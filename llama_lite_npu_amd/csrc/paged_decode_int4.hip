@@ -33,6 +33,7 @@ typedef uint32_t uint2v_t __attribute__((ext_vector_type(2)));
 constexpr int kInt4Waves = 4;            // most wavefronts of a workgroup
 constexpr float kInt4Top = 7.0f;         // log2 of where the largest p s' is put
 constexpr float kInt4Grown = 32768.0f;   // and what it may grow to
+constexpr int kFold = 32;                // blocks between two subtractions of the zero points
 constexpr float kLog2eI4 = 1.4426950408889634f, kLn2I4 = 0.6931471805599453f;
 
 // A block of 16 tokens as a lane (n = lane % 16, g = lane / 16) holds it: of K row n the g-th quarter, of V rows 4g .. 4g + 3
@@ -43,7 +44,26 @@ struct Int4Regs {
   uint32_t kw[2], vw[2];
 };
 
-// Eight codes of a dword as fp16 pairs, times 2^-20.
+// Codes of K as the matrix cores take them in the first product: a nibble on its own in a byte is the fp8 (E4M3) number
+// c * 2^-9, subnormal up to 7 and in the lowest binade from 8, which have one spacing.
+typedef int int8v_t __attribute__((ext_vector_type(8)));
+template <int D>
+__device__ __forceinline__ int8v_t int4_k_bytes(const uint32_t (&k)[D / 32]) {
+  int8v_t a;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {   // (D = 64: the same elements twice, for two parts of q)
+    const uint32_t x = k[i % (D / 32)];
+    a[2 * i] = (int)(x & 0x0f0f0f0fu);
+    a[2 * i + 1] = (int)((x >> 4) & 0x0f0f0f0fu);
+  }
+  return a;
+}
+// D(16x16) += A(16x128) * B(128x16), fp8: lane l supplies 32 bytes of row (column) l % 16, at 32 * (l / 16).
+__device__ __forceinline__ float4_t mfma_16x16x128_fp8(int8v_t a, int8v_t b, float4_t c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+}
+
+// Eight codes of V in a dword as fp16 pairs, times 2^-20.
 __device__ __forceinline__ void int4_pairs(uint32_t x, uint32_t (&out)[4]) {
   out[0] = (x << 4) & 0x00f000f0u;
   out[1] = x & 0x00f000f0u;
@@ -119,10 +139,11 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   const uint32_t v_off = (uint32_t)(int4_codes_at(num_kv_heads + h, D) + g * (2 * D) + n * (D / 8));
   const uint32_t kw_off = (uint32_t)(int4_words_at(h, num_kv_heads, D) + 8 * g);
   const uint32_t vw_off = (uint32_t)(int4_words_at(num_kv_heads + h, num_kv_heads, D) + 8 * g);
-  auto request = [&](int p, Int4Regs<D> &r) {
-    const uint8_t *block = pool + (int64_t)page_id(p) * block_bytes;
+  auto request = [&](int id, Int4Regs<D> &r) {
+    const uint8_t *block = pool + (int64_t)id * block_bytes;
     typedef uint32_t vec __attribute__((ext_vector_type(kSteps)));
-    const vec kk = *(const vec *)(block + k_off), vv = *(const vec *)(block + v_off);
+    const vec kk = __builtin_nontemporal_load((const vec *)(block + k_off));
+    const vec vv = __builtin_nontemporal_load((const vec *)(block + v_off));
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       r.k[i] = kk[i];
@@ -135,12 +156,18 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
     r.vw[1] = vw[1];
   };
   Int4Regs<D> buf[2][2];
-  request(p0, buf[0][0]);
-  request(p0 + 1, buf[0][1]);
+  // (page ids are read a step before the requests that they are for)
+  int id0 = page_id(p0), id1 = page_id(p0 + 1);
+  request(id0, buf[0][0]);
+  request(id1, buf[0][1]);
+  id0 = page_id(p0 + 2);
+  id1 = page_id(p0 + 3);
 
-  // q as the right operand: column n, of every dword of K that the lane of the same g holds the eight elements, scaled by a
-  // power of two that puts the row's largest at 2^14 or above.
-  half8_t qf[kSteps];
+  // q as the right operand of the first product: column n, the elements of the bytes that the lane of the same g holds of K,
+  // as a sum of three fp8 numbers (4 + 4 + 4 bits), scaled by a power of two that puts the row's largest between 224 and 448. What
+  // that leaves of an element is 2^-10, some 2^-18 of the largest.
+  constexpr int kParts = 3, kProducts = D == 128 ? 3 : 2;   // D = 64: two parts side by side in the 128 of one product
+  int8v_t qf[kProducts];
   float q_sum = 0.f, k_mul;
   {
     const int col = TWO ? n : (n & 7);
@@ -158,114 +185,176 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
     }
     most = __builtin_fmaxf(most, xor_lane(most, 16));
     most = __builtin_fmaxf(most, xor_lane(most, 32));
-    const int up = most > 0.f ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+    int up = most > 0.f ? 9 - __builtin_amdgcn_frexp_expf(most) : 0;
+    if (__builtin_amdgcn_ldexpf(most, up) > 448.f) --up;
+    bool odd = false;   // an element that is not finite: fp8 would saturate it
 #pragma unroll
     for (int t = 0; t < kSteps; ++t) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const half_t y = (half_t)__builtin_amdgcn_ldexpf(x[t][i], up);
-        q_sum += (float)y;
-        qf[t][i] = y;
+        odd |= !(__builtin_fabsf(x[t][i]) < INFINITY);
+        x[t][i] = __builtin_amdgcn_ldexpf(x[t][i], up);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) qf[kProducts - 1][i] = 0;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          constexpr int kOrder[2][4] = {{0, 4, 1, 5}, {2, 6, 3, 7}};   // elements of the lower and of the upper nibbles
+          float *y[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = &x[t][kOrder[u][i]];
+          int bytes = __builtin_amdgcn_cvt_pk_fp8_f32(*y[0], *y[1], 0, false);
+          bytes = __builtin_amdgcn_cvt_pk_fp8_f32(*y[2], *y[3], bytes, true);
+          const float back[4] = {__builtin_amdgcn_cvt_f32_fp8(bytes, 0), __builtin_amdgcn_cvt_f32_fp8(bytes, 1),
+                                 __builtin_amdgcn_cvt_f32_fp8(bytes, 2), __builtin_amdgcn_cvt_f32_fp8(bytes, 3)};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            q_sum += back[i];
+            *y[i] -= back[i];
+          }
+          if constexpr (D == 128) {
+            qf[part][2 * t + u] = bytes;
+          } else {
+            qf[part >> 1][4 * (part & 1) + 2 * t + u] = bytes;
+          }
+        }
       }
     }
     q_sum += xor_lane(q_sum, 16);
     q_sum += xor_lane(q_sum, 32);
-    k_mul = __builtin_amdgcn_ldexpf(scale_log2, 20 - up);
+    q_sum *= 0x1p15f;    // the zero points come as z * 2^-24, the products in units of 2^-9
+    odd = (__builtin_amdgcn_ballot_w64(odd) >> n & 0x0001000100010001ull) != 0;
+    k_mul = odd ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(scale_log2, 9 - up);
   }
-  const uint32_t hi_mask = !TWO && n >= 8 ? ~0u : 0u;   // of the columns that carry the second part
+  const bool second = n >= 8;   // !TWO: the lane's scores are those of the second block's keys
 
-  float4_t acc[kTiles];
+  // O^T, and what is to be subtracted from every element of it (see kFold)
+  float4_t acc[kTiles], acc_z = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < kTiles; ++j) acc[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+  auto fold_zeros = [&]() {
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) acc[j] -= acc_z;
+    acc_z = float4_t{0.f, 0.f, 0.f, 0.f};
+  };
   float ref = -1e30f, total = 0.f;   // reference of the exponentials; sum of p
   const int end = len < p1 * kInt4Block ? len : p1 * kInt4Block;
 
   auto attend = [&](Int4Regs<D> (&r)[2], int p, auto masked_tag) {
     constexpr bool MASKED = decltype(masked_tag)::value;
+    constexpr int kKeys = TWO ? 8 : 4;   // keys a lane has the scores of: of its column all of 4g .. 4g + 3, or one block's
     float4_t st[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
+      const int8v_t a = int4_k_bytes<D>(r[u].k);
       st[u] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int t = 0; t < kSteps; ++t) {
-        uint32_t x[4];
-        int4_pairs(r[u].k[t], x);
-        st[u] = mfma_16x16x32(as_half8(x[0], x[1], x[2], x[3]), qf[t], st[u]);
-      }
+      for (int i = 0; i < kProducts; ++i) st[u] = mfma_16x16x128_fp8(a, qf[i], st[u]);
     }
-    half2_t ks[4], kz[4], vs[4];   // of the lane's keys 2i, 2i + 1 (0, 1: the first block's)
-    uint32_t vz[4];                       // -z' of those keys, times 2^-20
+    uint32_t kw[kKeys / 2], vw[kKeys / 2];   // words of the lane's keys 2i, 2i + 1
+    uint32_t vz[4];                          // z' of the eight keys of its g, times 2^-20
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t kw = r[i >> 1].kw[i & 1], vw = r[i >> 1].vw[i & 1];
+    for (int i = 0; i < 2; ++i) {
       if constexpr (MASKED) {
         // rows past the end: finite values for zero probabilities to multiply
-        const int left = end - p * kInt4Block - 16 * (i >> 1) - 4 * g - 2 * (i & 1);
-        const uint32_t keep = left >= 2 ? ~0u : left == 1 ? 0xffffu : 0u;
-        kw &= keep;
-        vw &= keep;
-      }
-      ks[i] = int4_scales(kw);
-      kz[i] = __builtin_bit_cast(half2_t, (kw << 4) & 0x00f000f0u);
-      vs[i] = int4_scales(vw);
-      vz[i] = ((vw << 4) & 0x00f000f0u) | 0x80008000u;
-    }
-    float x[8];   // scores in log2 units
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y = __builtin_fmaf(-(float)kz[i >> 1][i & 1], q_sum, st[i >> 2][i & 3]) * k_mul;
-      x[i] = y * (float)ks[i >> 1][i & 1];
-      if constexpr (MASKED) {
-        if (p * kInt4Block + 16 * (i >> 2) + 4 * g + (i & 3) >= end) x[i] = -INFINITY;
+        for (int u = 0; u < 2; ++u) {
+          const int left = end - (p + u) * kInt4Block - 4 * g - 2 * i;
+          const uint32_t keep = left >= 2 ? ~0u : left == 1 ? 0xffffu : 0u;
+          r[u].kw[i] &= keep;
+          r[u].vw[i] &= keep;
+        }
+      }
+      vz[i] = (r[0].vw[i] << 4) & 0x00f000f0u;
+      vz[2 + i] = (r[1].vw[i] << 4) & 0x00f000f0u;
+      if constexpr (TWO) {
+        kw[i] = r[0].kw[i];
+        kw[2 + i] = r[1].kw[i];
+        vw[i] = r[0].vw[i];
+        vw[2 + i] = r[1].vw[i];
+      } else {
+        kw[i] = second ? r[1].kw[i] : r[0].kw[i];
+        vw[i] = second ? r[1].vw[i] : r[0].vw[i];
       }
     }
-    float pr[8], w[8], sum;
+    float x[kKeys], vs[kKeys];   // scores in log2 units, scales of V
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+      const half2_t ks = int4_scales(kw[i >> 1]), kz = __builtin_bit_cast(half2_t, kw[i >> 1] & 0x000f000fu);
+      vs[i] = (float)int4_scales(vw[i >> 1])[i & 1];
+      const float dot = TWO ? st[i >> 2][i & 3] : second ? st[1][i] : st[0][i];
+      x[i] = __builtin_fmaf(-(float)kz[i & 1], q_sum, dot) * k_mul * (float)ks[i & 1];
+      if constexpr (MASKED) {
+        const int u = TWO ? i >> 2 : second ? 1 : 0;
+        if ((p + u) * kInt4Block + 4 * g + (i & 3) >= end) x[i] = -INFINITY;
+      }
+    }
+    float w[kKeys], sum;   // p s'; sum of p
     auto exponentials = [&]() {
       sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        pr[i] = fast_exp2(x[i] - ref);
-        sum += pr[i];
-        w[i] = __builtin_fmaf(pr[i], (float)vs[i >> 1][i & 1], 0.0f);
+      for (int i = 0; i < kKeys; ++i) {
+        const float pr = fast_exp2(x[i] - ref);
+        sum += pr;
+        w[i] = __builtin_fmaf(pr, vs[i], 0.0f);
       }
     };
     exponentials();
     float most = sum * 0x1p-40f;   // (p alone may outgrow fp32 where s' is tiny or 0)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) most = __builtin_fmaxf(most, w[i]);
+    for (int i = 0; i < kKeys; ++i) most = __builtin_fmaxf(most, w[i]);
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > kInt4Grown) != 0, false)) {
       float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        top = __builtin_fmaxf(top, x[i] + fast_log2(__builtin_fmaxf((float)vs[i >> 1][i & 1], 0x1p-24f)));
+      for (int i = 0; i < kKeys; ++i) {
+        top = __builtin_fmaxf(top, x[i] + fast_log2(__builtin_fmaxf(vs[i], 0x1p-24f)));
       }
+      if constexpr (!TWO) top = __builtin_fmaxf(top, dpp<kDppRotate8>(top));
       top = __builtin_fmaxf(top, xor_lane(top, 16));
       top = __builtin_fmaxf(top, xor_lane(top, 32)) - kInt4Top;
       const float next = __builtin_fmaxf(ref, top);
       const float alpha = fast_exp2(ref - next);
       ref = next;
       total *= alpha;
+      acc_z *= alpha;
 #pragma unroll
       for (int j = 0; j < kTiles; ++j) acc[j] *= alpha;
       exponentials();
     }
     total += sum;
-    uint32_t hi[4], lo[4];   // p s' of keys 2i, 2i + 1: what a column carries, and TWO: what that leaves
+    // p s' as two fp16 numbers, the second what the first leaves, of keys 2i, 2i + 1
+    auto toward_zero = [&](float a, float b) {
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+    };
+    uint32_t hi[kKeys / 2], lo[kKeys / 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      auto toward_zero = [&](float a, float b) {
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-      };
-      const uint32_t first = toward_zero(w[2 * i], w[2 * i + 1]);
-      const half2_t off = __builtin_bit_cast(half2_t, TWO ? first : first & hi_mask);
-      const uint32_t rest = toward_zero(w[2 * i] - (float)off[0], w[2 * i + 1] - (float)off[1]);
-      hi[i] = TWO ? first : rest;
-      lo[i] = rest;
+    for (int i = 0; i < kKeys / 2; ++i) {
+      hi[i] = toward_zero(w[2 * i], w[2 * i + 1]);
+      const half2_t off = __builtin_bit_cast(half2_t, hi[i]);
+      lo[i] = toward_zero(w[2 * i] - (float)off[0], w[2 * i + 1] - (float)off[1]);
     }
-    const half8_t ph = as_half8(hi[0], hi[1], hi[2], hi[3]), pl = as_half8(lo[0], lo[1], lo[2], lo[3]);
-    const half8_t z = as_half8(vz[0], vz[1], vz[2], vz[3]);
+    half8_t ph, pl;
+    if constexpr (TWO) {
+      ph = as_half8(hi[0], hi[1], hi[2], hi[3]);
+      pl = as_half8(lo[0], lo[1], lo[2], lo[3]);
+      acc_z = mfma_16x16x32(as_half8(vz[0], vz[1], vz[2], vz[3]), ph, acc_z);
+      acc_z = mfma_16x16x32(as_half8(vz[0], vz[1], vz[2], vz[3]), pl, acc_z);
+    } else {
+      // columns 0 .. 7 carry the first numbers of both blocks' keys, columns 8 .. 15 the second: each half has one block's
+      uint32_t x0[2], x1[2];
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) acc[j] = mfma_16x16x32(z, ph, acc[j]);
+      for (int i = 0; i < 2; ++i) {
+        x0[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)hi[i], (int)lo[i], kDppRotate8, 0xf, 0xc, false);
+        x1[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)lo[i], (int)hi[i], kDppRotate8, 0xf, 0x3, false);
+      }
+      ph = pl = as_half8(x0[0], x0[1], x1[0], x1[1]);
+      acc_z = mfma_16x16x32(as_half8(vz[0], vz[1], vz[2], vz[3]), ph, acc_z);
+    }
 #pragma unroll
     for (int e = 0; e < kUnits; ++e) {
       uint32_t x0[4], x1[4], x2[4], x3[4];   // rows 4g, 4g + 1 of the first block, 4g + 2, 4g + 3, the same of the second
@@ -277,10 +366,7 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
       for (int j = 0; j < 4; ++j) {
         const half8_t a = as_half8(x0[j], x1[j], x2[j], x3[j]);
         acc[4 * e + j] = mfma_16x16x32(a, ph, acc[4 * e + j]);
-        if constexpr (TWO) {   // (the small parts only once the large ones have met their zero points)
-          acc[4 * e + j] = mfma_16x16x32(z, pl, acc[4 * e + j]);
-          acc[4 * e + j] = mfma_16x16x32(a, pl, acc[4 * e + j]);
-        }
+        if constexpr (TWO) acc[4 * e + j] = mfma_16x16x32(a, pl, acc[4 * e + j]);
       }
     }
   };
@@ -288,16 +374,22 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   // Two blocks a step, the next two in flight.
   auto request_pair = [&](int p, Int4Regs<D> (&r)[2]) {
     if (p < p1) {
-      request(p, r[0]);
-      request(p + 1, r[1]);
+      request(id0, r[0]);
+      request(id1, r[1]);
+      id0 = page_id(p + 2);
+      id1 = page_id(p + 3);
     }
   };
   int p = p0;
-  for (; (p + 4) * kInt4Block <= end; p += 4) {
-    request_pair(p + 2, buf[1]);
-    attend(buf[0], p, std::false_type{});
-    request_pair(p + 4, buf[0]);
-    attend(buf[1], p + 2, std::false_type{});
+  while ((p + 4) * kInt4Block <= end) {
+    const int fold_at = p + kFold;
+    for (; (p + 4) * kInt4Block <= end && p < fold_at; p += 4) {
+      request_pair(p + 2, buf[1]);
+      attend(buf[0], p, std::false_type{});
+      request_pair(p + 4, buf[0]);
+      attend(buf[1], p + 2, std::false_type{});
+    }
+    fold_zeros();
   }
 #pragma unroll 1
   for (; p < p1; p += 2) {   // less than 64 tokens
@@ -307,6 +399,8 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
     buf[0][1] = buf[1][1];
   }
 
+  fold_zeros();
+  if constexpr (!TWO) total += dpp<kDppRotate8>(total);
   total += xor_lane(total, 16);
   total += xor_lane(total, 32);
   const float inv = 0x1p20f / total;
