@@ -33,6 +33,12 @@ typedef uint32_t uint2v_t __attribute__((ext_vector_type(2)));
 constexpr int kInt4Waves = 4;            // most wavefronts of a workgroup
 constexpr float kInt4Top = 7.0f;         // log2 of where the largest p s' is put
 constexpr float kInt4Grown = 32768.0f;   // and what it may grow to
+#ifndef DEPTH
+#define DEPTH 2
+#define WPE 3
+#define AUX 0
+#endif
+constexpr int kDepth = DEPTH;
 constexpr int kFold = 32;                // blocks between two subtractions of the zero points
 constexpr float kLog2eI4 = 1.4426950408889634f, kLn2I4 = 0.6931471805599453f;
 
@@ -76,7 +82,7 @@ __device__ __forceinline__ half8_t as_half8(uint32_t a, uint32_t b, uint32_t c, 
 
 // TWO: more than 8 query heads, whose second part of p s' has MFMAs of its own.
 template <int D, bool TWO>
-__global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_eu(3, 3))) void paged_decode_int4_kernel(
+__global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void paged_decode_int4_kernel(
     const half_t *__restrict__ q, int64_t q_batch_stride, uint8_t *pool, const int32_t *__restrict__ block_table,
     int32_t bt_stride, const int32_t *__restrict__ seq_lens, const half_t *__restrict__ k_new,
     const half_t *__restrict__ v_new, int64_t k_new_stride, int64_t v_new_stride, half_t *__restrict__ out,
@@ -139,29 +145,46 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   const uint32_t v_off = (uint32_t)(int4_codes_at(num_kv_heads + h, D) + g * (2 * D) + n * (D / 8));
   const uint32_t kw_off = (uint32_t)(int4_words_at(h, num_kv_heads, D) + 8 * g);
   const uint32_t vw_off = (uint32_t)(int4_words_at(num_kv_heads + h, num_kv_heads, D) + 8 * g);
-  auto request = [&](int id, Int4Regs<D> &r) {
-    const uint8_t *block = pool + (int64_t)id * block_bytes;
-    typedef uint32_t vec __attribute__((ext_vector_type(kSteps)));
-    const vec kk = __builtin_nontemporal_load((const vec *)(block + k_off));
-    const vec vv = __builtin_nontemporal_load((const vec *)(block + v_off));
+  // Loads of pages past the split's last name a buffer of no bytes: they return zeros and touch no memory, and the loop has the
+  // same number of them in flight at every step, so that each wait covers the page it needs and no younger one.
+  auto request = [&](int p, int id, Int4Regs<D> &r) {
+    const auto block = __builtin_amdgcn_make_buffer_rsrc(pool + (int64_t)id * block_bytes, 0, p < p1 ? (int)block_bytes : 0,
+                                                         0x00020000);
+    if constexpr (D == 128) {
+      const uint4_t kk = __builtin_amdgcn_raw_buffer_load_b128(block, k_off, 0, AUX);
+      const uint4_t vv = __builtin_amdgcn_raw_buffer_load_b128(block, v_off, 0, AUX);
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      r.k[i] = kk[i];
-      r.v[i] = vv[i];
+      for (int i = 0; i < kSteps; ++i) {
+        r.k[i] = kk[i];
+        r.v[i] = vv[i];
+      }
+    } else {
+      const uint2v_t kk = __builtin_amdgcn_raw_buffer_load_b64(block, k_off, 0, AUX);
+      const uint2v_t vv = __builtin_amdgcn_raw_buffer_load_b64(block, v_off, 0, AUX);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        r.k[i] = kk[i];
+        r.v[i] = vv[i];
+      }
     }
-    const uint2v_t kw = *(const uint2v_t *)(block + kw_off), vw = *(const uint2v_t *)(block + vw_off);
+    const uint2v_t kw = __builtin_amdgcn_raw_buffer_load_b64(block, kw_off, 0, 0);
+    const uint2v_t vw = __builtin_amdgcn_raw_buffer_load_b64(block, vw_off, 0, 0);
     r.kw[0] = kw[0];
     r.kw[1] = kw[1];
     r.vw[0] = vw[0];
     r.vw[1] = vw[1];
   };
-  Int4Regs<D> buf[2][2];
-  // (page ids are read a step before the requests that they are for)
+  // Two blocks a step, kDepth steps' in flight; page ids are read a step before the requests that they are for.
+  Int4Regs<D> buf[kDepth][2];
   int id0 = page_id(p0), id1 = page_id(p0 + 1);
-  request(id0, buf[0][0]);
-  request(id1, buf[0][1]);
-  id0 = page_id(p0 + 2);
-  id1 = page_id(p0 + 3);
+  auto request_pair = [&](int p, Int4Regs<D> (&r)[2]) {
+    request(p, id0, r[0]);
+    request(p + 1, id1, r[1]);
+    id0 = page_id(p + 2);
+    id1 = page_id(p + 3);
+  };
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i) request_pair(p0 + 2 * i, buf[i]);
 
   // q as the right operand of the first product: column n, the elements of the bytes that the lane of the same g holds of K,
   // as a sum of three fp8 numbers (4 + 4 + 4 bits), scaled by a power of two that puts the row's largest between 224 and 448. What
@@ -371,32 +394,23 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
     }
   };
 
-  // Two blocks a step, the next two in flight.
-  auto request_pair = [&](int p, Int4Regs<D> (&r)[2]) {
-    if (p < p1) {
-      request(id0, r[0]);
-      request(id1, r[1]);
-      id0 = page_id(p + 2);
-      id1 = page_id(p + 3);
-    }
-  };
   int p = p0;
-  while ((p + 4) * kInt4Block <= end) {
-    const int fold_at = p + kFold;
-    for (; (p + 4) * kInt4Block <= end && p < fold_at; p += 4) {
-      request_pair(p + 2, buf[1]);
-      attend(buf[0], p, std::false_type{});
-      request_pair(p + 4, buf[0]);
-      attend(buf[1], p + 2, std::false_type{});
+  int fold_at = p + kFold;
+  while ((p + 2 * kDepth) * kInt4Block <= end) {
+#pragma unroll
+    for (int i = 0; i < kDepth; ++i) {
+      attend(buf[i], p + 2 * i, std::false_type{});
+      request_pair(p + 2 * i + 2 * kDepth, buf[i]);
     }
-    fold_zeros();
+    p += 2 * kDepth;
+    if (p >= fold_at) {
+      fold_zeros();
+      fold_at = p + kFold;
+    }
   }
-#pragma unroll 1
-  for (; p < p1; p += 2) {   // less than 64 tokens
-    request_pair(p + 2, buf[1]);
-    attend(buf[0], p, std::true_type{});
-    buf[0][0] = buf[1][0];
-    buf[0][1] = buf[1][1];
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i) {
+    if (p + 2 * i < p1) attend(buf[i], p + 2 * i, std::true_type{});
   }
 
   fold_zeros();
