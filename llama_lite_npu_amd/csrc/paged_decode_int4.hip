@@ -1,26 +1,38 @@
-// Paged flash-decoding over a 4-bit pool (kv_int4.h): one wavefront per (sequence, kv head, split), partial rows
-// merged by litekv_paged_decode_merge.
+// Paged flash-decoding over a 4-bit pool (kv_int4.h): a workgroup per (sequence, kv head, split), whose wavefronts attend a
+// part of the split's keys each; partial rows of several splits are merged by litekv_paged_decode_merge.
 //
 // The kernel works on the codes. With q the rows of up to 16 query heads of the kv head as columns, key i's score is
 //     S[i] = s_i * (sum_d c_id q_d - z_i * sum_d q_d)
 // and an output row
 //     O[d] = sum_i (p_i s'_i) (c'_id - z'_i)       p = softmax of S, s', z', c' those of V
 // so a scale and a zero point cost a few instructions per key instead of one per element. Codes reach the matrix cores with
-// nothing but a shift and a mask: c in bits 4 .. 7 of an fp16 number is the subnormal c * 2^-20. The matrix cores take it as it
-// is, but do not normalise it: products are lined up by the exponents of their factors and cut off some 27 bits below the largest of
-// a sum. From bits 4 .. 7 that leaves 24 bits of a code's own size; in bits 0 .. 3, which need two instructions fewer for eight
-// codes, 20 (333 keys with one that carries nearly all of the weight: outputs 1e-5 of sum p |v| off, all to one side).
-// For the same reason the z' are subtracted step by step, by an MFMA of their own per tile, and not at the end from an accumulator
-// that would have grown to some twenty times the result.
+// nothing but shifts and masks:
+//  * K as bytes. A nibble in the low half of a byte is the fp8 number c * 2^-9, exactly; q is a sum of three fp8 numbers, which
+//    leaves 2^-18 of its row's largest. S^T is three 16x16x128 products per 16 keys, two with heads of 64.
+//  * V as fp16. c in bits 4 .. 7 is the subnormal c * 2^-20. The matrix cores take it as it is, but do not normalise it: products are
+//    lined up by the exponents of their factors and cut off some 27 bits below the largest of a sum. From bits 4 .. 7 that leaves 24
+//    bits of a code's own size; in bits 0 .. 3, which need two instructions fewer for eight codes, 20 (333 keys with one that
+//    carries nearly all of the weight: outputs 1e-5 of sum p |v| off, all to one side). For the same reason the z' are
+//    summed by an MFMA of their own and taken off every kFold blocks, and not at the end from accumulators that would have
+//    grown to some twenty times the result.
 //
-// S^T[key][col] is the accumulator of the first product (16x16x32: 16 keys, 32 of D) and in the same lanes the right operand of the
-// second, O^T[d][col] += V^T[d][key] P^T[key][col], whose 32 keys are two blocks of 16: nothing crosses lanes and no LDS
-// is used. p s' as fp16 would cost the result as much again as its own rounding: up to 8 query heads, which leave half
-// of the columns empty, columns 8..15 carry the same heads and hold what the rounding left; with more
-// a second MFMA does. So a result is as good as with fp32 probabilities.
+// A wavefront takes two blocks of 16 keys a step. S^T[key][col] is the accumulator of the first product and in the same lanes
+// the right operand of the second, O^T[d][col] += V^T[d][key] P^T[key][col] (16x16x32): no LDS. p s' as fp16 would
+// cost the result as much again as its own rounding, so it is kept as two fp16 numbers, the second what the first leaves. Up to
+// 8 query heads leave half of the columns empty: there columns 0 .. 7 do the softmax of the first block and columns 8 .. 15 that of
+// the second, and one exchange of 8 lanes makes the second product's operand, the first numbers in columns 0 .. 7, the others in
+// 8 .. 15. With more heads a second MFMA takes the others.
 //
 // The reference of the exponentials is the largest p s' so far, not the largest p: in fp16 it is p s' that has to fit. It is put
 // at 2^7 and may grow to 2^15 before the accumulators are rescaled.
+//
+// Bound: by vector instructions and the latency of the loads, then by memory. A step is 157 vector instructions for 32 keys and 8 heads
+// (D = 128), which leaves room for three wavefronts per SIMD with two steps' loads in flight each (147 registers; four with one
+// step's in flight took 3 to 10% longer). 64 sequences of 8192 tokens, 32 / 4 heads of 128: 48.5 us, 5.7 TB/s of cache read (a copy
+// reads and writes 5.0). Of its twelve wavefronts a compute unit holds one workgroup of eight or three of four. Eight are faster
+// while there are no more workgroups than compute units (the case above with four: 53 us; 20 sequences of 4096, 8 kv heads: 22.7
+// against 25), four where there are more (38 of them: 39 us against 44; 100 of 2048: 44 against 55). Streaming loads, whose lines
+// are the first to leave the caches, took 10% less than ordinary ones.
 #include <type_traits>
 
 #include "common.h"
@@ -30,15 +42,11 @@ namespace litekv {
 
 typedef uint32_t uint2v_t __attribute__((ext_vector_type(2)));
 
-constexpr int kInt4Waves = 4;            // most wavefronts of a workgroup
+constexpr int kInt4Waves = 8;            // of a workgroup, at most
 constexpr float kInt4Top = 7.0f;         // log2 of where the largest p s' is put
 constexpr float kInt4Grown = 32768.0f;   // and what it may grow to
-#ifndef DEPTH
-#define DEPTH 2
-#define WPE 3
-#define AUX 0
-#endif
-constexpr int kDepth = DEPTH;
+constexpr int kDepth = 2;                // steps whose loads are in flight
+constexpr int kStreaming = 2;            // of a buffer load: not read again soon
 constexpr int kFold = 32;                // blocks between two subtractions of the zero points
 constexpr float kLog2eI4 = 1.4426950408889634f, kLn2I4 = 0.6931471805599453f;
 
@@ -82,26 +90,34 @@ __device__ __forceinline__ half8_t as_half8(uint32_t a, uint32_t b, uint32_t c, 
 
 // TWO: more than 8 query heads, whose second part of p s' has MFMAs of its own.
 template <int D, bool TWO>
-__global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void paged_decode_int4_kernel(
+__global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_eu(3, 3))) void paged_decode_int4_kernel(
     const half_t *__restrict__ q, int64_t q_batch_stride, uint8_t *pool, const int32_t *__restrict__ block_table,
     int32_t bt_stride, const int32_t *__restrict__ seq_lens, const half_t *__restrict__ k_new,
     const half_t *__restrict__ v_new, int64_t k_new_stride, int64_t v_new_stride, half_t *__restrict__ out,
     float *__restrict__ part_o, float *__restrict__ part_lse, int32_t num_q_heads, int32_t num_kv_heads,
-    int32_t group_all, int32_t slices, int32_t max_splits, int32_t min_pages_per_split, int32_t num_pages,
-    int32_t page_shift, float scale_log2) {
+    int32_t batch, int32_t group_all, int32_t slices, int32_t max_splits, int32_t min_pages_per_split,
+    int32_t num_pages, int32_t page_shift, float scale_log2) {
   constexpr int kSteps = D / 32;   // MFMAs of a block's scores; dwords a lane holds of K and of V
   constexpr int kTiles = D / 16;   // 16-row tiles of O^T
   constexpr int kUnits = D / 64;   // see int4_v_unit
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
-  const HeadSlice hs = head_slice(blockIdx.x * (blockDim.x >> 6) + wave, slices, group_all);
+  // Workgroups with the same pages -- the heads of a sequence's split, whose words share cache lines -- land on one XCD: they
+  // are dealt out round robin, so eight (sequence, split) pairs' take turns. Splits are the slowest index: a launch of more
+  // workgroups than the device holds ends with splits of one size.
+  const int pairs = batch * max_splits, heads_x = gridDim.x / pairs;
+  const int deal = (int)blockIdx.x / (8 * heads_x), at = (int)blockIdx.x - deal * 8 * heads_x;
+  const int turns = pairs - 8 * deal < 8 ? pairs - 8 * deal : 8;
+  const int pair = 8 * deal + at % turns;
+  const int split = pair / batch, b = pair - split * batch;
+  const HeadSlice hs = head_slice(at / turns, slices, group_all);
+  const int share = (int)(blockDim.x >> 6), part = wave;   // the wavefronts attend a part of the split's keys each
   const int h = hs.kv_head, group = hs.q_heads, hq0 = hs.q_head0;
-  const int split = blockIdx.y, b = blockIdx.z;
   const int len = as_uniform(seq_lens)[b];
   half_t *out_row = out + ((int64_t)b * num_q_heads + hq0) * D;
   if (len <= 0) {
-    if (split == 0) {
+    if (split == 0 && part == 0) {
       for (int i = lane; i < group * (D / 8); i += kWave) *(half8_t *)(out_row + 8 * i) = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
     }
     return;
@@ -109,8 +125,12 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   const int pages = pages_of(len);
   const int n_splits = splits_for_pages(pages, max_splits, min_pages_per_split);
   if (split >= n_splits) return;
-  const int p0 = (int)(((int64_t)split * pages) / n_splits);
-  const int p1 = (int)(((int64_t)(split + 1) * pages) / n_splits);
+  const int first = (int)(((int64_t)split * pages) / n_splits);
+  const int last = (int)(((int64_t)(split + 1) * pages) / n_splits);
+  const int steps = (last - first + 1) / 2;   // of two blocks
+  const int p0 = first + 2 * ((steps * part) / share);
+  const int p1 = part + 1 < share ? first + 2 * ((steps * (part + 1)) / share) : last;
+  const bool any = p0 < p1;   // (a wavefront without a part has nothing to add)
 
   const int64_t block_bytes = int4_block_bytes(num_kv_heads, D);
   const uniform_i32_ptr table = as_uniform(block_table) + (int64_t)b * bt_stride;
@@ -123,7 +143,7 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
 
   // The step's new token goes into the last block before anything of it is read (by this wavefront, the only one that reads it
   // in this launch; the slices of a wide group all write the same bytes).
-  if (k_new != nullptr && p1 == pages && pages <= (bt_stride << page_shift)) {
+  if (k_new != nullptr && any && p1 == pages && pages <= (bt_stride << page_shift)) {
     constexpr int L = D / 8;
     if (lane < 2 * L) {
       const bool is_v = lane >= L;
@@ -151,16 +171,16 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
     const auto block = __builtin_amdgcn_make_buffer_rsrc(pool + (int64_t)id * block_bytes, 0, p < p1 ? (int)block_bytes : 0,
                                                          0x00020000);
     if constexpr (D == 128) {
-      const uint4_t kk = __builtin_amdgcn_raw_buffer_load_b128(block, k_off, 0, AUX);
-      const uint4_t vv = __builtin_amdgcn_raw_buffer_load_b128(block, v_off, 0, AUX);
+      const uint4_t kk = __builtin_amdgcn_raw_buffer_load_b128(block, k_off, 0, kStreaming);
+      const uint4_t vv = __builtin_amdgcn_raw_buffer_load_b128(block, v_off, 0, kStreaming);
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         r.k[i] = kk[i];
         r.v[i] = vv[i];
       }
     } else {
-      const uint2v_t kk = __builtin_amdgcn_raw_buffer_load_b64(block, k_off, 0, AUX);
-      const uint2v_t vv = __builtin_amdgcn_raw_buffer_load_b64(block, v_off, 0, AUX);
+      const uint2v_t kk = __builtin_amdgcn_raw_buffer_load_b64(block, k_off, 0, kStreaming);
+      const uint2v_t vv = __builtin_amdgcn_raw_buffer_load_b64(block, v_off, 0, kStreaming);
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         r.k[i] = kk[i];
@@ -176,12 +196,12 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   };
   // Two blocks a step, kDepth steps' in flight; page ids are read a step before the requests that they are for.
   Int4Regs<D> buf[kDepth][2];
-  int id0 = page_id(p0), id1 = page_id(p0 + 1);
+  int id0 = any ? page_id(p0) : 0, id1 = any ? page_id(p0 + 1) : 0;
   auto request_pair = [&](int p, Int4Regs<D> (&r)[2]) {
     request(p, id0, r[0]);
     request(p + 1, id1, r[1]);
-    id0 = page_id(p + 2);
-    id1 = page_id(p + 3);
+    id0 = any ? page_id(p + 2) : 0;
+    id1 = any ? page_id(p + 3) : 0;
   };
 #pragma unroll
   for (int i = 0; i < kDepth; ++i) request_pair(p0 + 2 * i, buf[i]);
@@ -417,43 +437,63 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   if constexpr (!TWO) total += dpp<kDppRotate8>(total);
   total += xor_lane(total, 16);
   total += xor_lane(total, 32);
-  const float inv = 0x1p20f / total;
   const int head = TWO ? n : (n & 7);
   const bool whole = n_splits == 1;
-  const int64_t cell = ((int64_t)b * num_q_heads + hq0 + head) * max_splits + split;
-  // O^T tile (e, j): row m is element m * D / 16 + kUnits * j + e of the output row; a lane has rows 4g .. 4g + 3
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float y[kTiles];   // elements (4g + i) * D / 16 ...
+  const int64_t cell0 = ((int64_t)b * num_q_heads + hq0) * max_splits + split;
+  // O^T tile (e, j): row m is element m * D / 16 + kUnits * j + e of the output row; a lane has rows 4g .. 4g + 3: row i of them
+  // as kTiles neighbours of the output row, from (4g + i) * kTiles on
+  auto elements = [&](int i, float scale, float (&y)[kTiles]) {
 #pragma unroll
     for (int e = 0; e < kUnits; ++e) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float a = acc[4 * e + j][i];
         if constexpr (!TWO) a += dpp<kDppRotate8>(a);
-        y[kUnits * j + e] = a * inv;
+        y[kUnits * j + e] = a * scale;
       }
     }
-    // (both halves of the columns have the rows: each stores two of the four)
-    if (head < group && (TWO || (i >> 1) == (n >> 3))) {
-      const int at = (4 * g + i) * kTiles;
-      if (whole) {
-        half_t *o = out_row + (int64_t)head * D + at;
+  };
+  // (!TWO: both halves of the columns have the rows, each stores two of the four)
+  auto mine = [&](int i) { return head < group && (TWO || (i >> 1) == (n >> 3)); };
+  // The wavefronts that share a split leave their rows, references and sums in LDS, and fold them in order.
+  extern __shared__ __attribute__((aligned(16))) float int4_rows[];
+  constexpr int kHeads = TWO ? 16 : 8, kArea = kHeads * D + 32;   // of a wavefront: rows, references, sums
+  float *area = int4_rows + part * kArea;
 #pragma unroll
-        for (int j = 0; j < kTiles; j += 4) {
-          *(half4_t *)(o + j) = half4_t{(half_t)y[j], (half_t)y[j + 1], (half_t)y[j + 2], (half_t)y[j + 3]};
-        }
-      } else {
-        float *o = part_o + cell * D + at;
+  for (int i = 0; i < 4; ++i) {
+    float y[kTiles];
+    elements(i, 0x1p20f, y);
+    if (!mine(i)) continue;
 #pragma unroll
-        for (int j = 0; j < kTiles; j += 4) {
-          __builtin_nontemporal_store(float4_t{y[j], y[j + 1], y[j + 2], y[j + 3]}, (float4_t *)(o + j));
-        }
-      }
+    for (int j = 0; j < kTiles; j += 4) {
+      *(float4_t *)(area + head * D + (4 * g + i) * kTiles + j) = float4_t{y[j], y[j + 1], y[j + 2], y[j + 3]};
     }
   }
-  if (!whole && g == 0 && n < group) {
-    __builtin_nontemporal_store((ref + fast_log2(total)) * kLn2I4, part_lse + cell);
+  if (g == 0 && n < kHeads) {
+    area[kHeads * D + n] = ref;
+    area[kHeads * D + 16 + n] = total;
+  }
+  __syncthreads();
+  for (int i = part * kWave + lane; i < group * (D / 4); i += share * kWave) {
+    const int of = i / (D / 4), at_row = 4 * (i % (D / 4));
+    const float *stats = int4_rows + kHeads * D + of;
+    float top = stats[0];
+    for (int s = 1; s < share; ++s) top = __builtin_fmaxf(top, stats[s * kArea]);
+    float sum = 0.f;
+    float4_t y = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < share; ++s) {
+      const float weight = fast_exp2(stats[s * kArea] - top);
+      sum += weight * stats[s * kArea + 16];
+      y += weight * *(const float4_t *)(int4_rows + s * kArea + of * D + at_row);
+    }
+    y *= 1.0f / sum;
+    if (whole) {
+      *(half4_t *)(out_row + (int64_t)of * D + at_row) = half4_t{(half_t)y[0], (half_t)y[1], (half_t)y[2], (half_t)y[3]};
+    } else {
+      const int64_t cell = cell0 + (int64_t)of * max_splits;
+      __builtin_nontemporal_store(y, (float4_t *)(part_o + cell * D + at_row));
+      if (at_row == 0) __builtin_nontemporal_store((top + fast_log2(sum)) * kLn2I4, part_lse + cell);
+    }
   }
 }
 
@@ -510,22 +550,21 @@ extern "C" int litekv_paged_decode_int4(const void *q, int64_t q_batch_stride, v
   LITEKV_REQUIRE(slice_heads <= 65535, "%s: num_q_heads %d too large", what, num_q_heads);
   float *part_o = max_splits > 1 ? static_cast<float *>(workspace) : nullptr;
   float *part_lse = max_splits > 1 ? part_o + (size_t)batch * num_q_heads * max_splits * head_dim : nullptr;
-  // Wavefronts per workgroup: as many kv heads of one (sequence, split), whose codes and words are neighbours in memory, as
-  // leave at least two workgroups per compute unit.
   const int64_t units = (int64_t)batch * slice_heads * max_splits;
-  int waves = kInt4Waves;
-  while (waves > 1 && (units / waves < 512 || slice_heads % waves != 0)) waves >>= 1;
-  auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(slice_heads / waves), (unsigned)max_splits, (unsigned)batch),
-                       dim3((unsigned)(waves * kWave)), 0, static_cast<hipStream_t>(stream),
-                       static_cast<const half_t *>(q), q_batch_stride, static_cast<uint8_t *>(kv_pool_int4),
-                       block_table, block_table_stride, seq_lens, static_cast<const half_t *>(k_new),
-                       static_cast<const half_t *>(v_new), k_new_stride, v_new_stride, static_cast<half_t *>(out),
-                       part_o, part_lse, num_q_heads, num_kv_heads, group, slices, max_splits,
-                       (int32_t)(min16 < 0x7fffffffLL ? min16 : 0x7fffffffLL), (int32_t)num_pages, page_shift,
-                       softmax_scale * kLog2eI4);
-  };
+  // (256 compute units: see the top of the file)
+  const int share = units > 256 ? kInt4Waves / 2 : kInt4Waves;
+  LITEKV_REQUIRE(units <= 0x7fffffffLL / 8, "%s: too many workgroups", what);
   const bool two = (group + slices - 1) / slices > 8;
+  const size_t lds = (size_t)share * ((two ? 16 : 8) * head_dim + 32) * sizeof(float);
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)units), dim3((unsigned)(share * kWave)), lds,
+                       static_cast<hipStream_t>(stream), static_cast<const half_t *>(q), q_batch_stride,
+                       static_cast<uint8_t *>(kv_pool_int4), block_table, block_table_stride, seq_lens,
+                       static_cast<const half_t *>(k_new), static_cast<const half_t *>(v_new), k_new_stride,
+                       v_new_stride, static_cast<half_t *>(out), part_o, part_lse, num_q_heads, num_kv_heads, batch, group,
+                       slices, max_splits, (int32_t)(min16 < 0x7fffffffLL ? min16 : 0x7fffffffLL),
+                       (int32_t)num_pages, page_shift, softmax_scale * kLog2eI4);
+  };
   if (head_dim == 64) {
     two ? launch(paged_decode_int4_kernel<64, true>) : launch(paged_decode_int4_kernel<64, false>);
   } else {

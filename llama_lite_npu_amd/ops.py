@@ -359,24 +359,26 @@ def decode_split_plan(batch: int, num_kv_heads: int, max_blocks: int,
     return max(1, (max_blocks + pps - 1) // pps), pps
 
 
-# A split of a decode step over 4-bit codes is at least this many tokens long.
-INT4_SPLIT_TOKENS = 128
+def int4_split_tokens(batch: int, num_kv_heads: int) -> int:
+    """Least tokens of a split of a decode step over 4-bit codes. Up to 256 (sequence, kv head) pairs, a compute unit has at
+    most one and shorter splits fill the device (8 sequences of 4096 tokens, 8 kv heads: splits of 1024 / 2048 / 4096 tokens
+    15.1 / 17.6 / 21.1 us); with more, splits only even out the lengths (8 kv heads, 40 of 16384
+    tokens: 144 / 122 / 115 us, 135 unsplit; 64 of them: 224 / 189 / 180 us, 170 unsplit)."""
+    return 1024 if batch * num_kv_heads <= 256 else 4096
 
 
 def int4_decode_splits(batch: int, num_kv_heads: int, max_pages: int, total_pages: Optional[int] = None,
                        page_size: int = PAGE_SIZE) -> tuple[int, int]:
     """(max_splits, min_pages_per_split) of a decode step over a 4-bit pool whose longest sequence has ``max_pages`` pages and
-    all of them together ``total_pages`` (None: as many for every sequence)."""
-    min_pages = max(1, INT4_SPLIT_TOKENS // page_size)
-    steps = max(1, page_size // PAGE_SIZE)
-    total = batch * max_pages if total_pages is None else total_pages
-    wavefronts = 2048 / max(1, num_kv_heads)                 # per kv head
-    each = max(1.0, total * steps / wavefronts)              # 16-token pages a wavefront should get
-    want = max_pages * steps / each
-    splits = 1
-    while splits < want and splits * min_pages < max_pages:
-        splits *= 2
-    return splits, min_pages
+    all of them together ``total_pages`` (None: as many for every sequence): as many splits as fill 256 compute units, but no
+    more than 16 where that makes them shorter than 4096 tokens, since their merge takes longer the more there are (one
+    sequence of 32768 tokens, 8 kv heads: 8 / 16 / 32 splits 24 / 19.5 / 22 us)."""
+    min_pages = max(1, int4_split_tokens(batch, num_kv_heads) // page_size)
+    most = min(-(-max_pages // min_pages), max(16, max_pages * page_size // 4096), 65535)
+    if batch * num_kv_heads <= 256:
+        total = batch * max_pages if total_pages is None else total_pages
+        most = min(most, 256 * max_pages // max(1, total * num_kv_heads))
+    return max(1, most), min_pages
 
 
 def decode_workspace(batch: int, num_q_heads: int, max_splits: int, device) -> Optional[torch.Tensor]:
@@ -599,10 +601,10 @@ class DecodePlan:
     def set_schedule(self, splits: int) -> None:
         """0: balanced; otherwise the per-sequence schedule with that many splits per sequence
         (the partial-result buffer of several splits is allocated here, not at the launch). A step over 4-bit codes has
-        no balanced form: 0 is one split, and several are at least ``INT4_SPLIT_TOKENS`` long."""
+        no balanced form: 0 is one split, and several are at least ``int4_split_tokens`` long."""
         if self.int4:
             splits = max(1, int(splits))
-            self.min_pages_per_split = max(1, INT4_SPLIT_TOKENS // self.page_size)
+            self.min_pages_per_split = max(1, int4_split_tokens(self.batch, self.num_kv_heads) // self.page_size)
         self.per_sequence = splits > 0
         self.splits = max(1, int(splits))
         if self.splits > 1:
