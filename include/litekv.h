@@ -791,7 +791,9 @@ int litekv_paged_prefill_int8(const void *q, int64_t q_token_stride,
  *
  * litekv_paged_decode_int4: litekv_paged_decode (splits, both stages; workspace from
  * litekv_paged_decode_workspace_bytes) over a 4-bit pool, with the step's append fused in where k_new / v_new are not
- * NULL (see litekv_paged_decode_append).
+ * NULL (see litekv_paged_decode_append). litekv_paged_decode_int4_splits: the max_splits that suits a step
+ * whose longest sequence has max_pages pages and all of them total_pages (-1: batch * max_pages); *min_pages_per_split
+ * depends on batch, num_kv_heads and page_size only. 0 for arguments that no step has.
  *
  * litekv_paged_prefill_int4: litekv_paged_prefill_bounded over a 4-bit pool (key_slices 1), or
  * litekv_paged_prefill_split (key_slices 2 .. 8, with its workspace; max_kv_len is then not read).
@@ -814,6 +816,10 @@ int litekv_page_dequant_int4(const void *kv_pool_int4, void *dst_pool, const int
                              const int32_t *dst_ids, int32_t n, int32_t num_kv_heads,
                              int32_t head_dim, int32_t page_size, int64_t num_src_pages,
                              int64_t num_dst_pages, void *stream);
+
+int32_t litekv_paged_decode_int4_splits(int32_t batch, int32_t num_kv_heads, int64_t max_pages,
+                                        int64_t total_pages, int32_t page_size,
+                                        int32_t *min_pages_per_split);
 
 int litekv_paged_decode_int4(const void *q, int64_t q_batch_stride, void *kv_pool_int4,
                              const int32_t *block_table, int32_t block_table_stride,

@@ -235,6 +235,10 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int64,
          c_int64, c_void_p],
     ),
+    "litekv_paged_decode_int4_splits": (
+        c_int32,
+        [c_int32, c_int32, c_int64, c_int64, c_int32, c_void_p],
+    ),
     "litekv_paged_decode_int4": (
         c_int32,
         [c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_int64,

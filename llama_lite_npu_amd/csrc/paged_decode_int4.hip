@@ -499,6 +499,33 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
 
 }  // namespace litekv
 
+// Up to 256 (sequence, kv head) pairs, a compute unit has at most one, and splits of 1024 tokens and more fill the device
+// (8 sequences of 4096 tokens, 8 kv heads: splits of 1024 / 2048 / 4096 tokens 15.1 / 17.6 / 21.1 us). With more, splits only even out
+// the lengths (40 of 16384 tokens, 8 kv heads: 144 / 122 / 115 us, 135 unsplit; 64 of them: 224 / 189 / 180 us, 170 unsplit).
+// No more than 16 where that makes them shorter than 4096 tokens: their merge takes longer the more there are (one sequence of 32768
+// tokens, 8 kv heads: 8 / 16 / 32 splits 24 / 19.5 / 22 us).
+extern "C" int32_t litekv_paged_decode_int4_splits(int32_t batch, int32_t num_kv_heads, int64_t max_pages, int64_t total_pages,
+                                                   int32_t page_size, int32_t *min_pages_per_split) {
+  using namespace litekv;
+  if (batch < 0 || num_kv_heads < 1 || max_pages < 0 || max_pages > 0x7fffffff || total_pages > (int64_t)batch * max_pages ||
+      page_shift_of(page_size) < 0 || min_pages_per_split == nullptr) {
+    return 0;
+  }
+  const int64_t pairs = (int64_t)batch * num_kv_heads;
+  const bool few = pairs <= 256;
+  const int64_t least = (few ? 1024 : 4096) / page_size;
+  *min_pages_per_split = (int32_t)least;
+  int64_t most = (max_pages + least - 1) / least;
+  const int64_t merged = max_pages * page_size / 4096 > 16 ? max_pages * page_size / 4096 : 16;
+  if (most > merged) most = merged;
+  if (few) {
+    const int64_t rows = total_pages < 0 ? pairs * max_pages : total_pages * num_kv_heads;   // of pages, a head's share each
+    const int64_t fill = 256 * max_pages / (rows > 0 ? rows : 1);
+    if (most > fill) most = fill;
+  }
+  return most < 1 ? 1 : most > 65535 ? 65535 : (int32_t)most;
+}
+
 extern "C" int litekv_paged_decode_int4(const void *q, int64_t q_batch_stride, void *kv_pool_int4,
                                         const int32_t *block_table, int32_t block_table_stride,
                                         const int32_t *seq_lens, const void *k_new, const void *v_new,

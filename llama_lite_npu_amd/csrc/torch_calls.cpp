@@ -12,6 +12,8 @@
 #include <Python.h>
 #include <stdio.h>
 
+#include <cmath>
+
 #include <ATen/ATen.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
@@ -254,9 +256,153 @@ PyObject *paged_prefill(PyObject *, PyObject *const *a, Py_ssize_t n) {
   }
 }
 
+// (q, kv_pool, block_table, seq_lens, softmax_scale or None, page_size, k_new, v_new, stream), the pool one of 4-bit codes
+// -> the output, or the library's status if that is not 0, or None. The partial rows' workspace as in paged_prefill.
+PyObject *paged_decode_int4(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (n != 9) Py_RETURN_NONE;
+  try {
+    const at::Tensor *q = half_tensor(a[0]);
+    if (q == nullptr || q->dim() != 3) Py_RETURN_NONE;
+    const Pool pool = pool_of(a[1], Py_None);
+    if (pool.format != kInt4) Py_RETURN_NONE;
+    const int64_t b = q->size(0), hq = q->size(1), d = pool.d;
+    const int64_t qs = row_stride(*q, b, hq, d);
+    const at::Tensor *table = index_tensor(a[2], -1), *lens = index_tensor(a[3], b);
+    if (b < 1 || qs < 0 || lens == nullptr || table == nullptr || table->dim() != 2 || table->size(0) != b) Py_RETURN_NONE;
+    const int64_t width = table->size(1);
+    const at::Tensor *kn = nullptr, *vn = nullptr;
+    int64_t ks = 0, vs = 0;
+    if (a[6] != Py_None || a[7] != Py_None) {
+      kn = half_tensor(a[6]);
+      vn = half_tensor(a[7]);
+      if (kn == nullptr || vn == nullptr) Py_RETURN_NONE;
+      ks = row_stride(*kn, b, pool.hkv, d);
+      vs = row_stride(*vn, b, pool.hkv, d);
+      if (ks < 0 || vs < 0) Py_RETURN_NONE;
+    }
+    const double scale = a[4] == Py_None ? 1.0 / std::sqrt((double)d) : PyFloat_AsDouble(a[4]);
+    const int64_t page = PyLong_AsLongLong(a[5]);
+    void *stream = PyLong_AsVoidPtr(a[8]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    if (page < 1 || page > 65536 || pool.slots % page != 0 || b > INT32_MAX || hq > INT32_MAX || pool.hkv > INT32_MAX ||
+        width < 1 || width > INT32_MAX) {
+      Py_RETURN_NONE;
+    }
+    int32_t least = 1;
+    const int32_t splits = litekv_paged_decode_int4_splits((int32_t)b, (int32_t)pool.hkv, width, -1, (int32_t)page, &least);
+    if (splits < 1) Py_RETURN_NONE;
+    const size_t partial_bytes = litekv_paged_decode_workspace_bytes((int32_t)b, (int32_t)hq, (int32_t)d, splits);
+    at::Tensor out = at::empty({b, hq, d}, q->options());
+    at::Tensor partials;
+    if (partial_bytes > 0) partials = at::empty({(int64_t)((partial_bytes + 3) / 4)}, q->options().dtype(at::kFloat));
+    const void *qp = address(q), *knp = address(kn), *vnp = address(vn);
+    void *pp = address(pool.t), *op = address(&out), *wp = partial_bytes > 0 ? partials.data_ptr() : nullptr;
+    const int32_t *tp = static_cast<const int32_t *>(address(table)), *lp = static_cast<const int32_t *>(address(lens));
+    PyObject *result = THPVariable_Wrap(std::move(out));  // (before the launch: it may throw)
+    const int rc = unlocked([&] {
+      return litekv_paged_decode_int4(qp, qs, pp, tp, (int32_t)width, lp, knp, vnp, ks, vs, op, wp, partial_bytes, (int32_t)b,
+                                      (int32_t)hq, (int32_t)pool.hkv, (int32_t)d, (int32_t)page, pool.slots / page, splits, least,
+                                      (float)scale, stream);
+    });
+    if (rc == 0) return result;
+    Py_DECREF(result);
+    return PyLong_FromLong(rc);
+  } catch (...) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+}
+
+// (k, v, slot_mapping, kv_pool, scales, stream) -> the library's status, or None
+PyObject *kv_append_quantised(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (n != 6) Py_RETURN_NONE;
+  try {
+    const at::Tensor *k = half_tensor(a[0]), *v = half_tensor(a[1]);
+    if (k == nullptr || v == nullptr || k->dim() != 3) Py_RETURN_NONE;
+    const Pool pool = pool_of(a[3], a[4]);
+    if (pool.format == kNone || pool.format == kF16) Py_RETURN_NONE;
+    const int64_t t = k->size(0), ks = row_stride(*k, t, pool.hkv, pool.d), vs = row_stride(*v, t, pool.hkv, pool.d);
+    const at::Tensor *slots = index_tensor(a[2], t);
+    if (ks < 0 || vs < 0 || slots == nullptr || t > INT32_MAX || pool.hkv > INT32_MAX || pool.d > INT32_MAX) Py_RETURN_NONE;
+    void *stream = PyLong_AsVoidPtr(a[5]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    const void *kp = address(k), *vp = address(v);
+    void *pp = address(pool.t);
+    const int32_t *slp = static_cast<const int32_t *>(address(slots));
+    const float *scales = static_cast<const float *>(pool.scales);
+    const int32_t t32 = (int32_t)t, h = (int32_t)pool.hkv, d = (int32_t)pool.d;
+    return PyLong_FromLong(unlocked([&] {
+      switch (pool.format) {
+        case kInt4:
+          return litekv_kv_append_int4(kp, vp, ks, vs, slp, pp, t32, h, d, pool.slots, stream);
+        case kFp8:
+          return litekv_kv_append_fp8(kp, vp, ks, vs, slp, pp, scales, t32, h, d, pool.slots, stream);
+        default:
+          return litekv_kv_append_int8(kp, vp, ks, vs, slp, pp, scales, t32, h, d, pool.slots, stream);
+      }
+    }));
+  } catch (...) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+}
+
+// (kv_pool, dst_pool, src_ids, dst_ids or None, scales, page_size, stream) -> the library's status, or None
+PyObject *page_dequant(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (n != 7) Py_RETURN_NONE;
+  try {
+    const Pool pool = pool_of(a[0], a[4]), to = pool_of(a[1], Py_None);
+    if (pool.format == kNone || pool.format == kF16 || to.format != kF16 || to.hkv != pool.hkv || to.d != pool.d) Py_RETURN_NONE;
+    const at::Tensor *src = index_tensor(a[2], -1), *dst = nullptr;
+    if (src == nullptr) Py_RETURN_NONE;
+    if (a[3] != Py_None) {
+      dst = index_tensor(a[3], src->numel());
+      if (dst == nullptr) Py_RETURN_NONE;
+    }
+    const int64_t page = PyLong_AsLongLong(a[5]);
+    void *stream = PyLong_AsVoidPtr(a[6]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    if (page < 1 || page > 65536 || pool.slots % page != 0 || to.slots % page != 0 || src->numel() > INT32_MAX ||
+        pool.hkv > INT32_MAX || pool.d > INT32_MAX) {
+      Py_RETURN_NONE;
+    }
+    const void *pp = address(pool.t);
+    void *tp = address(to.t);
+    const int32_t *sp = static_cast<const int32_t *>(address(src)), *dp = static_cast<const int32_t *>(address(dst));
+    const float *scales = static_cast<const float *>(pool.scales);
+    const int32_t count = (int32_t)src->numel(), h = (int32_t)pool.hkv, d = (int32_t)pool.d;
+    const int64_t from_pages = pool.slots / page, to_pages = to.slots / page;
+    return PyLong_FromLong(unlocked([&] {
+      switch (pool.format) {
+        case kInt4:
+          return litekv_page_dequant_int4(pp, tp, sp, dp, count, h, d, (int32_t)page, from_pages, to_pages, stream);
+        case kFp8:
+          return litekv_page_dequant(pp, tp, sp, dp, count, scales, h, d, (int32_t)page, from_pages, to_pages, stream);
+        default:
+          return litekv_page_dequant_int8(pp, tp, sp, dp, count, scales, h, d, (int32_t)page, from_pages, to_pages, stream);
+      }
+    }));
+  } catch (...) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+}
+
 PyMethodDef methods[] = {
     {"qk_norm_rope_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(qk_norm_rope_append)), METH_FASTCALL, nullptr},
     {"paged_prefill", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(paged_prefill)), METH_FASTCALL, nullptr},
+    {"paged_decode_int4", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(paged_decode_int4)), METH_FASTCALL, nullptr},
+    {"kv_append_quantised", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(kv_append_quantised)), METH_FASTCALL, nullptr},
+    {"page_dequant", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(page_dequant)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -190,6 +190,11 @@ def kv_append_quantised(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Te
     A pool of 4-bit codes (uint8 [slots, 2 * Hkv, D / 2 + 2], D 64 or 128) takes no scales: every row (token, kv head)
     is quantised over its own range, 0 included, and keeps its scale s and zero point z beside its codes: a code c
     stands for s * (c - z), at most s / 2 from the element, s = (max - min) / 15 rounded up to 7 bits."""
+    if k.is_cuda:
+        done = _lib.calls().kv_append_quantised(k, v, slot_mapping, kv_pool, scales, _stream())
+        if done is not None:
+            return _lib.check(done)
+    # (not a plain call)
     _dev_half("k", k), _dev_half("v", v)
     slots, hkv, d, _, _ = pool_geometry(kv_pool, 1)
     int4 = is_int4_pool(kv_pool)
@@ -218,6 +223,11 @@ def page_dequant(kv_pool: torch.Tensor, dst_pool: torch.Tensor, src_ids: torch.T
                  dst_ids: Optional[torch.Tensor], scales: Optional[torch.Tensor], page_size: int = PAGE_SIZE) -> None:
     """dst_pool[page dst_ids[i]] (fp16) = decoded page src_ids[i] of the fp8, int8 or (scales None) 4-bit pool; dst_ids
     None means page i."""
+    if kv_pool.is_cuda:
+        done = _lib.calls().page_dequant(kv_pool, dst_pool, src_ids, dst_ids, scales, page_size, _stream())
+        if done is not None:
+            return _lib.check(done)
+    # (not a plain call)
     _dev_half("dst_pool", dst_pool)
     _, hkv, d, n_src, _ = pool_geometry(kv_pool, page_size)
     _, hkv_d, d_d, n_dst, _ = pool_geometry(dst_pool, page_size)
@@ -359,26 +369,16 @@ def decode_split_plan(batch: int, num_kv_heads: int, max_blocks: int,
     return max(1, (max_blocks + pps - 1) // pps), pps
 
 
-def int4_split_tokens(batch: int, num_kv_heads: int) -> int:
-    """Least tokens of a split of a decode step over 4-bit codes. Up to 256 (sequence, kv head) pairs, a compute unit has at
-    most one and shorter splits fill the device (8 sequences of 4096 tokens, 8 kv heads: splits of 1024 / 2048 / 4096 tokens
-    15.1 / 17.6 / 21.1 us); with more, splits only even out the lengths (8 kv heads, 40 of 16384
-    tokens: 144 / 122 / 115 us, 135 unsplit; 64 of them: 224 / 189 / 180 us, 170 unsplit)."""
-    return 1024 if batch * num_kv_heads <= 256 else 4096
-
-
 def int4_decode_splits(batch: int, num_kv_heads: int, max_pages: int, total_pages: Optional[int] = None,
                        page_size: int = PAGE_SIZE) -> tuple[int, int]:
     """(max_splits, min_pages_per_split) of a decode step over a 4-bit pool whose longest sequence has ``max_pages`` pages and
-    all of them together ``total_pages`` (None: as many for every sequence): as many splits as fill 256 compute units, but no
-    more than 16 where that makes them shorter than 4096 tokens, since their merge takes longer the more there are (one
-    sequence of 32768 tokens, 8 kv heads: 8 / 16 / 32 splits 24 / 19.5 / 22 us)."""
-    min_pages = max(1, int4_split_tokens(batch, num_kv_heads) // page_size)
-    most = min(-(-max_pages // min_pages), max(16, max_pages * page_size // 4096), 65535)
-    if batch * num_kv_heads <= 256:
-        total = batch * max_pages if total_pages is None else total_pages
-        most = min(most, 256 * max_pages // max(1, total * num_kv_heads))
-    return max(1, most), min_pages
+    all of them together ``total_pages`` (None: as many for every sequence). The second depends on ``batch``,
+    ``num_kv_heads`` and ``page_size`` only."""
+    least = ctypes.c_int32()
+    splits = _lib.load().litekv_paged_decode_int4_splits(batch, num_kv_heads, max_pages, -1 if total_pages is None else total_pages,
+                                                         page_size, ctypes.byref(least))
+    _need(splits > 0, f"no decode step has batch {batch}, {num_kv_heads} kv heads, {max_pages} pages of {page_size} tokens")
+    return splits, least.value
 
 
 def decode_workspace(batch: int, num_q_heads: int, max_splits: int, device) -> Optional[torch.Tensor]:
@@ -601,10 +601,10 @@ class DecodePlan:
     def set_schedule(self, splits: int) -> None:
         """0: balanced; otherwise the per-sequence schedule with that many splits per sequence
         (the partial-result buffer of several splits is allocated here, not at the launch). A step over 4-bit codes has
-        no balanced form: 0 is one split, and several are at least ``int4_split_tokens`` long."""
+        no balanced form: 0 is one split, and the least length of several is that of ``int4_decode_splits``."""
         if self.int4:
             splits = max(1, int(splits))
-            self.min_pages_per_split = max(1, int4_split_tokens(self.batch, self.num_kv_heads) // self.page_size)
+            self.min_pages_per_split = int4_decode_splits(self.batch, self.num_kv_heads, 1, page_size=self.page_size)[1]
         self.per_sequence = splits > 0
         self.splits = max(1, int(splits))
         if self.splits > 1:
@@ -851,8 +851,17 @@ def paged_decode(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tens
     ``k_new`` / ``v_new`` [B, Hkv, D] (splits schedule, both stages): the step's new token of every
     sequence is written at logical position seq_lens[b] - 1 by the same launch and attended.
     """
-    _dev_half("q", q)
     int4 = is_int4_pool(kv_pool)
+    if (int4 and q.is_cuda and out is None and workspace is None and num_splits is None and max_splits is None
+            and min_pages_per_split is None and chunks is None and plan is None and kv_scales is None and not shared_pages
+            and stage == "both" and (schedule is None or schedule == "splits")):
+        done = _lib.calls().paged_decode_int4(q, kv_pool, block_table, seq_lens, softmax_scale, page_size, k_new, v_new, _stream())
+        if done is not None:
+            if type(done) is int:
+                _lib.check(done)
+            return done
+    # (not a plain call)
+    _dev_half("q", q)
     if int4:
         _dev_int4_pool(kv_pool, kv_scales)
     elif not is_quantised_pool(kv_pool):
