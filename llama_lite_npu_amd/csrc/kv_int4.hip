@@ -6,6 +6,9 @@
 // which would move one element in some hundred over a code's border. The sum of squares is taken in fp64, where the order
 // of its additions does not show, and each product and sum behind it is rounded by itself (no contraction): codes next
 // to a border are then the same however a row's lanes are laid out.
+//
+// Bound by memory: 10366 tokens of 64 + 16 heads of 128 in 78 to 83 us, 5 TB/s of q read and written, k, v and the codes, which is
+// what a large copy reaches; a few tokens in 3.5 us, which is a launch.
 #include <type_traits>
 
 #include "common.h"
@@ -13,16 +16,15 @@
 
 namespace litekv {
 
-// Rows [0, num_q_heads) of a token are q's, the next num_kv_heads K's, then V's. num_q_heads 0: the append alone. TOK tokens a
-// lane, see qk_norm_rope_append_kernel.
-template <int L, int TOK>
+// Rows [0, num_q_heads) of a token are q's, the next num_kv_heads K's, then V's. num_q_heads 0: the append alone. A lane has 16 bytes of
+// one token (of two or four, with their loads ahead of the work: 1 to 3% longer for many rows, up to 70% for few).
+template <int L>
 __global__ __launch_bounds__(256) void int4_append_kernel(
     half_t *__restrict__ q, int64_t q_stride, const half_t *__restrict__ k, int64_t k_stride,
     const half_t *__restrict__ v, int64_t v_stride, const half_t *__restrict__ q_weight,
     const half_t *__restrict__ k_weight, const half_t *__restrict__ cos_rows,
     const half_t *__restrict__ sin_rows, int64_t cs_stride, const int32_t *__restrict__ slot_mapping,
-    uint8_t *__restrict__ pool, int64_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads, int64_t num_slots,
-    float eps) {
+    uint8_t *__restrict__ pool, int32_t num_q_heads, int32_t num_kv_heads, int64_t num_slots, float eps) {
 #pragma clang fp contract(off)
   constexpr int kDim = 8 * L;
   const int l = threadIdx.x & (L - 1);
@@ -31,114 +33,114 @@ __global__ __launch_bounds__(256) void int4_append_kernel(
   const bool is_v = r >= num_q_heads + num_kv_heads;
   const bool is_q = r < num_q_heads;
   const int head = is_q ? r : (is_v ? r - num_q_heads - num_kv_heads : r - num_q_heads);
-  int64_t token[TOK], slot[TOK];
-  bool live[TOK];
-  half8_t x[TOK], c[TOK], sn[TOK];
-#pragma unroll
-  for (int t = 0; t < TOK; ++t) {
-    token[t] = (int64_t)blockIdx.x * TOK + t;
-    live[t] = token[t] < num_tokens;
-    if (!live[t]) token[t] = num_tokens - 1;  // loads repeat the last token; nothing is stored
-    const half_t *src = is_q   ? q + token[t] * q_stride + (int64_t)head * kDim
-                        : is_v ? v + token[t] * v_stride + (int64_t)head * kDim
-                               : k + token[t] * k_stride + (int64_t)head * kDim;
-    x[t] = *(const half8_t *)(src + 8 * l);
-    slot[t] = slot_mapping[token[t]];
-    if (cos_rows != nullptr && !is_v) {
-      const int j = 8 * (l & (L / 2 - 1));  // the first D / 2 entries of a cos / sin row
-      c[t] = *(const half8_t *)(cos_rows + token[t] * cs_stride + j);
-      sn[t] = *(const half8_t *)(sin_rows + token[t] * cs_stride + j);
-    }
+  const int64_t token = blockIdx.x;
+  const half_t *src = is_q   ? q + token * q_stride + (int64_t)head * kDim
+                      : is_v ? v + token * v_stride + (int64_t)head * kDim
+                             : k + token * k_stride + (int64_t)head * kDim;
+  const half8_t x = *(const half8_t *)(src + 8 * l);
+  const int64_t slot = slot_mapping[token];
+  half8_t c = half8_t{0, 0, 0, 0, 0, 0, 0, 0}, sn = c, w = c;
+  if (cos_rows != nullptr && !is_v) {
+    const int j = 8 * (l & (L / 2 - 1));  // the first D / 2 entries of a cos / sin row
+    c = *(const half8_t *)(cos_rows + token * cs_stride + j);
+    sn = *(const half8_t *)(sin_rows + token * cs_stride + j);
   }
   const half_t *weight = is_q ? q_weight : k_weight;
-  half8_t w = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
   if (weight != nullptr && !is_v) w = *(const half8_t *)(weight + 8 * l);
 
+  float y[8];
 #pragma unroll
-  for (int t = 0; t < TOK; ++t) {
-    float y[8];
+  for (int i = 0; i < 8; ++i) y[i] = (float)x[i];
+  if (weight != nullptr && !is_v) {
+    double ss = 0.0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = (float)x[t][i];
-    if (weight != nullptr && !is_v) {
-      double ss = 0.0;
+    for (int i = 0; i < 8; ++i) ss = __builtin_fma((double)y[i], (double)y[i], ss);
+    ss = over_row<L>(ss, [](double a, double b) { return a + b; });
+    const double ms = ss * (1.0 / kDim) + (double)eps;
+    // 1 / sqrt(ms): the hardware's approximation, twice improved (one step leaves about 2^-50 of it)
+    double rs = __builtin_amdgcn_rsq(ms);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = __builtin_fma((double)y[i], (double)y[i], ss);
-      ss = over_row<L>(ss, [](double a, double b) { return a + b; });
-      const double ms = ss * (1.0 / kDim) + (double)eps;
-      // 1 / sqrt(ms): the hardware's approximation, twice improved (one step leaves about 2^-50 of it)
-      double rs = __builtin_amdgcn_rsq(ms);
-#pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        const double e = __builtin_fma(-ms * rs, rs, 1.0);
-        rs = __builtin_fma(0.5 * rs, e, rs);
-      }
-      const float rrms = (float)rs;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = y[i] * rrms * (float)w[i];
+    for (int step = 0; step < 2; ++step) {
+      const double e = __builtin_fma(-ms * rs, rs, 1.0);
+      rs = __builtin_fma(0.5 * rs, e, rs);
     }
-    if (cos_rows != nullptr && !is_v) {
-      // partner: element i + D / 2 for the first half of the row, i - D / 2 for the second
-      const float sign = l < L / 2 ? -1.0f : 1.0f;
-      float p[8];
+    const float rrms = (float)rs;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = half_a_row_away<L>(y[i]);
+    for (int i = 0; i < 8; ++i) y[i] = y[i] * rrms * (float)w[i];
+  }
+  if (cos_rows != nullptr && !is_v) {
+    // partner: element i + D / 2 for the first half of the row, i - D / 2 for the second
+    const float sign = l < L / 2 ? -1.0f : 1.0f;
+    float p[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float own = y[i] * (float)c[t][i], other = p[i] * (float)sn[t][i];
-        y[i] = own + sign * other;
-      }
+    for (int i = 0; i < 8; ++i) p[i] = half_a_row_away<L>(y[i]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float own = y[i] * (float)c[i], other = p[i] * (float)sn[i];
+      y[i] = own + sign * other;
     }
-    if (is_q) {
-      half8_t o;
+  }
+  if (is_q) {
+    half8_t o;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = (half_t)y[i];
-      if (live[t]) *(half8_t *)(q + token[t] * q_stride + (int64_t)head * kDim + 8 * l) = o;
-    } else {
-      const Int4Row row = int4_row<L>(y);
-      if (live[t] && slot[t] >= 0 && slot[t] < num_slots) {
-        int4_store<kDim>(pool, slot[t], num_kv_heads, is_v ? num_kv_heads + head : head, l, row);
-      }
+    for (int i = 0; i < 8; ++i) o[i] = (half_t)y[i];
+    *(half8_t *)(q + token * q_stride + (int64_t)head * kDim + 8 * l) = o;
+  } else {
+    const Int4Row row = int4_row<L>(y);
+    if (slot >= 0 && slot < num_slots) {
+      int4_store<kDim>(pool, slot, num_kv_heads, is_v ? num_kv_heads + head : head, l, row);
     }
   }
 }
 
 // Pages as fp16 [slots][2 * Hkv][D]: a lane makes 8 elements of a row, neighbouring lanes neighbouring ones, so that stores
-// are whole lines; a block's codes are read in pieces of 4 (K) and 2 bytes (V) that share lines.
+// are whole lines; a block's codes are read in pieces of 4 (K) and 2 bytes (V) that share lines. A lane has the loads of two rows in
+// flight: 4000 pages of 16 tokens, 8 heads of 128, in 82 us (4.0 TB/s read and written), 106 with one row, 78 with four, which takes
+// longer for few pages (40 of them: 3.0 / 3.0 / 3.6 us).
+constexpr int kDequant = 2;
 template <int D>
 __global__ __launch_bounds__(256) void page_dequant_int4_kernel(
     const uint8_t *__restrict__ src_pool, half_t *__restrict__ dst_pool, const int32_t *__restrict__ src_ids,
     const int32_t *__restrict__ dst_ids, int32_t kv_heads, int32_t page_size, int64_t num_src_pages,
     int64_t num_dst_pages, int32_t tiles) {
   const int64_t i = blockIdx.x / (uint32_t)tiles;
-  const int32_t item = (int32_t)(blockIdx.x - i * tiles) * 256 + (int32_t)threadIdx.x;
   constexpr int kPieces = D / 8;   // of a row
-  if (item >= page_size * 2 * kv_heads * kPieces) return;
+  constexpr int kRows = 256 / kPieces;
+  const int32_t row0 = (int32_t)(blockIdx.x - i * tiles) * (kDequant * kRows) + (int32_t)threadIdx.x / kPieces;
+  const int w = (int)threadIdx.x % kPieces;
+  const int32_t rows = page_size * 2 * kv_heads;
   const int64_t sp = src_ids[i];
   const int64_t dp = dst_ids ? (int64_t)dst_ids[i] : i;
   if (sp < 0 || sp >= num_src_pages || dp < 0 || dp >= num_dst_pages) return;
-  const int w = item % kPieces;
-  const int row = item / kPieces;
-  const int head = row % (2 * kv_heads);
-  const int in_page = row / (2 * kv_heads);
-  const int t = in_page & 15;
-  const uint8_t *block = src_pool + ((sp * page_size + in_page) >> 4) * int4_block_bytes(kv_heads, D);
-  const uint8_t *codes = block + int4_codes_at(head, D);
-  const uint32_t word = *(const uint16_t *)(block + int4_words_at(head, kv_heads, D) + 2 * t);
-  uint32_t x;
-  if (head < kv_heads) {
-    x = *(const uint32_t *)(codes + t * (D / 2) + 4 * w);
-  } else if constexpr (D == 128) {
-    x = *(const uint16_t *)(codes + int4_v_unit<D>(t, w, 0)) |
-        ((uint32_t)*(const uint16_t *)(codes + int4_v_unit<D>(t, w, 1)) << 16);
-  } else {
-    const uint32_t a = *(const uint16_t *)(codes + int4_v_unit<D>(t, 2 * w, 0));
-    const uint32_t b = *(const uint16_t *)(codes + int4_v_unit<D>(t, 2 * w + 1, 0));
-    // even elements down, odd ones up, as in int4_pack
-    x = (a & 0xfu) | ((a >> 4) & 0xf0u) | ((b & 0xfu) << 8) | ((b & 0xf00u) << 4) | ((a & 0xf0u) << 12) |
-        ((a & 0xf000u) << 8) | ((b & 0xf0u) << 20) | ((b & 0xf000u) << 16);
+  uint32_t x[kDequant], word[kDequant];
+#pragma unroll
+  for (int u = 0; u < kDequant; ++u) {
+    const int row = row0 + u * kRows < rows ? row0 + u * kRows : rows - 1;   // (of the page, [slot][head])
+    const int head = row % (2 * kv_heads);
+    const int in_page = row / (2 * kv_heads);
+    const int t = in_page & 15;
+    const uint8_t *block = src_pool + ((sp * page_size + in_page) >> 4) * int4_block_bytes(kv_heads, D);
+    const uint8_t *codes = block + int4_codes_at(head, D);
+    word[u] = *(const uint16_t *)(block + int4_words_at(head, kv_heads, D) + 2 * t);
+    if (head < kv_heads) {
+      x[u] = *(const uint32_t *)(codes + t * (D / 2) + 4 * w);
+    } else if constexpr (D == 128) {
+      x[u] = *(const uint16_t *)(codes + int4_v_unit<D>(t, w, 0)) |
+             ((uint32_t)*(const uint16_t *)(codes + int4_v_unit<D>(t, w, 1)) << 16);
+    } else {
+      const uint32_t a = *(const uint16_t *)(codes + int4_v_unit<D>(t, 2 * w, 0));
+      const uint32_t b = *(const uint16_t *)(codes + int4_v_unit<D>(t, 2 * w + 1, 0));
+      // even elements down, odd ones up, as in int4_pack
+      x[u] = (a & 0xfu) | ((a >> 4) & 0xf0u) | ((b & 0xfu) << 8) | ((b & 0xf00u) << 4) | ((a & 0xf0u) << 12) |
+             ((a & 0xf000u) << 8) | ((b & 0xf0u) << 20) | ((b & 0xf000u) << 16);
+    }
   }
-  const half8_t y = int4x8_to_half(x, word | (word << 16));
-  *(half8_t *)(dst_pool + ((dp * page_size + in_page) * (int64_t)(2 * kv_heads) + head) * D + 8 * w) = y;
+#pragma unroll
+  for (int u = 0; u < kDequant; ++u) {
+    if (row0 + u * kRows >= rows) return;
+    const half8_t y = int4x8_to_half(x[u], word[u] | (word[u] << 16));
+    *(half8_t *)(dst_pool + (dp * rows + row0 + u * kRows) * D + 8 * w) = y;
+  }
 }
 
 static int launch_int4_append(const char *what, void *q, int64_t q_token_stride, const void *k,
@@ -177,19 +179,19 @@ static int launch_int4_append(const char *what, void *q, int64_t q_token_stride,
   const int rows_per_wg = 256 / (head_dim / 8);
   const int row_blocks = (num_q_heads + 2 * num_kv_heads + rows_per_wg - 1) / rows_per_wg;
   LITEKV_REQUIRE(row_blocks <= 65535, "%s: too many heads", what);
-  auto launch = [&](auto kernel, int tok) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((num_tokens + tok - 1) / tok), (unsigned)row_blocks), dim3(256), 0,
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)num_tokens, (unsigned)row_blocks), dim3(256), 0,
                        static_cast<hipStream_t>(stream), static_cast<half_t *>(q), q_token_stride,
                        static_cast<const half_t *>(k), k_token_stride, static_cast<const half_t *>(v), v_token_stride,
                        static_cast<const half_t *>(q_norm_weight), static_cast<const half_t *>(k_norm_weight),
                        static_cast<const half_t *>(cos_rows), static_cast<const half_t *>(sin_rows),
-                       cos_sin_token_stride, slot_mapping, static_cast<uint8_t *>(kv_pool), (int64_t)num_tokens,
-                       num_q_heads, num_kv_heads, num_slots, rms_eps);
+                       cos_sin_token_stride, slot_mapping, static_cast<uint8_t *>(kv_pool), num_q_heads, num_kv_heads,
+                       num_slots, rms_eps);
   };
   if (head_dim == 64) {
-    launch(int4_append_kernel<8, 1>, 1);
+    launch(int4_append_kernel<8>);
   } else {
-    launch(int4_append_kernel<16, 1>, 1);
+    launch(int4_append_kernel<16>);
   }
   return check_launch(what);
 }
@@ -240,7 +242,7 @@ extern "C" int litekv_page_dequant_int4(const void *kv_pool_int4, void *dst_pool
   LITEKV_REQUIRE(dst_ids != nullptr || n <= num_dst_pages,
                  "page_dequant_int4: %d pages do not fit a destination of %lld", n, (long long)num_dst_pages);
   const int64_t items = (int64_t)page_size * 2 * num_kv_heads * (head_dim / 8);
-  const int64_t tiles = (items + 255) / 256;
+  const int64_t tiles = (items + 256 * kDequant - 1) / (256 * kDequant);
   LITEKV_REQUIRE(items <= 0x7fffffffLL && tiles * n <= 0x7fffffffLL,
                  "page_dequant_int4: %d pages are too many for one launch", n);
   auto launch = [&](auto kernel) {
