@@ -796,7 +796,11 @@ int litekv_paged_prefill_int8(const void *q, int64_t q_token_stride,
  * depends on batch, num_kv_heads and page_size only. 0 for arguments that no step has.
  *
  * litekv_paged_prefill_int4: litekv_paged_prefill_bounded over a 4-bit pool (key_slices 1), or
- * litekv_paged_prefill_split (key_slices 2 .. 8, with its workspace; max_kv_len is then not read).
+ * litekv_paged_prefill_split (key_slices 2 .. 8, with its workspace). With a workspace (16-byte aligned) of
+ * litekv_paged_prefill_int4_workspace_bytes, which counts those partial rows in, a launch whose keys are attended by
+ * several blocks of rows decodes them into it once, max_kv_len tokens a sequence: with such a workspace no
+ * sequence may have more keys (those past it are not attended). max_kv_len 0, or a smaller workspace: every block
+ * of rows decodes for itself. The results are the same to the rounding of the sums' order.
  */
 int litekv_kv_append_int4(const void *k, const void *v, int64_t k_token_stride,
                           int64_t v_token_stride, const int32_t *slot_mapping,
@@ -829,6 +833,11 @@ int litekv_paged_decode_int4(const void *q, int64_t q_batch_stride, void *kv_poo
                              int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                              int32_t page_size, int64_t num_pages, int32_t max_splits,
                              int32_t min_pages_per_split, float softmax_scale, void *stream);
+
+size_t litekv_paged_prefill_int4_workspace_bytes(int32_t batch, int32_t num_q_heads,
+                                                 int32_t num_kv_heads, int32_t head_dim,
+                                                 int32_t max_q_len, int64_t max_kv_len,
+                                                 int64_t num_tokens, int32_t key_slices);
 
 int litekv_paged_prefill_int4(const void *q, int64_t q_token_stride, const void *kv_pool_int4,
                               const int32_t *block_table, int32_t block_table_stride,

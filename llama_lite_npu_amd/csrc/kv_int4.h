@@ -38,6 +38,13 @@ __host__ __device__ constexpr int int4_codes_at(int head, int d) { return head *
 __host__ __device__ constexpr int int4_words_at(int head, int kv_heads, int d) {
   return 2 * kv_heads * 8 * d + head * 2 * kInt4Block;
 }
+// The keys of a prefill launch decoded once (see kv_int4.hip): fp16 pages of kInt4StagePage tokens and their block table.
+constexpr int kInt4StagePage = 256;
+int launch_int4_stage(const char *what, const void *pool, void *staged, int32_t *staged_table, const int32_t *block_table,
+                      int32_t block_table_stride, const int32_t *cu_q_lens, const int32_t *context_lens, int32_t batch,
+                      int32_t num_kv_heads, int32_t head_dim, int32_t page_shift, int64_t num_pages, int64_t capacity,
+                      void *stream);
+
 // Inside a V head's codes: unit e of column c of row t (two bytes).
 template <int D>
 __device__ __forceinline__ int int4_v_unit(int t, int c, int e) {

@@ -93,54 +93,104 @@ __global__ __launch_bounds__(256) void int4_append_kernel(
   }
 }
 
-// Pages as fp16 [slots][2 * Hkv][D]: a lane makes 8 elements of a row, neighbouring lanes neighbouring ones, so that stores
-// are whole lines; a block's codes are read in pieces of 4 (K) and 2 bytes (V) that share lines. A lane has the loads of two rows in
-// flight: 4000 pages of 16 tokens, 8 heads of 128, in 82 us (4.0 TB/s read and written), 106 with one row, 78 with four, which takes
-// longer for few pages (40 of them: 3.0 / 3.0 / 3.6 us).
-constexpr int kDequant = 2;
+// Tokens as fp16 [slots][2 * Hkv][D]. A lane makes 8 elements of four consecutive tokens' rows of a head, neighbouring lanes
+// neighbouring elements and heads, so that stores are whole lines; the four rows' codes are four dwords of K and one load of
+// V, whose column holds them together. This is workgroup `tile` of those that take `tokens` slots from `block` on (the first of a block).
+template <int D>
+__device__ __forceinline__ void int4_to_half(const uint8_t *block, half_t *dst, int32_t kv_heads, int32_t tokens, int32_t tile) {
+  constexpr int kPieces = D / 8;   // of a row
+  const int32_t item = tile * 256 + (int32_t)threadIdx.x;
+  const int w = item % kPieces, row = item / kPieces;
+  const int quad = row / (2 * kv_heads), head = row - quad * (2 * kv_heads);
+  if (quad >= tokens / 4) return;
+  const int g = quad & 3;
+  const uint8_t *at = block + (int64_t)(quad >> 2) * int4_block_bytes(kv_heads, D);
+  const uint8_t *codes = at + int4_codes_at(head, D);
+  const uint2_t words = *(const uint2_t *)(at + int4_words_at(head, kv_heads, D) + 8 * g);
+  half8_t y[4];
+  auto twice = [&](int i) { return __builtin_amdgcn_perm(0u, words[i >> 1], i & 1 ? 0x03020302u : 0x01000100u); };
+  if (head < kv_heads) {
+    uint32_t x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *(const uint32_t *)(codes + (4 * g + i) * (D / 2) + 4 * w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = int4x8_to_half(x[i], twice(i));
+  } else {
+    const uint4_t x = *(const uint4_t *)(codes + g * (2 * D) + 16 * w);
+    if constexpr (D == 128) {   // column w: two units of rows 4g, 4g + 1, then of 4g + 2, 4g + 3
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t c = __builtin_amdgcn_perm(x[2 * (i >> 1) + 1], x[2 * (i >> 1)], i & 1 ? 0x07060302u : 0x05040100u);
+        y[i] = int4x8_to_half(c, twice(i));
+      }
+    } else {                    // columns 2w, 2w + 1: four elements of two rows at once, each row's under its own scale
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const half8_t left = int4x8_to_half(x[p], words[p]), right = int4x8_to_half(x[2 + p], words[p]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          y[2 * p + i] = half8_t{left[i], left[2 + i], left[4 + i], left[6 + i], right[i], right[2 + i], right[4 + i], right[6 + i]};
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *(half8_t *)(dst + ((int64_t)(4 * quad + i) * (2 * kv_heads) + head) * D + 8 * w) = y[i];
+}
+
 template <int D>
 __global__ __launch_bounds__(256) void page_dequant_int4_kernel(
     const uint8_t *__restrict__ src_pool, half_t *__restrict__ dst_pool, const int32_t *__restrict__ src_ids,
     const int32_t *__restrict__ dst_ids, int32_t kv_heads, int32_t page_size, int64_t num_src_pages,
     int64_t num_dst_pages, int32_t tiles) {
   const int64_t i = blockIdx.x / (uint32_t)tiles;
-  constexpr int kPieces = D / 8;   // of a row
-  constexpr int kRows = 256 / kPieces;
-  const int32_t row0 = (int32_t)(blockIdx.x - i * tiles) * (kDequant * kRows) + (int32_t)threadIdx.x / kPieces;
-  const int w = (int)threadIdx.x % kPieces;
-  const int32_t rows = page_size * 2 * kv_heads;
   const int64_t sp = src_ids[i];
   const int64_t dp = dst_ids ? (int64_t)dst_ids[i] : i;
   if (sp < 0 || sp >= num_src_pages || dp < 0 || dp >= num_dst_pages) return;
-  uint32_t x[kDequant], word[kDequant];
-#pragma unroll
-  for (int u = 0; u < kDequant; ++u) {
-    const int row = row0 + u * kRows < rows ? row0 + u * kRows : rows - 1;   // (of the page, [slot][head])
-    const int head = row % (2 * kv_heads);
-    const int in_page = row / (2 * kv_heads);
-    const int t = in_page & 15;
-    const uint8_t *block = src_pool + ((sp * page_size + in_page) >> 4) * int4_block_bytes(kv_heads, D);
-    const uint8_t *codes = block + int4_codes_at(head, D);
-    word[u] = *(const uint16_t *)(block + int4_words_at(head, kv_heads, D) + 2 * t);
-    if (head < kv_heads) {
-      x[u] = *(const uint32_t *)(codes + t * (D / 2) + 4 * w);
-    } else if constexpr (D == 128) {
-      x[u] = *(const uint16_t *)(codes + int4_v_unit<D>(t, w, 0)) |
-             ((uint32_t)*(const uint16_t *)(codes + int4_v_unit<D>(t, w, 1)) << 16);
-    } else {
-      const uint32_t a = *(const uint16_t *)(codes + int4_v_unit<D>(t, 2 * w, 0));
-      const uint32_t b = *(const uint16_t *)(codes + int4_v_unit<D>(t, 2 * w + 1, 0));
-      // even elements down, odd ones up, as in int4_pack
-      x[u] = (a & 0xfu) | ((a >> 4) & 0xf0u) | ((b & 0xfu) << 8) | ((b & 0xf00u) << 4) | ((a & 0xf0u) << 12) |
-             ((a & 0xf000u) << 8) | ((b & 0xf0u) << 20) | ((b & 0xf000u) << 16);
-    }
+  int4_to_half<D>(src_pool + (sp * (page_size / kInt4Block)) * int4_block_bytes(kv_heads, D),
+                  dst_pool + dp * page_size * (int64_t)(2 * kv_heads) * D, kv_heads, page_size, (int32_t)(blockIdx.x - i * tiles));
+}
+
+// The keys of a prefill launch as fp16 pages of kInt4StagePage tokens, `capacity` tokens a sequence (a multiple of that), and
+// their block table. A workgroup has part `x % tiles` of block x / tiles of sequence y.
+template <int D>
+__global__ __launch_bounds__(256) void int4_stage_kernel(
+    const uint8_t *__restrict__ pool, half_t *__restrict__ staged, int32_t *__restrict__ staged_table,
+    const int32_t *__restrict__ block_table, int32_t bt_stride, const int32_t *__restrict__ cu_q_lens,
+    const int32_t *__restrict__ context_lens, int32_t kv_heads, int32_t page_shift, int32_t num_pages, int32_t capacity,
+    int32_t tiles) {
+  const int b = (int)blockIdx.y, p = (int)blockIdx.x / tiles, tile = (int)blockIdx.x - p * tiles;
+  constexpr int kBlocks = kInt4StagePage / kInt4Block;
+  const int64_t page = ((int64_t)b * capacity) / kInt4StagePage + p / kBlocks;
+  if (tile == 0 && p % kBlocks == 0 && threadIdx.x == 0) staged_table[page] = (int32_t)page;
+  const int at = p >> page_shift;
+  const int entry = as_uniform(block_table)[(int64_t)b * bt_stride + (at < bt_stride ? at : bt_stride - 1)];
+  const int rows = as_uniform(cu_q_lens)[b + 1] - as_uniform(cu_q_lens)[b];
+  const int64_t keys = (int64_t)rows + (context_lens != nullptr ? as_uniform(context_lens)[b] : 0);
+  if (rows <= 0 || (int64_t)p * kInt4Block >= keys) return;
+  int4_to_half<D>(pool + (int64_t)sub_page_id(entry, p, page_shift, num_pages) * int4_block_bytes(kv_heads, D),
+                  staged + ((int64_t)b * capacity + (int64_t)p * kInt4Block) * (2 * kv_heads) * D, kv_heads, kInt4Block, tile);
+}
+
+int launch_int4_stage(const char *what, const void *pool, void *staged, int32_t *staged_table, const int32_t *block_table,
+                      int32_t block_table_stride, const int32_t *cu_q_lens, const int32_t *context_lens, int32_t batch,
+                      int32_t num_kv_heads, int32_t head_dim, int32_t page_shift, int64_t num_pages, int64_t capacity,
+                      void *stream) {
+  const int64_t tiles = ((int64_t)(kInt4Block / 4) * 2 * num_kv_heads * (head_dim / 8) + 255) / 256;
+  const int64_t blocks = capacity / kInt4Block * tiles;
+  LITEKV_REQUIRE(batch <= 65535 && blocks <= 0x7fffffffLL, "%s: too many keys to stage", what);
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, (unsigned)batch), dim3(256), 0, static_cast<hipStream_t>(stream),
+                       static_cast<const uint8_t *>(pool), static_cast<half_t *>(staged), staged_table, block_table,
+                       block_table_stride, cu_q_lens, context_lens, num_kv_heads, page_shift, (int32_t)num_pages,
+                       (int32_t)capacity, (int32_t)tiles);
+  };
+  if (head_dim == 64) {
+    launch(int4_stage_kernel<64>);
+  } else {
+    launch(int4_stage_kernel<128>);
   }
-#pragma unroll
-  for (int u = 0; u < kDequant; ++u) {
-    if (row0 + u * kRows >= rows) return;
-    const half8_t y = int4x8_to_half(x[u], word[u] | (word[u] << 16));
-    *(half8_t *)(dst_pool + (dp * rows + row0 + u * kRows) * D + 8 * w) = y;
-  }
+  return check_launch(what);
 }
 
 static int launch_int4_append(const char *what, void *q, int64_t q_token_stride, const void *k,
@@ -241,8 +291,8 @@ extern "C" int litekv_page_dequant_int4(const void *kv_pool_int4, void *dst_pool
   LITEKV_REQUIRE(num_src_pages > 0 && num_dst_pages > 0, "page_dequant_int4: empty pool");
   LITEKV_REQUIRE(dst_ids != nullptr || n <= num_dst_pages,
                  "page_dequant_int4: %d pages do not fit a destination of %lld", n, (long long)num_dst_pages);
-  const int64_t items = (int64_t)page_size * 2 * num_kv_heads * (head_dim / 8);
-  const int64_t tiles = (items + 256 * kDequant - 1) / (256 * kDequant);
+  const int64_t items = (int64_t)(page_size / 4) * 2 * num_kv_heads * (head_dim / 8);
+  const int64_t tiles = (items + 255) / 256;
   LITEKV_REQUIRE(items <= 0x7fffffffLL && tiles * n <= 0x7fffffffLL,
                  "page_dequant_int4: %d pages are too many for one launch", n);
   auto launch = [&](auto kernel) {

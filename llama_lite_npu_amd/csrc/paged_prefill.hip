@@ -608,6 +608,46 @@ extern "C" int litekv_paged_prefill_int8(const void *q, int64_t q_token_stride, 
                                       litekv::kKvInt8, litekv::PrefillKeySplit{});
 }
 
+// Where the keys of a launch over 4-bit codes lie as fp16, in its workspace behind the partial rows of its key slices. Decoded once
+// they cost a launch and their bytes, some 14 us for 33 MB; decoded by every block of rows, a third of its tile loop. 512
+// rows over 7601 tokens, 64 / 8 heads: 172 -> 151 us (fp16 pool: 129 to 135); 8 prompts of 128 to 2048 tokens 263 -> 241 (225 to
+// 235); four chunks of up to 512 over up to 8000, 32 / 8 heads of 64, 163 -> 128 (107); 16 prompts of 1024 118 -> 109. With fewer blocks:
+// 128 rows over 4000, 64 / 8 heads (8 blocks), 44.7 -> 45.2; 32 / 8 heads (4 blocks), 26.7 -> 33.9; 8 prompts of 512, 32 / 8 heads
+// (16 blocks, a key attended by 8 on the average), 43.5 -> 45.2. Up to 1 GiB: a cache in 4 bits is there to save memory.
+struct Int4Staging {
+  int64_t capacity = 0;   // tokens of a sequence, 0: they are decoded where they are attended
+  size_t table_at = 0, pool_at = 0, bytes = 0;
+};
+static Int4Staging int4_staging(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_q_len,
+                                int64_t max_kv_len, int64_t num_tokens, int32_t key_slices) {
+  Int4Staging s;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  s.table_at = up(litekv_paged_prefill_split_workspace_bytes(num_tokens, num_q_heads, head_dim, key_slices));
+  s.bytes = s.table_at;
+  if (batch < 1 || batch > 65535 || num_kv_heads < 1 || num_kv_heads > 1024 || num_q_heads < num_kv_heads || max_q_len < 1 ||
+      max_kv_len < 1 || max_kv_len > 0x3fffffff) {
+    return s;
+  }
+  // Blocks of rows that attend a key, on the average (a chunk's own keys by half of its blocks)
+  const double blocks = (double)(((int64_t)(num_q_heads / num_kv_heads) * max_q_len + 127) / 128);
+  const double visits = blocks * (1.0 - 0.5 * std::min<double>(1.0, (double)max_q_len / (double)max_kv_len));
+  if (visits < 12.0) return s;
+  const int64_t capacity = (max_kv_len + litekv::kInt4StagePage - 1) / litekv::kInt4StagePage * litekv::kInt4StagePage;
+  const double bytes = (double)batch * (double)capacity * 4.0 * num_kv_heads * head_dim;
+  if (bytes > 1073741824.0) return s;
+  s.capacity = capacity;
+  s.pool_at = s.table_at + up((size_t)batch * (size_t)(capacity / litekv::kInt4StagePage) * sizeof(int32_t));
+  s.bytes = s.pool_at + (size_t)bytes;
+  return s;
+}
+
+extern "C" size_t litekv_paged_prefill_int4_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                                            int32_t head_dim, int32_t max_q_len, int64_t max_kv_len,
+                                                            int64_t num_tokens, int32_t key_slices) {
+  if (!litekv::int4_head_dim(head_dim)) return 0;
+  return int4_staging(batch, num_q_heads, num_kv_heads, head_dim, max_q_len, max_kv_len, num_tokens, key_slices).bytes;
+}
+
 extern "C" int litekv_paged_prefill_int4(const void *q, int64_t q_token_stride, const void *kv_pool_int4,
                                          const int32_t *block_table, int32_t block_table_stride,
                                          const int32_t *cu_q_lens, const int32_t *context_lens,
@@ -617,17 +657,40 @@ extern "C" int litekv_paged_prefill_int4(const void *q, int64_t q_token_stride, 
                                          int64_t max_kv_len, int64_t num_tokens, int32_t key_slices,
                                          void *workspace, size_t workspace_bytes, float softmax_scale,
                                          void *stream) {
-  LITEKV_REQUIRE(litekv::int4_head_dim(head_dim), "paged_prefill_int4: head_dim %d unsupported (64 or 128)", head_dim);
-  litekv::PrefillKeySplit split;
+  using namespace litekv;
+  const char *what = "paged_prefill_int4";
+  LITEKV_REQUIRE(int4_head_dim(head_dim), "%s: head_dim %d unsupported (64 or 128)", what, head_dim);
+  PrefillKeySplit split;
   split.key_slices = key_slices;
   split.workspace = workspace;
   split.workspace_bytes = workspace_bytes;
   split.num_tokens = num_tokens;
   split.max_kv_len = max_kv_len;
-  return litekv::launch_paged_prefill("paged_prefill_int4", q, q_token_stride, kv_pool_int4, nullptr, block_table,
-                                      block_table_stride, cu_q_lens, context_lens, out, out_token_stride, batch,
-                                      num_q_heads, num_kv_heads, head_dim, page_size, num_pages, max_q_len,
-                                      softmax_scale, stream, litekv::kKvInt4, split);
+  int format = kKvInt4;
+  const Int4Staging s = int4_staging(batch, num_q_heads, num_kv_heads, head_dim, max_q_len, max_kv_len, num_tokens, key_slices);
+  if (s.capacity > 0 && workspace != nullptr && workspace_bytes >= s.bytes) {
+    const int page_shift = page_shift_of(page_size);
+    LITEKV_REQUIRE(page_shift >= 0, "%s: page_size %d unsupported (16, 32, 64, 128 or 256)", what, page_size);
+    LITEKV_REQUIRE(kv_pool_int4 && block_table && cu_q_lens, "%s: null pointer", what);
+    LITEKV_REQUIRE(aligned16(kv_pool_int4) && aligned16(workspace), "%s: kv_pool and workspace must be 16-byte aligned", what);
+    LITEKV_REQUIRE(block_table_stride >= 1, "%s: block_table_stride %d < 1", what, block_table_stride);
+    LITEKV_REQUIRE(num_pages >= 1 && num_pages <= 0x7fffffffLL / page_size, "%s: num_pages %lld out of range", what,
+                   (long long)num_pages);
+    char *base = static_cast<char *>(workspace);
+    int32_t *table = reinterpret_cast<int32_t *>(base + s.table_at);
+    const int rc = launch_int4_stage(what, kv_pool_int4, base + s.pool_at, table, block_table, block_table_stride, cu_q_lens,
+                                     context_lens, batch, num_kv_heads, head_dim, page_shift, num_pages, s.capacity, stream);
+    if (rc != LITEKV_OK) return rc;
+    kv_pool_int4 = base + s.pool_at;
+    block_table = table;
+    block_table_stride = (int32_t)(s.capacity / kInt4StagePage);
+    page_size = kInt4StagePage;
+    num_pages = batch * (s.capacity / kInt4StagePage);
+    format = kKvF16;
+  }
+  return launch_paged_prefill(what, q, q_token_stride, kv_pool_int4, nullptr, block_table, block_table_stride, cu_q_lens,
+                              context_lens, out, out_token_stride, batch, num_q_heads, num_kv_heads, head_dim, page_size,
+                              num_pages, max_q_len, softmax_scale, stream, format, split);
 }
 
 extern "C" int litekv_varlen_prefill(const void *q, int64_t q_token_stride, const void *k,

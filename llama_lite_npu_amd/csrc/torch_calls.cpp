@@ -214,10 +214,13 @@ PyObject *paged_prefill(PyObject *, PyObject *const *a, Py_ssize_t n) {
     at::Tensor out = at::empty({t, hq, d}, q->options());
     at::Tensor partials;
     size_t partial_bytes = 0;
-    if (slices > 1) {
+    if (pool.format == kInt4) {
+      partial_bytes = litekv_paged_prefill_int4_workspace_bytes((int32_t)b, (int32_t)hq, (int32_t)pool.hkv, (int32_t)d,
+                                                                (int32_t)max_q, max_kv, t, slices);
+    } else if (slices > 1) {
       partial_bytes = litekv_paged_prefill_split_workspace_bytes(t, (int32_t)hq, (int32_t)d, slices);
-      partials = at::empty({(int64_t)(partial_bytes / sizeof(float))}, q->options().dtype(at::kFloat));
     }
+    if (partial_bytes > 0) partials = at::empty({(int64_t)(partial_bytes / sizeof(float))}, q->options().dtype(at::kFloat));
     const void *qp = address(q), *pp = address(pool.t);
     const int32_t *tp = static_cast<const int32_t *>(address(table)), *cup = static_cast<const int32_t *>(address(cu));
     const int32_t *ctxp = static_cast<const int32_t *>(address(ctx));
@@ -226,7 +229,7 @@ PyObject *paged_prefill(PyObject *, PyObject *const *a, Py_ssize_t n) {
     PyObject *result = THPVariable_Wrap(std::move(out));  // (before the launch: it may throw)
     const int32_t ts = (int32_t)table->stride(0);
     const int64_t pages = pool.slots / page;
-    void *wp = slices > 1 ? partials.data_ptr() : nullptr;
+    void *wp = partial_bytes > 0 ? partials.data_ptr() : nullptr;
     const int rc = unlocked([&] {
       if (pool.format == kInt4) {
         return litekv_paged_prefill_int4(qp, qs, pp, tp, ts, cup, ctxp, op, hq * d, (int32_t)b, (int32_t)hq, (int32_t)pool.hkv,

@@ -1068,17 +1068,23 @@ def paged_prefill(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Ten
     key_slices = int(key_slices)
     if key_slices > 1:
         need = paged_prefill_workspace_floats(t, hq, d, key_slices)
-        if workspace is None:
+        if workspace is None and not int4:
             workspace = torch.empty(need, dtype=torch.float32, device=q.device)
-        if not (workspace.is_cuda and workspace.dtype == torch.float32
-                and workspace.is_contiguous() and workspace.numel() >= need):
+        if workspace is not None and not (workspace.is_cuda and workspace.dtype == torch.float32
+                                          and workspace.is_contiguous() and workspace.numel() >= need):
             raise ValueError(f"workspace must be {need} contiguous float32 on the device")
     if int4:
+        if workspace is None:
+            need = int(lib.litekv_paged_prefill_int4_workspace_bytes(b, hq, hkv, d, int(max_q_len), int(max_kv_len or 0), t,
+                                                                     max(1, key_slices))) // 4
+            workspace = torch.empty(need, dtype=torch.float32, device=q.device) if need > 0 else None
+        elif not (workspace.is_cuda and workspace.dtype == torch.float32 and workspace.is_contiguous()):
+            raise ValueError("workspace must be contiguous float32 on the device")
         _lib.check(lib.litekv_paged_prefill_int4(
             _ptr(q), q_stride, _ptr(kv_pool), _ptr(block_table), block_table.stride(0), _ptr(cu_q_lens),
             _ptr(context_lens), _ptr(out), _rows("out", out), b, hq, hkv, d, page_size, n_pages, int(max_q_len),
             0 if max_kv_len is None else int(max_kv_len), t, max(1, key_slices),
-            _ptr(workspace) if key_slices > 1 else None, workspace.numel() * 4 if key_slices > 1 else 0,
+            _ptr(workspace), 0 if workspace is None else workspace.numel() * 4,
             float(softmax_scale), _stream()))
         return out
     if key_slices <= 1:

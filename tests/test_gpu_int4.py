@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from llama_lite_npu_amd import ops
+from llama_lite_npu_amd import _lib, ops
 from oracle import int4
 
 pytestmark = pytest.mark.gpu
@@ -400,3 +400,55 @@ def test_refusals_on_the_gpu():
         with pytest.raises((ValueError, RuntimeError)):
             call()
             raise AssertionError(f"call {i} was taken")
+
+
+@pytest.mark.parametrize("hq,hkv,d,page,rows,history", [
+    (64, 8, 128, 16, [300], [2000]), (64, 8, 128, 64, [1, 0, 333, 260], [500, 20, 0, 77]), (32, 8, 64, 64, [513, 400], [1000, 30]),
+    (16, 2, 64, 256, [250, 1], [255, 256]), (48, 3, 128, 32, [129] * 5, [3, 700, 250, 251, 511])])
+def test_prefill_with_keys_decoded_once(hq, hkv, d, page, rows, history):
+    lib = _lib.load()
+    lens = [r + h if r else 0 for r, h in zip(rows, history)]
+    s = Sequences(lens, hq, hkv, d, page, seed=sum(rows))
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    q = half(s.rng, int(cu[-1]), hq, d)
+    picks = [sorted({0, r // 2, max(0, r - 2), r - 1}) if r else [] for r in rows]
+    of = lambda b: ([cu[b] + i for i in picks[b]], [history[b] + i + 1 for i in picks[b]])  # noqa: E731
+    args = (dev(q), dev(s.pool), dev(s.table), dev(cu, torch.int32), dev(np.array(history), torch.int32), max(rows), 1 / math.sqrt(d))
+    p_error = HALF + 2.0 ** -25 * max(lens)
+    for slices in (1, 3):
+        need = lib.litekv_paged_prefill_int4_workspace_bytes(len(rows), hq, hkv, d, max(rows), max(lens), len(q), slices) // 4
+        least = ops.paged_prefill_workspace_floats(len(q), hq, d, slices) if slices > 1 else 4
+        assert need > least + sum(lens) * hkv * d
+        outs = []
+        for floats in (need, least):           # decoded once; where they are attended
+            room = torch.full((floats,), math.nan, device=DEV)
+            out = ops.paged_prefill(*args, page_size=page, key_slices=slices, max_kv_len=max(lens), workspace=room)
+            check(out.cpu().numpy(), q, s, of, 1 / math.sqrt(d), p_error)
+            outs.append(out)
+        again = torch.full((need,), math.nan, device=DEV)
+        assert torch.equal(outs[0], ops.paged_prefill(*args, page_size=page, key_slices=slices, max_kv_len=max(lens), workspace=again))
+    out = ops.paged_prefill(*args, page_size=page, max_kv_len=max(lens) + 300)     # the lengths need only be bounded
+    check(out.cpu().numpy(), q, s, of, 1 / math.sqrt(d), p_error)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_native_calls_and_wrappers_agree(d):
+    """A plain call goes through native code, one with an argument of its own through the wrapper's."""
+    lens = [70, 1, 0, 333]
+    s = Sequences(lens, 16, 4, d, 16, seed=d)
+    q, kv = dev(half(s.rng, 4, 16, d)), dev(half(s.rng, 4, 8, d))
+    table, n = dev(s.table), dev(np.array(lens), torch.int32)
+    pools = [dev(s.pool) for _ in range(2)]
+    out = ops.paged_decode(q, pools[0], table, n, k_new=kv[:, :4], v_new=kv[:, 4:])
+    mine = torch.empty_like(q)
+    ops.paged_decode(q, pools[1], table, n, k_new=kv[:, :4], v_new=kv[:, 4:], out=mine)
+    assert torch.equal(out, mine) and torch.equal(*pools)
+    slots = dev(np.array([3, -1, 40, 17]), torch.int32)
+    ops.kv_append_quantised(kv[:, :4], kv[:, 4:], slots, pools[0])
+    ops.kv_append_quantised(kv[:, :4], kv[:, 4:], slots.long(), pools[1])       # (int64 slots: the wrapper converts them)
+    assert torch.equal(*pools)
+    a, b = (torch.full((s.pool.shape[0], 8, d), 3.0, dtype=torch.float16, device=DEV) for _ in range(2))
+    ids = torch.arange(s.pages, dtype=torch.int32, device=DEV).flip(0).contiguous()
+    ops.page_dequant(pools[0], a, ids, None, None)
+    ops.page_dequant(pools[0], b, ids.long(), None, None)
+    assert torch.equal(a.view(torch.int16), b.view(torch.int16))
