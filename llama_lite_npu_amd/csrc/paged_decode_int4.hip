@@ -503,7 +503,8 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
 // (8 sequences of 4096 tokens, 8 kv heads: splits of 1024 / 2048 / 4096 tokens 15.1 / 17.6 / 21.1 us). With more, splits only even out
 // the lengths (40 of 16384 tokens, 8 kv heads: 144 / 122 / 115 us, 135 unsplit; 64 of them: 224 / 189 / 180 us, 170 unsplit).
 // No more than 16 where that makes them shorter than 4096 tokens: their merge takes longer the more there are (one sequence of 32768
-// tokens, 8 kv heads: 8 / 16 / 32 splits 24 / 19.5 / 22 us).
+// tokens, 8 kv heads: 8 / 16 / 32 splits 24 / 19.5 / 22 us). Powers of two: a captured step holds their number, and growing
+// sequences should not ask for a new one every thousand tokens.
 extern "C" int32_t litekv_paged_decode_int4_splits(int32_t batch, int32_t num_kv_heads, int64_t max_pages, int64_t total_pages,
                                                    int32_t page_size, int32_t *min_pages_per_split) {
   using namespace litekv;
@@ -515,15 +516,15 @@ extern "C" int32_t litekv_paged_decode_int4_splits(int32_t batch, int32_t num_kv
   const bool few = pairs <= 256;
   const int64_t least = (few ? 1024 : 4096) / page_size;
   *min_pages_per_split = (int32_t)least;
-  int64_t most = (max_pages + least - 1) / least;
-  const int64_t merged = max_pages * page_size / 4096 > 16 ? max_pages * page_size / 4096 : 16;
-  if (most > merged) most = merged;
+  int64_t most = max_pages * page_size / 4096 > 16 ? max_pages * page_size / 4096 : 16;
   if (few) {
     const int64_t rows = total_pages < 0 ? pairs * max_pages : total_pages * num_kv_heads;   // of pages, a head's share each
     const int64_t fill = 256 * max_pages / (rows > 0 ? rows : 1);
     if (most > fill) most = fill;
   }
-  return most < 1 ? 1 : most > 65535 ? 65535 : (int32_t)most;
+  int64_t splits = 1;
+  while (2 * splits <= most && splits * least < max_pages && splits < 32768) splits *= 2;
+  return (int32_t)splits;
 }
 
 extern "C" int litekv_paged_decode_int4(const void *q, int64_t q_batch_stride, void *kv_pool_int4,

@@ -632,10 +632,16 @@ class DecodePlan:
             self.set_schedule(0)
             return self.per_sequence
         if self.int4:
-            splits = int4_decode_splits(self.batch, self.num_kv_heads, max(pages), sum(pages), self.page_size)[0]
-            # a batch that grows past a power of two does not flip back with the next length
-            if hysteresis > 1.0 and self.per_sequence and splits < self.splits and splits * 4 > self.splits:
-                splits = self.splits
+            def rule(longest: int) -> int:
+                total = min(sum(pages), self.batch * longest)
+                return int4_decode_splits(self.batch, self.num_kv_heads, longest, total, self.page_size)[0]
+            splits, longest = rule(max(pages)), max(pages)
+            if hysteresis > 1.0 and self.per_sequence:
+                # another number only where a longest sequence a little shorter (longer) than it is would have it too
+                if splits > self.splits:
+                    splits = max(self.splits, rule(max(1, int(longest / hysteresis))))
+                elif splits < self.splits:
+                    splits = min(self.splits, rule(int(longest * hysteresis) + 1))
             self.set_schedule(splits)
             return True
         # the rule is told what its defaults do not say

@@ -169,3 +169,36 @@ def test_refusals_of_the_wrappers():
                  lambda: ops.page_dequant(four, q, lens, None, None)):
         with pytest.raises(ValueError, match="must live on the GPU"):
             call()
+
+
+def test_splits_are_powers_of_two_that_hold_still():
+    """Growing sequences ask for a new number of splits (a new captured step) a handful of times, and never back and forth."""
+    for batch, hkv, start in ((1, 8, 1), (4, 2, 900), (12, 8, 100), (40, 8, 3000)):
+        seen = []
+        for tokens in range(start, 140000, 160):
+            splits, least = ops.int4_decode_splits(batch, hkv, -(-tokens // 16))
+            assert splits & (splits - 1) == 0 and (splits, least) == ops.int4_decode_splits(batch, hkv, -(-tokens // 16), batch * -(-tokens // 16))
+            assert splits == 1 or splits // 2 * least * 16 < tokens
+            seen.append(splits)
+        assert seen == sorted(seen) and seen[0] == 1 and len(set(seen)) <= 7
+    assert ops.int4_decode_splits(32, 8, 256)[0] == 1               # 256 pairs fill the device
+    # one long sequence among short ones
+    assert ops.int4_decode_splits(32, 8, 4096, 4096 + 31)[0] >= 8
+    for bad in ((-1, 8, 1, None, 16), (1, 0, 1, None, 16), (1, 8, 4, 5, 16), (1, 8, 1, None, 17), (1, 8, -1, None, 16)):
+        with pytest.raises(ValueError):
+            ops.int4_decode_splits(*bad)
+
+
+def test_prefill_workspace_holds_the_keys_where_they_are_decoded_once():
+    lib = _lib.load()
+
+    def room(b=1, hq=64, hkv=8, d=128, rows=512, kv=8113, tokens=512, slices=1):
+        return lib.litekv_paged_prefill_int4_workspace_bytes(b, hq, hkv, d, rows, kv, tokens, slices)
+
+    pages = -(-8113 // 256)
+    assert room() >= pages * 256 * 16 * 128 * 2 + 4 * pages
+    assert room(slices=4) >= room() + lib.litekv_paged_prefill_split_workspace_bytes(512, 64, 128, 4)
+    assert room(d=64, rows=1024) >= pages * 256 * 16 * 64 * 2 + 4 * pages
+    # few blocks of rows a key, lengths not known, more than 1 GiB of keys, heads of another size: the partial rows' alone, or nothing
+    assert room(rows=64) == room(kv=0) == room(kv=-1) == room(kv=300000) == room(d=96) == room(b=0) == 0
+    assert 0 < room(rows=64, slices=2) < 1 << 26
