@@ -26,10 +26,12 @@
 // The reference of the exponentials is the largest p s' so far, not the largest p: in fp16 it is p s' that has to fit. It is put
 // at 2^7 and may grow to 2^15 before the accumulators are rescaled.
 //
-// Bound: by vector instructions and the latency of the loads, then by memory. A step is 157 vector instructions for 32 keys and 8 heads
-// (D = 128), which leaves room for three wavefronts per SIMD with two steps' loads in flight each (147 registers; four with one
-// step's in flight took 3 to 10% longer). 64 sequences of 8192 tokens, 32 / 4 heads of 128: 48.5 us, 5.7 TB/s of cache read (a copy
-// reads and writes 5.0). Of its twelve wavefronts a compute unit holds one workgroup of eight or three of four. Eight are faster
+// Bound: by what one compute unit takes in, some 40 GB/s at one sequence per head (32768 tokens on 8 compute units: 104 us; neither more
+// loads in flight nor the scores of the next step beside the second product of this one make it faster), and by memory once
+// there are as many workgroups as compute units: 64 sequences of 8192 tokens, 32 / 4 heads of 128, take 47 us, 5.9 TB/s of cache read (a
+// large copy reads and writes 5.0). A step is 149 vector and 15 matrix instructions for 32 keys and 8 heads (D = 128); 146
+// registers leave room for three wavefronts per SIMD with two steps' loads in flight each (four with one step's took 3 to 40%
+// longer). Of its twelve wavefronts a compute unit holds one workgroup of eight or three of four. Eight are faster
 // while there are no more workgroups than compute units (the case above with four: 53 us; 20 sequences of 4096, 8 kv heads: 22.7
 // against 25), four where there are more (38 of them: 39 us against 44; 100 of 2048: 44 against 55). Streaming loads, whose lines
 // are the first to leave the caches, took 10% less than ordinary ones.
@@ -134,12 +136,17 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
 
   const int64_t block_bytes = int4_block_bytes(num_kv_heads, D);
   const uniform_i32_ptr table = as_uniform(block_table) + (int64_t)b * bt_stride;
-  // A length beyond what a block-table row can name re-reads the row's last entry; pages past the split's re-read its last.
-  auto page_id = [&](int p) {
+  // The block-table entry of a page, and the block it means. A length beyond what a row can name re-reads the row's last entry;
+  // pages past the wavefront's last re-read that.
+  auto place = [&](int p) {
     const int pp = p < p1 ? p : p1 - 1;
-    const int at = pp >> page_shift;
-    return sub_page_id(table[at < bt_stride ? at : bt_stride - 1], pp, page_shift, num_pages);
+    return pp > 0 ? pp : 0;
   };
+  auto entry_of = [&](int p) {
+    const int at = place(p) >> page_shift;
+    return table[at < bt_stride ? at : bt_stride - 1];
+  };
+  auto block_of = [&](int p, int entry) { return sub_page_id(entry, place(p), page_shift, num_pages); };
 
   // The step's new token goes into the last block before anything of it is read (by this wavefront, the only one that reads it
   // in this launch; the slices of a wide group all write the same bytes).
@@ -153,7 +160,7 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
       float x[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = (float)x16[i];
-      const int64_t slot = (int64_t)page_id(pages - 1) * kInt4Block + ((len - 1) & (kInt4Block - 1));
+      const int64_t slot = (int64_t)block_of(pages - 1, entry_of(pages - 1)) * kInt4Block + ((len - 1) & (kInt4Block - 1));
       int4_store<D>(pool, slot, num_kv_heads, is_v ? num_kv_heads + h : h, l, int4_row<L>(x));
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
@@ -167,8 +174,8 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   const uint32_t vw_off = (uint32_t)(int4_words_at(num_kv_heads + h, num_kv_heads, D) + 8 * g);
   // Loads of pages past the split's last name a buffer of no bytes: they return zeros and touch no memory, and the loop has the
   // same number of them in flight at every step, so that each wait covers the page it needs and no younger one.
-  auto request = [&](int p, int id, Int4Regs<D> &r) {
-    const auto block = __builtin_amdgcn_make_buffer_rsrc(pool + (int64_t)id * block_bytes, 0, p < p1 ? (int)block_bytes : 0,
+  auto request = [&](int p, int entry, Int4Regs<D> &r) {
+    const auto block = __builtin_amdgcn_make_buffer_rsrc(pool + (int64_t)block_of(p, entry) * block_bytes, 0, p < p1 ? (int)block_bytes : 0,
                                                          0x00020000);
     if constexpr (D == 128) {
       const uint4_t kk = __builtin_amdgcn_raw_buffer_load_b128(block, k_off, 0, kStreaming);
@@ -194,14 +201,15 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
     r.vw[0] = vw[0];
     r.vw[1] = vw[1];
   };
-  // Two blocks a step, kDepth steps' in flight; page ids are read a step before the requests that they are for.
+  // Two blocks a step, kDepth steps' in flight. Block-table entries are read a step before the requests that they are for, and not
+  // looked at before: a scalar load that is waited for on the spot cost every step its whole trip.
   Int4Regs<D> buf[kDepth][2];
-  int id0 = any ? page_id(p0) : 0, id1 = any ? page_id(p0 + 1) : 0;
+  int entry0 = entry_of(p0), entry1 = entry_of(p0 + 1);
   auto request_pair = [&](int p, Int4Regs<D> (&r)[2]) {
-    request(p, id0, r[0]);
-    request(p + 1, id1, r[1]);
-    id0 = any ? page_id(p + 2) : 0;
-    id1 = any ? page_id(p + 3) : 0;
+    request(p, entry0, r[0]);
+    request(p + 1, entry1, r[1]);
+    entry0 = entry_of(p + 2);
+    entry1 = entry_of(p + 3);
   };
 #pragma unroll
   for (int i = 0; i < kDepth; ++i) request_pair(p0 + 2 * i, buf[i]);
