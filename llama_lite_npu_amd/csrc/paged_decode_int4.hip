@@ -35,6 +35,12 @@
 // while there are no more workgroups than compute units (the case above with four: 53 us; 20 sequences of 4096, 8 kv heads: 22.7
 // against 25), four where there are more (38 of them: 39 us against 44; 100 of 2048: 44 against 55). Streaming loads, whose lines
 // are the first to leave the caches, took 10% less than ordinary ones.
+//
+// Around its keys a workgroup spends some 5 us, most of it one memory trip after another and the first run through its code: the
+// sequence's length, block-table entries, keys, the fold. So q, the first 64 entries of the table row and the new rows are
+// requested ahead of the length, q is converted once for the workgroup and not by every wavefront for itself (9.8 -> 8.2 us a launch
+// for one sequence of 778 tokens, 22.0 -> 20.4 for 32 of 256 to 4096), and the last, masked steps are one piece of code
+// (8.2 -> 7.6, with the fold's loads ahead of its arithmetic).
 #include <type_traits>
 
 #include "common.h"
@@ -43,6 +49,7 @@
 namespace litekv {
 
 typedef uint32_t uint2v_t __attribute__((ext_vector_type(2)));
+typedef float float2v_t __attribute__((ext_vector_type(2)));
 
 constexpr int kInt4Waves = 8;            // of a workgroup, at most
 constexpr float kInt4Top = 7.0f;         // log2 of where the largest p s' is put
@@ -116,6 +123,22 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   const HeadSlice hs = head_slice(at / turns, slices, group_all);
   const int share = (int)(blockDim.x >> 6), part = wave;   // the wavefronts attend a part of the split's keys each
   const int h = hs.kv_head, group = hs.q_heads, hq0 = hs.q_head0;
+  constexpr int L = D / 8;                 // lanes of a row, 8 elements each
+  constexpr int kHeads = TWO ? 16 : 8;     // rows of q (the last one again past the group)
+  // What does not depend on the sequence's length is requested ahead of it: rows of q, the first entries of the block-table row (one
+  // a lane), the step's new rows (K's in the first L lanes, V's in the next).
+  const int32_t *row_of_table = block_table + (int64_t)b * bt_stride;
+  const int first_entries = row_of_table[lane < bt_stride ? lane : bt_stride - 1];
+  half8_t q_in = half8_t{0, 0, 0, 0, 0, 0, 0, 0}, new_row = q_in;
+  if (wave < kHeads * L / kWave) {
+    const int head = (int)threadIdx.x / L;
+    q_in = *(const half8_t *)(q + (int64_t)b * q_batch_stride + (int64_t)(hq0 + (head < group ? head : group - 1)) * D +
+                              8 * (threadIdx.x % L));
+  }
+  if (k_new != nullptr) {
+    const half_t *src = lane & L ? v_new + (int64_t)b * v_new_stride : k_new + (int64_t)b * k_new_stride;
+    new_row = *(const half8_t *)(src + (int64_t)h * D + 8 * (lane & (L - 1)));
+  }
   const int len = as_uniform(seq_lens)[b];
   half_t *out_row = out + ((int64_t)b * num_q_heads + hq0) * D;
   if (len <= 0) {
@@ -130,37 +153,40 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   const int first = (int)(((int64_t)split * pages) / n_splits);
   const int last = (int)(((int64_t)(split + 1) * pages) / n_splits);
   const int steps = (last - first + 1) / 2;   // of two blocks
-  const int p0 = first + 2 * ((steps * part) / share);
-  const int p1 = part + 1 < share ? first + 2 * ((steps * (part + 1)) / share) : last;
+  // (the last wavefront, which has the new token and the keys to be masked, has no more of them than the others)
+  const int p0 = first + 2 * ((steps * part + share - 1) / share);
+  const int p1_even = first + 2 * ((steps * (part + 1) + share - 1) / share);
+  const int p1 = p1_even < last ? p1_even : last;
   const bool any = p0 < p1;   // (a wavefront without a part has nothing to add)
 
   const int64_t block_bytes = int4_block_bytes(num_kv_heads, D);
-  const uniform_i32_ptr table = as_uniform(block_table) + (int64_t)b * bt_stride;
   // The block-table entry of a page, and the block it means. A length beyond what a row can name re-reads the row's last entry;
   // pages past the wavefront's last re-read that.
   auto place = [&](int p) {
     const int pp = p < p1 ? p : p1 - 1;
     return pp > 0 ? pp : 0;
   };
-  auto entry_of = [&](int p) {
+  auto entry_at = [&](int p) {
     const int at = place(p) >> page_shift;
-    return table[at < bt_stride ? at : bt_stride - 1];
+    return at < bt_stride ? at : bt_stride - 1;
+  };
+  auto entry_of = [&](int p) { return as_uniform(row_of_table)[entry_at(p)]; };
+  auto first_entry_of = [&](int p) {   // from the registers where it is there
+    const int at = entry_at(p);
+    return at < kWave ? __builtin_amdgcn_readlane(first_entries, at) : entry_of(p);
   };
   auto block_of = [&](int p, int entry) { return sub_page_id(entry, place(p), page_shift, num_pages); };
 
   // The step's new token goes into the last block before anything of it is read (by this wavefront, the only one that reads it
   // in this launch; the slices of a wide group all write the same bytes).
   if (k_new != nullptr && any && p1 == pages && pages <= (bt_stride << page_shift)) {
-    constexpr int L = D / 8;
     if (lane < 2 * L) {
       const bool is_v = lane >= L;
       const int l = lane & (L - 1);
-      const half_t *src = is_v ? v_new + (int64_t)b * v_new_stride : k_new + (int64_t)b * k_new_stride;
-      const half8_t x16 = *(const half8_t *)(src + (int64_t)h * D + 8 * l);
       float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = (float)x16[i];
-      const int64_t slot = (int64_t)block_of(pages - 1, entry_of(pages - 1)) * kInt4Block + ((len - 1) & (kInt4Block - 1));
+      for (int i = 0; i < 8; ++i) x[i] = (float)new_row[i];
+      const int64_t slot = (int64_t)block_of(pages - 1, first_entry_of(pages - 1)) * kInt4Block + ((len - 1) & (kInt4Block - 1));
       int4_store<D>(pool, slot, num_kv_heads, is_v ? num_kv_heads + h : h, l, int4_row<L>(x));
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
@@ -204,7 +230,7 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   // Two blocks a step, kDepth steps' in flight. Block-table entries are read a step before the requests that they are for, and not
   // looked at before: a scalar load that is waited for on the spot cost every step its whole trip.
   Int4Regs<D> buf[kDepth][2];
-  int entry0 = entry_of(p0), entry1 = entry_of(p0 + 1);
+  int entry0 = first_entry_of(p0), entry1 = first_entry_of(p0 + 1);
   auto request_pair = [&](int p, Int4Regs<D> (&r)[2]) {
     request(p, entry0, r[0]);
     request(p + 1, entry1, r[1]);
@@ -216,71 +242,79 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
 
   // q as the right operand of the first product: column n, the elements of the bytes that the lane of the same g holds of K,
   // as a sum of three fp8 numbers (4 + 4 + 4 bits), scaled by a power of two that puts the row's largest between 224 and 448. What
-  // that leaves of an element is 2^-10, some 2^-18 of the largest.
+  // that leaves of an element is 2^-10, some 2^-18 of the largest. Made once for the workgroup and handed out through LDS.
   constexpr int kParts = 3, kProducts = D == 128 ? 3 : 2;   // D = 64: two parts side by side in the 128 of one product
-  int8v_t qf[kProducts];
-  float q_sum = 0.f, k_mul;
-  {
-    const int col = TWO ? n : (n & 7);
-    const half_t *row = q + (int64_t)b * q_batch_stride + (int64_t)(hq0 + (col < group ? col : group - 1)) * D +
-                        (D / 4) * g;
-    float x[kSteps][8], most = 0.f;
+  extern __shared__ __attribute__((aligned(16))) float int4_lds[];
+  constexpr int kRowBytes = kParts * D + 16;                // of a row of q: the parts, the sum and the factor of its scores
+  char *const q_rows = (char *)int4_lds;
+  float *const int4_rows = int4_lds + kHeads * kRowBytes / 4;
+  if (wave < kHeads * L / kWave) {
+    const int l = threadIdx.x % L;
+    char *row = q_rows + (threadIdx.x / L) * kRowBytes;
+    float x[8], most = 0.f, sum = 0.f, odd = 0.f;   // odd: an element that is not finite, which fp8 would saturate
 #pragma unroll
-    for (int t = 0; t < kSteps; ++t) {
-      const half8_t y = *(const half8_t *)(row + 8 * t);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[t][i] = (float)y[i];
-        most = __builtin_fmaxf(most, __builtin_fabsf(x[t][i]));
-      }
+    for (int i = 0; i < 8; ++i) {
+      x[i] = (float)q_in[i];
+      most = __builtin_fmaxf(most, __builtin_fabsf(x[i]));
+      odd = __builtin_fabsf(x[i]) < INFINITY ? odd : 1.f;
     }
-    most = __builtin_fmaxf(most, xor_lane(most, 16));
-    most = __builtin_fmaxf(most, xor_lane(most, 32));
+    most = over_row<L>(most, [](float a, float b) { return __builtin_fmaxf(a, b); });
+    odd = over_row<L>(odd, [](float a, float b) { return a + b; });
     int up = most > 0.f ? 9 - __builtin_amdgcn_frexp_expf(most) : 0;
     if (__builtin_amdgcn_ldexpf(most, up) > 448.f) --up;
-    bool odd = false;   // an element that is not finite: fp8 would saturate it
 #pragma unroll
-    for (int t = 0; t < kSteps; ++t) {
+    for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_ldexpf(x[i], up);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        odd |= !(__builtin_fabsf(x[t][i]) < INFINITY);
-        x[t][i] = __builtin_amdgcn_ldexpf(x[t][i], up);
+    for (int part = 0; part < kParts; ++part) {
+      uint2v_t bytes;   // elements of the lower and of the upper nibbles
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        constexpr int kOrder[2][4] = {{0, 4, 1, 5}, {2, 6, 3, 7}};
+        int four = __builtin_amdgcn_cvt_pk_fp8_f32(x[kOrder[u][0]], x[kOrder[u][1]], 0, false);
+        four = __builtin_amdgcn_cvt_pk_fp8_f32(x[kOrder[u][2]], x[kOrder[u][3]], four, true);
+        const float back[4] = {__builtin_amdgcn_cvt_f32_fp8(four, 0), __builtin_amdgcn_cvt_f32_fp8(four, 1),
+                               __builtin_amdgcn_cvt_f32_fp8(four, 2), __builtin_amdgcn_cvt_f32_fp8(four, 3)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sum += back[i];
+          x[kOrder[u][i]] -= back[i];
+        }
+        bytes[u] = (uint32_t)four;
       }
+      *(uint2v_t *)(row + part * D + 8 * l) = bytes;
     }
+    sum = over_row<L>(sum, [](float a, float b) { return a + b; });
+    if (l == 0) {
+      *(float2v_t *)(row + kParts * D) =
+          float2v_t{sum * 0x1p15f,   // the zero points come as z * 2^-24, the products in units of 2^-9
+                    odd > 0.f ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(scale_log2, 9 - up)};
+    }
+  }
+  __syncthreads();
+  int8v_t qf[kProducts];
+  float q_sum, k_mul;
+  {
+    const char *row = q_rows + (TWO ? n : (n & 7)) * kRowBytes;
+    const float2v_t both = *(const float2v_t *)(row + kParts * D);
+    q_sum = both[0];
+    k_mul = both[1];
 #pragma unroll
     for (int i = 0; i < 8; ++i) qf[kProducts - 1][i] = 0;
 #pragma unroll
     for (int part = 0; part < kParts; ++part) {
 #pragma unroll
-      for (int t = 0; t < kSteps; ++t) {
+      for (int j = 0; j < D / 64; ++j) {   // 16 bytes: elements of two dwords of K
+        const uint4_t x = *(const uint4_t *)(row + part * D + (D / 4) * g + 16 * j);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          constexpr int kOrder[2][4] = {{0, 4, 1, 5}, {2, 6, 3, 7}};   // elements of the lower and of the upper nibbles
-          float *y[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = &x[t][kOrder[u][i]];
-          int bytes = __builtin_amdgcn_cvt_pk_fp8_f32(*y[0], *y[1], 0, false);
-          bytes = __builtin_amdgcn_cvt_pk_fp8_f32(*y[2], *y[3], bytes, true);
-          const float back[4] = {__builtin_amdgcn_cvt_f32_fp8(bytes, 0), __builtin_amdgcn_cvt_f32_fp8(bytes, 1),
-                                 __builtin_amdgcn_cvt_f32_fp8(bytes, 2), __builtin_amdgcn_cvt_f32_fp8(bytes, 3)};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            q_sum += back[i];
-            *y[i] -= back[i];
-          }
+        for (int i = 0; i < 4; ++i) {
           if constexpr (D == 128) {
-            qf[part][2 * t + u] = bytes;
+            qf[part][4 * j + i] = (int)x[i];
           } else {
-            qf[part >> 1][4 * (part & 1) + 2 * t + u] = bytes;
+            qf[part >> 1][4 * (part & 1) + i] = (int)x[i];
           }
         }
       }
     }
-    q_sum += xor_lane(q_sum, 16);
-    q_sum += xor_lane(q_sum, 32);
-    q_sum *= 0x1p15f;    // the zero points come as z * 2^-24, the products in units of 2^-9
-    odd = (__builtin_amdgcn_ballot_w64(odd) >> n & 0x0001000100010001ull) != 0;
-    k_mul = odd ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(scale_log2, 9 - up);
   }
   const bool second = n >= 8;   // !TWO: the lane's scores are those of the second block's keys
 
@@ -436,9 +470,12 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
       fold_at = p + kFold;
     }
   }
+  static_assert(kDepth == 2, "the last steps, one after the other");
+#pragma unroll 1
+  for (; p < p1; p += 2) {
+    attend(buf[0], p, std::true_type{});
 #pragma unroll
-  for (int i = 0; i < kDepth; ++i) {
-    if (p + 2 * i < p1) attend(buf[i], p + 2 * i, std::true_type{});
+    for (int u = 0; u < 2; ++u) buf[0][u] = buf[1][u];
   }
 
   fold_zeros();
@@ -464,8 +501,7 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   // (!TWO: both halves of the columns have the rows, each stores two of the four)
   auto mine = [&](int i) { return head < group && (TWO || (i >> 1) == (n >> 3)); };
   // The wavefronts that share a split leave their rows, references and sums in LDS, and fold them in order.
-  extern __shared__ __attribute__((aligned(16))) float int4_rows[];
-  constexpr int kHeads = TWO ? 16 : 8, kArea = kHeads * D + 32;   // of a wavefront: rows, references, sums
+  constexpr int kArea = kHeads * D + 32;   // of a wavefront: rows, references, sums
   float *area = int4_rows + part * kArea;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -485,14 +521,25 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   for (int i = part * kWave + lane; i < group * (D / 4); i += share * kWave) {
     const int of = i / (D / 4), at_row = 4 * (i % (D / 4));
     const float *stats = int4_rows + kHeads * D + of;
-    float top = stats[0];
-    for (int s = 1; s < share; ++s) top = __builtin_fmaxf(top, stats[s * kArea]);
+    float refs[kInt4Waves], sums[kInt4Waves];
+    float4_t parts[kInt4Waves];
+#pragma unroll
+    for (int s = 0; s < kInt4Waves; ++s) {
+      const int at = s < share ? s : share - 1;
+      refs[s] = stats[at * kArea];
+      sums[s] = stats[at * kArea + 16];
+      parts[s] = *(const float4_t *)(int4_rows + at * kArea + of * D + at_row);
+    }
+    float top = refs[0];
+#pragma unroll
+    for (int s = 1; s < kInt4Waves; ++s) top = __builtin_fmaxf(top, refs[s]);
     float sum = 0.f;
     float4_t y = float4_t{0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < share; ++s) {
-      const float weight = fast_exp2(stats[s * kArea] - top);
-      sum += weight * stats[s * kArea + 16];
-      y += weight * *(const float4_t *)(int4_rows + s * kArea + of * D + at_row);
+#pragma unroll
+    for (int s = 0; s < kInt4Waves; ++s) {
+      const float weight = s < share ? fast_exp2(refs[s] - top) : 0.f;
+      sum += weight * sums[s];
+      y += weight * parts[s];
     }
     y *= 1.0f / sum;
     if (whole) {
@@ -591,7 +638,8 @@ extern "C" int litekv_paged_decode_int4(const void *q, int64_t q_batch_stride, v
   const int share = units > 256 ? kInt4Waves / 2 : kInt4Waves;
   LITEKV_REQUIRE(units <= 0x7fffffffLL / 8, "%s: too many workgroups", what);
   const bool two = (group + slices - 1) / slices > 8;
-  const size_t lds = (size_t)share * ((two ? 16 : 8) * head_dim + 32) * sizeof(float);
+  const int heads = two ? 16 : 8;
+  const size_t lds = (size_t)share * (heads * head_dim + 32) * sizeof(float) + (size_t)heads * (3 * head_dim + 16);
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)units), dim3((unsigned)(share * kWave)), lds,
                        static_cast<hipStream_t>(stream), static_cast<const half_t *>(q), q_batch_stride,
