@@ -801,6 +801,8 @@ int litekv_paged_prefill_int8(const void *q, int64_t q_token_stride,
  * several blocks of rows decodes them into it once, max_kv_len tokens a sequence: with such a workspace no
  * sequence may have more keys (those past it are not attended). max_kv_len 0, or a smaller workspace: every block
  * of rows decodes for itself. The results are the same to the rounding of the sums' order.
+ * litekv_paged_prefill_int4_key_slices: the key_slices that suit a launch of few rows (num_tokens *
+ * num_q_heads <= 65536; 1 for more).
  */
 int litekv_kv_append_int4(const void *k, const void *v, int64_t k_token_stride,
                           int64_t v_token_stride, const int32_t *slot_mapping,
@@ -833,6 +835,10 @@ int litekv_paged_decode_int4(const void *q, int64_t q_batch_stride, void *kv_poo
                              int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                              int32_t page_size, int64_t num_pages, int32_t max_splits,
                              int32_t min_pages_per_split, float softmax_scale, void *stream);
+
+int32_t litekv_paged_prefill_int4_key_slices(int32_t batch, int32_t num_q_heads,
+                                             int32_t num_kv_heads, int32_t head_dim,
+                                             int32_t max_q_len, int64_t max_kv_len);
 
 size_t litekv_paged_prefill_int4_workspace_bytes(int32_t batch, int32_t num_q_heads,
                                                  int32_t num_kv_heads, int32_t head_dim,

@@ -245,6 +245,10 @@ SIGNATURES = {
          c_void_p, c_void_p, c_size_t, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int32,
          c_int32, c_float, c_void_p],
     ),
+    "litekv_paged_prefill_int4_key_slices": (
+        c_int32,
+        [c_int32, c_int32, c_int32, c_int32, c_int32, c_int64],
+    ),
     "litekv_paged_prefill_int4_workspace_bytes": (
         c_size_t,
         [c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, c_int32],

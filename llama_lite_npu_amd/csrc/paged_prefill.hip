@@ -641,6 +641,17 @@ static Int4Staging int4_staging(int32_t batch, int32_t num_q_heads, int32_t num_
   return s;
 }
 
+// As litekv_paged_prefill_key_slices, but two for three chunks and more over long histories that it leaves uncut: the launch then
+// takes as long as its longest chain of keys, which chunks of one batch seldom share evenly. 4 chunks of up to 512 rows over 2000 to
+// 8000 tokens, 32 / 8 heads of 64: 126 -> 97 us, of 128 175 -> 131; 3 of up to 400 over up to 30000 609 -> 467; 4 equal ones of 512
+// over 8000 239 -> 234; 16 of up to 128 over up to 4000, heads of 64, 98 -> 84, but over up to 2000, heads of 128, 73 -> 75, 6 of up to
+// 300 over up to 1000 48 -> 53, and two of up to 1000 over 4000 88 -> 104. (Other pools would gain as much.)
+extern "C" int32_t litekv_paged_prefill_int4_key_slices(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                                        int32_t max_q_len, int64_t max_kv_len) {
+  const int32_t slices = litekv_paged_prefill_key_slices(batch, num_q_heads, num_kv_heads, head_dim, max_q_len, max_kv_len);
+  return slices == 1 && batch >= 3 && max_kv_len >= 3000 && max_kv_len >= 2 * (int64_t)max_q_len ? 2 : slices;
+}
+
 extern "C" size_t litekv_paged_prefill_int4_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                                             int32_t head_dim, int32_t max_q_len, int64_t max_kv_len,
                                                             int64_t num_tokens, int32_t key_slices) {

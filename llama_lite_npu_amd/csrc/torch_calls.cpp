@@ -209,7 +209,8 @@ PyObject *paged_prefill(PyObject *, PyObject *const *a, Py_ssize_t n) {
     // (the count's rule and the rows it looks at as in the wrapper)
     int32_t slices = 1;
     if (a[9] != Py_None && t * hq > 0 && t * hq <= 128 * 512) {
-      slices = litekv_paged_prefill_key_slices((int32_t)b, (int32_t)hq, (int32_t)pool.hkv, (int32_t)d, (int32_t)max_q, max_kv);
+      const auto rule = pool.format == kInt4 ? litekv_paged_prefill_int4_key_slices : litekv_paged_prefill_key_slices;
+      slices = rule((int32_t)b, (int32_t)hq, (int32_t)pool.hkv, (int32_t)d, (int32_t)max_q, max_kv);
     }
     at::Tensor out = at::empty({t, hq, d}, q->options());
     at::Tensor partials;

@@ -1070,7 +1070,8 @@ def paged_prefill(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Ten
         # and without the lengths on the host there is nothing to choose by (what the block table
         # could name says little: a fresh prompt cut into eight slices takes twice as long)
         few_rows = 0 < t * hq <= 128 * 512 and max_kv_len is not None
-        key_slices = int(lib.litekv_paged_prefill_key_slices(b, hq, hkv, d, int(max_q_len), int(max_kv_len))) if few_rows else 1
+        rule = lib.litekv_paged_prefill_int4_key_slices if int4 else lib.litekv_paged_prefill_key_slices
+        key_slices = int(rule(b, hq, hkv, d, int(max_q_len), int(max_kv_len))) if few_rows else 1
     key_slices = int(key_slices)
     if key_slices > 1:
         need = paged_prefill_workspace_floats(t, hq, d, key_slices)
