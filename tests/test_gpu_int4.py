@@ -452,3 +452,47 @@ def test_native_calls_and_wrappers_agree(d):
     ops.page_dequant(pools[0], a, ids, None, None)
     ops.page_dequant(pools[0], b, ids.long(), None, None)
     assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+def test_prefill_that_was_told_of_too_few_keys():
+    """Keys decoded once, for the most keys the caller named: a longer sequence's rows are not numbers, the others' are right."""
+    hq, hkv, d, rows, history = 64, 8, 128, [300, 280], [900, 100]
+    lens = [1200, 380]
+    s = Sequences(lens, hq, hkv, d, 16, seed=9)
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    q = half(s.rng, 580, hq, d)
+    out = ops.paged_prefill(dev(q), dev(s.pool), dev(s.table), dev(cu, torch.int32), dev(np.array(history), torch.int32), 300,
+                            1 / math.sqrt(d), max_kv_len=1000).cpu().numpy()
+    assert np.isnan(out[:300]).all()
+    s.lens = [0, 380]
+    check(out, q, s, lambda b: ([300, 301, 440, 579], [101, 102, 241, 380]) if b else ([], []), 1 / math.sqrt(d),
+          HALF + 2.0 ** -25 * 380)
+
+
+def test_a_pool_of_more_than_4_gib():
+    """The last pages of a large pool give what the first pages of a small one give."""
+    hq, hkv, d, rows = 64, 8, 128, 300
+    small = torch.zeros(64 * 16, 2 * hkv, 66, dtype=torch.uint8, device=DEV)
+    large = torch.zeros((5 << 30) // (2 * hkv * 66) // 16 * 16, 2 * hkv, 66, dtype=torch.uint8, device=DEV)
+    shift = large.shape[0] // 16 - 64
+    rng = np.random.default_rng(3)
+    k, v, q = (dev(half(rng, 900, h, d)) for h in (hkv, hkv, hq))
+    table = dev(rng.permutation(64)[:57].reshape(1, -1), torch.int32)
+    slots = (table[0].long()[:, None] * 16 + torch.arange(16, device=DEV)).reshape(-1)[:900].to(torch.int32)
+    outs = []
+    for pool, pages in ((small, 0), (large, shift)):
+        at = slots + 16 * pages
+        ops.kv_append_quantised(k[:450], v[:450], at[:450].contiguous(), pool)
+        q_in = q[450:].clone()
+        ops.qk_norm_rope_append(q_in, k[450:], v[450:], at[450:].contiguous(), pool)
+        t, n = table + pages, torch.tensor([900], dtype=torch.int32, device=DEV)
+        values = torch.empty(57 * 16, 2 * hkv, d, dtype=torch.float16, device=DEV)
+        step = ops.paged_decode(q[:1], pool, t, n, k_new=k[7:8], v_new=v[7:8])
+        ops.page_dequant(pool, values, t[0].contiguous(), None, None)
+        cu = torch.tensor([0, rows], dtype=torch.int32, device=DEV)
+        ctx = torch.tensor([600], dtype=torch.int32, device=DEV)
+        chunk = ops.paged_prefill(q[:rows], pool, t, cu, ctx, rows, 0.1, max_kv_len=900)
+        direct = ops.paged_prefill(q[:rows], pool, t, cu, ctx, rows, 0.1)
+        outs.append((step, values[:900], chunk, direct, pool[16 * pages:16 * pages + 1024]))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert large[: 16 * shift].any() == False  # noqa: E712
