@@ -26,15 +26,16 @@
 // The reference of the exponentials is the largest p s' so far, not the largest p: in fp16 it is p s' that has to fit. It is put
 // at 2^7 and may grow to 2^15 before the accumulators are rescaled.
 //
-// Bound: by what one compute unit takes in, some 40 GB/s at one sequence per head (32768 tokens on 8 compute units: 104 us; neither more
+// Bound: by what one compute unit takes in, some 40 GB/s at one sequence per head (32768 tokens on 8 compute units: 103 us; neither more
 // loads in flight nor the scores of the next step beside the second product of this one make it faster), and by memory once
 // there are as many workgroups as compute units: 64 sequences of 8192 tokens, 32 / 4 heads of 128, take 47 us, 5.9 TB/s of cache read (a
 // large copy reads and writes 5.0). A step is 149 vector and 15 matrix instructions for 32 keys and 8 heads (D = 128); 146
 // registers leave room for three wavefronts per SIMD with two steps' loads in flight each (four with one step's took 3 to 40%
 // longer). Of its twelve wavefronts a compute unit holds one workgroup of eight or three of four. Eight are faster
-// while there are no more workgroups than compute units (the case above with four: 53 us; 20 sequences of 4096, 8 kv heads: 22.7
-// against 25), four where there are more (38 of them: 39 us against 44; 100 of 2048: 44 against 55). Streaming loads, whose lines
-// are the first to leave the caches, took 10% less than ordinary ones.
+// while there are no more workgroups than compute units (20 sequences of 4096, 8 kv heads: 20.4 us against 23.3; 4096 to 16384
+// tokens in 64: 71 against 79), four where there are more (38 of 4096: 36.4 against 40.8; 100 of 2048: 42.6 against 51). Streaming
+// loads, whose lines are the first to leave the caches, suit a cache larger than those (the case above with ordinary ones: 52.5 us), as
+// that of a model's layers one after the other is; inside them ordinary ones are faster (20 of 4096: 19.2 against 20.5).
 //
 // Around its keys a workgroup spends some 5 us, most of it one memory trip after another and the first run through its code: the
 // sequence's length, block-table entries, keys, the fold. So q, the first 64 entries of the table row and the new rows are
@@ -555,10 +556,10 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
 }  // namespace litekv
 
 // Up to 256 (sequence, kv head) pairs, a compute unit has at most one, and splits of 1024 tokens and more fill the device
-// (8 sequences of 4096 tokens, 8 kv heads: splits of 1024 / 2048 / 4096 tokens 15.1 / 17.6 / 21.1 us). With more, splits only even out
-// the lengths (40 of 16384 tokens, 8 kv heads: 144 / 122 / 115 us, 135 unsplit; 64 of them: 224 / 189 / 180 us, 170 unsplit).
+// (8 sequences of 4096 tokens, 8 kv heads: splits of 1024 / 2048 / 4096 tokens 12.9 / 15.7 / 18.4 us). With more, splits only even out
+// the lengths (40 of 16384 tokens, 8 kv heads: 137 / 117 / 112 us, 135 unsplit; 64 of them: 214 / 191 / 175 us, 166 unsplit).
 // No more than 16 where that makes them shorter than 4096 tokens: their merge takes longer the more there are (one sequence of 32768
-// tokens, 8 kv heads: 8 / 16 / 32 splits 24 / 19.5 / 22 us). Powers of two: a captured step holds their number, and growing
+// tokens, 8 kv heads: 8 / 16 / 32 splits 21.7 / 17.6 / 19.5 us). Powers of two: a captured step holds their number, and growing
 // sequences should not ask for a new one every thousand tokens.
 extern "C" int32_t litekv_paged_decode_int4_splits(int32_t batch, int32_t num_kv_heads, int64_t max_pages, int64_t total_pages,
                                                    int32_t page_size, int32_t *min_pages_per_split) {

@@ -54,38 +54,46 @@ static PrefillShape prefill_shape(int group, int max_q_len, int wg_col_tiles = k
   return s;
 }
 
-// Folds the key slices of a split prefill: one wavefront per (query row, head) reads the row's
-// `slices` log-sum-exps and partial rows (fp32, normalised per slice) and writes the fp16 row.
-// A slice without keys has log-sum-exp -inf and weight 0; the last slice always has keys.
+// Folds the key slices of a split prefill: the lanes of a (query row, head), four elements each, read the row's
+// `slices` log-sum-exps and partial rows (fp32, normalised per slice) and write the fp16 row. A slice without keys has
+// log-sum-exp -inf and weight 0; the last slice always has keys. Bound by memory trips, then by memory: no lane needs another's
+// numbers, and all loads are ahead of the arithmetic (64 rows of 16 heads of 128 in 8 slices 3.8 us, 1224 rows of 32 heads
+// of 64 in 2 7.7; with a wavefront a row that gathers them by shuffles 5.5 and 15).
+constexpr int kMergeLanes = kHD / 4, kMergeRows = 4 * kWave / kMergeLanes;   // of a row; rows of a workgroup
 __global__ __launch_bounds__(4 * kWave) void prefill_split_merge_kernel(
     const float *__restrict__ part_o, const float *__restrict__ part_lse, half_t *__restrict__ out,
     int64_t out_stride, int64_t num_tokens, int32_t num_q_heads, int32_t slices) {
-  const int lane = threadIdx.x & (kWave - 1);
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (id >= num_tokens * num_q_heads) return;  // whole wavefronts
+  const int at = 4 * (threadIdx.x % kMergeLanes);
+  const int64_t id = (int64_t)blockIdx.x * kMergeRows + threadIdx.x / kMergeLanes;
+  if (id >= num_tokens * num_q_heads) return;
   const int64_t token = id / num_q_heads;
   const int head = (int)(id - token * num_q_heads);
   const int64_t piece_stride = num_tokens * num_q_heads;  // cells between the slices of a row
-  const float l = lane < slices ? part_lse[lane * piece_stride + id] : -INFINITY;
-  float mx = l;
+  float w[kMaxPrefillKeySlices];
+  float4_t row[kMaxPrefillKeySlices];
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, xor_lane(mx, off));
-  const float w = lane < slices ? fast_exp2((l - mx) * 1.4426950408889634f) : 0.f;
-  float den = w;
+  for (int i = 0; i < kMaxPrefillKeySlices; ++i) {
+    w[i] = i < slices ? part_lse[i * piece_stride + id] : -INFINITY;
+    row[i] = i < slices ? *(const float4_t *)(part_o + (i * piece_stride + id) * kHD + at) : float4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  float mx = w[0];
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) den += xor_lane(den, off);
-  if (2 * lane >= kHD) return;
-  float o0 = 0.f, o1 = 0.f;
-  for (int sidx = 0; sidx < slices; ++sidx) {  // in slice order: the sum does not depend on timing
-    const float ws = __shfl(w, sidx, kWave);
-    const float2 r = *(const float2 *)(part_o + (sidx * piece_stride + id) * kHD + 2 * lane);
-    o0 += ws * r.x;
-    o1 += ws * r.y;
+  for (int i = 1; i < kMaxPrefillKeySlices; ++i) mx = fmaxf(mx, w[i]);
+#pragma unroll
+  for (int i = 0; i < kMaxPrefillKeySlices; ++i) w[i] = i < slices ? fast_exp2((w[i] - mx) * 1.4426950408889634f) : 0.f;
+  static_assert(kMaxPrefillKeySlices == 8, "the order of the sum");
+  const float den = ((w[0] + w[4]) + (w[2] + w[6])) + ((w[1] + w[5]) + (w[3] + w[7]));
+  float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kMaxPrefillKeySlices; ++i) {  // in slice order: the sum does not depend on timing
+    if (i < slices) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += w[i] * row[i][j];
+    }
   }
   const float inv = 1.0f / den;
-  typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-  *(half2_t *)(out + token * out_stride + (int64_t)head * kHD + 2 * lane) =
-      half2_t{(half_t)(o0 * inv), (half_t)(o1 * inv)};
+  *(half4_t *)(out + token * out_stride + (int64_t)head * kHD + at) =
+      half4_t{(half_t)(o[0] * inv), (half_t)(o[1] * inv), (half_t)(o[2] * inv), (half_t)(o[3] * inv)};
 }
 
 static size_t prefill_split_workspace_bytes(int64_t num_tokens, int32_t num_q_heads, int32_t key_slices) {
@@ -329,7 +337,7 @@ static int launch_paged_prefill(const char *what, const void *q, int64_t q_token
     int rc2 = check_launch(what);
     if (rc2 != LITEKV_OK) return rc2;
     const int64_t merge_rows = rows * num_q_heads;
-    hipLaunchKernelGGL(prefill_split_merge_kernel, dim3((unsigned)((merge_rows + 3) / 4)), dim3(4 * kWave), 0,
+    hipLaunchKernelGGL(prefill_split_merge_kernel, dim3((unsigned)((merge_rows + kMergeRows - 1) / kMergeRows)), dim3(4 * kWave), 0,
                        static_cast<hipStream_t>(stream), part_o, part_lse, static_cast<half_t *>(out),
                        out_token_stride, rows, num_q_heads, slices);
     return check_launch(what);
@@ -610,10 +618,10 @@ extern "C" int litekv_paged_prefill_int8(const void *q, int64_t q_token_stride, 
 
 // Where the keys of a launch over 4-bit codes lie as fp16, in its workspace behind the partial rows of its key slices. Decoded once
 // they cost a launch and their bytes, some 14 us for 33 MB; decoded by every block of rows, a third of its tile loop. 512
-// rows over 7601 tokens, 64 / 8 heads: 172 -> 151 us (fp16 pool: 129 to 135); 8 prompts of 128 to 2048 tokens 263 -> 241 (225 to
-// 235); four chunks of up to 512 over up to 8000, 32 / 8 heads of 64, 163 -> 128 (107); 16 prompts of 1024 118 -> 109. With fewer blocks:
-// 128 rows over 4000, 64 / 8 heads (8 blocks), 44.7 -> 45.2; 32 / 8 heads (4 blocks), 26.7 -> 33.9; 8 prompts of 512, 32 / 8 heads
-// (16 blocks, a key attended by 8 on the average), 43.5 -> 45.2. Up to 1 GiB: a cache in 4 bits is there to save memory.
+// rows over 7601 tokens, 64 / 8 heads: 178 -> 153 us (fp16 pool: 129 to 135); 8 prompts of 128 to 2048 tokens 261 -> 236 (225 to
+// 235); four chunks of up to 512 over up to 8000, 32 / 8 heads of 64, uncut, 163 -> 128 (107); 16 prompts of 1024 118 -> 107; 200 rows over
+// 8000, 64 / 8 heads (13 blocks), 91 -> 83. With fewer blocks: 128 rows over 4000, 64 / 8 heads (8 blocks), 44 in both forms; 32 / 8 heads
+// (4 blocks), 26.6 -> 33.8; 8 prompts of 512, 32 / 8 heads (16 blocks, a key attended by 8 on the average), 44.3 -> 45.3. Up to 1 GiB: a cache in 4 bits is there to save memory.
 struct Int4Staging {
   int64_t capacity = 0;   // tokens of a sequence, 0: they are decoded where they are attended
   size_t table_at = 0, pool_at = 0, bytes = 0;
