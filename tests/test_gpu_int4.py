@@ -496,3 +496,24 @@ def test_a_pool_of_more_than_4_gib():
         outs.append((step, values[:900], chunk, direct, pool[16 * pages:16 * pages + 1024]))
     assert all(torch.equal(a, b) for a, b in zip(*outs))
     assert large[: 16 * shift].any() == False  # noqa: E712
+
+
+@pytest.mark.parametrize("hq,hkv,d,page", [(16, 8, 128, 16), (8, 2, 64, 64), (12, 1, 128, 32), (32, 2, 64, 16)])
+def test_a_new_token_in_every_row_of_its_block(hq, hkv, d, page):
+    """The wavefront that attends the last block has the new token in registers: every row of a block, blocks of every place."""
+    lens = list(range(1, 52)) + [256 + n for n in (1, 2, 7, 10, 16)] + [2048 + n for n in (0, 4, 11)]
+    s = Sequences(lens, hq, hkv, d, page, seed=hq)
+    q, kv = half(s.rng, len(lens), hq, d), half(s.rng, len(lens), 2 * hkv, d)
+    kv[:, :, 5] *= 4.0                     # (so that a row's element somewhere else would show)
+    kv[:, hkv:, d - 9] *= -3.0
+    both, slots = dev(kv), [int4.tokens_of(s.table[b], n, page)[-1] for b, n in enumerate(lens)]
+    pools = [dev(s.pool) for _ in range(2)]
+    args = dev(s.table), dev(np.array(lens), torch.int32), 1 / math.sqrt(d)
+    for kw in (dict(), dict(num_splits=4)):
+        out = ops.paged_decode(dev(q), pools[0], *args, page_size=page, k_new=both[:, :hkv], v_new=both[:, hkv:], **kw)
+        ops.kv_append_quantised(both[:, :hkv], both[:, hkv:], dev(np.array(slots), torch.int32), pools[1])
+        assert torch.equal(out, ops.paged_decode(dev(q), pools[1], *args, page_size=page, **kw))
+        assert torch.equal(*pools)
+        pools[0].copy_(dev(s.pool)), pools[1].copy_(dev(s.pool))
+    int4.store(s.pool, slots, kv[:, :hkv], kv[:, hkv:])
+    check(out.cpu().numpy(), q, s, lambda b: ([b], [lens[b]]), 1 / math.sqrt(d), 2.0 ** -19)
