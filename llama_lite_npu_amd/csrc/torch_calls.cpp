@@ -15,6 +15,7 @@
 #include <cmath>
 
 #include <ATen/ATen.h>
+#include <ATen/detail/CUDAHooksInterface.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
@@ -72,7 +73,7 @@ Pool pool_of(PyObject *pool, PyObject *scales) {
       return p;
     case at::kByte:
       if (p.d == 34 || p.d == 66) {  // 4-bit codes: rows of head_dim / 2 + 2 bytes, in blocks of 16 slots, no scales
-        if (scales != Py_None || p.slots % 16 != 0) return p;
+        if (scales != Py_None || p.slots % 16 != 0 || p.t->get_device() != at::detail::getCUDAHooks().getCurrentDevice()) return p;
         p.d = 2 * (p.d - 2);
         p.format = kInt4;
         return p;
@@ -92,6 +93,12 @@ Pool pool_of(PyObject *pool, PyObject *scales) {
 }
 
 void *address(const at::Tensor *t) { return t != nullptr ? t->data_ptr() : nullptr; }
+
+// A pool of 4-bit codes and tensors elsewhere: the wrapper says so.
+template <typename... Tensors>
+bool apart(const Pool &pool, const Tensors *...others) {
+  return pool.format == kInt4 && ((others != nullptr && others->get_device() != pool.t->get_device()) || ...);
+}
 
 // Runs `call` without the interpreter lock, as ctypes does.
 template <typename Call>
@@ -136,6 +143,7 @@ PyObject *qk_norm_rope_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
       }
       cs = cos->stride(0);
     }
+    if (apart(pool, q, k, v, slots, qw, kw, cos, sin)) Py_RETURN_NONE;
     const double eps = PyFloat_AsDouble(a[9]);
     void *stream = PyLong_AsVoidPtr(a[11]);
     if (PyErr_Occurred()) {
@@ -194,6 +202,7 @@ PyObject *paged_prefill(PyObject *, PyObject *const *a, Py_ssize_t n) {
       ctx = index_tensor(a[4], b);
       if (ctx == nullptr) Py_RETURN_NONE;
     }
+    if (apart(pool, q, cu, table, ctx)) Py_RETURN_NONE;
     const int64_t max_q = PyLong_AsLongLong(a[5]), page = PyLong_AsLongLong(a[7]);
     const int64_t max_kv = a[9] == Py_None ? -1 : PyLong_AsLongLong(a[9]);
     const double scale = PyFloat_AsDouble(a[6]);
@@ -284,6 +293,7 @@ PyObject *paged_decode_int4(PyObject *, PyObject *const *a, Py_ssize_t n) {
       vs = row_stride(*vn, b, pool.hkv, d);
       if (ks < 0 || vs < 0) Py_RETURN_NONE;
     }
+    if (apart(pool, q, table, lens, kn, vn)) Py_RETURN_NONE;
     const double scale = a[4] == Py_None ? 1.0 / std::sqrt((double)d) : PyFloat_AsDouble(a[4]);
     const int64_t page = PyLong_AsLongLong(a[5]);
     void *stream = PyLong_AsVoidPtr(a[8]);
@@ -330,6 +340,7 @@ PyObject *kv_append_quantised(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (pool.format == kNone || pool.format == kF16) Py_RETURN_NONE;
     const int64_t t = k->size(0), ks = row_stride(*k, t, pool.hkv, pool.d), vs = row_stride(*v, t, pool.hkv, pool.d);
     const at::Tensor *slots = index_tensor(a[2], t);
+    if (apart(pool, k, v, slots)) Py_RETURN_NONE;
     if (ks < 0 || vs < 0 || slots == nullptr || t > INT32_MAX || pool.hkv > INT32_MAX || pool.d > INT32_MAX) Py_RETURN_NONE;
     void *stream = PyLong_AsVoidPtr(a[5]);
     if (PyErr_Occurred()) {
@@ -369,6 +380,7 @@ PyObject *page_dequant(PyObject *, PyObject *const *a, Py_ssize_t n) {
       dst = index_tensor(a[3], src->numel());
       if (dst == nullptr) Py_RETURN_NONE;
     }
+    if (apart(pool, to.t, src, dst)) Py_RETURN_NONE;
     const int64_t page = PyLong_AsLongLong(a[5]);
     void *stream = PyLong_AsVoidPtr(a[6]);
     if (PyErr_Occurred()) {

@@ -108,9 +108,13 @@ def _dev_fp8_pool(kv_pool: torch.Tensor, scales: Optional[torch.Tensor], num_kv_
         raise ValueError("scales must be float32 [2 * Hkv] on the GPU (K heads, then V heads)")
 
 
-def _dev_int4_pool(kv_pool: torch.Tensor, scales: Optional[torch.Tensor]) -> None:
+def _dev_int4_pool(kv_pool: torch.Tensor, scales: Optional[torch.Tensor], *others: Optional[torch.Tensor]) -> None:
     if not kv_pool.is_cuda:
         raise ValueError("kv_pool must live on the GPU")
+    if kv_pool.get_device() != torch._C._cuda_getDevice():       # a launch goes to the current device
+        raise ValueError(f"kv_pool lives on {kv_pool.device}, which is not the current device")
+    if any(t is not None and t.is_cuda and t.get_device() != kv_pool.get_device() for t in others):
+        raise ValueError(f"kv_pool lives on {kv_pool.device}, another tensor on another device")
     if scales is not None:
         raise ValueError("a pool of 4-bit codes has no scales per head: its rows carry their own")
     if kv_pool.shape[0] % 16 != 0:
@@ -199,7 +203,7 @@ def kv_append_quantised(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Te
     slots, hkv, d, _, _ = pool_geometry(kv_pool, 1)
     int4 = is_int4_pool(kv_pool)
     if int4:
-        _dev_int4_pool(kv_pool, scales)
+        _dev_int4_pool(kv_pool, scales, k, v, slot_mapping)
     else:
         _dev_fp8_pool(kv_pool, scales, hkv)
     _need(k.shape == v.shape and k.shape[1] == hkv and k.shape[2] == d, "k / v must be [T, Hkv, D] matching the pool")
@@ -233,7 +237,7 @@ def page_dequant(kv_pool: torch.Tensor, dst_pool: torch.Tensor, src_ids: torch.T
     _, hkv_d, d_d, n_dst, _ = pool_geometry(dst_pool, page_size)
     int4 = is_int4_pool(kv_pool)
     if int4:
-        _dev_int4_pool(kv_pool, scales)
+        _dev_int4_pool(kv_pool, scales, dst_pool, src_ids, dst_ids)
     else:
         _dev_fp8_pool(kv_pool, scales, hkv)
     _need((hkv, d) == (hkv_d, d_d), "pools differ in head geometry")
@@ -275,7 +279,7 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_
     if fp8:
         _dev_fp8_pool(kv_pool, kv_scales, hkv)
     elif int4:
-        _dev_int4_pool(kv_pool, kv_scales)
+        _dev_int4_pool(kv_pool, kv_scales, q, k, v, slot_mapping, q_norm_weight, k_norm_weight, cos, sin)
     else:
         _dev_half("kv_pool", kv_pool)
     t, hq = q.shape[0], q.shape[1]
@@ -869,7 +873,7 @@ def paged_decode(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tens
     # (not a plain call)
     _dev_half("q", q)
     if int4:
-        _dev_int4_pool(kv_pool, kv_scales)
+        _dev_int4_pool(kv_pool, kv_scales, q, block_table, seq_lens, out, workspace, k_new, v_new)
     elif not is_quantised_pool(kv_pool):
         _dev_half("kv_pool", kv_pool)
     if not (q.dim() == 3 and q.stride(2) == 1 and q.stride(1) == q.shape[2]):
@@ -1041,7 +1045,7 @@ def paged_prefill(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Ten
     _dev_half("q", q)
     fp8, int4 = is_quantised_pool(kv_pool), is_int4_pool(kv_pool)
     if int4:
-        _dev_int4_pool(kv_pool, kv_scales)
+        _dev_int4_pool(kv_pool, kv_scales, q, block_table, cu_q_lens, context_lens, out, workspace)
     elif not fp8:
         _dev_half("kv_pool", kv_pool)
         if not (kv_scales is None):

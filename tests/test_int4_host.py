@@ -202,3 +202,22 @@ def test_prefill_workspace_holds_the_keys_where_they_are_decoded_once():
     # few blocks of rows a key, lengths not known, more than 1 GiB of keys, heads of another size: the partial rows' alone, or nothing
     assert room(rows=64) == room(kv=0) == room(kv=-1) == room(kv=300000) == room(d=96) == room(b=0) == 0
     assert 0 < room(rows=64, slices=2) < 1 << 26
+
+
+def test_refusal_of_another_device(monkeypatch):
+    """Launches go to the current device: a pool, or a tensor beside it, that lives elsewhere is refused."""
+    class Elsewhere:
+        is_cuda, shape = True, (32, 4, 66)
+
+        def __init__(self, index):
+            self.index, self.device = index, f"cuda:{index}"
+
+        def get_device(self):
+            return self.index
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    ops._dev_int4_pool(Elsewhere(0), None, Elsewhere(0), None)
+    with pytest.raises(ValueError, match="not the current device"):
+        ops._dev_int4_pool(Elsewhere(1), None)
+    with pytest.raises(ValueError, match="another device"):
+        ops._dev_int4_pool(Elsewhere(0), None, Elsewhere(0), Elsewhere(1))
