@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void int4_append_kernel(
       const double e = __builtin_fma(-ms * rs, rs, 1.0);
       rs = __builtin_fma(0.5 * rs, e, rs);
     }
-    const float rrms = (float)rs;
+    const float rrms = ms == (double)INFINITY ? 0.f : (float)rs;   // (where a step has made NaN of it)
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = y[i] * rrms * (float)w[i];
   }

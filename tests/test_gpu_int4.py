@@ -517,3 +517,56 @@ def test_a_new_token_in_every_row_of_its_block(hq, hkv, d, page):
         pools[0].copy_(dev(s.pool)), pools[1].copy_(dev(s.pool))
     int4.store(s.pool, slots, kv[:, :hkv], kv[:, hkv:])
     check(out.cpu().numpy(), q, s, lambda b: ([b], [lens[b]]), 1 / math.sqrt(d), 2.0 ** -19)
+
+
+def test_epilogue_of_rows_that_are_not_finite():
+    """An infinite element makes its row's norm infinite: it is not a number itself (nor is what the rotation mixes it into), the others
+    are 0; a NaN makes the whole row NaN. In the pool NaN counts as 0."""
+    rng = np.random.default_rng(4)
+    d, hq, hkv, t = 128, 4, 2, 6
+    q, k, v = half(rng, t, hq, d), half(rng, t, hkv, d), half(rng, t, hkv, d)
+    q[1, 2, 5], q[2, 1, 100], q[3, 0, 9] = np.inf, -np.inf, np.nan
+    k[1, 0, 70], k[2, 1, 3], k[4, 0, 0] = np.inf, np.nan, -np.inf
+    w = half(rng, 2, d) + np.float16(2)
+    angle = rng.uniform(0, 6, (t, d // 2))
+    cos, sin = (np.concatenate([f(angle)] * 2, -1).astype(np.float16) for f in (np.cos, np.sin))
+    pool, got = torch.full((16, 2 * hkv, 66), 255, dtype=torch.uint8, device=DEV), dev(q)
+    ops.qk_norm_rope_append(got, dev(k), dev(v), torch.arange(t, dtype=torch.int32, device=DEV), pool, dev(w[0]), dev(w[1]), dev(cos),
+                            dev(sin), 1e-6)
+
+    def epilogue(x, weight):
+        with np.errstate(invalid="ignore"):
+            x = x.astype(np.float64)
+            y = x * (1 / np.sqrt((x * x).mean(-1, keepdims=True) + 1e-6)) * weight.astype(np.float64)
+            turned = np.concatenate([-y[..., d // 2:], y[..., :d // 2]], -1)
+            return y * cos[:, None].astype(np.float64) + turned * sin[:, None].astype(np.float64)
+
+    want, got = epilogue(q, w[0]), got.cpu().numpy()
+    assert np.array_equal(np.isnan(want), np.isnan(got)) and np.isnan(want).sum() == 4 + d
+    ok = ~np.isnan(want)
+    # one rounding to fp16 and a few of fp32
+    assert (np.abs(got[ok] - want[ok]) <= HALF * np.abs(want[ok]) + 2.0 ** -25 + 2.0 ** -20 * np.abs(want[ok]).max()).all()
+    values, _ = int4.decode_pool(pool.cpu().numpy(), hkv, d)
+    k_want = np.nan_to_num(epilogue(k, w[1]))
+    span = np.maximum(k_want.max(-1), 0) - np.minimum(k_want.min(-1), 0)
+    # half a step, the scale's rounding to 7 bits, an element next to a border
+    assert (np.abs(values[:t, :hkv] - k_want) <= (span * (0.5 / 15) * (1 + 2.0 ** -6) + 1e-5 * np.abs(k_want).max() + 2.0 ** -20)[..., None]).all()
+    assert (values[[1, 2, 4], [0, 1, 0]] == 0).all()
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(16, 2, 128), (32, 2, 64)])
+def test_decode_of_a_query_that_is_not_finite(hq, hkv, d):
+    """Its head's outputs are not numbers; every other head's and sequence's are what they are without it."""
+    lens = [40, 700, 33]
+    s = Sequences(lens, hq, hkv, d, 16, seed=d)
+    q = half(s.rng, 3, hq, d)
+    args = dev(s.pool), dev(s.table), dev(np.array(lens), torch.int32)
+    want = ops.paged_decode(dev(q), *args).cpu().numpy()
+    bad = [(0, 3, np.inf), (1, hq - 1, np.nan), (1, 0, -np.inf)]
+    for b, h, x in bad:
+        q[b, h, 7] = x
+    got = ops.paged_decode(dev(q), *args).cpu().numpy()
+    for b, h, _ in bad:
+        assert np.isnan(got[b, h]).all()
+        got[b, h] = want[b, h]
+    assert np.array_equal(got, want)
