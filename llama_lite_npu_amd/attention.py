@@ -13,7 +13,7 @@ arguments, driven by the same ``AttentionInfo``. Differences:
   chunks), so one kernel serves both branches of the reference;
 * ``qkv_epilogue`` folds the step before the append (QK RMSNorm, rotary embedding,
   qwen3.py:124-129) into the append itself; the forward calls are then made with ``xk=None``;
-* a layer whose pool holds fp8 or int8 codes (or 4-bit ones, which need no scales) (``atten_info.kv_scales[layer]`` set) quantises on append
+* a layer whose pool holds fp8 or int8 codes (``atten_info.kv_scales[layer]`` set) or 4-bit ones (no scales) quantises on append
   and attends straight from the codes, in decode and in chunks over cached history; fresh
   prompts attend to their own fp16 K/V.
 

@@ -270,9 +270,10 @@ PyObject *paged_prefill(PyObject *, PyObject *const *a, Py_ssize_t n) {
 }
 
 // (q, kv_pool, block_table, seq_lens, softmax_scale or None, page_size, k_new, v_new, stream), the pool one of 4-bit codes
-// -> the output, or the library's status if that is not 0, or None. The partial rows' workspace as in paged_prefill.
+// -> the output, or the library's status if that is not 0, or None. The partial rows' workspace as in paged_prefill. A plan's
+// splits, their least pages and its workspace (or None) may follow.
 PyObject *paged_decode_int4(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  if (n != 9) Py_RETURN_NONE;
+  if (n != 9 && n != 12) Py_RETURN_NONE;
   try {
     const at::Tensor *q = half_tensor(a[0]);
     if (q == nullptr || q->dim() != 3) Py_RETURN_NONE;
@@ -306,12 +307,30 @@ PyObject *paged_decode_int4(PyObject *, PyObject *const *a, Py_ssize_t n) {
       Py_RETURN_NONE;
     }
     int32_t least = 1;
-    const int32_t splits = litekv_paged_decode_int4_splits((int32_t)b, (int32_t)pool.hkv, width, -1, (int32_t)page, &least);
-    if (splits < 1) Py_RETURN_NONE;
-    const size_t partial_bytes = litekv_paged_decode_workspace_bytes((int32_t)b, (int32_t)hq, (int32_t)d, splits);
-    at::Tensor out = at::empty({b, hq, d}, q->options());
+    int32_t splits = 0;
     at::Tensor partials;
-    if (partial_bytes > 0) partials = at::empty({(int64_t)((partial_bytes + 3) / 4)}, q->options().dtype(at::kFloat));
+    size_t partial_bytes = 0;
+    if (n == 12) {
+      const int64_t given = PyLong_AsLongLong(a[9]), given_least = PyLong_AsLongLong(a[10]);
+      if (PyErr_Occurred() || given < 1 || given > 65535 || given_least < 1 || given_least > INT32_MAX) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+      }
+      splits = (int32_t)given;
+      least = (int32_t)given_least;
+      if (a[11] != Py_None) {
+        const at::Tensor *room = gpu_tensor(a[11]);
+        if (room == nullptr || room->scalar_type() != at::kFloat || !room->is_contiguous() || apart(pool, room)) Py_RETURN_NONE;
+        partials = *room;
+        partial_bytes = (size_t)room->numel() * sizeof(float);
+      }
+    } else {
+      splits = litekv_paged_decode_int4_splits((int32_t)b, (int32_t)pool.hkv, width, -1, (int32_t)page, &least);
+      if (splits < 1) Py_RETURN_NONE;
+      partial_bytes = litekv_paged_decode_workspace_bytes((int32_t)b, (int32_t)hq, (int32_t)d, splits);
+      if (partial_bytes > 0) partials = at::empty({(int64_t)((partial_bytes + 3) / 4)}, q->options().dtype(at::kFloat));
+    }
+    at::Tensor out = at::empty({b, hq, d}, q->options());
     const void *qp = address(q), *knp = address(kn), *vnp = address(vn);
     void *pp = address(pool.t), *op = address(&out), *wp = partial_bytes > 0 ? partials.data_ptr() : nullptr;
     const int32_t *tp = static_cast<const int32_t *>(address(table)), *lp = static_cast<const int32_t *>(address(lens));

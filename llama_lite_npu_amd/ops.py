@@ -770,6 +770,15 @@ def decode_step(q: torch.Tensor, kv_pool: torch.Tensor, plan: DecodePlan,
     schedule (``plan.per_sequence``): the same by ``plan.splits`` wavefronts per (sequence, kv
     head); one launch and no merge with one split. An fp8 pool (uint8 / float8_e4m3fn) comes with
     its per-head ``kv_scales``."""
+    if plan.int4 and out is None and kv_scales is None and q.is_cuda:
+        done = _lib.calls().paged_decode_int4(q, kv_pool, plan.block_table, plan.seq_lens, softmax_scale, plan.page_size, k_new, v_new,
+                                              _stream(), plan.splits, plan.min_pages_per_split,
+                                              plan.split_workspace if plan.splits > 1 else None)
+        if done is not None:
+            if type(done) is int:
+                _lib.check(done)
+            return done
+    # (not a plain call, or another pool)
     if plan.per_sequence:
         return paged_decode(q, kv_pool, plan.block_table, plan.seq_lens, softmax_scale, num_splits=plan.splits,
                             min_pages_per_split=plan.min_pages_per_split if plan.int4 else None,

@@ -570,3 +570,23 @@ def test_decode_of_a_query_that_is_not_finite(hq, hkv, d):
         assert np.isnan(got[b, h]).all()
         got[b, h] = want[b, h]
     assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_plan_s_steps_native_and_through_the_wrapper(d):
+    lens = [1500, 3, 0, 2600]
+    s = Sequences(lens, 8, 2, d, 16, seed=d)
+    q, kv = dev(half(s.rng, 4, 8, d)), dev(half(s.rng, 4, 4, d))
+    table, n = dev(s.table), dev(np.array(lens), torch.int32)
+    for splits in (1, 2, 16):
+        pools = [dev(s.pool) for _ in range(2)]
+        plan = ops.DecodePlan(table, n, 8, 2, s.pages, kv_dtype=torch.uint4)
+        plan.set_schedule(splits)
+        out = ops.decode_step(q, pools[0], plan, kv[:, :2], kv[:, 2:], 0.1)
+        mine = torch.empty_like(q)
+        assert ops.decode_step(q, pools[1], plan, kv[:, :2], kv[:, 2:], 0.1, out=mine) is mine
+        assert torch.equal(out, mine) and torch.equal(*pools) and torch.isfinite(out).all()
+        assert torch.equal(out, ops.decode_step(q, pools[0], plan, None, None, 0.1))
+    with pytest.raises(_lib.LiteKVError):
+        plan.split_workspace = plan.split_workspace[:64]
+        ops.decode_step(q, pools[0], plan, None, None, 0.1)
