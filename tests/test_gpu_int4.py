@@ -590,3 +590,30 @@ def test_a_plan_s_steps_native_and_through_the_wrapper(d):
     with pytest.raises(_lib.LiteKVError):
         plan.split_workspace = plan.split_workspace[:64]
         ops.decode_step(q, pools[0], plan, None, None, 0.1)
+
+
+def test_views_strides_and_alignment():
+    """Columns of a wider block table, 64-bit lengths, rows of a fused projection; rows that are not 16-byte aligned are refused."""
+    hq, hkv, d = 16, 4, 128
+    lens = [300, 17, 0, 64]
+    s = Sequences(lens, hq, hkv, d, 16, seed=2)
+    wide = np.full((4, s.table.shape[1] + 9), 7, np.int32)
+    wide[:, 4:4 + s.table.shape[1]] = s.table
+    table = dev(wide)[:, 4:4 + s.table.shape[1]]
+    fused = dev(half(s.rng, 4, hq + 2 * hkv + 1, d))
+    q, k, v = fused[:, :hq], fused[:, hq:hq + hkv], fused[:, hq + hkv:hq + 2 * hkv]
+    n32, n64 = dev(np.array(lens), torch.int32), dev(np.array(lens), torch.int64)
+    pools = [dev(s.pool) for _ in range(3)]
+    want = ops.paged_decode(q.contiguous(), pools[0], dev(s.table), n32, k_new=k.contiguous(), v_new=v.contiguous())
+    assert torch.equal(want, ops.paged_decode(q, pools[1], table, n64, k_new=k, v_new=v)) and torch.equal(pools[0], pools[1])
+    plan = ops.DecodePlan(table, n64, hq, hkv, s.pages, kv_dtype=torch.uint4)
+    assert torch.allclose(want.float(), ops.decode_step(q, pools[2], plan, k, v).float(), atol=2e-3, rtol=1e-2)
+    assert torch.equal(pools[0], pools[2])
+    cu, ctx = torch.tensor([0, 2, 3, 3, 4], device=DEV), torch.tensor([298, 16, 0, 63], device=DEV)
+    chunk = ops.paged_prefill(q, pools[0], table, cu, ctx, 2)
+    assert torch.equal(chunk, ops.paged_prefill(q.contiguous(), pools[0], dev(s.table), cu.int(), ctx.int(), 2))
+    odd = torch.zeros(4 * hq * d + 4, dtype=torch.float16, device=DEV)[4:].view(4, hq, d)
+    with pytest.raises(_lib.LiteKVError, match="aligned"):
+        ops.paged_decode(odd, pools[0], table, n32)
+    with pytest.raises((_lib.LiteKVError, ValueError)):
+        ops.kv_append_quantised(odd[:, :hkv], odd[:, :hkv], n32, pools[0])
