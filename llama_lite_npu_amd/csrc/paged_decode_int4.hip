@@ -555,8 +555,10 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
 
 }  // namespace litekv
 
-// Up to 256 (sequence, kv head) pairs, a compute unit has at most one, and splits of 1024 tokens and more fill the device
-// (8 sequences of 4096 tokens, 8 kv heads: splits of 1024 / 2048 / 4096 tokens 12.9 / 15.7 / 18.4 us). With more, splits only even out
+// Up to 256 (sequence, kv head) pairs, a compute unit has at most one, and splits fill the device: of 512 tokens and more where
+// the longest sequence has over 1024 (8 kv heads: one sequence of 2000 tokens in splits of 512 / 1024 tokens, or unsplit, 9.4 / 11.1 /
+// 11.4 us, six of 2048 10.5 / 11.6 / 11.8, eight of 4096 in splits of 1024 / 2048 12.9 / 15.7, unsplit 18.4; one of 778 in two 9.5 us, unsplit
+// 7.6). With more, splits only even out
 // the lengths (40 of 16384 tokens, 8 kv heads: 137 / 117 / 112 us, 135 unsplit; 64 of them: 214 / 191 / 175 us, 166 unsplit).
 // No more than 16 where that makes them shorter than 4096 tokens: their merge takes longer the more there are (one sequence of 32768
 // tokens, 8 kv heads: 8 / 16 / 32 splits 21.7 / 17.6 / 19.5 us). Powers of two: a captured step holds their number, and growing
@@ -570,8 +572,9 @@ extern "C" int32_t litekv_paged_decode_int4_splits(int32_t batch, int32_t num_kv
   }
   const int64_t pairs = (int64_t)batch * num_kv_heads;
   const bool few = pairs <= 256;
-  const int64_t least = (few ? 1024 : 4096) / page_size;
+  const int64_t least = (few ? 512 : 4096) / page_size;
   *min_pages_per_split = (int32_t)least;
+  if (max_pages * page_size <= 1024) return 1;
   int64_t most = max_pages * page_size / 4096 > 16 ? max_pages * page_size / 4096 : 16;
   if (few) {
     const int64_t rows = total_pages < 0 ? pairs * max_pages : total_pages * num_kv_heads;   // of pages, a head's share each
