@@ -792,7 +792,8 @@ int litekv_paged_prefill_int8(const void *q, int64_t q_token_stride,
  *
  * litekv_paged_decode_int4: litekv_paged_decode (splits, both stages; workspace from
  * litekv_paged_decode_workspace_bytes) over a 4-bit pool, with the step's append fused in where k_new / v_new are not
- * NULL (see litekv_paged_decode_append). litekv_paged_decode_int4_splits: the max_splits that suits a step
+ * NULL (see litekv_paged_decode_append); nothing is stored where the block-table entry of the token names no page of
+ * the pool, which a read takes as the nearest one that there is. litekv_paged_decode_int4_splits: the max_splits that suits a step
  * whose longest sequence has max_pages pages and all of them total_pages (-1: batch * max_pages); *min_pages_per_split
  * depends on batch, num_kv_heads and page_size only. 0 for arguments that no step has.
  *

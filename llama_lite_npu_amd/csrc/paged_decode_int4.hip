@@ -179,15 +179,17 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   auto block_of = [&](int p, int entry) { return sub_page_id(entry, place(p), page_shift, num_pages); };
 
   // The step's new token goes into the last block before anything of it is read (by this wavefront, the only one that reads it
-  // in this launch; the slices of a wide group all write the same bytes).
+  // in this launch; the slices of a wide group all write the same bytes). Reads take a page id outside the pool as the nearest one
+  // inside, whose rows are another sequence's: nothing is stored through such an id.
   if (k_new != nullptr && any && p1 == pages && pages <= (bt_stride << page_shift)) {
-    if (lane < 2 * L) {
+    const int entry = first_entry_of(pages - 1);
+    if (lane < 2 * L && entry >= 0 && entry < num_pages) {
       const bool is_v = lane >= L;
       const int l = lane & (L - 1);
       float x[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = (float)new_row[i];
-      const int64_t slot = (int64_t)block_of(pages - 1, first_entry_of(pages - 1)) * kInt4Block + ((len - 1) & (kInt4Block - 1));
+      const int64_t slot = (int64_t)block_of(pages - 1, entry) * kInt4Block + ((len - 1) & (kInt4Block - 1));
       int4_store<D>(pool, slot, num_kv_heads, is_v ? num_kv_heads + h : h, l, int4_row<L>(x));
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
