@@ -7,8 +7,10 @@
 //     O[d] = sum_i (p_i s'_i) (c'_id - z'_i)       p = softmax of S, s', z', c' those of V
 // so a scale and a zero point cost a few instructions per key instead of one per element. Codes reach the matrix cores with
 // nothing but shifts and masks:
-//  * K as bytes. A nibble in the low half of a byte is the fp8 number c * 2^-9, exactly; q is a sum of three fp8 numbers, which
-//    leaves 2^-18 of its row's largest. S^T is three 16x16x128 products per 16 keys, two with heads of 64.
+//  * K as bytes. A nibble in the low half of a byte is the fp8 (E4M3) number c * 2^-9, exactly. q is a sum of three E5M2 numbers, whose
+//    3 + 4 + 4 bits (a sign between them is a bit) are an fp16 number's 11: exact for elements down to 2^-21 of their row's
+//    largest, off by at most 2^-31 of that below. (Three E4M3 numbers are 12 bits of the largest, but end 2^-18 below it: beside
+//    a channel of 1000, elements of 0.1 are up to 4% off.) S^T is three 16x16x128 products per 16 keys, two with heads of 64.
 //  * V as fp16. c in bits 4 .. 7 is the subnormal c * 2^-20. The matrix cores take it as it is, but do not normalise it: products are
 //    lined up by the exponents of their factors and cut off some 27 bits below the largest of a sum. From bits 4 .. 7 that leaves 24
 //    bits of a code's own size; in bits 0 .. 3, which need two instructions fewer for eight codes, 20 (333 keys with one that
@@ -82,9 +84,9 @@ __device__ __forceinline__ int8v_t int4_k_bytes(const uint32_t (&k)[D / 32]) {
   }
   return a;
 }
-// D(16x16) += A(16x128) * B(128x16), fp8: lane l supplies 32 bytes of row (column) l % 16, at 32 * (l / 16).
-__device__ __forceinline__ float4_t mfma_16x16x128_fp8(int8v_t a, int8v_t b, float4_t c) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+// D(16x16) += A(16x128) * B(128x16), A in E4M3, B in E5M2: lane l supplies 32 bytes of row (column) l % 16, at 32 * (l / 16).
+__device__ __forceinline__ float4_t mfma_16x16x128_bytes(int8v_t a, int8v_t b, float4_t c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 1, 0, 0, 0, 0);
 }
 
 // Eight codes of V in a dword as fp16 pairs, times 2^-20.
@@ -244,8 +246,8 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   for (int i = 0; i < kDepth; ++i) request_pair(p0 + 2 * i, buf[i]);
 
   // q as the right operand of the first product: column n, the elements of the bytes that the lane of the same g holds of K,
-  // as a sum of three fp8 numbers (4 + 4 + 4 bits), scaled by a power of two that puts the row's largest between 224 and 448. What
-  // that leaves of an element is 2^-10, some 2^-18 of the largest. Made once for the workgroup and handed out through LDS.
+  // as a sum of three E5M2 numbers, scaled by a power of two that puts the row's largest between 28672 and 57344. What that leaves of an
+  // element of less than 2^-6 is at most 2^-17, of the others nothing. Made once for the workgroup and handed out through LDS.
   constexpr int kParts = 3, kProducts = D == 128 ? 3 : 2;   // D = 64: two parts side by side in the 128 of one product
   extern __shared__ __attribute__((aligned(16))) float int4_lds[];
   constexpr int kRowBytes = kParts * D + 16;                // of a row of q: the parts, the sum and the factor of its scores
@@ -254,7 +256,7 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   if (wave < kHeads * L / kWave) {
     const int l = threadIdx.x % L;
     char *row = q_rows + (threadIdx.x / L) * kRowBytes;
-    float x[8], most = 0.f, sum = 0.f, odd = 0.f;   // odd: an element that is not finite, which fp8 would saturate
+    float x[8], most = 0.f, sum = 0.f, odd = 0.f;   // odd: an element that is not finite
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       x[i] = (float)q_in[i];
@@ -263,25 +265,25 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
     }
     most = over_row<L>(most, [](float a, float b) { return __builtin_fmaxf(a, b); });
     odd = over_row<L>(odd, [](float a, float b) { return a + b; });
-    int up = most > 0.f ? 9 - __builtin_amdgcn_frexp_expf(most) : 0;
-    if (__builtin_amdgcn_ldexpf(most, up) > 448.f) --up;
+    int up = most > 0.f ? 16 - __builtin_amdgcn_frexp_expf(most) : 0;
+    if (__builtin_amdgcn_ldexpf(most, up) > 57344.f) --up;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_ldexpf(x[i], up);
+    for (int i = 0; i < 8; ++i) {
+      x[i] = __builtin_amdgcn_ldexpf(x[i], up);
+      sum += x[i];
+    }
 #pragma unroll
     for (int part = 0; part < kParts; ++part) {
       uint2v_t bytes;   // elements of the lower and of the upper nibbles
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         constexpr int kOrder[2][4] = {{0, 4, 1, 5}, {2, 6, 3, 7}};
-        int four = __builtin_amdgcn_cvt_pk_fp8_f32(x[kOrder[u][0]], x[kOrder[u][1]], 0, false);
-        four = __builtin_amdgcn_cvt_pk_fp8_f32(x[kOrder[u][2]], x[kOrder[u][3]], four, true);
-        const float back[4] = {__builtin_amdgcn_cvt_f32_fp8(four, 0), __builtin_amdgcn_cvt_f32_fp8(four, 1),
-                               __builtin_amdgcn_cvt_f32_fp8(four, 2), __builtin_amdgcn_cvt_f32_fp8(four, 3)};
+        int four = __builtin_amdgcn_cvt_pk_bf8_f32(x[kOrder[u][0]], x[kOrder[u][1]], 0, false);
+        four = __builtin_amdgcn_cvt_pk_bf8_f32(x[kOrder[u][2]], x[kOrder[u][3]], four, true);
+        const float back[4] = {__builtin_amdgcn_cvt_f32_bf8(four, 0), __builtin_amdgcn_cvt_f32_bf8(four, 1),
+                               __builtin_amdgcn_cvt_f32_bf8(four, 2), __builtin_amdgcn_cvt_f32_bf8(four, 3)};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sum += back[i];
-          x[kOrder[u][i]] -= back[i];
-        }
+        for (int i = 0; i < 4; ++i) x[kOrder[u][i]] -= back[i];
         bytes[u] = (uint32_t)four;
       }
       *(uint2v_t *)(row + part * D + 8 * l) = bytes;
@@ -342,7 +344,7 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
       const int8v_t a = int4_k_bytes<D>(r[u].k);
       st[u] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < kProducts; ++i) st[u] = mfma_16x16x128_fp8(a, qf[i], st[u]);
+      for (int i = 0; i < kProducts; ++i) st[u] = mfma_16x16x128_bytes(a, qf[i], st[u]);
     }
     uint32_t kw[kKeys / 2], vw[kKeys / 2];   // words of the lane's keys 2i, 2i + 1
     uint32_t vz[4];                          // z' of the eight keys of its g, times 2^-20

@@ -1,4 +1,5 @@
-"""4-bit pools where a call can go wrong without showing it: page ids that name no page."""
+"""4-bit pools where a call can go wrong without showing it: page ids that name no page, queries with a large
+channel."""
 
 import math
 
@@ -8,7 +9,7 @@ import torch
 
 from llama_lite_npu_amd import ops
 from oracle import int4
-from tests.test_gpu_int4 import Sequences, check, dev, half
+from tests.test_gpu_int4 import HALF, Sequences, check, dev, half
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +41,38 @@ def test_nothing_is_appended_through_an_id_that_names_no_page(hq, hkv, d, page, 
     assert np.array_equal(stepped.cpu().numpy(), want)
     s.pool = want
     check(out, q, s, lambda b: ([b], [lens[b]]) if b in good else ([], []), 1 / math.sqrt(d), 2.0 ** -19)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(16, 4, 128), (16, 4, 64), (12, 1, 128), (12, 1, 64)])
+@pytest.mark.parametrize("large", [100.0, 1000.0, 30000.0])
+def test_a_large_channel_of_q_leaves_the_others_their_bits(hq, hkv, d, large):
+    """One channel of q is hundreds of times the others, as in models without norms of q and k, and K is small there: scores are made by
+    the small elements, every one of which is an error of the same sign if it is held relative to the row's largest."""
+    lens = [2, 3, 17, 40, 300]
+    at = d // 3
+
+    def rows(rng, n, h2, d):
+        x = half(rng, n, h2, d)
+        x[:, : h2 // 2] = np.float16(0.5) * rng.choice([-1.0, 1.0], (n, h2 // 2, 1))
+        x[:, : h2 // 2, at] = 0
+        return x
+
+    s = Sequences(lens, hq, hkv, d, 16, seed=d, rows=rows)
+    q = (np.ones((len(lens), hq, d)) * s.rng.uniform(0.05, 0.2, (len(lens), hq, 1))).astype(np.float16)
+    q[..., at] = large
+    scale = 1 / math.sqrt(d)
+    for n in (1, 3):
+        got = ops.paged_decode(dev(q), dev(s.pool), dev(s.table), dev(np.array(lens), torch.int32), scale, num_splits=n).cpu().numpy()
+        for b, length in enumerate(lens):
+            k, v = s.values(b)
+            want, size = int4.attend(q[[b]], k, v, scale, [length])
+            # a score: codes up to 15 steps of 0.5 / 15, whose products with q are summed in fp32. The row's own sum, times the zero
+            # point, goes the same way. Three sums of 128 products and the zero point's: 2^-24 of the whole's size each, and 2^-27 of the
+            # largest product for each one added to it
+            codes = 0.5 * 1.02
+            whole = codes * (large + 0.2 * d) * scale
+            error = 2 * 2.0 ** -24 * 4 * whole + 2 * d * 2.0 ** -27 * codes * large * scale
+            rel = 2 * (math.expm1(error) + 2.0 ** -19) + 2.0 ** -18
+            allowed = HALF * np.abs(want) + 2.0 ** -25 + rel * (size + np.abs(want)) + 2.0 ** -20 * np.abs(v).max()
+            off = np.abs(got[[b]].astype(np.float64) - want)
+            assert (off <= allowed).all(), (b, n, float((off / allowed).max()))
