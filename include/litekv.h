@@ -595,7 +595,8 @@ int litekv_paged_prefill_bounded(const void *q, int64_t q_token_stride,
  *       gives, against a merge launch and a partial row per query row, head
  *       and slice; 1: do not split (call litekv_paged_prefill) -- launches
  *       that fill the device, short histories, fresh prompts
- *   num_tokens    T, the query rows of the launch (= cu_q_lens[batch])
+ *   num_tokens    T, the query rows of the launch (cu_q_lens[batch] of them, or
+ *                 more: those behind are not written)
  *   workspace     litekv_paged_prefill_split_workspace_bytes(T, Hq, D,
  *                 key_slices) bytes, 16-byte aligned; launches that share it
  *                 must be ordered on one stream

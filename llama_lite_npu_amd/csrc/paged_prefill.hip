@@ -56,13 +56,15 @@ static PrefillShape prefill_shape(int group, int max_q_len, int wg_col_tiles = k
 
 // Folds the key slices of a split prefill: the lanes of a (query row, head), four elements each, read the row's
 // `slices` log-sum-exps and partial rows (fp32, normalised per slice) and write the fp16 row. A slice without keys has
-// log-sum-exp -inf and weight 0; the last slice always has keys. Bound by memory trips, then by memory: no lane needs another's
+// log-sum-exp -inf and weight 0; the last slice always has keys. Rows behind the last sequence, which no slice wrote, are left as they
+// are in `out` (their cells are read, and only the store waits for the number of rows). Bound by memory trips, then by memory: no lane needs another's
 // numbers, and all loads are ahead of the arithmetic (64 rows of 16 heads of 128 in 8 slices 3.8 us, 1224 rows of 32 heads
 // of 64 in 2 7.7; with a wavefront a row that gathers them by shuffles 5.5 and 15).
 constexpr int kMergeLanes = kHD / 4, kMergeRows = 4 * kWave / kMergeLanes;   // of a row; rows of a workgroup
 __global__ __launch_bounds__(4 * kWave) void prefill_split_merge_kernel(
     const float *__restrict__ part_o, const float *__restrict__ part_lse, half_t *__restrict__ out,
-    int64_t out_stride, int64_t num_tokens, int32_t num_q_heads, int32_t slices) {
+    int64_t out_stride, int64_t num_tokens, int32_t num_q_heads, int32_t slices, const int32_t *__restrict__ live_rows) {
+  const int live = *as_uniform(live_rows);
   const int at = 4 * (threadIdx.x % kMergeLanes);
   const int64_t id = (int64_t)blockIdx.x * kMergeRows + threadIdx.x / kMergeLanes;
   if (id >= num_tokens * num_q_heads) return;
@@ -92,6 +94,7 @@ __global__ __launch_bounds__(4 * kWave) void prefill_split_merge_kernel(
     }
   }
   const float inv = 1.0f / den;
+  if (token >= live) return;
   *(half4_t *)(out + token * out_stride + (int64_t)head * kHD + at) =
       half4_t{(half_t)(o[0] * inv), (half_t)(o[1] * inv), (half_t)(o[2] * inv), (half_t)(o[3] * inv)};
 }
@@ -339,7 +342,7 @@ static int launch_paged_prefill(const char *what, const void *q, int64_t q_token
     const int64_t merge_rows = rows * num_q_heads;
     hipLaunchKernelGGL(prefill_split_merge_kernel, dim3((unsigned)((merge_rows + kMergeRows - 1) / kMergeRows)), dim3(4 * kWave), 0,
                        static_cast<hipStream_t>(stream), part_o, part_lse, static_cast<half_t *>(out),
-                       out_token_stride, rows, num_q_heads, slices);
+                       out_token_stride, rows, num_q_heads, slices, cu_q_lens + batch);
     return check_launch(what);
   }
 #endif  // LITEKV_HD != 256

@@ -1,5 +1,5 @@
-"""4-bit pools where a call can go wrong without showing it: page ids that name no page, queries with a large
-channel."""
+"""4-bit pools where a call can go wrong without showing it: page ids that name no page, queries with a large channel, rows
+behind the last sequence."""
 
 import math
 
@@ -9,7 +9,7 @@ import torch
 
 from llama_lite_npu_amd import ops
 from oracle import int4
-from tests.test_gpu_int4 import HALF, Sequences, check, dev, half
+from tests.test_gpu_int4 import DEV, HALF, Sequences, check, dev, half
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +76,26 @@ def test_a_large_channel_of_q_leaves_the_others_their_bits(hq, hkv, d, large):
             allowed = HALF * np.abs(want) + 2.0 ** -25 + rel * (size + np.abs(want)) + 2.0 ** -20 * np.abs(v).max()
             off = np.abs(got[[b]].astype(np.float64) - want)
             assert (off <= allowed).all(), (b, n, float((off / allowed).max()))
+
+
+@pytest.mark.parametrize("fmt", ["fp16", "int4"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_behind_the_last_sequence_are_left_as_they_were(fmt, d):
+    """A launch over key slices folds the rows that cu_q_lens names, whatever the tensors have behind them."""
+    hq, hkv, rows, history, behind = 16, 4, [40, 25], [300, 700], 9
+    lens = [r + h for r, h in zip(rows, history)]
+    s = Sequences(lens, hq, hkv, d, 16, seed=d)
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    q = half(s.rng, int(cu[-1]) + behind, hq, d)
+    pool = dev(s.pool)
+    if fmt == "fp16":
+        values, _ = int4.decode_pool(s.pool, hkv, d)
+        pool = dev(np.nan_to_num(values).astype(np.float16))
+    args = dev(s.table), dev(cu, torch.int32), dev(np.array(history), torch.int32), max(rows), 1 / math.sqrt(d)
+    for slices in (1, 2, 8):
+        room = torch.full((ops.paged_prefill_workspace_floats(len(q), hq, d, max(2, slices)),), 77.0, device=DEV)
+        out = torch.full((len(q), hq, d), 5.0, dtype=torch.float16, device=DEV)
+        assert ops.paged_prefill(dev(q), pool, *args, out=out, key_slices=slices, workspace=room) is out
+        assert (out[cu[-1]:] == 5.0).all(), slices
+        check(out.cpu().numpy(), q, s, lambda b: (list(range(cu[b], cu[b + 1])), [history[b] + i + 1 for i in range(rows[b])]),
+              1 / math.sqrt(d), HALF + 2.0 ** -25 * max(lens))
