@@ -821,11 +821,16 @@ __device__ __forceinline__ void prefill_tile_body(
       const uint32_t tile_at = (uint32_t)((kt & 1) * kTileHalfs + kRowsPerWave * wave * kHD) * 2u;
       const uint32_t kw = raw4_kw | (raw4_kw << 16);
       const int kr = lane >> 2;
+      // The swizzles are linear in these numbers (the low bits of a chunk, of a row), so one address each for K and V, made
+      // in the tile, serves all stores: an address a store, made ahead of the loop, was six registers.
+      const uint32_t k_to = k_lds + tile_at + (uint32_t)(2 * kHD * kr) + 16u * (uint32_t)((kHD / 32) * (lane & 3) ^ k_swz(kr));
+      const uint32_t v_to = v_lds + tile_at + (uint32_t)(2 * kHD * 4 * g) +
+                            (kHD == 128 ? 16u * (uint32_t)(n ^ v_swz(4 * g))
+                                        : 16u * (uint32_t)((n >> 1) ^ v_swz(4 * g)) + 8u * (uint32_t)(n & 1));
+      auto v_row_to = [&](int i) { return (v_to ^ (16u * (uint32_t)v_swz(i))) + (uint32_t)(2 * kHD * i); };   // of rows 4g + i
 #pragma unroll
       for (int j = 0; j < kHD / 32; ++j) {
-        const int chunk = (kHD / 32) * (lane & 3) + j;
-        *(lds_half8_t *)(uintptr_t)(k_lds + tile_at + (uint32_t)(2 * kHD * kr) + 16u * (uint32_t)(chunk ^ k_swz(kr))) =
-            int4x8_to_half(raw4_k[j], kw);
+        *(lds_half8_t *)(uintptr_t)(k_to ^ (16u * (uint32_t)j)) = int4x8_to_half(raw4_k[j], kw);
       }
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
@@ -835,18 +840,14 @@ __device__ __forceinline__ void prefill_tile_body(
             // row 4g + 2p + b2: its halves of the two units' dwords
             const uint32_t x = __builtin_amdgcn_perm(raw4_v[2 * p + 1], raw4_v[2 * p], b2 ? 0x07060302u : 0x05040100u);
             const uint32_t w = __builtin_amdgcn_perm(0u, raw4_vw[p], b2 ? 0x03020302u : 0x01000100u);
-            const int r = 4 * g + 2 * p + b2;
-            *(lds_half8_t *)(uintptr_t)(v_lds + tile_at + (uint32_t)(2 * kHD * r) + 16u * (uint32_t)(n ^ v_swz(r))) =
-                int4x8_to_half(x, w);
+            *(lds_half8_t *)(uintptr_t)v_row_to(2 * p + b2) = int4x8_to_half(x, w);
           }
         } else {
           // four elements of two rows at once, each row's under its own scale, then row by row
           const half8_t y = int4x8_to_half(raw4_v[p], raw4_vw[p]);  // element j of rows 4g + 2p, 4g + 2p + 1
 #pragma unroll
           for (int b2 = 0; b2 < 2; ++b2) {
-            const int r = 4 * g + 2 * p + b2;
-            *(__attribute__((address_space(3))) half4_t *)(uintptr_t)(
-                v_lds + tile_at + (uint32_t)(2 * kHD * r) + 16u * (uint32_t)((n >> 1) ^ v_swz(r)) + 8u * (uint32_t)(n & 1)) =
+            *(__attribute__((address_space(3))) half4_t *)(uintptr_t)v_row_to(2 * p + b2) =
                 half4_t{y[b2], y[2 + b2], y[4 + b2], y[6 + b2]};
           }
         }
