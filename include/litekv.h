@@ -256,7 +256,8 @@ int litekv_paged_decode_static(const void *q, int64_t q_batch_stride, const void
  * strides given) the launch also performs this step's KV append: the rows are
  * written, bit exact, to logical position seq_lens[b] - 1 of sequence b (the
  * slot the reference passes as cur_select_index, paged_attention.py:310-317)
- * and take part in the attention. It replaces
+ * and take part in the attention; where the block-table entry of that position
+ * names no page of the pool nothing is stored. It replaces
  * the separate update_kv_buffer launch of Attention.token_forward
  * (lite_llama/models/qwen3.py:53-75).
  *
@@ -426,7 +427,8 @@ int litekv_paged_decode_fp8(const void *q, int64_t q_batch_stride, const void *k
  * attends a sequence's last page first writes the step's token (rows k_new[b],
  * v_new[b] of [batch][num_kv_heads][128] fp16, element strides per sequence)
  * at logical position seq_lens[b] - 1 of the pages the block table names, as
- * litekv_kv_append would through that token's slot, and attends it. Replaces,
+ * litekv_kv_append would through that token's slot (nothing is stored where
+ * the entry names no page of the pool), and attends it. Replaces,
  * in one launch for max_splits == 1, the reference's per-layer pair
  * update_kv_buffer + flash_decoding (models/qwen3.py:62-74;
  * kernels/update_kv_buffer.py:46-81, kernels/flashdecoding.py:294-342) for

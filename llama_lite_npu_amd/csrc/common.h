@@ -79,6 +79,9 @@ constexpr int kMaxPrefixSplits = 8;
 // spans); per sequence the position of its first 16-token page on the line; the chunk entries.
 constexpr int kPlanMeta = 16;      // int32 words of plan meta data
 constexpr int kEntryHeader = 8;    // int32 words of an entry before its page ids
+// Beside a page id of a plan: the block-table entry names no page of the pool. The id is where reads go all the same, and nothing
+// is stored through it. (Ids of 16-token pages, whose slots are numbered in 32 bits, end at 2^27.)
+constexpr int kNoPage = 1 << 30;
 // plan meta words
 constexpr int kMetaTotal = 0, kMetaChunkPages = 1, kMetaChunks = 2, kMetaBatch = 3,
               kMetaEntryStride = 4, kMetaKvHeads = 5, kMetaSkip = 6;
@@ -228,9 +231,12 @@ int launch_generic_attention(const char *what, const GenericLaunch &a);
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float fast_log2(float x) { return __builtin_amdgcn_logf(x); }
 
+// Reads take a page id outside the pool as the nearest one inside (block tables live on the device, where the host cannot check
+// them). Nothing is stored through such an id: the row would be another sequence's.
 __device__ __forceinline__ int clamp_page(int pid, int num_pages) {
   return pid < 0 ? 0 : (pid >= num_pages ? num_pages - 1 : pid);
 }
+__device__ __forceinline__ bool names_page(int pid, int num_pages) { return (uint32_t)pid < (uint32_t)num_pages; }
 
 // Pools whose pages hold 16 << shift tokens: the kernels keep working on 16-token pages, and the
 // 16-token page j of a sequence is part j % (1 << shift) of the sequence's page j >> shift, whose

@@ -177,15 +177,16 @@ __global__ __launch_bounds__(kWave) void generic_attention_kernel(GenericTask t)
   const int entry_stride = planned ? t.plan[kMetaEntryStride] : 0;
   const int before = planned ? t.plan[plan_seq_before_offset(plan_batch) + b] : 0;
   // the K row of key `tok` (V: + num_kv_heads * D elements in a pool)
+  auto planned_id = [&](int tok) -> int {
+    // the plan holds at most a block-table row's worth of 16-token pages per sequence
+    const int cap16 = t.bt_stride * (t.page_size >> 4);
+    const int f = before + ((tok >> 4) < cap16 ? (tok >> 4) : cap16 - 1);
+    const int c = cut.chunk_of(f);
+    return t.plan[plan_entries_offset(plan_batch) + (int64_t)c * entry_stride + kEntryHeader + (f - cut.chunk_start(c))];
+  };
   auto k_row_of = [&](int tok) -> const char * {
     if (planned) {
-      // the plan holds at most a block-table row's worth of 16-token pages per sequence
-      const int cap16 = t.bt_stride * (t.page_size >> 4);
-      const int f = before + ((tok >> 4) < cap16 ? (tok >> 4) : cap16 - 1);
-      const int c = cut.chunk_of(f);
-      const int pid16 = t.plan[plan_entries_offset(plan_batch) + (int64_t)c * entry_stride + kEntryHeader +
-                               (f - cut.chunk_start(c))];
-      const int64_t slot = (int64_t)pid16 * 16 + (tok & 15);
+      const int64_t slot = (int64_t)(planned_id(tok) & ~kNoPage) * 16 + (tok & 15);
       return (const char *)t.kv_pool + slot * slot_bytes + (int64_t)h * D * elem;
     }
     if (paged) {
@@ -206,9 +207,12 @@ __global__ __launch_bounds__(kWave) void generic_attention_kernel(GenericTask t)
   };
 
   // the step's new rows of this head, if this launch appends them (not for a length beyond what
-  // the block-table row can name: the row's last page is not where that token belongs)
-  const bool appends = t.k_new != nullptr &&
-                       (int64_t)n_keys <= (int64_t)t.bt_stride * t.page_size;
+  // the block-table row can name, whose last page is not where that token belongs, nor where its entry names
+  // no page)
+  bool appends = t.k_new != nullptr && (int64_t)n_keys <= (int64_t)t.bt_stride * t.page_size;
+  if (appends) {
+    appends = planned ? (planned_id(n_keys - 1) & kNoPage) == 0 : names_page(table[(n_keys - 1) / t.page_size], t.num_pages);
+  }
   const half_t *k_new = appends ? t.k_new + (int64_t)b * t.k_new_stride + (int64_t)h * D : nullptr;
   const half_t *v_new = appends ? t.v_new + (int64_t)b * t.v_new_stride + (int64_t)h * D : nullptr;
 

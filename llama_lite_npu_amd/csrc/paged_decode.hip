@@ -784,17 +784,20 @@ paged_decode_split_kernel(
   // first: there an id per page, through scalar loads a step ahead of their use, is faster than
   // the window and requests in front of the length (16 splits, 32 / 4 heads: 64 sequences of 4k to
   // 16k tokens 230.6 against 237.6 us, 128 of 8k to 32k 816 against 824).
-  auto page_id = [&](int p) {
-    const int pp = p < p1 ? p : p1 - 1;
+  auto entry_of = [&](int pp) {   // the block-table entry of page pp, as it stands there
     int at = pp >> page_shift;
     at = at < bt_stride ? at : bt_stride - 1;
-    if constexpr (ORDERED) return sub_page_id(table[at], pp, page_shift, num_pages);
+    if constexpr (ORDERED) return table[at];
     if (at - win0 >= kWave) {
       win0 = at;
       ids = table[at + lane < bt_stride ? at + lane : bt_stride - 1];
       wait_vector_loads();
     }
-    return sub_page_id(__builtin_amdgcn_readlane(ids, at - win0), pp, page_shift, num_pages);
+    return (int32_t)__builtin_amdgcn_readlane(ids, at - win0);
+  };
+  auto page_id = [&](int p) {
+    const int pp = p < p1 ? p : p1 - 1;
+    return sub_page_id(entry_of(pp), pp, page_shift, num_pages);
   };
   int pid_next = page_id(p0);
   auto request = [&](int p, Page &r) {
@@ -816,7 +819,7 @@ paged_decode_split_kernel(
   auto last_pair = [&](int p, auto at) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      if (APPEND && fits_table && p + u < p1 && (p + u + 1) * kPageSize >= len) {
+      if (APPEND && fits_table && p + u < p1 && (p + u + 1) * kPageSize >= len && names_page(entry_of(p + u), num_pages)) {
         // The sequence's last page: the step's new token (logical position len - 1) goes to
         // the pool and replaces the stale values this wavefront loaded before the write; an
         // fp8 pool gets the codes the append kernel would store and is attended as stored.
@@ -1060,7 +1063,7 @@ __global__ __launch_bounds__(kWave) void paged_decode_merge_kernel(
 //   entry[2] sequence of the first page (low half) and the next sequence with pages (high half)
 //   entry[3], entry[4] the first sequence's [first, last) page, entry[7] its length
 //   entry[5], entry[6] for the merge by chunk boundary (see decode_plan_kernel)
-//   entry[8 ..] the chunk's physical page ids, in line order
+//   entry[8 ..] the chunk's physical page ids, in line order (with kNoPage where the block-table entry named none)
 // so a wavefront needs one dependent hop (its entry) before it can request q, K and V.
 //
 // The piece of sequence b inside chunk c is partial slot c + b (strictly increasing along the
@@ -1172,8 +1175,9 @@ __global__ __launch_bounds__(256) void decode_plan_kernel(
     const int c = chunk_of(f);
     const int first = chunk_start(c);
     int32_t *e = entries + (int64_t)c * entry_stride;
+    const int entry = row[(p + skip) >> page_shift];
     e[kEntryHeader + (f - first)] =
-        sub_page_id(row[(p + skip) >> page_shift], p + skip, page_shift, num_pages);
+        sub_page_id(entry, p + skip, page_shift, num_pages) | (names_page(entry, num_pages) ? 0 : kNoPage);
     if (f == first) {
       e[0] = f;
       e[1] = chunk_start(c + 1);

@@ -181,11 +181,10 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   auto block_of = [&](int p, int entry) { return sub_page_id(entry, place(p), page_shift, num_pages); };
 
   // The step's new token goes into the last block before anything of it is read (by this wavefront, the only one that reads it
-  // in this launch; the slices of a wide group all write the same bytes). Reads take a page id outside the pool as the nearest one
-  // inside, whose rows are another sequence's: nothing is stored through such an id.
+  // in this launch; the slices of a wide group all write the same bytes).
   if (k_new != nullptr && any && p1 == pages && pages <= (bt_stride << page_shift)) {
     const int entry = first_entry_of(pages - 1);
-    if (lane < 2 * L && entry >= 0 && entry < num_pages) {
+    if (lane < 2 * L && names_page(entry, num_pages)) {
       const bool is_v = lane >= L;
       const int l = lane & (L - 1);
       float x[8];

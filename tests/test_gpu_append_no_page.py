@@ -1,0 +1,86 @@
+"""The append fused into a decode step, where the block-table entry of the new token names no page of the pool: nothing is stored for
+that sequence (as the append on its own skips a slot outside the pool), and the other sequences' steps are what they are without it."""
+
+import pytest
+import torch
+
+from llama_lite_npu_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+LENS = [33, 70, 1, 129, 600, 16, 257, 48, 0]
+BAD = {0: -1, 1: "pages", 3: 2 ** 31 - 1, 4: -2 ** 31, 7: "beyond"}
+FORMATS = {"fp16": torch.float16, "fp8": torch.float8_e4m3fn, "int8": torch.int8}
+
+
+class Case:
+    def __init__(self, fmt, hq, hkv, d, page, shared=0):
+        g = torch.Generator(device=DEV).manual_seed(hq + d + page)
+        randn = lambda *s: torch.randn(s, generator=g, device=DEV).half()  # noqa: E731
+        self.hq, self.hkv, self.page, self.shared = hq, hkv, page, shared
+        lens = [n + shared * page if n else 0 for n in LENS]
+        each = [-(-n // page) - (shared if n else 0) for n in lens]
+        self.pages = shared + sum(each) + 2
+        order = torch.randperm(self.pages - 1, generator=g, device=DEV) + 1     # (page 0 is nobody's, the last one is somebody's)
+        table = torch.zeros((len(lens), shared + max(each) + 1), dtype=torch.int32, device=DEV)
+        table[:, :shared] = order[:shared]
+        at = shared
+        for b, n in enumerate(each):
+            table[b, shared:shared + n] = order[at:at + n]
+            at += n
+        self.slots = torch.full((len(lens),), -1, dtype=torch.int32, device=DEV)
+        for b, n in enumerate(lens):
+            if b in BAD:
+                table[b, (n - 1) // page] = {"pages": self.pages, "beyond": self.pages + 9}.get(BAD[b], BAD[b])
+            elif n:
+                self.slots[b] = int(table[b, (n - 1) // page]) * page + (n - 1) % page
+        self.table, self.lens = table, torch.tensor(lens, dtype=torch.int32, device=DEV)
+        self.good = [b for b in range(len(lens)) if b not in BAD]
+        self.scales = None if fmt == "fp16" else torch.full((2 * hkv,), 0.03, device=DEV)
+        values = randn(self.pages * page, 2 * hkv, d)
+        if fmt == "fp16":
+            self.pool = values
+        else:
+            self.pool = torch.zeros(values.shape, dtype=torch.uint8, device=DEV).view(FORMATS[fmt])
+            slots = torch.arange(self.pages * page, dtype=torch.int32, device=DEV)
+            ops.kv_append_quantised(values[:, :hkv], values[:, hkv:], slots, self.pool, self.scales)
+        self.q, self.k, self.v = randn(len(lens), hq, d), randn(len(lens), hkv, d), randn(len(lens), hkv, d)
+
+    def appended(self):
+        pool = self.pool.clone()
+        if self.scales is None:
+            ops.kv_append(self.k, self.v, self.slots, pool)
+        else:
+            ops.kv_append_quantised(self.k, self.v, self.slots, pool, self.scales)
+        return pool
+
+    def check(self, step):
+        want, got = self.appended(), self.pool.clone()
+        out = step(got, self.k, self.v)
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+        plain = step(want, None, None)
+        assert torch.equal(out[self.good], plain[self.good]) and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("fmt", list(FORMATS))
+@pytest.mark.parametrize("hq,hkv,d,page", [(16, 4, 128, 16), (16, 4, 64, 64), (20, 1, 128, 32), (6, 2, 32, 16), (4, 2, 256, 16)])
+@pytest.mark.parametrize("splits", [1, 4])
+def test_splits(fmt, hq, hkv, d, page, splits):
+    c = Case(fmt, hq, hkv, d, page)
+    c.check(lambda pool, k, v: ops.paged_decode(c.q, pool, c.table, c.lens, page_size=page, num_splits=splits, kv_scales=c.scales,
+                                                k_new=k, v_new=v))
+
+
+@pytest.mark.parametrize("fmt", list(FORMATS))
+@pytest.mark.parametrize("hq,hkv,d,page", [(16, 4, 128, 16), (16, 4, 64, 64), (20, 1, 128, 32), (6, 2, 32, 16), (4, 2, 256, 16)])
+@pytest.mark.parametrize("chunks", [None, 3])
+@pytest.mark.parametrize("shared", [0, 4])
+def test_balanced_schedule_and_shared_prefix(fmt, hq, hkv, d, page, chunks, shared):
+    if shared and d not in (64, 128):
+        pytest.skip("a shared prefix takes head_dim 64 or 128")
+    c = Case(fmt, hq, hkv, d, page, shared)
+    plan = ops.DecodePlan(c.table, c.lens, hq, hkv, c.pages, page_size=page, shared_pages=shared, chunks=chunks,
+                          token_bytes=2 * hkv * d * c.pool.element_size(), kv_dtype=c.pool.dtype)
+    plan.set_schedule(0)
+    plan.refresh()
+    c.check(lambda pool, k, v: ops.decode_step(c.q, pool, plan, k, v, 0.1, kv_scales=c.scales))
