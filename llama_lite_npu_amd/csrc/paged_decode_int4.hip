@@ -7,10 +7,12 @@
 //     O[d] = sum_i (p_i s'_i) (c'_id - z'_i)       p = softmax of S, s', z', c' those of V
 // so a scale and a zero point cost a few instructions per key instead of one per element. Codes reach the matrix cores with
 // nothing but shifts and masks:
-//  * K as bytes. A nibble in the low half of a byte is the fp8 (E4M3) number c * 2^-9, exactly. q is a sum of three E5M2 numbers, whose
-//    3 + 4 + 4 bits (a sign between them is a bit) are an fp16 number's 11: exact for elements down to 2^-21 of their row's
-//    largest, off by at most 2^-31 of that below. (Three E4M3 numbers are 12 bits of the largest, but end 2^-18 below it: beside
-//    a channel of 1000, elements of 0.1 are up to 4% off.) S^T is three 16x16x128 products per 16 keys, two with heads of 64.
+//  * K as int8: a nibble in the low half of a byte. q is a fixed-point number in four int8 digits to the base 256, with the row's
+//    largest element between 2^29 and 2^30 units: elements are exact down to 2^-19 of the largest, off by half a unit below that.
+//    Products of integers are exact, whatever they stand beside. (Three 8-bit floating-point numbers hold q as well, for 28 vector
+//    instructions of a step fewer, but their matrix products add neighbours in a window of some 14 bits: beside one element of
+//    300, scores were up to 6e-3 off.) S^T is four products of 16x16x64 per 16 keys, two with heads of 64, and twice as many
+//    with more than 8 heads: up to 8, the columns that they leave empty take the lower two digits.
 //  * V as fp16. c in bits 4 .. 7 is the subnormal c * 2^-20. The matrix cores take it as it is, but do not normalise it: products are
 //    lined up by the exponents of their factors and cut off some 27 bits below the largest of a sum. From bits 4 .. 7 that leaves 24
 //    bits of a code's own size; in bits 0 .. 3, which need two instructions fewer for eight codes, 20 (333 keys with one that
@@ -31,7 +33,7 @@
 // Bound: by what one compute unit takes in, some 40 GB/s at one sequence per head (32768 tokens on 8 compute units: 103 us; neither more
 // loads in flight nor the scores of the next step beside the second product of this one make it faster), and by memory once
 // there are as many workgroups as compute units: 64 sequences of 8192 tokens, 32 / 4 heads of 128, take 47 us, 5.9 TB/s of cache read (a
-// large copy reads and writes 5.0). A step is 149 vector and 15 matrix instructions for 32 keys and 8 heads (D = 128); 146
+// large copy reads and writes 5.0). A step is 177 vector and 17 matrix instructions for 32 keys and 8 heads (D = 128); 164
 // registers leave room for three wavefronts per SIMD with two steps' loads in flight each (four with one step's took 3 to 40%
 // longer). Of its twelve wavefronts a compute unit holds one workgroup of eight or three of four. Eight are faster
 // while there are no more workgroups than compute units (20 sequences of 4096, 8 kv heads: 20.4 us against 23.3; 4096 to 16384
@@ -70,23 +72,19 @@ struct Int4Regs {
   uint32_t kw[2], vw[2];
 };
 
-// Codes of K as the matrix cores take them in the first product: a nibble on its own in a byte is the fp8 (E4M3) number
-// c * 2^-9, subnormal up to 7 and in the lowest binade from 8, which have one spacing.
-typedef int int8v_t __attribute__((ext_vector_type(8)));
+// Codes of K as the matrix cores take them in the first product: each nibble on its own in a byte.
+typedef int int4v_t __attribute__((ext_vector_type(4)));
 template <int D>
-__device__ __forceinline__ int8v_t int4_k_bytes(const uint32_t (&k)[D / 32]) {
-  int8v_t a;
+__device__ __forceinline__ void int4_k_bytes(const uint32_t (&k)[D / 32], int4v_t (&a)[D / 64]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {   // (D = 64: the same elements twice, for two parts of q)
-    const uint32_t x = k[i % (D / 32)];
-    a[2 * i] = (int)(x & 0x0f0f0f0fu);
-    a[2 * i + 1] = (int)((x >> 4) & 0x0f0f0f0fu);
+  for (int i = 0; i < D / 32; ++i) {
+    a[i / 2][2 * (i & 1)] = (int)(k[i] & 0x0f0f0f0fu);
+    a[i / 2][2 * (i & 1) + 1] = (int)((k[i] >> 4) & 0x0f0f0f0fu);
   }
-  return a;
 }
-// D(16x16) += A(16x128) * B(128x16), A in E4M3, B in E5M2: lane l supplies 32 bytes of row (column) l % 16, at 32 * (l / 16).
-__device__ __forceinline__ float4_t mfma_16x16x128_bytes(int8v_t a, int8v_t b, float4_t c) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 1, 0, 0, 0, 0);
+// D(16x16) += A(16x64) * B(64x16), int8: lane l supplies 16 bytes of row (column) l % 16, at 16 * (l / 16).
+__device__ __forceinline__ int4v_t mfma_16x16x64_i8(int4v_t a, int4v_t b, int4v_t c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
 // Eight codes of V in a dword as fp16 pairs, times 2^-20.
@@ -245,11 +243,12 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   for (int i = 0; i < kDepth; ++i) request_pair(p0 + 2 * i, buf[i]);
 
   // q as the right operand of the first product: column n, the elements of the bytes that the lane of the same g holds of K,
-  // as a sum of three E5M2 numbers, scaled by a power of two that puts the row's largest between 28672 and 57344. What that leaves of an
-  // element of less than 2^-6 is at most 2^-17, of the others nothing. Made once for the workgroup and handed out through LDS.
-  constexpr int kParts = 3, kProducts = D == 128 ? 3 : 2;   // D = 64: two parts side by side in the 128 of one product
+  // in four digits. Up to 8 heads: the upper two in columns 0 .. 7, the lower two in 8 .. 15. More: the lower two in a sum of their own.
+  // Made once for the workgroup and handed out through LDS.
+  constexpr int kDigits = 4, kSets = TWO ? 4 : 2;   // of a row; of a lane's column
+  constexpr float kUpper = 0x1p16f;                 // what a sum over the upper two counts for
   extern __shared__ __attribute__((aligned(16))) float int4_lds[];
-  constexpr int kRowBytes = kParts * D + 16;                // of a row of q: the parts, the sum and the factor of its scores
+  constexpr int kRowBytes = kDigits * D + 16;                 // of a row of q: the digits, the sum and the factor of its scores
   char *const q_rows = (char *)int4_lds;
   float *const int4_rows = int4_lds + kHeads * kRowBytes / 4;
   if (wave < kHeads * L / kWave) {
@@ -264,60 +263,48 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
     }
     most = over_row<L>(most, [](float a, float b) { return __builtin_fmaxf(a, b); });
     odd = over_row<L>(odd, [](float a, float b) { return a + b; });
-    int up = most > 0.f ? 16 - __builtin_amdgcn_frexp_expf(most) : 0;
-    if (__builtin_amdgcn_ldexpf(most, up) > 57344.f) --up;
+    const int up = most > 0.f ? 30 - __builtin_amdgcn_frexp_expf(most) : 0;
+    uint32_t digits[8];   // an element's, lowest first: signed, since each borrows 128 from the next
+    constexpr uint32_t kBorrow = 0x00808080u;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      x[i] = __builtin_amdgcn_ldexpf(x[i], up);
-      sum += x[i];
+      const float units = __builtin_rintf(__builtin_amdgcn_ldexpf(x[i], up));
+      sum += units;
+      digits[i] = ((uint32_t)(odd > 0.f ? 0 : (int)units) + kBorrow) ^ kBorrow;
     }
 #pragma unroll
-    for (int part = 0; part < kParts; ++part) {
+    for (int of = 0; of < kDigits; ++of) {   // highest digit first
+      const uint32_t sel = (uint32_t)(kDigits - 1 - of);
       uint2v_t bytes;   // elements of the lower and of the upper nibbles
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         constexpr int kOrder[2][4] = {{0, 4, 1, 5}, {2, 6, 3, 7}};
-        int four = __builtin_amdgcn_cvt_pk_bf8_f32(x[kOrder[u][0]], x[kOrder[u][1]], 0, false);
-        four = __builtin_amdgcn_cvt_pk_bf8_f32(x[kOrder[u][2]], x[kOrder[u][3]], four, true);
-        const float back[4] = {__builtin_amdgcn_cvt_f32_bf8(four, 0), __builtin_amdgcn_cvt_f32_bf8(four, 1),
-                               __builtin_amdgcn_cvt_f32_bf8(four, 2), __builtin_amdgcn_cvt_f32_bf8(four, 3)};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[kOrder[u][i]] -= back[i];
-        bytes[u] = (uint32_t)four;
+        const uint32_t low = __builtin_amdgcn_perm(digits[kOrder[u][1]], digits[kOrder[u][0]], 0x0c0c0000u | ((sel + 4) << 8) | sel);
+        const uint32_t high = __builtin_amdgcn_perm(digits[kOrder[u][3]], digits[kOrder[u][2]], 0x00000c0cu | ((sel + 4) << 24) | (sel << 16));
+        bytes[u] = low | high;
       }
-      *(uint2v_t *)(row + part * D + 8 * l) = bytes;
+      *(uint2v_t *)(row + of * D + 8 * l) = bytes;
     }
     sum = over_row<L>(sum, [](float a, float b) { return a + b; });
     if (l == 0) {
-      *(float2v_t *)(row + kParts * D) =
-          float2v_t{sum * 0x1p15f,   // the zero points come as z * 2^-24, the products in units of 2^-9
-                    odd > 0.f ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(scale_log2, 9 - up)};
+      const float mul = odd > 0.f ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(scale_log2, -up);
+      *(float2v_t *)(row + kDigits * D) = float2v_t{sum * 0x1p24f * mul, mul};   // (the zero points come as z * 2^-24)
     }
   }
   __syncthreads();
-  int8v_t qf[kProducts];
-  float q_sum, k_mul;
+  int4v_t qf[kSets][D / 64];
+  float q_sum, mul_own, mul_other;   // of the lane's own sums, and of those that it gets (TWO: of the upper digits' sums, of the lower ones')
   {
     const char *row = q_rows + (TWO ? n : (n & 7)) * kRowBytes;
-    const float2v_t both = *(const float2v_t *)(row + kParts * D);
+    const float2v_t both = *(const float2v_t *)(row + kDigits * D);
     q_sum = both[0];
-    k_mul = both[1];
+    mul_own = TWO || n < 8 ? both[1] * kUpper : both[1];
+    mul_other = TWO || n < 8 ? both[1] : both[1] * kUpper;
+    if constexpr (!TWO) row += n < 8 ? 0 : 2 * D;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) qf[kProducts - 1][i] = 0;
+    for (int of = 0; of < kSets; ++of) {
 #pragma unroll
-    for (int part = 0; part < kParts; ++part) {
-#pragma unroll
-      for (int j = 0; j < D / 64; ++j) {   // 16 bytes: elements of two dwords of K
-        const uint4_t x = *(const uint4_t *)(row + part * D + (D / 4) * g + 16 * j);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (D == 128) {
-            qf[part][4 * j + i] = (int)x[i];
-          } else {
-            qf[part >> 1][4 * (part & 1) + i] = (int)x[i];
-          }
-        }
-      }
+      for (int j = 0; j < D / 64; ++j) qf[of][j] = *(const int4v_t *)(row + of * D + (D / 4) * g + 16 * j);   // of two dwords of K
     }
   }
   const bool second = n >= 8;   // !TWO: the lane's scores are those of the second block's keys
@@ -337,14 +324,26 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
   auto attend = [&](Int4Regs<D> (&r)[2], int p, auto masked_tag) {
     constexpr bool MASKED = decltype(masked_tag)::value;
     constexpr int kKeys = TWO ? 8 : 4;   // keys a lane has the scores of: of its column all of 4g .. 4g + 3, or one block's
-    float4_t st[2];
+    int4v_t st[2], st_low[2];   // sums over two digits; TWO: over the upper and the lower two
+    int4v_t a[2][D / 64];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int8v_t a = int4_k_bytes<D>(r[u].k);
-      st[u] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < 2; ++u) int4_k_bytes<D>(r[u].k, a[u]);
+    auto add_digit = [&](const int4v_t (&digit)[D / 64], int4v_t (&sums)[2]) {
 #pragma unroll
-      for (int i = 0; i < kProducts; ++i) st[u] = mfma_16x16x128_bytes(a, qf[i], st[u]);
-    }
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) sums[u] = mfma_16x16x64_i8(a[u][j], digit[j], sums[u]);
+      }
+    };
+    auto two_digits = [&](const int4v_t (&high)[D / 64], const int4v_t (&low)[D / 64], int4v_t (&sums)[2]) {
+      sums[0] = sums[1] = int4v_t{0, 0, 0, 0};
+      add_digit(high, sums);
+      sums[0] <<= 8;
+      sums[1] <<= 8;
+      add_digit(low, sums);
+    };
+    two_digits(qf[0], qf[1], st);
+    if constexpr (TWO) two_digits(qf[2], qf[3], st_low);
     uint32_t kw[kKeys / 2], vw[kKeys / 2];   // words of the lane's keys 2i, 2i + 1
     uint32_t vz[4];                          // z' of the eight keys of its g, times 2^-20
 #pragma unroll
@@ -376,8 +375,11 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
     for (int i = 0; i < kKeys; ++i) {
       const half2_t ks = int4_scales(kw[i >> 1]), kz = __builtin_bit_cast(half2_t, kw[i >> 1] & 0x000f000fu);
       vs[i] = (float)int4_scales(vw[i >> 1])[i & 1];
-      const float dot = TWO ? st[i >> 2][i & 3] : second ? st[1][i] : st[0][i];
-      x[i] = __builtin_fmaf(-(float)kz[i & 1], q_sum, dot) * k_mul * (float)ks[i & 1];
+      // (the other digits of the block that the lane's scores are of are in the other half of the columns)
+      const float own = (float)(TWO ? st[i >> 2][i & 3] : second ? st[1][i] : st[0][i]);
+      const float other = TWO ? (float)st_low[i >> 2][i & 3] : dpp<kDppRotate8>((float)(second ? st[0][i] : st[1][i]));
+      const float dot = __builtin_fmaf(-(float)kz[i & 1], q_sum, own * mul_own);
+      x[i] = __builtin_fmaf(other, mul_other, dot) * (float)ks[i & 1];
       if constexpr (MASKED) {
         const int u = TWO ? i >> 2 : second ? 1 : 0;
         if ((p + u) * kInt4Block + 4 * g + (i & 3) >= end) x[i] = -INFINITY;
@@ -646,7 +648,7 @@ extern "C" int litekv_paged_decode_int4(const void *q, int64_t q_batch_stride, v
   LITEKV_REQUIRE(units <= 0x7fffffffLL / 8, "%s: too many workgroups", what);
   const bool two = (group + slices - 1) / slices > 8;
   const int heads = two ? 16 : 8;
-  const size_t lds = (size_t)share * (heads * head_dim + 32) * sizeof(float) + (size_t)heads * (3 * head_dim + 16);
+  const size_t lds = (size_t)share * (heads * head_dim + 32) * sizeof(float) + (size_t)heads * (4 * head_dim + 16);
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)units), dim3((unsigned)(share * kWave)), lds,
                        static_cast<hipStream_t>(stream), static_cast<const half_t *>(q), q_batch_stride,

@@ -74,10 +74,12 @@ def test_splits(fmt, hq, hkv, d, page, splits):
 @pytest.mark.parametrize("fmt", list(FORMATS))
 @pytest.mark.parametrize("hq,hkv,d,page", [(16, 4, 128, 16), (16, 4, 64, 64), (20, 1, 128, 32), (6, 2, 32, 16), (4, 2, 256, 16)])
 @pytest.mark.parametrize("chunks", [None, 3])
-@pytest.mark.parametrize("shared", [0, 4])
-def test_balanced_schedule_and_shared_prefix(fmt, hq, hkv, d, page, chunks, shared):
-    if shared and d not in (64, 128):
-        pytest.skip("a shared prefix takes head_dim 64 or 128")
+def test_balanced_schedule_and_shared_prefix(fmt, hq, hkv, d, page, chunks):
+    for shared in (0, 4) if d in (64, 128) else (0,):       # (a shared prefix takes these head dims)
+        balanced(fmt, hq, hkv, d, page, chunks, shared)
+
+
+def balanced(fmt, hq, hkv, d, page, chunks, shared):
     c = Case(fmt, hq, hkv, d, page, shared)
     plan = ops.DecodePlan(c.table, c.lens, hq, hkv, c.pages, page_size=page, shared_pages=shared, chunks=chunks,
                           token_bytes=2 * hkv * d * c.pool.element_size(), kv_dtype=c.pool.dtype)
