@@ -40,6 +40,12 @@ __host__ __device__ constexpr int int4_words_at(int head, int kv_heads, int d) {
 }
 // The keys of a prefill launch decoded once (see kv_int4.hip): fp16 pages of kInt4StagePage tokens and their block table.
 constexpr int kInt4StagePage = 256;
+// The block-table entry of 16-token page p of a sequence with that many keys, -1 for a page that it has not: the row may end behind
+// its last one. (A sequence with more keys than the row can name re-reads the row's last entry.)
+__host__ __device__ constexpr int int4_stage_entry(int p, int64_t keys, int page_shift, int bt_stride) {
+  if (p < 0 || (int64_t)p * kInt4Block >= keys) return -1;
+  return (p >> page_shift) < bt_stride ? p >> page_shift : bt_stride - 1;
+}
 int launch_int4_stage(const char *what, const void *pool, void *staged, int32_t *staged_table, const int32_t *block_table,
                       int32_t block_table_stride, const int32_t *cu_q_lens, const int32_t *context_lens, int32_t batch,
                       int32_t num_kv_heads, int32_t head_dim, int32_t page_shift, int64_t num_pages, int64_t capacity,

@@ -169,11 +169,11 @@ __global__ __launch_bounds__(256) void int4_stage_kernel(
   constexpr int kBlocks = kInt4StagePage / kInt4Block;
   const int64_t page = ((int64_t)b * capacity) / kInt4StagePage + p / kBlocks;
   if (tile == 0 && p % kBlocks == 0 && threadIdx.x == 0) staged_table[page] = (int32_t)page;
-  const int at = p >> page_shift;
-  const int entry = as_uniform(block_table)[(int64_t)b * bt_stride + (at < bt_stride ? at : bt_stride - 1)];
   const int rows = as_uniform(cu_q_lens)[b + 1] - as_uniform(cu_q_lens)[b];
   const int64_t keys = (int64_t)rows + (context_lens != nullptr ? as_uniform(context_lens)[b] : 0);
-  if (rows <= 0 || (int64_t)p * kInt4Block >= keys) return;
+  const int at = rows > 0 ? int4_stage_entry(p, keys, page_shift, bt_stride) : -1;
+  if (at < 0) return;
+  const int entry = as_uniform(block_table)[(int64_t)b * bt_stride + at];
   int4_to_half<D>(pool + (int64_t)sub_page_id(entry, p, page_shift, num_pages) * int4_block_bytes(kv_heads, D),
                   staged + ((int64_t)b * capacity + (int64_t)p * kInt4Block) * (2 * kv_heads) * D, kv_heads, kInt4Block, tile,
                   p == 0 && keys > capacity);   // the launch was told of fewer: rows of NaN, not rows that lack their last keys
