@@ -212,7 +212,7 @@ PyObject *paged_prefill(PyObject *, PyObject *const *a, Py_ssize_t n) {
       Py_RETURN_NONE;
     }
     if (page < 1 || page > 65536 || pool.slots % page != 0 || max_q < 0 || max_q > INT32_MAX || t > INT32_MAX || b > INT32_MAX ||
-        hq > INT32_MAX || pool.hkv > INT32_MAX || d > INT32_MAX || table->stride(0) > INT32_MAX) {
+        hq > INT32_MAX || pool.hkv > INT32_MAX || d > INT32_MAX || table->size(1) > INT32_MAX) {
       Py_RETURN_NONE;
     }
     // (the count's rule and the rows it looks at as in the wrapper)
@@ -237,7 +237,7 @@ PyObject *paged_prefill(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const float *scales = static_cast<const float *>(pool.scales);
     void *op = address(&out);
     PyObject *result = THPVariable_Wrap(std::move(out));  // (before the launch: it may throw)
-    const int32_t ts = (int32_t)table->stride(0);
+    const int32_t ts = (int32_t)std::max<int64_t>(1, table->size(1));  // (the one row of a view may have any stride)
     const int64_t pages = pool.slots / page;
     void *wp = partial_bytes > 0 ? partials.data_ptr() : nullptr;
     const int rc = unlocked([&] {

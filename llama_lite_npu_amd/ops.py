@@ -1070,7 +1070,7 @@ def paged_prefill(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Ten
     b = cu_q_lens.numel() - 1
     if not (block_table.dim() == 2 and block_table.shape[0] == b):
         raise ValueError("block_table must be [B, max_blocks]")
-    block_table = _dev_i32("block_table", block_table)
+    block_table, bt_stride = _table_rows(_dev_i32("block_table", block_table))
     if context_lens is not None:
         context_lens = _dev_i32("context_lens", context_lens)
         if not (context_lens.numel() == b):
@@ -1103,7 +1103,7 @@ def paged_prefill(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Ten
         elif not (workspace.is_cuda and workspace.dtype == torch.float32 and workspace.is_contiguous()):
             raise ValueError("workspace must be contiguous float32 on the device")
         _lib.check(lib.litekv_paged_prefill_int4(
-            _ptr(q), q_stride, _ptr(kv_pool), _ptr(block_table), block_table.stride(0), _ptr(cu_q_lens),
+            _ptr(q), q_stride, _ptr(kv_pool), _ptr(block_table), bt_stride, _ptr(cu_q_lens),
             _ptr(context_lens), _ptr(out), _rows("out", out), b, hq, hkv, d, page_size, n_pages, int(max_q_len),
             0 if max_kv_len is None else int(max_kv_len), t, max(1, key_slices),
             _ptr(workspace), 0 if workspace is None else workspace.numel() * 4,
@@ -1113,19 +1113,19 @@ def paged_prefill(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Ten
         # (max_kv_len 0: not known)
         _lib.check(lib.litekv_paged_prefill_bounded(
             _ptr(q), q_stride, _ptr(kv_pool), _ptr(kv_scales), 1 if is_int8_pool(kv_pool) else 0, _ptr(block_table),
-            block_table.stride(0), _ptr(cu_q_lens), _ptr(context_lens), _ptr(out), _rows("out", out), b, hq, hkv, d,
+            bt_stride, _ptr(cu_q_lens), _ptr(context_lens), _ptr(out), _rows("out", out), b, hq, hkv, d,
             page_size, n_pages, int(max_q_len), 0 if max_kv_len is None else int(max_kv_len), float(softmax_scale),
             _stream()))
         return out
     if fp8:
         _lib.check(lib.litekv_paged_prefill_split_q8(
             _ptr(q), q_stride, _ptr(kv_pool), _ptr(kv_scales), 1 if is_int8_pool(kv_pool) else 0,
-            _ptr(block_table), block_table.stride(0), _ptr(cu_q_lens), _ptr(context_lens), _ptr(out),
+            _ptr(block_table), bt_stride, _ptr(cu_q_lens), _ptr(context_lens), _ptr(out),
             _rows("out", out), b, hq, hkv, d, page_size, n_pages, int(max_q_len), t, key_slices,
             _ptr(workspace), workspace.numel() * 4, float(softmax_scale), _stream()))
         return out
     _lib.check(lib.litekv_paged_prefill_split(_ptr(q), q_stride, _ptr(kv_pool), _ptr(block_table),
-                                              block_table.stride(0), _ptr(cu_q_lens), _ptr(context_lens),
+                                              bt_stride, _ptr(cu_q_lens), _ptr(context_lens),
                                               _ptr(out), _rows("out", out), b, hq, hkv, d, page_size, n_pages,
                                               int(max_q_len), t, key_slices, _ptr(workspace),
                                               workspace.numel() * 4, float(softmax_scale), _stream()))
