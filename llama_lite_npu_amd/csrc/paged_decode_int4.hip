@@ -13,10 +13,10 @@
 //    instructions of a step fewer, but their matrix products add neighbours in a window of some 14 bits: beside one element of
 //    300, scores were up to 6e-3 off.) S^T is four products of 16x16x64 per 16 keys, two with heads of 64, and twice as many
 //    with more than 8 heads: up to 8, the columns that they leave empty take the lower two digits.
-//  * V as fp16. c in bits 4 .. 7 is the subnormal c * 2^-20. The matrix cores take it as it is, but do not normalise it: products are
-//    lined up by the exponents of their factors and cut off some 27 bits below the largest of a sum. From bits 4 .. 7 that leaves 24
-//    bits of a code's own size; in bits 0 .. 3, which need two instructions fewer for eight codes, 20 (333 keys with one that
-//    carries nearly all of the weight: outputs 1e-5 of sum p |v| off, all to one side). For the same reason the z' are
+//  * V as fp16. c in bits 4 .. 7 is the subnormal c * 2^-20. The matrix cores take it as it is, but do not normalise it: the eight
+//    products of a lane are lined up by the exponents of their factors and cut off some 24 bits below the largest. From bits 4 .. 7
+//    that leaves 21 bits of a code's own size; in bits 0 .. 3, which need two instructions fewer for eight codes, 17 (333 keys with
+//    one that carries nearly all of the weight: outputs 1e-5 of sum p |v| off, all to one side). For the same reason the z' are
 //    summed by an MFMA of their own and taken off every kFold blocks, and not at the end from accumulators that would have
 //    grown to some twenty times the result.
 //
@@ -30,16 +30,16 @@
 // The reference of the exponentials is the largest p s' so far, not the largest p: in fp16 it is p s' that has to fit. It is put
 // at 2^7 and may grow to 2^15 before the accumulators are rescaled.
 //
-// Bound: by what one compute unit takes in, some 40 GB/s at one sequence per head (32768 tokens on 8 compute units: 103 us; neither more
-// loads in flight nor the scores of the next step beside the second product of this one make it faster), and by memory once
+// Bound: by what one compute unit takes in, some 40 GB/s at one sequence per head (32768 tokens on 8 compute units: 110 us), and by memory once
 // there are as many workgroups as compute units: 64 sequences of 8192 tokens, 32 / 4 heads of 128, take 47 us, 5.9 TB/s of cache read (a
-// large copy reads and writes 5.0). A step is 177 vector and 17 matrix instructions for 32 keys and 8 heads (D = 128); 164
-// registers leave room for three wavefronts per SIMD with two steps' loads in flight each (four with one step's took 3 to 40%
-// longer). Of its twelve wavefronts a compute unit holds one workgroup of eight or three of four. Eight are faster
-// while there are no more workgroups than compute units (20 sequences of 4096, 8 kv heads: 20.4 us against 23.3; 4096 to 16384
-// tokens in 64: 71 against 79), four where there are more (38 of 4096: 36.4 against 40.8; 100 of 2048: 42.6 against 51). Streaming
-// loads, whose lines are the first to leave the caches, suit a cache larger than those (the case above with ordinary ones: 52.5 us), as
-// that of a model's layers one after the other is; inside them ordinary ones are faster (20 of 4096: 19.2 against 20.5).
+// large copy reads and writes 5.0). A step is 177 vector and 17 matrix instructions for 32 keys and 8 heads (D = 128), 219 and 34
+// with more: 64 / 4 heads take 51 us over the same bytes, 8 sequences of 4096 tokens 24.0 with 16 heads per kv head and 19.4 with
+// 8. 164 registers leave room for three wavefronts per SIMD with two steps' loads in flight each. Of its twelve wavefronts a
+// compute unit holds one workgroup of eight or three of four. Eight are faster while there are no more workgroups than compute
+// units (20 sequences of 4096, 8 kv heads: 20.8 us against 23.6; 4096 to 16384 tokens in 64: 71.6 against 80.4), four where there
+// are more (38 of 4096: 37.1 against 41.8; 100 of 2048: 42.6 against 51.4). Streaming loads, whose lines are the first to leave the
+// caches, suit a cache larger than those (the case above with ordinary ones: 52 us), as that of a model's layers one after the
+// other is; inside them ordinary ones are faster (20 of 4096: 20.1 against 20.7).
 //
 // Around its keys a workgroup spends some 5 us, most of it one memory trip after another and the first run through its code: the
 // sequence's length, block-table entries, keys, the fold. So q, the first 64 entries of the table row and the new rows are
@@ -561,12 +561,13 @@ __global__ __launch_bounds__(kInt4Waves *kWave) __attribute__((amdgpu_waves_per_
 }  // namespace litekv
 
 // Up to 256 (sequence, kv head) pairs, a compute unit has at most one, and splits fill the device: of 512 tokens and more where
-// the longest sequence has over 1024 (8 kv heads: one sequence of 2000 tokens in splits of 512 / 1024 tokens, or unsplit, 9.4 / 11.1 /
-// 11.4 us, six of 2048 10.5 / 11.6 / 11.8, eight of 4096 in splits of 1024 / 2048 12.9 / 15.7, unsplit 18.4; one of 778 in two 9.5 us, unsplit
-// 7.6). With more, splits only even out
-// the lengths (40 of 16384 tokens, 8 kv heads: 137 / 117 / 112 us, 135 unsplit; 64 of them: 214 / 191 / 175 us, 166 unsplit).
+// the longest sequence has over 1024 (8 kv heads: one sequence of 2000 tokens in splits of 512 / 1024 tokens, or unsplit, 9.6 / 11.0 /
+// 11.8 us, six of 2048 10.2 / 11.7 / 12.2, eight of 4096 in splits of 1024 / 2048 12.9 / 15.3, unsplit 19.1; one of 778 in two 9.4 us, unsplit
+// 7.7). With more, splits only even out the lengths and the last turn of the workgroups, from 4096 tokens a split (in splits of 1024 /
+// 2048 / 4096 tokens, 8 kv heads: 40 sequences of 16384 131 / 117 / 110 us, 131 unsplit; 64 of them, which are even as they are, 199 / 182 /
+// 177, 171 unsplit: the rule does not look at that, and costs them 3%).
 // No more than 16 where that makes them shorter than 4096 tokens: their merge takes longer the more there are (one sequence of 32768
-// tokens, 8 kv heads: 8 / 16 / 32 splits 21.7 / 17.6 / 19.5 us). Powers of two: a captured step holds their number, and growing
+// tokens, 8 kv heads: 8 / 16 / 32 splits 22.7 / 17.4 / 19.5 us). Powers of two: a captured step holds their number, and growing
 // sequences should not ask for a new one every thousand tokens.
 extern "C" int32_t litekv_paged_decode_int4_splits(int32_t batch, int32_t num_kv_heads, int64_t max_pages, int64_t total_pages,
                                                    int32_t page_size, int32_t *min_pages_per_split) {

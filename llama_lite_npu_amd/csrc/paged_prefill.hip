@@ -624,7 +624,9 @@ extern "C" int litekv_paged_prefill_int8(const void *q, int64_t q_token_stride, 
 // rows over 7601 tokens, 64 / 8 heads: 178 -> 153 us (fp16 pool: 129 to 135); 8 prompts of 128 to 2048 tokens 261 -> 236 (225 to
 // 235); four chunks of up to 512 over up to 8000, 32 / 8 heads of 64, uncut, 163 -> 128 (107); 16 prompts of 1024 118 -> 107; 200 rows over
 // 8000, 64 / 8 heads (13 blocks), 91 -> 83. With fewer blocks: 128 rows over 4000, 64 / 8 heads (8 blocks), 44 in both forms; 32 / 8 heads
-// (4 blocks), 26.6 -> 33.8; 8 prompts of 512, 32 / 8 heads (16 blocks, a key attended by 8 on the average), 44.3 -> 45.3. Up to 1 GiB: a cache in 4 bits is there to save memory.
+// (4 blocks), 26.6 -> 33.8; 8 prompts of 512, 32 / 8 heads (16 blocks, a key attended by 8 on the average), 44.3 -> 45.3. Up to 1 GiB: a cache in 4 bits is there to save memory. (The room is the longest
+// sequence's for each, whatever the others' lengths, which the host does not know: one of 8000 tokens and 15 short ones, 8 kv heads of
+// 128, 537 MB for some 34 MB of keys; workgroups of tokens that a sequence has not leave at once.)
 struct Int4Staging {
   int64_t capacity = 0;   // tokens of a sequence, 0: they are decoded where they are attended
   size_t table_at = 0, pool_at = 0, bytes = 0;
@@ -656,7 +658,10 @@ static Int4Staging int4_staging(int32_t batch, int32_t num_q_heads, int32_t num_
 // takes as long as its longest chain of keys, which chunks of one batch seldom share evenly. 4 chunks of up to 512 rows over 2000 to
 // 8000 tokens, 32 / 8 heads of 64: 126 -> 97 us, of 128 175 -> 131; 3 of up to 400 over up to 30000 609 -> 467; 4 equal ones of 512
 // over 8000 239 -> 234; 16 of up to 128 over up to 4000, heads of 64, 98 -> 84, but over up to 2000, heads of 128, 73 -> 75, 6 of up to
-// 300 over up to 1000 48 -> 53, and two of up to 1000 over 4000 88 -> 104. (Other pools would gain as much.)
+// 300 over up to 1000 48 -> 53, and two of up to 1000 over 4000 88 -> 104. (Other pools would gain as much.) One chunk of 64 rows, 16 / 8
+// heads, in 8 slices takes 11 to 12 us with one key tile a slice over any pool (of them the merge 3.2, the rest one memory trip after another:
+// lengths, page ids, keys, partial rows), and a tile more 0.7 us over fp16, 0.9 over int8 and 1.1 over 4-bit codes, whose conversion nothing
+// covers in so short a chain.
 extern "C" int32_t litekv_paged_prefill_int4_key_slices(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                                                         int32_t max_q_len, int64_t max_kv_len) {
   const int32_t slices = litekv_paged_prefill_key_slices(batch, num_q_heads, num_kv_heads, head_dim, max_q_len, max_kv_len);
