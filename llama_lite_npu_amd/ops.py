@@ -1040,8 +1040,9 @@ def paged_prefill(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Ten
     (head_dim 64 / 128, any pool format). None lets the library choose from the launch shape and
     ``max_kv_len`` (the most keys a row sees: history + chunk, as the host knows it; without it
     the launch is not cut, and its form is the one for few keys); 1 switches it off. Over 4-bit codes the keys that
-    many blocks of rows attend are decoded once, into the workspace, for ``max_kv_len`` tokens a sequence: there it has to
-    be true (the rows of a longer sequence are NaN). ``workspace`` (float32, see ``paged_prefill_workspace_floats``) is
+    many blocks of rows attend are decoded once, into the workspace, for ``max_kv_len`` tokens a sequence (up to 1 GiB of fp16): there
+    it has to be true, in a captured launch for every replay (the rows of a longer sequence are NaN). Rows behind the last
+    sequence are left as they are. ``workspace`` (float32, see ``paged_prefill_workspace_floats``) is
     allocated when not given."""
     if q.is_cuda and out is None and key_slices is None and workspace is None and softmax_scale is not None:
         done = _lib.calls().paged_prefill(q, kv_pool, block_table, cu_q_lens, context_lens, max_q_len, softmax_scale,
