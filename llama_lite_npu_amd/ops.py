@@ -868,7 +868,8 @@ def paged_decode(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tens
     An fp8 pool comes with its ``kv_scales``; either schedule reads it. A pool of 4-bit codes is read on the "splits"
     schedule, whatever is left open here (see ``int4_decode_splits``).
     ``k_new`` / ``v_new`` [B, Hkv, D] (splits schedule, both stages): the step's new token of every
-    sequence is written at logical position seq_lens[b] - 1 by the same launch and attended.
+    sequence is written at logical position seq_lens[b] - 1 by the same launch and attended (a block-table entry there
+    that names no page of the pool is read as the nearest one that does, and nothing is written).
     """
     int4 = is_int4_pool(kv_pool)
     if (int4 and q.is_cuda and out is None and workspace is None and num_splits is None and max_splits is None
