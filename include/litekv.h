@@ -50,7 +50,7 @@ extern "C" {
 #define LITEKV_ERR_INVALID_ARGUMENT 1
 #define LITEKV_ERR_LAUNCH 2
 
-#define LITEKV_ABI_VERSION 5
+#define LITEKV_ABI_VERSION 6
 
 /* ABI version of the loaded library (LITEKV_ABI_VERSION at build time). */
 int litekv_abi_version(void);
@@ -858,6 +858,102 @@ int litekv_paged_prefill_int4(const void *q, int64_t q_token_stride, const void 
                               int64_t num_pages, int32_t max_q_len, int64_t max_kv_len,
                               int64_t num_tokens, int32_t key_slices, void *workspace,
                               size_t workspace_bytes, float softmax_scale, void *stream);
+
+/*
+ * Formats of a pool, where an entry point takes any of them. The 8-bit ones come with
+ * kv_scales [2 * Hkv] (K heads, then V heads), the others with NULL.
+ */
+#define LITEKV_POOL_FP16 0
+#define LITEKV_POOL_FP8 1
+#define LITEKV_POOL_INT8 2
+#define LITEKV_POOL_INT4 3
+
+/*
+ * The QKV projection's epilogue (see litekv_qk_norm_rope_append) for tokens whose position
+ * has several axes, as images and video give them (time, height, width): pair i of a row,
+ * elements i and i + head_dim / 2, turns by entry i of the cos and sin row of position
+ * positions[axis_of_pair[i]][t]:
+ *     q[t][h]                           = rope(norm(q[t][h]) * q_norm_weight)     in place
+ *     kv_pool[slot_mapping[t]][h]       = rope(norm(k[t][h]) * k_norm_weight)
+ *     kv_pool[slot_mapping[t]][Hkv + h] = v[t][h]
+ * Everything is fp32 from the fp16 inputs to the one rounding of q and to the pool's format,
+ * each operation rounded by itself; the sum of squares is fp64.
+ *   cos_table, sin_table  [table_rows][table_stride] fp16, the rows of positions 0, 1, ..;
+ *                         a position outside reads the nearest row
+ *   positions             element (axis a, token t) at a * axis_stride + t * token_stride,
+ *                         int32, or int64 if positions_int64; either stride may be 0
+ *   num_axes              1 to 4
+ *   axis_of_pair          HOST pointer, head_dim / 2 bytes, read before the call returns
+ *   q_norm_weight, k_norm_weight  [head_dim] fp16, or both NULL
+ *   slot outside [0, num_slots)   k / v of that token are not stored; q is still processed
+ * Head dims 32, 64, 128 and 256; over 4-bit codes 64 and 128.
+ */
+int litekv_qk_norm_mrope_append(void *q, int64_t q_token_stride, const void *k,
+                                int64_t k_token_stride, const void *v, int64_t v_token_stride,
+                                const void *q_norm_weight, const void *k_norm_weight,
+                                const void *cos_table, const void *sin_table,
+                                int64_t table_stride, int64_t table_rows,
+                                const void *positions, int32_t positions_int64,
+                                int64_t axis_stride, int64_t token_stride, int32_t num_axes,
+                                const uint8_t *axis_of_pair, const int32_t *slot_mapping,
+                                void *kv_pool, const float *kv_scales, int32_t pool_format,
+                                int32_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                                int32_t head_dim, int64_t num_slots, float rms_eps,
+                                void *stream);
+
+/*
+ * Attention of packed rows over all keys of another sequence, an encoder's states in pages of
+ * their own (appended as any tokens are):
+ *     out[t][h] = softmax(q[t][h] . K_b[h / (Hq/Hkv)]^T * scale) V_b
+ * for the rows t in [cu_q_lens[b], cu_q_lens[b+1]) of sequence b, over its kv_lens[b] keys
+ * (at most what a row of the block table can name). A sequence without keys gets rows of zeros;
+ * rows behind the last sequence are left as they are. q, out, block_table, page_size, num_pages
+ * and softmax_scale (above 0) as in litekv_paged_prefill; head dims 64 and 128. max_q_len is the most rows of a
+ * sequence and has to be true; max_kv_len the most keys as the host knows it, 0 if it does
+ * not, and only a choice of form goes by it. key_slices above 1 cuts the keys, for launches of
+ * few rows: litekv_paged_prefill_key_slices says into how many, and
+ * litekv_paged_prefill_split_workspace_bytes what workspace that takes (num_tokens rows,
+ * those behind the last sequence among them). One row a sequence: litekv_paged_decode and its
+ * like, with kv_lens for seq_lens, stream the keys without a tile.
+ */
+int litekv_paged_cross_attention(const void *q, int64_t q_token_stride, const void *kv_pool,
+                                 const float *kv_scales, int32_t pool_format,
+                                 const int32_t *block_table, int32_t block_table_stride,
+                                 const int32_t *cu_q_lens, const int32_t *kv_lens, void *out,
+                                 int64_t out_token_stride, int32_t batch, int32_t num_q_heads,
+                                 int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                                 int64_t num_pages, int32_t max_q_len, int64_t max_kv_len,
+                                 int64_t num_tokens, int32_t key_slices, void *workspace,
+                                 size_t workspace_bytes, float softmax_scale, void *stream);
+
+/*
+ * One token per row of logits, from a given uniform number (the reference draws after
+ * lite_llama/sampling.py). With p_i = exp((x_i - max x) / T), 0 where (x_i - max x) < -40 T,
+ * and the tokens ordered by p, ties the lowest index first, kept are: the first top_k; of
+ * them the shortest run whose mass reaches top_p of theirs; of them those with
+ * p_i >= min_p; always the first. tokens[r] is the first token, by index, at which the kept
+ * mass exceeds uniforms[r] times all of it, logprobs[r] its logarithm of probability among the
+ * kept. Masses are exact to 2^-41 of themselves. T <= 0 (or NaN) takes the first
+ * largest logit, with logprob 0.
+ *   logits       [batch][row_stride], logits_type 0 fp16, 1 bf16, 2 fp32; aligned to an
+ *                element. NaN and -inf are never drawn, +inf counts as the largest finite fp32
+ *                number. A row without any other: token -1, logprob -inf
+ *   uniforms     [batch], in [0, 1) (what is outside counts as the nearest inside, NaN as 0)
+ *   temperature  [batch], NULL: 1
+ *   top_k        [batch], below 1: off. NULL: off
+ *   top_p        [batch], 1 and above (or NaN): off. NULL: off
+ *   min_p        [batch], 0 and below (or NaN): off. NULL: off
+ *   logprobs     [batch] or NULL
+ * vocab at most 2^20. Reads the 16-byte blocks that hold an element of a row. The same inputs give the same
+ * outputs, whatever the order the device works in.
+ */
+size_t litekv_sample_tokens_workspace_bytes(int32_t logits_type, int32_t batch, int32_t vocab);
+
+int litekv_sample_tokens(const void *logits, int32_t logits_type, int64_t row_stride,
+                         const float *uniforms, const float *temperature,
+                         const int32_t *top_k, const float *top_p, const float *min_p,
+                         int64_t *tokens, float *logprobs, int32_t batch, int32_t vocab,
+                         void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -19,7 +19,7 @@ import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "csrc" / "liblitekv.so"
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 # name -> (restype, argtypes); mirrors include/litekv.h declaration by declaration.
 SIGNATURES = {
@@ -263,6 +263,24 @@ SIGNATURES = {
         c_int32,
         [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
          c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_float, c_void_p],
+    ),
+    "litekv_qk_norm_mrope_append": (
+        c_int32,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_int64, c_int64, c_void_p, c_int32, c_int64, c_int64, c_int32, c_char_p, c_void_p, c_void_p, c_void_p,
+         c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_float, c_void_p],
+    ),
+    "litekv_paged_cross_attention": (
+        c_int32,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
+         c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int32, c_int64, c_int64, c_int32,
+         c_void_p, c_size_t, c_float, c_void_p],
+    ),
+    "litekv_sample_tokens_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32]),
+    "litekv_sample_tokens": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_int32, c_int32, c_void_p, c_size_t, c_void_p],
     ),
 }
 

@@ -56,6 +56,27 @@ class Attention:
         return ops.qk_norm_rope_append(xq, xk, xv, atten_info.cur_select_index, pool, q_norm_weight,
                                        k_norm_weight, cos, sin, rms_eps, kv_scales=scales)
 
+    def qkv_epilogue_axes(self, xq, xk, xv, atten_info, layer_index: int, positions, sections, cos_table, sin_table,
+                          q_norm_weight=None, k_norm_weight=None, rms_eps: float = 1e-6,
+                          interleaved: bool = False) -> torch.Tensor:
+        """``qkv_epilogue`` for tokens whose position has several axes (images, video): ``positions`` [A, T], of which each pair
+        of a row takes the axis that ``sections`` gives it (``ops.qk_norm_mrope_append``); the rows of the cos and sin tables are
+        gathered on the way."""
+        pool = atten_info.kv_buffer[layer_index]
+        scales = atten_info.kv_scales[layer_index] if ops.is_quantised_pool(pool) else None
+        return ops.qk_norm_mrope_append(xq, xk, xv, atten_info.cur_select_index, pool, positions, sections, cos_table, sin_table,
+                                        q_norm_weight, k_norm_weight, rms_eps, kv_scales=scales, interleaved=interleaved)
+
+    def cross_forward(self, xq, states, layer_index: int, cu_q_lens=None, max_q_len: int = 1, qk_scale=None) -> torch.Tensor:
+        """Attention over an encoder's states (``executor.encoder_states.EncoderStates``): packed rows xq [T, Hq, D] with the
+        batch's ``cu_q_lens``, or one row a sequence without them. ``qk_scale`` is the natural 1/sqrt(D) in both."""
+        scale = (1.0 / math.sqrt(self.head_dim)) if qk_scale is None else float(qk_scale)
+        pool, scales = states.kv_buffer[layer_index], states.kv_scales[layer_index]
+        if cu_q_lens is None:
+            return ops.decode_step(xq, pool, states.decode_plan(self.num_q_heads), None, None, scale, kv_scales=scales)
+        return ops.paged_cross_attention(xq, pool, states.block_table, states.kv_lens, cu_q_lens, max_q_len, scale,
+                                         page_size=states.page_size, kv_scales=scales, max_kv_len=states.max_kv_len)
+
     def context_forward(self, xq, xk, xv, atten_info, layer_index: int, qk_scale=None) -> torch.Tensor:
         """Prefill: xq [T, Hq, D], xk / xv [T, Hkv, D] packed rows of the batch's prompts or chunks
         (None when ``qkv_epilogue`` already stored them)."""

@@ -38,7 +38,11 @@ SOURCES = (
     "paged_prefill.hip",
     "paged_prefill_hd64.hip",
     "paged_prefill_hd256.hip",
+    "paged_cross.hip",
+    "paged_cross_hd64.hip",
     "generic_attention.hip",
+    "mrope_append.hip",
+    "sample_tokens.hip",
 )
 
 # Packed fp32 VALU forms are switched off for device code: the compiler would
@@ -63,6 +67,8 @@ HIPCC_FLAGS = (
 PER_FILE_FLAGS = {
     "paged_prefill.hip": ("-fno-honor-nans", "-Wno-inline-asm"),
     "paged_prefill_hd64.hip": ("-fno-honor-nans", "-Wno-inline-asm"),
+    "paged_cross.hip": ("-fno-honor-nans", "-Wno-inline-asm"),
+    "paged_cross_hd64.hip": ("-fno-honor-nans", "-Wno-inline-asm"),
     # at head dim 256 not a number goes where fp32 arithmetic takes it: no NaN flag (231 more
     # v_max_f32 in its four kernels, none in the loop over tiles below the diagonal)
     "paged_prefill_hd256.hip": ("-Wno-inline-asm",),

@@ -27,9 +27,12 @@ What is different underneath:
 from __future__ import annotations
 
 import logging
+import random
 from typing import Callable, Optional, Sequence
 
 import torch
+
+from . import ops
 
 logger = logging.getLogger(__name__)
 
@@ -43,9 +46,12 @@ class BatchRequest:
     completion events belong to the scheduler and are not modelled."""
 
     def __init__(self, request_id: str, prompt_tokens: Sequence[int], max_new_tokens: int,
-                 temperature: float, top_p: float, control_id: Optional[int] = None) -> None:
+                 temperature: float, top_p: float, control_id: Optional[int] = None, top_k: int = 0,
+                 min_p: float = 0.0, seed: Optional[int] = None) -> None:
+        """``top_k`` (0: off), ``min_p`` (0: off) and ``seed`` are beside the reference's: see ``draw_tokens``."""
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens must be positive")
+        self.top_k, self.min_p, self.seed = int(top_k), float(min_p), seed
         self.request_id = request_id
         self.control_id = control_id
         self.prompt_tokens = list(prompt_tokens)
@@ -101,6 +107,26 @@ def sample_next_token(logits: torch.Tensor, temperature: Sequence[float], top_p:
     drawn = order.gather(1, pick).reshape(-1)
     is_greedy = torch.tensor([float(t) == 0.0 for t in temperature], device=rows.device)
     return torch.where(is_greedy, greedy, drawn)
+
+
+def draw_tokens(logits: torch.Tensor, requests: Sequence) -> torch.Tensor:
+    """One token per row of ``logits`` [n, vocab] (or [n, seq, vocab]: last position), by each request's temperature, top_k, top_p
+    and min_p (``ops.sample_tokens``; one small upload, two launches). The uniform number of a request with a ``seed`` depends
+    on that and on the number of tokens it has generated, so its answer is the same in any batch; the others' come
+    from Python's generator."""
+    rows = logits[:, -1, :] if logits.dim() == 3 else logits
+    numbers = []
+    for r in requests:
+        seed = getattr(r, "seed", None)
+        source = random if seed is None else random.Random(f"{seed}/{len(r.generated_token_ids)}")
+        numbers.append(int(source.random() * 2 ** 24) / 2 ** 24)          # a float32 below 1
+    # top_k as the bits of an int32 in a float32's place
+    top_k = [min(int(getattr(r, "top_k", 0)), 2 ** 31 - 1) for r in requests]
+    floats = [numbers, [float(r.temperature) for r in requests], [float(r.top_p) for r in requests],
+              [float(getattr(r, "min_p", 0.0)) for r in requests]]
+    packed = torch.cat((torch.tensor(floats, dtype=torch.float32), torch.tensor([top_k], dtype=torch.int32).view(torch.float32)))
+    uniforms, temperature, top_p, min_p, bits = packed.to(rows.device).unbind(0)
+    return ops.sample_tokens(rows, uniforms, temperature, bits.view(torch.int32), top_p, min_p)
 
 
 class _TokenRows(dict):
@@ -174,6 +200,10 @@ class ContinuousBatchModelBackend:
         return torch.tensor(values, dtype=torch.long, device=self.executor.device)
 
     def _sample(self, logits, requests: Sequence[BatchRequest]) -> torch.Tensor:
+        if self._sampler is sample_next_token and not getattr(self.executor, "logits_are_sharded", False) and any(
+                getattr(r, "top_k", 0) > 0 or getattr(r, "min_p", 0.0) > 0.0 or getattr(r, "seed", None) is not None
+                for r in requests):
+            return draw_tokens(logits, requests)
         return self._sampler(logits, temperature=[r.temperature for r in requests],
                              top_p=[r.top_p for r in requests],
                              vocab_parallel=bool(getattr(self.executor, "logits_are_sharded", False)))

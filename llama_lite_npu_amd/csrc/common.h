@@ -174,6 +174,12 @@ struct PrefillBuild {
 };
 const PrefillBuild &hd64_prefill();
 const PrefillBuild &hd256_prefill();
+// ... and of its builds in which every row sees all of kv_lens[b] keys (paged_cross.hip, paged_cross_hd64.hip).
+int hd64_cross(const char *what, const void *q, int64_t q_token_stride, const void *kv_pool, const float *kv_scales,
+               const int32_t *block_table, int32_t block_table_stride, const int32_t *cu_q_lens,
+               const int32_t *kv_lens, void *out, int64_t out_token_stride, int32_t batch, int32_t num_q_heads,
+               int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int64_t num_pages, int32_t max_q_len,
+               float softmax_scale, void *stream, int format, const PrefillKeySplit &split);
 
 // The launchers of the head dim 64 build of paged_decode.hip (paged_decode_hd64.hip), to which the
 // head dim 128 build, which owns the C ABI, hands calls with head_dim == 64. `scales` marks a pool

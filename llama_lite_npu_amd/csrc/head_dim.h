@@ -8,7 +8,16 @@
 #ifndef LITEKV_HD
 #define LITEKV_HD 128
 #endif
-#if LITEKV_HD == 128
+#ifndef LITEKV_CROSS
+#define LITEKV_CROSS 0   // paged_cross.hip, paged_cross_hd64.hip: the same launches, every row seeing all keys
+#endif
+#if LITEKV_CROSS && LITEKV_HD == 128
+#define LITEKV_HD_NS cross128
+#elif LITEKV_CROSS && LITEKV_HD == 64
+#define LITEKV_HD_NS cross64
+#elif LITEKV_CROSS
+#error "LITEKV_CROSS takes LITEKV_HD 128 or 64"
+#elif LITEKV_HD == 128
 #define LITEKV_HD_NS hd128
 #elif LITEKV_HD == 64
 #define LITEKV_HD_NS hd64

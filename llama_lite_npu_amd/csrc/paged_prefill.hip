@@ -6,6 +6,9 @@ namespace litekv {
 inline namespace LITEKV_HD_NS {
 using namespace prefill_tile;
 
+// What is added to the modes of this build's launches (see kCross in prefill_tile.h).
+constexpr int kCrossBit = LITEKV_CROSS ? kCross : 0;
+
 static int validate_prefill(const char *what, const void *q, int64_t q_stride, const void *out,
                             int64_t out_stride, int32_t batch, int32_t hq, int32_t hkv,
                             int32_t head_dim, int32_t max_q_len) {
@@ -81,6 +84,7 @@ __global__ __launch_bounds__(4 * kWave) void prefill_split_merge_kernel(
   float mx = w[0];
 #pragma unroll
   for (int i = 1; i < kMaxPrefillKeySlices; ++i) mx = fmaxf(mx, w[i]);
+  if (kCrossBit != 0 && mx == -INFINITY) mx = 0.f;   // a sequence without keys: no slice has any
 #pragma unroll
   for (int i = 0; i < kMaxPrefillKeySlices; ++i) w[i] = i < slices ? fast_exp2((w[i] - mx) * 1.4426950408889634f) : 0.f;
   static_assert(kMaxPrefillKeySlices == 8, "the order of the sum");
@@ -93,7 +97,7 @@ __global__ __launch_bounds__(4 * kWave) void prefill_split_merge_kernel(
       for (int j = 0; j < 4; ++j) o[j] += w[i] * row[i][j];
     }
   }
-  const float inv = 1.0f / den;
+  const float inv = kCrossBit == 0 || den > 0.f ? 1.0f / den : 0.f;
   if (token >= live) return;
   *(half4_t *)(out + token * out_stride + (int64_t)head * kHD + at) =
       half4_t{(half_t)(o[0] * inv), (half_t)(o[1] * inv), (half_t)(o[2] * inv), (half_t)(o[3] * inv)};
@@ -227,7 +231,17 @@ static int launch_paged_prefill(const char *what, const void *q, int64_t q_token
                  "%s: key_slices %d out of [1, %d]", what, split.key_slices, kMaxPrefillKeySlices);
   LITEKV_REQUIRE(split.key_slices == 1 || head_dim == 128 || head_dim == 64,
                  "%s: key slices take head_dim 64 or 128", what);
-#if LITEKV_HD == 128
+#if LITEKV_CROSS
+  LITEKV_REQUIRE(head_dim == 128 || head_dim == 64, "%s: head_dim %d unsupported (64 or 128)", what, head_dim);
+  LITEKV_REQUIRE(batch == 0 || max_q_len == 0 || context_lens != nullptr, "%s: null pointer (kv_lens)", what);
+#endif
+#if LITEKV_CROSS && LITEKV_HD == 128
+  if (head_dim == 64) {  // another head dim's build of this file
+    return hd64_cross(what, q, q_token_stride, kv_pool, kv_scales, block_table, block_table_stride, cu_q_lens,
+                      context_lens, out, out_token_stride, batch, num_q_heads, num_kv_heads, head_dim, page_size,
+                      num_pages, max_q_len, softmax_scale, stream, format, split);
+  }
+#elif LITEKV_HD == 128
   const PrefillBuild *build = head_dim == 64 ? &hd64_prefill()
                               : head_dim == 256 && tiled_256(q_token_stride, out_token_stride, num_kv_heads,
                                                                  softmax_scale)
@@ -329,13 +343,13 @@ static int launch_paged_prefill(const char *what, const void *q, int64_t q_token
       }
     };
     if (format == kKvInt4) {
-      by_width(std::integral_constant<int, kPagedPrefillSplitInt4>{});
+      by_width(std::integral_constant<int, kPagedPrefillSplitInt4 | kCrossBit>{});
     } else if (format == kKvInt8) {
-      by_width(std::integral_constant<int, kPagedPrefillSplitInt8>{});
+      by_width(std::integral_constant<int, kPagedPrefillSplitInt8 | kCrossBit>{});
     } else if (format == kKvFp8) {
-      by_width(std::integral_constant<int, kPagedPrefillSplitFp8>{});
+      by_width(std::integral_constant<int, kPagedPrefillSplitFp8 | kCrossBit>{});
     } else {
-      by_width(std::integral_constant<int, kPagedPrefillSplit>{});
+      by_width(std::integral_constant<int, kPagedPrefillSplit | kCrossBit>{});
     }
     int rc2 = check_launch(what);
     if (rc2 != LITEKV_OK) return rc2;
@@ -376,20 +390,21 @@ static int launch_paged_prefill(const char *what, const void *q, int64_t q_token
   };
 #if LITEKV_HD != 256
   if (format == kKvInt4) {
-    launch(std::integral_constant<int, kPagedPrefillInt4>{});
+    launch(std::integral_constant<int, kPagedPrefillInt4 | kCrossBit>{});
     return check_launch(what);
   }
 #endif
   if (format == kKvInt8) {
-    launch(std::integral_constant<int, kPagedPrefillInt8>{});
+    launch(std::integral_constant<int, kPagedPrefillInt8 | kCrossBit>{});
   } else if (format == kKvFp8) {
-    launch(std::integral_constant<int, kPagedPrefillFp8>{});
+    launch(std::integral_constant<int, kPagedPrefillFp8 | kCrossBit>{});
   } else {
-    launch(std::integral_constant<int, kPagedPrefill>{});
+    launch(std::integral_constant<int, kPagedPrefill | kCrossBit>{});
   }
   return check_launch(what);
 }
 
+#if !LITEKV_CROSS
 // Causal attention over packed, contiguous K/V.
 static int launch_varlen_prefill(const void *q, int64_t q_token_stride, const void *k,
                                  int64_t k_token_stride, const void *v, int64_t v_token_stride,
@@ -479,9 +494,21 @@ static int launch_varlen_prefill(const void *q, int64_t q_token_stride, const vo
   launch(varlen_prefill_tiled_kernel<kPackedPrefill>, prefill_waves(kPackedPrefill));
   return check_launch("varlen_prefill");
 }
+#endif  // !LITEKV_CROSS
 }  // namespace LITEKV_HD_NS
 
-#if LITEKV_HD == 64
+#if LITEKV_CROSS && LITEKV_HD == 64
+int hd64_cross(const char *what, const void *q, int64_t q_token_stride, const void *kv_pool, const float *kv_scales,
+               const int32_t *block_table, int32_t block_table_stride, const int32_t *cu_q_lens,
+               const int32_t *kv_lens, void *out, int64_t out_token_stride, int32_t batch, int32_t num_q_heads,
+               int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int64_t num_pages, int32_t max_q_len,
+               float softmax_scale, void *stream, int format, const PrefillKeySplit &split) {
+  return launch_paged_prefill(what, q, q_token_stride, kv_pool, kv_scales, block_table, block_table_stride, cu_q_lens,
+                              kv_lens, out, out_token_stride, batch, num_q_heads, num_kv_heads, head_dim, page_size,
+                              num_pages, max_q_len, softmax_scale, stream, format, split);
+}
+#elif LITEKV_CROSS
+#elif LITEKV_HD == 64
 const PrefillBuild &hd64_prefill() {
   static const PrefillBuild build{launch_paged_prefill, launch_varlen_prefill, prefill_key_slices};
   return build;
@@ -494,7 +521,33 @@ const PrefillBuild &hd256_prefill() {
 #endif
 }  // namespace litekv
 
-#if LITEKV_HD == 128  // the C ABI lives in the head dim 128 build of this file
+#if LITEKV_CROSS && LITEKV_HD == 128
+extern "C" int litekv_paged_cross_attention(const void *q, int64_t q_token_stride, const void *kv_pool,
+                                            const float *kv_scales, int32_t pool_format,
+                                            const int32_t *block_table, int32_t block_table_stride,
+                                            const int32_t *cu_q_lens, const int32_t *kv_lens, void *out,
+                                            int64_t out_token_stride, int32_t batch, int32_t num_q_heads,
+                                            int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                                            int64_t num_pages, int32_t max_q_len, int64_t max_kv_len,
+                                            int64_t num_tokens, int32_t key_slices, void *workspace,
+                                            size_t workspace_bytes, float softmax_scale, void *stream) {
+  using namespace litekv;
+  const char *what = "paged_cross_attention";
+  LITEKV_REQUIRE(pool_format >= kKvF16 && pool_format <= kKvInt4, "%s: pool_format %d is not 0 (fp16), 1 (fp8), 2 (int8) or 3 (4-bit)",
+                 what, pool_format);
+  LITEKV_REQUIRE((pool_format == kKvFp8 || pool_format == kKvInt8) == (kv_scales != nullptr),
+                 "%s: pools of 8-bit codes have scales, others none", what);
+  PrefillKeySplit split;
+  split.key_slices = key_slices;
+  split.workspace = workspace;
+  split.workspace_bytes = workspace_bytes;
+  split.num_tokens = num_tokens;
+  split.max_kv_len = max_kv_len;
+  return launch_paged_prefill(what, q, q_token_stride, kv_pool, kv_scales, block_table, block_table_stride, cu_q_lens,
+                              kv_lens, out, out_token_stride, batch, num_q_heads, num_kv_heads, head_dim, page_size,
+                              num_pages, max_q_len, softmax_scale, stream, pool_format, split);
+}
+#elif LITEKV_HD == 128 && !LITEKV_CROSS  // the C ABI lives in the head dim 128 build of this file
 
 extern "C" int litekv_paged_prefill(const void *q, int64_t q_token_stride, const void *kv_pool,
                                     const int32_t *block_table, int32_t block_table_stride,

@@ -187,6 +187,12 @@ constexpr int kPagedPrefill = 0, kPackedPrefill = 1, kSharedPrefix = 2, kPagedPr
 // each; a slice leaves a normalised fp32 partial row + log-sum-exp per (query row, head), and a
 // merge launch folds the slices of a row (prefill_split_merge_kernel in paged_prefill.hip).
 
+// Added to a paged prefill's mode: every row of a sequence sees all of its kv_lens[b] keys (what is handed over as
+// context_lens), which are another sequence's than its own, an encoder's states say. All tiles but the last are then plain
+// ones, and the last is masked behind the last key. A sequence without keys has rows of zeros. (At most the keys that a row
+// of the block table can name.)
+constexpr int kCross = 16;
+
 // Column tiles per wavefront and wavefronts per workgroup of a prefill of 128 columns. Head dim 256 leaves one
 // workgroup per CU (LDS), which as four wavefronts of two column tiles is a lone wavefront per SIMD: its
 // softmax, LDS latencies and barrier waits stand in the open (MFMA busy 45 %). Eight wavefronts of one column tile
@@ -248,7 +254,7 @@ __device__ __forceinline__ void tile_by_rows(uint32_t lds, const half_t *q, int6
 template <int W>
 constexpr int tile_lds_bytes() { return (W == kWideWaves && kHD != 256 ? 6 : 4) * kTileHalfs * 2; }
 
-template <int MODE, int W, int KG = 1, int CT = kColTiles>
+template <int MODE_AND_CROSS, int W, int KG = 1, int CT = kColTiles>
 __device__ __forceinline__ void prefill_tile_body(
     const uint32_t lds_base, const int block_x, const int block_y, const int block_z, const int grid_y,
     const half_t *__restrict__ q, int64_t q_stride, half_t *__restrict__ out, int64_t out_stride,
@@ -257,6 +263,8 @@ __device__ __forceinline__ void prefill_tile_body(
     const int32_t *__restrict__ context_lens, int32_t group, int32_t head_splits,
     int32_t heads_per_wg, int32_t row_tiles, float scale_log2, const int key_slice = 0,
     const int key_slices = 1) {
+  constexpr int MODE = MODE_AND_CROSS & (kCross - 1);
+  constexpr bool CROSS = (MODE_AND_CROSS & kCross) != 0;
   constexpr bool PAGED = MODE != kPackedPrefill;
   // causal prefill over one slice of the block's keys
   constexpr bool KSPLIT = MODE == kPagedPrefillSplit || MODE == kPagedPrefillSplitFp8 ||
@@ -345,6 +353,32 @@ __device__ __forceinline__ void prefill_tile_body(
     kv_end = ctx + m0 + rows;
     diag = ctx + m0;
     last_key = ctx + q_len - 1;
+    if constexpr (CROSS) {
+      static_assert(PAGED && !SHARED && kHD != 256, "an encoder's states lie in pages");
+      const int64_t named = (int64_t)paged.bt_stride << (4 + paged.page_shift);
+      kv_end = ctx < named ? ctx : (int)named;
+      diag = last_key = kv_end - 1;
+      if (kv_end <= 0) {
+        for (int t = wave * CT; t < wave * CT + CT; ++t) {
+          const int head = t / row_tiles;
+          const int row = m0 + (t - head * row_tiles) * 16 + n;
+          if (head >= heads_here || row >= q_len) continue;
+          const int hq = h * group + head0 + head;
+          if constexpr (KSPLIT) {
+            const int64_t cell = ((int64_t)key_slice * prefix.batch + q_start + row) * prefix.num_q_heads + hq;
+            if (g == 0) prefix.part_lse[cell] = -INFINITY;
+            float4_t *dst = (float4_t *)(prefix.part_o + cell * kHD) + g * (kHD / 16);
+#pragma unroll
+            for (int i = 0; i < kHD / 16; ++i) dst[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+          } else {
+            half8_t *dst = (half8_t *)(out + (int64_t)(q_start + row) * out_stride + (int64_t)hq * kHD) + g * (kHD / 32);
+#pragma unroll
+            for (int i = 0; i < kHD / 32; ++i) dst[i] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+          }
+        }
+        return;
+      }
+    }
     if constexpr (KG == 2) {
       // The first group takes the first half of the tiles, the second the rest: as in a launch over key
       // slices, from no later than the last tile that every row of the block sees in full. (A block of
@@ -595,7 +629,7 @@ __device__ __forceinline__ void prefill_tile_body(
       ok = head < heads_here && row < q_len;
       hq = h * group + head0 + (head < heads_here ? head : 0);
       const int last = q_len - 1;
-      q_pos[u] = ctx + (row < last ? row : last);
+      q_pos[u] = CROSS ? last_key : ctx + (row < last ? row : last);
       out_row[u] = ok ? q_start + row : -1;
       qrow = q + (int64_t)(q_start + (ok ? row : 0)) * q_stride + (int64_t)hq * kHD + 8 * g;
     }
@@ -1322,8 +1356,9 @@ __global__ __launch_bounds__(prefill_waves(MODE) * kWave, kWgPerCu *prefill_wave
     const int32_t *__restrict__ context_lens, int32_t group, int32_t head_splits,
     int32_t heads_per_wg, int32_t row_tiles, float scale_log2, int32_t key_slices) {
   __shared__ __attribute__((aligned(1024))) half_t lds_all[tile_lds_bytes<prefill_waves(MODE)>() / 2];
-  if constexpr (MODE == kPagedPrefillSplit || MODE == kPagedPrefillSplitFp8 ||
-                MODE == kPagedPrefillSplitInt8 || MODE == kPagedPrefillSplitInt4) {
+  constexpr int KIND = MODE & (kCross - 1);
+  if constexpr (KIND == kPagedPrefillSplit || KIND == kPagedPrefillSplitFp8 ||
+                KIND == kPagedPrefillSplitInt8 || KIND == kPagedPrefillSplitInt4) {
     // blockIdx.y = row block * key_slices + slice: the slices of a block are neighbours
     const int by = (int)blockIdx.y / key_slices;
     prefill_tile_body<MODE, prefill_waves(MODE), 1, CT>((uint32_t)(uintptr_t)(lds_half_t *)lds_all, (int)blockIdx.x, by,

@@ -8,6 +8,7 @@ enqueue work on ``torch.cuda.current_stream()``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional, Sequence
 
@@ -1166,3 +1167,208 @@ def varlen_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts
                                          b, hq, hkv, d, int(max_seq_len), t, float(softmax_scale),
                                          _stream()))
     return out
+
+
+# ---- requests with images: positions of several axes, an encoder's states, the draw of a token -------------------------------
+
+POOL_FORMATS = {torch.float16: 0, torch.uint8: 1, torch.float8_e4m3fn: 1, torch.int8: 2, INT4_DTYPE: 3}   # LITEKV_POOL_*
+
+
+def _here(*tensors: Optional[torch.Tensor]) -> None:
+    """A launch goes to the current device, and so must every tensor of a call."""
+    device = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and not (t.is_cuda and t.get_device() == device):
+            raise ValueError(f"a tensor lives on {t.device}, which is not the current GPU")
+
+
+@functools.lru_cache(maxsize=64)
+def axis_of_pair(sections: tuple, head_dim: int, interleaved: bool = False) -> bytes:
+    """Which axis' position each of a row's head_dim / 2 pairs takes, a byte each. ``sections``: pairs of each axis, together
+    head_dim / 2. In runs, axis after axis; or ``interleaved``: pair i that of axis i mod A where i < A * sections[axis], all
+    others axis 0's (whose own number then does not matter)."""
+    if not (1 <= len(sections) <= 4 and all(type(s) is int and s >= 0 for s in sections) and 2 * sum(sections) == head_dim):
+        raise ValueError(f"sections {sections} must be 1 to 4 whole numbers that add up to head_dim / 2 = {head_dim // 2}")
+    axes = len(sections)
+    if not interleaved:
+        return bytes(a for a, n in enumerate(sections) for _ in range(n))
+    return bytes(i % axes if i < axes * sections[i % axes] else 0 for i in range(head_dim // 2))
+
+
+def qk_norm_mrope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor,
+                         kv_pool: torch.Tensor, positions: torch.Tensor, sections: Sequence[int], cos_table: torch.Tensor,
+                         sin_table: torch.Tensor, q_norm_weight: Optional[torch.Tensor] = None,
+                         k_norm_weight: Optional[torch.Tensor] = None, rms_eps: float = 1e-6,
+                         kv_scales: Optional[torch.Tensor] = None, interleaved: bool = False) -> torch.Tensor:
+    """``qk_norm_rope_append`` for tokens whose position has several axes (time, height, width), the rows of the cos and sin
+    tables [positions, >= D / 2] gathered on the way: pair i (elements i and i + D / 2) of token t turns by entry i of row
+    ``positions[a, t]``, a the pair's axis (see ``axis_of_pair``). ``positions`` [A, T] is int32 or int64 with any strides (one
+    row expanded to all axes: text); a position outside the tables reads the nearest row. Any pool format; fp32 from the
+    inputs to the one rounding of q and to the pool's format. q [T, Hq, D] is updated in place and returned."""
+    _dev_half("q", q), _dev_half("k", k), _dev_half("v", v)
+    slots, hkv, d, _, _ = pool_geometry(kv_pool, 1)
+    if is_int4_pool(kv_pool):
+        _dev_int4_pool(kv_pool, kv_scales)
+    elif is_quantised_pool(kv_pool):
+        _dev_fp8_pool(kv_pool, kv_scales, hkv)
+    else:
+        _dev_half("kv_pool", kv_pool)
+        _need(kv_scales is None, "kv_scales belong to an fp8 or int8 pool")
+    t = q.shape[0]
+    if not (q.dim() == 3 and q.shape[2] == d):
+        raise ValueError("q must be [T, Hq, D]")
+    if not (k.shape == (t, hkv, d) and v.shape == (t, hkv, d)):
+        raise ValueError("k / v must be [T, Hkv, D] matching the pool")
+    _need((q_norm_weight is None) == (k_norm_weight is None), "q_norm_weight and k_norm_weight go together")
+    if q_norm_weight is not None:
+        for name, w in (("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight)):
+            _dev_half(name, w)
+            _need(w.numel() == d and w.is_contiguous(), "norm weights must be contiguous [D]")
+    axes = axis_of_pair(tuple(sections), d, bool(interleaved))
+    if not (positions.dtype in (torch.int32, torch.int64) and positions.shape == (len(sections), t)):
+        raise ValueError(f"positions must be int32 or int64 [{len(sections)}, {t}]")
+    _dev_half("cos_table", cos_table), _dev_half("sin_table", sin_table)
+    if not (cos_table.dim() == 2 and cos_table.shape == sin_table.shape and cos_table.shape[0] > 0 and cos_table.shape[1] >= d // 2
+            and cos_table.stride(1) == 1 and cos_table.stride() == sin_table.stride()):
+        raise ValueError("cos_table / sin_table must be [positions, >= D / 2] with contiguous rows and equal strides")
+    slot_mapping = _dev_i32("slot_mapping", slot_mapping)
+    _need(slot_mapping.numel() == t, "slot_mapping must hold one slot per token")
+    _here(q, k, v, slot_mapping, kv_pool, positions, cos_table, sin_table, q_norm_weight, k_norm_weight, kv_scales)
+    table_stride = cos_table.stride(0) if cos_table.shape[0] > 1 else max(cos_table.stride(0), (d // 2 + 7) // 8 * 8)
+    _lib.check(_lib.load().litekv_qk_norm_mrope_append(
+        _ptr(q), _rows("q", q), _ptr(k), _rows("k", k), _ptr(v), _rows("v", v), _ptr(q_norm_weight), _ptr(k_norm_weight),
+        _ptr(cos_table), _ptr(sin_table), table_stride, cos_table.shape[0], _ptr(positions),
+        1 if positions.dtype is torch.int64 else 0, positions.stride(0), positions.stride(1), len(sections), axes,
+        _ptr(slot_mapping), _ptr(kv_pool), _ptr(kv_scales), POOL_FORMATS[pool_dtype(kv_pool)], t, q.shape[1], hkv, d, slots,
+        float(rms_eps), _stream()))
+    return q
+
+
+def paged_cross_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
+                          cu_q_lens: Optional[torch.Tensor] = None, max_q_len: int = 1,
+                          softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                          page_size: int = PAGE_SIZE, kv_scales: Optional[torch.Tensor] = None,
+                          max_kv_len: Optional[int] = None, key_slices: Optional[int] = None,
+                          workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of packed q [T, Hq, D] over all keys of another sequence, an encoder's states in pages of their own: the rows
+    [cu_q_lens[b], cu_q_lens[b + 1]) of sequence b attend its ``kv_lens[b]`` keys (at most what a row of ``block_table`` can
+    name), whatever their own number; a sequence without keys gets rows of zeros. Head dims 64 and 128, any pool format, a
+    softmax scale above 0.
+
+    ``cu_q_lens`` None: one row a sequence (a decode step), q [B, Hq, D], which streams the keys like ``paged_decode``.
+    ``max_q_len``: the most rows of a sequence. ``max_kv_len``: the most keys, as the host knows it; launches of few rows
+    are then cut along the keys as in ``paged_prefill``, and nothing but speed goes by it. Rows behind the last sequence are left as
+    they are. ``key_slices`` and ``workspace`` as there."""
+    _dev_half("q", q)
+    int4, fp8 = is_int4_pool(kv_pool), is_quantised_pool(kv_pool)
+    if q.dim() != 3:
+        raise ValueError("q must be [T, Hq, D]")
+    t, hq, d = q.shape
+    _, hkv, dk, n_pages, _ = pool_geometry(kv_pool, page_size)
+    if int4:
+        _dev_int4_pool(kv_pool, kv_scales)
+    elif fp8:
+        _dev_fp8_pool(kv_pool, kv_scales, hkv)
+    else:
+        _dev_half("kv_pool", kv_pool)
+        _need(kv_scales is None, "kv_scales belong to an fp8 or int8 pool")
+    if d != dk or d not in (64, 128):
+        raise ValueError(f"q and kv_pool must share a head_dim of 64 or 128, not {d} and {dk}")
+    q_stride = _rows("q", q)
+    b = t if cu_q_lens is None else cu_q_lens.numel() - 1
+    if not (b >= 0 and block_table.dim() == 2 and block_table.shape[0] == b and block_table.shape[1] > 0):
+        raise ValueError("block_table must be [B, max_blocks]")
+    kv_lens = _dev_i32("kv_lens", kv_lens)
+    _need(kv_lens.numel() == b, "kv_lens must be [B]")
+    softmax_scale = 1.0 / math.sqrt(d) if softmax_scale is None else float(softmax_scale)
+    _need(softmax_scale > 0.0, "softmax_scale must be above 0")
+    if out is None:
+        out = torch.empty((t, hq, d), dtype=torch.float16, device=q.device)
+    else:
+        _dev_half("out", out)
+        _need(out.shape == q.shape, "out must be [T, Hq, D]")
+    _here(q, kv_pool, block_table, kv_lens, cu_q_lens, out, kv_scales, workspace)
+    if cu_q_lens is None:
+        _need(key_slices is None and workspace is None, "key_slices and workspace belong to rows of several a sequence")
+        return _cross_rows(q, kv_pool, block_table, kv_lens, softmax_scale, out, page_size, kv_scales, max_kv_len, hkv, n_pages)
+    cu_q_lens = _dev_i32("cu_q_lens", cu_q_lens)
+    block_table, bt_stride = _table_rows(_dev_i32("block_table", block_table))
+    lib = _lib.load()
+    most = 0 if max_kv_len is None else int(max_kv_len)
+    if key_slices is None:
+        # (as in paged_prefill)
+        key_slices = int(lib.litekv_paged_prefill_key_slices(b, hq, hkv, d, int(max_q_len), most)) if most > 0 and 0 < t * hq <= 128 * 512 else 1
+    key_slices = max(1, int(key_slices))
+    if key_slices > 1:
+        need = paged_prefill_workspace_floats(t, hq, d, key_slices)
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.float32, device=q.device)
+        elif not (workspace.dtype == torch.float32 and workspace.is_contiguous() and workspace.numel() >= need):
+            raise ValueError(f"workspace must be {need} contiguous float32 on the device")
+    _lib.check(lib.litekv_paged_cross_attention(
+        _ptr(q), q_stride, _ptr(kv_pool), _ptr(kv_scales), POOL_FORMATS[pool_dtype(kv_pool)], _ptr(block_table), bt_stride,
+        _ptr(cu_q_lens), _ptr(kv_lens), _ptr(out), _rows("out", out), b, hq, hkv, d, page_size, n_pages, int(max_q_len), most, t,
+        key_slices, _ptr(workspace), 0 if workspace is None else workspace.numel() * 4, softmax_scale, _stream()))
+    return out
+
+
+def _cross_rows(q, kv_pool, block_table, kv_lens, softmax_scale, out, page_size, kv_scales, max_kv_len, hkv, n_pages):
+    """One row a sequence: the decode kernels, on the schedule for sequences of ``max_kv_len`` keys each."""
+    b, hq, d = q.shape
+    if b == 0:
+        return out
+    width = int(block_table.shape[1])
+    pages = width if max_kv_len is None else max(1, min(width, -(-int(max_kv_len) // page_size)))
+    if is_int4_pool(kv_pool):
+        splits, least = int4_decode_splits(b, hkv, pages, page_size=page_size)
+        return paged_decode(q, kv_pool, block_table, kv_lens, softmax_scale, max_splits=splits, min_pages_per_split=least, out=out,
+                            page_size=page_size)
+    splits = _cross_schedule(b, hkv, pages, 2 * hkv * d * kv_pool.element_size(), page_size, hq // hkv, d)
+    if splits > 0:
+        return paged_decode(q, kv_pool, block_table, kv_lens, softmax_scale, max_splits=splits, min_pages_per_split=1, out=out,
+                            page_size=page_size, kv_scales=kv_scales)
+    plan = DecodePlan(block_table, kv_lens, hq, hkv, n_pages, page_size=page_size, kv_dtype=kv_pool.dtype,
+                      token_bytes=2 * hkv * d * kv_pool.element_size())
+    return decode_step(q, kv_pool, plan, None, None, softmax_scale, out, kv_scales)
+
+
+@functools.lru_cache(maxsize=256)
+def _cross_schedule(batch: int, num_kv_heads: int, pages: int, token_bytes: int, page_size: int, group: int, head_dim: int) -> int:
+    return decode_schedule(batch, num_kv_heads, pages, batch * pages, token_bytes, page_size, group, head_dim=head_dim)
+
+
+_LOGITS_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+                  top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                  min_p: Optional[torch.Tensor] = None, return_logprobs: bool = False):
+    """One token (int64) per row of ``logits`` [B, vocab] (fp16, bf16 or fp32, rows with any stride), drawn with ``uniforms`` [B]
+    in [0, 1): the first token, by index, at which the kept mass exceeds u times all of it. Kept are the first ``top_k`` tokens by
+    probability (ties: the lowest index first), of them the shortest run that reaches ``top_p`` of their mass, of them those of at
+    least ``min_p`` times the largest probability; always the first. Each filter is a tensor of the batch or None; a row's top_k
+    below 1, top_p of 1 or more and min_p of 0 or less are off. Temperature 0 (or less) takes the first largest logit.
+    Tokens further than 40 * temperature below the largest are never drawn, nor are those of -inf or NaN; a row without any
+    other gives token -1. With ``return_logprobs`` (tokens, logprobs): the token's logarithm of probability among the kept."""
+    if not logits.is_cuda or logits.dtype not in _LOGITS_TYPES:
+        raise ValueError(f"logits must be float16, bfloat16 or float32 on the GPU, not {logits.dtype} on {logits.device}")
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be [B, vocab] with contiguous rows")
+    b, vocab = logits.shape
+    for name, x, dtype in (("uniforms", uniforms, torch.float32), ("temperature", temperature, torch.float32),
+                           ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if x is None and name != "uniforms":
+            continue
+        if not (x.is_cuda and x.dtype is dtype and x.is_contiguous() and x.numel() == b):
+            raise ValueError(f"{name} must be contiguous {dtype} [{b}] on the GPU")
+    _here(logits, uniforms, temperature, top_k, top_p, min_p)
+    lib = _lib.load()
+    kind = _LOGITS_TYPES[logits.dtype]
+    tokens = torch.empty(b, dtype=torch.int64, device=logits.device)
+    logprobs = torch.empty(b, dtype=torch.float32, device=logits.device) if return_logprobs else None
+    need = int(lib.litekv_sample_tokens_workspace_bytes(kind, b, vocab))
+    workspace = torch.empty((need + 7) // 8, dtype=torch.int64, device=logits.device)
+    _lib.check(lib.litekv_sample_tokens(_ptr(logits), kind, logits.stride(0) if b > 1 else vocab, _ptr(uniforms), _ptr(temperature),
+                                        _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(tokens), _ptr(logprobs), b, vocab,
+                                        _ptr(workspace), need, _stream()))
+    return (tokens, logprobs) if return_logprobs else tokens
