@@ -936,7 +936,7 @@ int litekv_paged_cross_attention(const void *q, int64_t q_token_stride, const vo
  * kept. Masses are exact to 2^-41 of themselves. T <= 0 (or NaN) takes the first
  * largest logit, with logprob 0.
  *   logits       [batch][row_stride], logits_type 0 fp16, 1 bf16, 2 fp32; aligned to an
- *                element. NaN and -inf are never drawn, +inf counts as the largest finite fp32
+ *                element. NaN and -inf are never drawn, +inf counts as the type's largest finite
  *                number. A row without any other: token -1, logprob -inf
  *   uniforms     [batch], in [0, 1) (what is outside counts as the nearest inside, NaN as 0)
  *   temperature  [batch], NULL: 1

@@ -4,39 +4,52 @@
 // first), so what is kept is the shortest of three prefixes: everything above one logit, and the first few of those that equal
 // it. The token is the first, by index, at which the kept mass exceeds u times all of it.
 //
-// Nothing is sorted. A first launch cuts the rows into slices, a workgroup each, and leaves per slice a histogram over y: bins of
-// 1/8 on a grid that all slices share, each with the number and the mass of its tokens. A second one, a workgroup per row, adds
-// them up, walks the bins to the one in which a filter's prefix ends, reads the row's tokens of that bin again and finds the
-// logit by their bits, ten at a time. Sums of mass are sums of whole numbers: the mass of a token is rounded to 2^-40
-// of its bin's top (y enters in fp64, and exp by a polynomial over the width of a bin), so no order of additions shows in a
-// token, and a bin's top is a factor applied once. A cumulative mass is then within 2^-41 of itself wherever it is compared, which
-// in a row of 150 000 tokens moves one draw in some millions to a neighbour of the token that exact arithmetic gives.
+// Nothing is sorted. A first launch cuts the rows into slices, a workgroup each, and leaves per slice a histogram over y (bins of
+// 1/8 on a grid that all slices share, each with the number and the mass of its tokens) and a list of its likeliest tokens. A
+// second one, a workgroup per row, adds the histograms up and walks the bins to the one in which a filter's prefix ends. Its
+// tokens come from the lists or, where these do not reach so far, from a pass over the row; the end among them, and
+// in the kept ones the token drawn, are found by the digits of their keys and, once they are few, by ranking them.
+//
+// Sums of mass are sums of whole numbers: the mass of a token is rounded to 2^-40 of its bin's top (y enters in fp64, and exp by a
+// polynomial over the width of a bin), so no order of additions shows in a token, and a bin's top is a factor applied once. A
+// cumulative mass is then within 2^-40 of itself wherever it is compared, which in a row of 150 000 tokens moves one draw in some
+// millions to a neighbour of the token that exact arithmetic gives.
 #include <cmath>
 
 #include "common.h"
+#include "kv_int4.h"
+
+// Products are rounded before they are subtracted from: z - floor(z) with a product z in one operation would leave z's own rounding
+// error beside the place in the bin, and of a large z nothing else.
+#pragma clang fp contract(off)
 
 namespace litekv {
 
 constexpr int kSampleBins = 322;              // of 1/8: what is further than 40 below a row's largest y is never drawn
+constexpr int kSampleSlots = 512;             // a slice's bins lie at their place on the grid modulo this
 constexpr int kSampleThreads = 256;           // of a slice's workgroup
 constexpr int kSampleSlice = 8192;            // tokens of a slice at most: their number has 14 bits of a bin's word
+constexpr int kSliceList = 128;               // tokens of a slice's list
 constexpr int kRowThreads = 1024;             // of a row's workgroup
+constexpr int kRowWaves = kRowThreads / kWave;
 constexpr int kSampleList = 8192;             // tokens that a row's workgroup holds
 constexpr int kSampleMaxVocab = 1 << 20;
-constexpr int kRadix = 1024;
-constexpr double kUnit = 0x1p-40;             // of a bin's top
-constexpr double kFloor = 0.875;              // below exp(-1/8): a bin's word has the sum of what is above it
-constexpr uint64_t kFloorUnits = 7ull << 37;
-constexpr uint64_t kMostUnits = (1ull << 37) - 1;
+constexpr int kMaxSlices = 520;
+constexpr int kRanked = 64;                   // tokens that are ranked against each other; more go by their digits
 constexpr int kCountShift = 50;
 constexpr uint64_t kUnitsMask = (1ull << kCountShift) - 1;
+constexpr uint64_t kFloorUnits = 7ull << 37;  // 7/8, below exp(-1/8): a bin's word has the sum of what is above it
+constexpr double kUnit = 0x1p-40 / (1.0 - 0x1p-20);   // of a bin's top (see mass_bits)
 constexpr double kCut = -40.0;
 constexpr double kReached = 1.0 - 0x1p-40;    // a border that rounding alone keeps from being reached is
+constexpr float kMostFloat = 3.4028234663852886e38f;
 
-struct SampleSlice {      // of the workspace, in front of the histograms
+struct SampleSlice {      // of the workspace, in front of the histograms and the lists
   double top;             // the bin of its largest y, counted from 0
   float most;             // its largest logit, -inf: nothing can be drawn
-  int32_t at;             // the first token that has it
+  int32_t at;             // greedy rows: the first token that has it
+  int32_t listed;         // tokens of its list: all of the `listed_bins` bins from its top on
+  int32_t listed_bins;
 };
 
 // The vectors of 16 bytes that a row's slices are counted in: of V elements, the first of them anywhere in its vector.
@@ -50,25 +63,23 @@ static int sample_slice_vectors(int32_t batch, int32_t vocab, int size) {
 enum { kLogitsF16 = 0, kLogitsBf16 = 1, kLogitsF32 = 2 };
 constexpr int logit_size(int type) { return type == kLogitsF32 ? 4 : 2; }
 
-// The elements of one vector as floats; what cannot be drawn is -inf. NaN is such a one; infinity is the largest finite number.
+// The largest finite logit of a type, which infinity counts as.
 template <int TYPE>
-__device__ __forceinline__ void logits_of(uint4_t raw, int64_t first, int32_t vocab, float (&x)[16 / logit_size(TYPE)]) {
-  constexpr int kPer = 16 / logit_size(TYPE);
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    float f;
-    if constexpr (TYPE == kLogitsF32) {
-      const uint32_t word = raw[i];        // (a bit cast of the element itself is one of the first)
-      f = __builtin_bit_cast(float, word);
-    } else if constexpr (TYPE == kLogitsBf16) {
-      f = __builtin_bit_cast(float, i & 1 ? raw[i >> 1] & 0xffff0000u : raw[i >> 1] << 16);
-    } else {
-      f = (float)__builtin_bit_cast(half_t, (uint16_t)(raw[i >> 1] >> (16 * (i & 1))));
-    }
-    const int64_t at = first + i;
-    const bool there = at >= 0 && at < vocab && f == f;
-    x[i] = there ? __builtin_fminf(f, 3.4028234663852886e38f) + 0.0f : -INFINITY;   // (+ 0: the two zeros are one)
+constexpr float kMostLogit = TYPE == kLogitsF16 ? 65504.0f : TYPE == kLogitsBf16 ? 0x1.fep+127f : kMostFloat;
+// Element i of a vector as a float. NaN cannot be drawn and becomes -inf.
+template <int TYPE>
+__device__ __forceinline__ float logit_of(uint4_t raw, int i) {
+  float f;
+  if constexpr (TYPE == kLogitsF32) {
+    const uint32_t word = raw[i];        // (a bit cast of the element itself is one of the first)
+    f = __builtin_bit_cast(float, word);
+  } else if constexpr (TYPE == kLogitsBf16) {
+    const uint32_t word = i & 1 ? raw[i >> 1] & 0xffff0000u : raw[i >> 1] << 16;
+    f = __builtin_bit_cast(float, word);
+  } else {
+    f = (float)__builtin_bit_cast(half_t, (uint16_t)(raw[i >> 1] >> (16 * (i & 1))));
   }
+  return __builtin_fminf(__builtin_fmaxf(f, -INFINITY), kMostLogit<TYPE>);
 }
 
 // Where the vector `at` of a row is; only those with an element of the row are read.
@@ -87,63 +98,151 @@ __device__ __forceinline__ LogitsRow logits_row(const void *logits, int64_t row_
   r.vectors = ((int64_t)(r.lead + vocab) * kSize + 15) / 16;
   return r;
 }
+// The elements of vector `at`, -inf in the places that are not the row's.
+template <int TYPE>
+__device__ __forceinline__ void logits_of(const LogitsRow &in, uint4_t raw, int64_t at, int32_t vocab,
+                                          float (&x)[16 / logit_size(TYPE)]) {
+  constexpr int kPer = 16 / logit_size(TYPE);
+  const int64_t first = at * kPer - in.lead;
+  const bool inside = first >= 0 && first + kPer <= vocab;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) x[i] = logit_of<TYPE>(raw, i);
+  if (!inside) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (first + i < 0 || first + i >= vocab) x[i] = -INFINITY;
+    }
+  }
+}
 
-// The bin of y = x / T counted from 0, and the token's mass in units of the bin's top, less the floor's.
-struct Binned {
-  double bin;
-  uint64_t units;
-};
-__device__ __forceinline__ double bin_of(float x, double inv_t) { return __builtin_floor((double)x * inv_t * 8.0); }
-__device__ __forceinline__ Binned binned(float x, double inv_t) {
-  const double y = (double)x * inv_t;
-  const double b = __builtin_floor(y * 8.0);
-  // exp(y - top), top = (b + 1) / 8: exp(-1/16) exp(r), |r| <= 1/16, to 2^-43 of itself
-  const double r = (y - b * 0.125) - 0.0625;
-  double e = 1.0 / 5040.0;
-  e = __builtin_fma(e, r, 1.0 / 720.0);
-  e = __builtin_fma(e, r, 1.0 / 120.0);
-  e = __builtin_fma(e, r, 1.0 / 24.0);
-  e = __builtin_fma(e, r, 1.0 / 6.0);
-  e = __builtin_fma(e, r, 0.5);
-  e = __builtin_fma(e, r, 1.0);
-  e = __builtin_fma(e, r, 1.0);
-  constexpr double kMiddle = 0.93941306281347578611;      // exp(-1/16)
-  // in whole units, as the low bits of a sum with 2^52
-  const double u = __builtin_fma(e, kMiddle / kUnit, -kFloor / kUnit);
-  const uint64_t bits = __builtin_bit_cast(uint64_t, __builtin_fmin(__builtin_fmax(u, 0.0), (double)kMostUnits) + 0x1p52);
-  return Binned{b, bits & ((1ull << 52) - 1)};
+// z = 8 y; its bin is floor(z).
+__device__ __forceinline__ double z_of(float x, double z_per_x) { return (double)x * z_per_x; }
+// (1 - 2^-20) exp((f - 1) / 8) - 7/8 in units of 2^-40, f in [0, 1) the place in a bin: below 2^37, and above 0. By the polynomial of
+// degree 6 that agrees with it in seven Chebyshev points, within 0.02 of a unit. As the low 52 bits of a double: 2^52 is added.
+__device__ __forceinline__ uint64_t mass_bits(double f) {
+  double e = 0x1.56123fcc468c2p+12;
+  e = __builtin_fma(e, f, 0x1.e10f01fb822cdp+17);
+  e = __builtin_fma(e, f, 0x1.2d3c27a6b0e5fp+23);
+  e = __builtin_fma(e, f, 0x1.2d39a7c5007cap+28);
+  e = __builtin_fma(e, f, 0x1.c3d68623f9176p+32);
+  e = __builtin_fma(e, f, 0x1.c3d686115b6e3p+36);
+  e = __builtin_fma(e, f, 0x1.eb4308b7019d4p+32);
+  return __builtin_bit_cast(uint64_t, e + 0x1p52);
+}
+constexpr uint64_t kMassOne = 0x4330000000000000ull;      // 2^52's bits
+__device__ __forceinline__ uint64_t units_of(double z) { return mass_bits(z - __builtin_floor(z)) - kMassOne; }
+// In whole numbers; out of their range the nearest, as the conversion does it, which C++ leaves open.
+__device__ __forceinline__ uint32_t whole_of(double x) {
+  uint32_t n;
+  asm("v_cvt_u32_f64 %0, %1" : "=v"(n) : "v"(x));
+  return n;
 }
 
 __device__ __forceinline__ uint32_t order_of(float x) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, x);
+  const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);         // (the two zeros are one)
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float logit_of_order(uint32_t k) {
   return __builtin_bit_cast(float, k ^ (k & 0x80000000u ? 0x80000000u : 0xffffffffu));
 }
 
+// Tokens are told apart, and ordered like p and the index, by a key: the order of the logit without the bits that its type leaves
+// alike, then the index from the last down.
+template <int TYPE>
+constexpr int kAlike = TYPE == kLogitsF16 ? 13 : TYPE == kLogitsBf16 ? 16 : 0;
+constexpr int kIndexBits = 20;
+template <int TYPE>
+__device__ __forceinline__ uint64_t key_of(uint32_t order, int32_t at) {
+  return (uint64_t)(order >> kAlike<TYPE>) << kIndexBits | (uint64_t)(kSampleMaxVocab - 1 - at);
+}
+__device__ __forceinline__ int32_t index_of_key(uint64_t key) {
+  return kSampleMaxVocab - 1 - (int32_t)(key & (uint64_t)(kSampleMaxVocab - 1));
+}
+template <int TYPE>
+__device__ __forceinline__ float logit_of_key(uint64_t key) {
+  const uint32_t o = (uint32_t)(key >> kIndexBits) << kAlike<TYPE>;
+  return logit_of_order(o & 0x80000000u ? o : o | ((1u << kAlike<TYPE>) - 1u));
+}
+// The lowest key of a token whose order is at least `order`.
+template <int TYPE>
+__device__ __forceinline__ uint64_t lowest_key(uint32_t order) {
+  const uint32_t up = order & 0x80000000u ? (1u << kAlike<TYPE>) - 1u : 0u;      // (a negative token's alike bits are ones)
+  return (((uint64_t)order + up) >> kAlike<TYPE>) << kIndexBits;
+}
+
 __device__ __forceinline__ float row_temperature(const float *temperature, int row) {
   const float t = temperature != nullptr ? temperature[row] : 1.0f;
-  return t > 3.4028234663852886e38f ? 3.4028234663852886e38f : t;      // (NaN stays)
+  return t > kMostFloat ? kMostFloat : t;      // (NaN stays)
 }
 __device__ __forceinline__ bool greedy_temperature(float t) { return !(t > 0.f); }
+__device__ __forceinline__ int slot_of(double bin) { return (int)(bin - 512.0 * __builtin_floor(bin * 0x1p-9)); }
 
-// A slice: its largest logit, then its histogram. Bound by memory, and behind it by the LDS additions.
+__device__ __forceinline__ float wave_max(float x) {
+  x = __builtin_fmaxf(x, dpp<kDppXor1>(x));
+  x = __builtin_fmaxf(x, dpp<kDppXor2>(x));
+  x = __builtin_fmaxf(x, dpp<kDppMirror8>(x));
+  x = __builtin_fmaxf(x, dpp<kDppMirror16>(x));
+  return max_over_lane_groups(x);
+}
+// What the lane `CTRL` names holds, 0 where there is none or the row of 16 is not in ROWS.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T lane_at(T x) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, true));
+  } else {
+    typedef int int2_t __attribute__((ext_vector_type(2)));
+    int2_t v = __builtin_bit_cast(int2_t, x);
+    v[0] = __builtin_amdgcn_update_dpp(0, v[0], CTRL, ROWS, 0xf, true);
+    v[1] = __builtin_amdgcn_update_dpp(0, v[1], CTRL, ROWS, 0xf, true);
+    return __builtin_bit_cast(T, v);
+  }
+}
+// Inclusive sums over a wavefront's lanes, in one order: rows of 16 by shifts, then their ends.
+template <typename T>
+__device__ __forceinline__ T wave_scan(T x) {
+  x += lane_at<0x111, 0xf>(x);
+  x += lane_at<0x112, 0xf>(x);
+  x += lane_at<0x114, 0xf>(x);
+  x += lane_at<0x118, 0xf>(x);
+  x += lane_at<0x142, 0xa>(x);
+  x += lane_at<0x143, 0xc>(x);
+  return x;
+}
+// The lowest logit, by order, that `above` holds for, which grows with the logit: within a few floats of a guess. (Each wavefront
+// finds it for itself.)
+template <typename Above>
+__device__ __forceinline__ uint32_t border(double guess, Above above) {
+  const float near = (float)__builtin_fmin(__builtin_fmax(guess, -(double)kMostFloat), (double)kMostFloat);
+  const int64_t lowest = order_of(-kMostFloat), highest = order_of(kMostFloat);
+  const int64_t o = (int64_t)order_of(near) + (int)(threadIdx.x % kWave) - 32;
+  const uint64_t all = __builtin_amdgcn_ballot_w64(o > highest || (o >= lowest && above(logit_of_order((uint32_t)o))));
+  const int64_t first = (int64_t)order_of(near) + (all != 0 ? __builtin_ctzll(all) : 63) - 32;
+  return (uint32_t)(first < lowest ? lowest : first);
+}
+// The lowest logit whose bin, counted from 0, is at least `limit`.
+__device__ __forceinline__ uint32_t lowest_of_bin(double limit, float t, double z_per_x) {
+  return border(limit * 0.125 * (double)t, [&](float x) { return __builtin_floor(z_of(x, z_per_x)) >= limit; });
+}
+
+// A slice: its largest logit, then its histogram, in two copies for two wavefronts each. A token adds its mass's bits as they are to
+// its bin: the words' top 12 bits then hold 0x433 times the number of tokens, modulo 4096.
 template <int TYPE>
 __global__ __launch_bounds__(kSampleThreads) void sample_slices_kernel(
     const void *__restrict__ logits, int64_t row_stride, const float *__restrict__ temperature, int32_t vocab,
-    int32_t slice_vectors, int32_t slices, SampleSlice *__restrict__ heads, uint64_t *__restrict__ bins) {
+    int32_t slice_vectors, int32_t slices, SampleSlice *__restrict__ heads, uint64_t *__restrict__ bins,
+    uint64_t *__restrict__ lists) {
   constexpr int kPer = 16 / logit_size(TYPE);
   constexpr int kMostVectors = kSampleSlice / kPer / kSampleThreads;
-  __shared__ uint64_t hist[kSampleBins];
-  __shared__ float wave_most[kSampleThreads / kWave];
-  __shared__ int wave_at[kSampleThreads / kWave];
-  const int tid = threadIdx.x, row = blockIdx.y, slice = blockIdx.x;
+  constexpr int kWaves = kSampleThreads / kWave, kCopies = 2;
+  static_assert(kSampleSlice / kCopies <= 4096, "a copy counts modulo 4096");
+  static_assert(2 * kSampleThreads >= kSampleBins, "two bins a thread");
+  __shared__ uint64_t hist[kCopies][2 * kSampleThreads];
+  __shared__ float wave_most[kWaves];
+  __shared__ int wave_at[kWaves];
+  __shared__ int found_bins, found_n;
+  const int tid = threadIdx.x, row = blockIdx.y, slice = blockIdx.x, wave = tid / kWave;
   const LogitsRow in = logits_row<TYPE>(logits, row_stride, row, vocab);
-  const float t = row_temperature(temperature, row);
-  for (int i = tid; i < kSampleBins; i += kSampleThreads) hist[i] = 0;
   const int64_t v0 = (int64_t)slice * slice_vectors;
-  float x[kMostVectors][kPer];
   uint4_t raw[kMostVectors];
 #pragma unroll
   for (int i = 0; i < kMostVectors; ++i) {
@@ -151,25 +250,31 @@ __global__ __launch_bounds__(kSampleThreads) void sample_slices_kernel(
     raw[i] = uint4_t{0, 0, 0, 0};
     if (v < slice_vectors && v0 + v < in.vectors) raw[i] = *(const uint4_t *)(in.base + (v0 + v) * 16);
   }
+  const float t = row_temperature(temperature, row);
+  const double z_per_x = 8.0 / (double)t;
+#pragma unroll
+  for (int i = tid; i < kCopies * 2 * kSampleThreads; i += kSampleThreads) hist[0][i] = 0;
+  if (tid == 0) {
+    found_bins = 0;
+    found_n = 0;
+  }
+  float x[kMostVectors][kPer];
   float most = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kMostVectors; ++i) {
     const int v = i * kSampleThreads + tid;
-    const bool there = v < slice_vectors && v0 + v < in.vectors;
-    logits_of<TYPE>(raw[i], there ? (v0 + v) * kPer - in.lead : -kPer, vocab, x[i]);
+    logits_of<TYPE>(in, raw[i], v < slice_vectors ? v0 + v : in.vectors, vocab, x[i]);      // (behind the row: nothing of it)
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) most = fmaxf(most, x[i][k]);
+    for (int k = 0; k < kPer; ++k) most = __builtin_fmaxf(most, x[i][k]);
   }
-  const int wave = tid / kWave;
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, kWave));
+  most = wave_max(most);
   if (tid % kWave == 0) wave_most[wave] = most;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kSampleThreads / kWave; ++w) most = fmaxf(most, wave_most[w]);
+  for (int w = 0; w < kWaves; ++w) most = __builtin_fmaxf(most, wave_most[w]);
   SampleSlice *head = heads + (int64_t)row * slices + slice;
   if (most == -INFINITY) {
-    if (tid == 0) *head = SampleSlice{0.0, -INFINITY, 0};
+    if (tid == 0) *head = SampleSlice{0.0, -INFINITY, 0, 0, kSampleBins};
     return;
   }
   if (greedy_temperature(t)) {
@@ -190,109 +295,188 @@ __global__ __launch_bounds__(kSampleThreads) void sample_slices_kernel(
     if (tid % kWave == 0) wave_at[wave] = at;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kSampleThreads / kWave; ++w) at = wave_at[w] < at ? wave_at[w] : at;
-    if (tid == 0) *head = SampleSlice{0.0, most, at};
+    for (int w = 0; w < kWaves; ++w) at = wave_at[w] < at ? wave_at[w] : at;
+    if (tid == 0) *head = SampleSlice{0.0, most, at, 0, 0};
     return;
   }
-  const double inv_t = 1.0 / (double)t;
-  const double top = bin_of(most, inv_t);
+  const double top = __builtin_floor(z_of(most, z_per_x));
+  uint64_t *mine = hist[wave / (kWaves / kCopies)];
 #pragma unroll
   for (int i = 0; i < kMostVectors; ++i) {
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      if (x[i][k] > -INFINITY) {
-        const Binned b = binned(x[i][k], inv_t);
-        const double d = top - b.bin;
-        if (d < (double)kSampleBins) {
-          atomicAdd((unsigned long long *)&hist[(int)d], (unsigned long long)(b.units | (1ull << kCountShift)));
-        }
-      }
+      const double z = z_of(x[i][k], z_per_x), b = __builtin_floor(z);
+      const uint32_t d = whole_of(top - b);                      // (-inf: far below)
+      if (d < (uint32_t)kSampleBins) atomicAdd((unsigned long long *)&mine[d], (unsigned long long)mass_bits(z - b));
     }
   }
   __syncthreads();
-  uint64_t *to = bins + ((int64_t)row * slices + slice) * kSampleBins;
-  for (int i = tid; i < kSampleBins; i += kSampleThreads) to[i] = hist[i];
-  if (tid == 0) *head = SampleSlice{top, most, 0};
+  // Two bins a thread, to their places; and how many from the top on have no more tokens than a list takes.
+  const int64_t place = (int64_t)row * slices + slice;
+  const int top_slot = slot_of(top);
+  int count = 0, count_first = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int b = 2 * tid + i;
+    uint64_t n_all = 0, units = 0;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      const uint64_t w = hist[c][b];
+      uint64_t n = ((w >> 52) * 1787u) & 4095u;            // 1787 * 0x433 = 1 modulo 4096
+      const uint64_t u = w & ((1ull << 52) - 1);
+      n = n == 0 && u != 0 ? 4096 : n;
+      n_all += n;
+      units += u;
+    }
+    if (b < kSampleBins) bins[place * kSampleSlots + ((top_slot - b) & (kSampleSlots - 1))] = units | n_all << kCountShift;
+    count += (int)n_all;
+    if (i == 0) count_first = count;
+  }
+  int upto = wave_scan(count);
+  if (tid % kWave == kWave - 1) wave_at[wave] = upto;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves - 1; ++w) upto += w < wave ? wave_at[w] : 0;
+  const int first_upto = upto - count + count_first;
+  if (first_upto <= kSliceList) atomicMax(&found_bins, upto <= kSliceList ? 2 * tid + 2 : 2 * tid + 1);
+  __syncthreads();
+  const int listed_bins = found_bins < kSampleBins ? found_bins : kSampleBins;
+  if (listed_bins > 0) {
+    const float least = logit_of_order(lowest_of_bin(top - (listed_bins - 1), t, z_per_x));
+#pragma unroll
+    for (int i = 0; i < kMostVectors; ++i) {
+      uint32_t those = 0;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) those |= (x[i][k] >= least ? 1u : 0u) << k;
+      while (those != 0) {
+        const int k = __builtin_ctz(those);
+        those &= those - 1;
+        float e = x[i][0];
+#pragma unroll
+        for (int j = 1; j < kPer; ++j) e = k == j ? x[i][j] : e;
+        const int slot = atomicAdd(&found_n, 1);
+        if (slot < kSliceList) {
+          lists[place * kSliceList + slot] = key_of<TYPE>(order_of(e), (int)((v0 + i * kSampleThreads + tid) * kPer - in.lead + k));
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (tid == 0) *head = SampleSlice{top, most, 0, found_n < kSliceList ? found_n : kSliceList, listed_bins};
 }
 
 // ---- a row ---------------------------------------------------------------------------------------------------------------------
-// Inclusive sums over the workgroup's threads, in one order.
+struct RowRoom {           // of a scan; two are used in turn, so that one barrier is enough
+  double mass[kRowWaves];
+  unsigned long long units[kRowWaves];
+  int32_t count[kRowWaves];
+};
+// Inclusive sums over the workgroup's threads, in one order, and all of them.
 template <typename T>
-__device__ __forceinline__ T wave_scan(T x) {
-  const int lane = threadIdx.x % kWave;
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) {
-    const T up = __shfl_up(x, off, kWave);
-    if (lane >= off) x += up;
-  }
-  return x;
-}
-template <typename T>
-__device__ __forceinline__ T row_scan(T x, T *room, T *total) {      // room: kRowThreads / kWave
+__device__ __forceinline__ T row_scan(T x, T *room, T *all) {
   const int wave = threadIdx.x / kWave;
   x = wave_scan(x);
-  __syncthreads();
   if (threadIdx.x % kWave == kWave - 1) room[wave] = x;
   __syncthreads();
-  T before = 0, all = 0;
+  T before = 0, sum = 0;
 #pragma unroll
-  for (int w = 0; w < kRowThreads / kWave; ++w) {
-    before += w < wave ? room[w] : T(0);
-    all += room[w];
+  for (int w = 0; w < kRowWaves; ++w) {
+    const T part = room[w];
+    before += w < wave ? part : T(0);
+    sum += part;
   }
-  *total = all;
+  *all = sum;
   return before + x;
 }
+template <typename T, typename U>
+__device__ __forceinline__ void row_scan2(T &x, T *room_x, U &y, U *room_y) {
+  const int wave = threadIdx.x / kWave;
+  x = wave_scan(x);
+  y = wave_scan(y);
+  if (threadIdx.x % kWave == kWave - 1) {
+    room_x[wave] = x;
+    room_y[wave] = y;
+  }
+  __syncthreads();
+  T bx = 0;
+  U by = 0;
+#pragma unroll
+  for (int w = 0; w < kRowWaves - 1; ++w) {
+    bx += w < wave ? room_x[w] : T(0);
+    by += w < wave ? room_y[w] : U(0);
+  }
+  x += bx;
+  y += by;
+}
 
-// What a filter's end in a bin comes to: of the bin's tokens those above `order`, and the first `ties` of those that equal it.
-struct Ending {
-  uint32_t order;
-  int32_t ties;
-  uint64_t units;       // of the bin's tokens that are kept
-};
-
+// Bound by latency: one memory trip or one pass over the row after another, with barriers between them. So loads are made whatever
+// their place (clamped, and masked where they are used), each piece of code stands once, and what few threads can find, each
+// wavefront finds for itself.
 template <int TYPE>
 __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     const void *__restrict__ logits, int64_t row_stride, const float *__restrict__ uniforms,
     const float *__restrict__ temperature, const int32_t *__restrict__ top_k, const float *__restrict__ top_p,
     const float *__restrict__ min_p, int64_t *__restrict__ tokens, float *__restrict__ logprobs, int32_t vocab,
-    int32_t slice_vectors, int32_t slices, const SampleSlice *__restrict__ heads, const uint64_t *__restrict__ bins) {
+    int32_t slice_vectors, int32_t slices, const SampleSlice *__restrict__ heads, const uint64_t *__restrict__ bins,
+    const uint64_t *__restrict__ lists) {
   constexpr int kPer = 16 / logit_size(TYPE);
-  constexpr int kMaxSlices = 520;
-  __shared__ double bin_top[kSampleBins];            // exp(the bin's top - the row's largest y), in units
-  __shared__ double mass_to[kSampleBins];            // inclusive
-  __shared__ int32_t count_to[kSampleBins];
-  __shared__ int32_t shift[kMaxSlices];              // of a slice's bins against the row's, kSampleBins: it has none
-  __shared__ int32_t slice_from[kMaxSlices + 1];     // where its tokens begin in the list
+  constexpr int kParts = kRowThreads / kSampleSlots;  // threads of a slot
+  static_assert(kParts == 2, "two threads a slot");
+  __shared__ double bin_top[kSampleSlots];            // exp(the bin's top - the row's largest y), in units
+  __shared__ double mass_to[kSampleSlots];            // inclusive
+  __shared__ int32_t count_to[kSampleSlots];
+  __shared__ int32_t shift[kMaxSlices];               // of a slice's bins against the row's, kSampleBins: it has none
+  __shared__ int32_t slice_listed[kMaxSlices];
   __shared__ double slice_mass[kMaxSlices];
   __shared__ unsigned long long slice_units[kMaxSlices];
-  __shared__ int32_t slice_ties[kMaxSlices];
-  __shared__ uint32_t list_order[kSampleList];
-  __shared__ int32_t list_at[kSampleList];
-  __shared__ unsigned long long radix_units[kRadix];
-  __shared__ int32_t radix_count[kRadix];
-  __shared__ double room_d[kRowThreads / kWave];
-  __shared__ unsigned long long room_u[kRowThreads / kWave];
-  __shared__ int32_t room_i[kRowThreads / kWave];
-  __shared__ float room_f[kRowThreads / kWave];
-  __shared__ int32_t found_bin, found_k, found_at, found_slice;
-  __shared__ uint32_t bound_low, bound_high;
-  __shared__ Ending ending;
-  const int tid = threadIdx.x, row = blockIdx.x, wave = tid / kWave, lane = tid % kWave;
+  __shared__ uint64_t list[kSampleList];              // keys, in any order
+  __shared__ unsigned long long radix_units[kRowThreads];
+  __shared__ int32_t radix_count[kRowThreads];
+  __shared__ unsigned long long rank_key[kRowThreads], rank_units[kRowThreads];
+  __shared__ RowRoom rooms[2];
+  __shared__ float room_f[kRowWaves];
+  __shared__ int32_t found_k, found_p, found_last, found_at, found_slice, found_n, complete;
+  __shared__ unsigned long long found_key, found_units;
+  const int tid = threadIdx.x, row = blockIdx.x, lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const LogitsRow in = logits_row<TYPE>(logits, row_stride, row, vocab);
   const SampleSlice *head = heads + (int64_t)row * slices;
-  const uint64_t *row_bins = bins + (int64_t)row * slices * kSampleBins;
+  const uint64_t *row_bins = bins + (int64_t)row * slices * kSampleSlots;
+  const uint64_t *row_lists = lists + (int64_t)row * slices * kSliceList;
+  int turn = 0;                                        // which room the next scan has
+
+  // The words of the first slices are asked for before it is known what they mean.
+  constexpr int kAhead = 10;
+  const int slot = tid % kSampleSlots, part = tid / kSampleSlots;
+  uint64_t words[kAhead];
+  auto load_words = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int s = s0 + i * kParts;
+      words[i] = row_bins[(int64_t)(s < slices ? s : slices - 1) * kSampleSlots + slot];
+    }
+  };
+  const SampleSlice own_head = head[tid < slices ? tid : slices - 1];
   const float t = row_temperature(temperature, row);
+  const int32_t k = top_k != nullptr ? top_k[row] : 0;
+  const float p = top_p != nullptr ? top_p[row] : 1.0f;
+  const float m = min_p != nullptr ? min_p[row] : 0.0f;
+  double u = (double)uniforms[row];
+  load_words(part);
+  u = u > 0.0 ? (u < 1.0 - 0x1p-24 ? u : 1.0 - 0x1p-24) : 0.0;
 
   // the row's largest logit
-  float most = -INFINITY;
-  for (int s = tid; s < slices; s += kRowThreads) most = fmaxf(most, head[s].most);
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) most = fmaxf(most, __shfl_xor(most, off, kWave));
+  static_assert(kMaxSlices <= kRowThreads, "a thread has a slice");
+  float most = wave_max(own_head.most);
   if (lane == 0) room_f[wave] = most;
+  if (tid == 0) {
+    found_k = complete = kSampleBins;
+    found_last = found_n = 0;
+    found_at = 0x7fffffff;
+  }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kRowThreads / kWave; ++w) most = fmaxf(most, room_f[w]);
+  for (int w = 0; w < kRowWaves; ++w) most = __builtin_fmaxf(most, room_f[w]);
   if (most == -INFINITY) {                            // nothing can be drawn
     if (tid == 0) {
       tokens[row] = -1;
@@ -301,496 +485,498 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     return;
   }
   if (greedy_temperature(t)) {
+    if (tid < slices && own_head.most == most) atomicMin(&found_at, own_head.at);
+    __syncthreads();
     if (tid == 0) {
-      int at = 0x7fffffff;
-      for (int s = 0; s < slices; ++s) {
-        if (head[s].most == most) {                   // (slices are in the tokens' order)
-          at = head[s].at;
-          break;
-        }
-      }
-      tokens[row] = at;
+      tokens[row] = found_at;
       if (logprobs != nullptr) logprobs[row] = 0.f;
     }
     return;
   }
-  const double inv_t = 1.0 / (double)t;
-  const double y_most = (double)most * inv_t;
-  const double top = __builtin_floor(y_most * 8.0);
-  for (int s = tid; s < slices; s += kRowThreads) {
-    const double d = head[s].most == -INFINITY ? (double)kSampleBins : top - head[s].top;
-    shift[s] = d < (double)kSampleBins ? (int)d : kSampleBins;
+  const double z_per_x = 8.0 / (double)t;
+  const double z_most = z_of(most, z_per_x), top = __builtin_floor(z_most);
+  const int top_slot = slot_of(top);
+  if (tid < slices) {
+    const uint32_t d = own_head.most == -INFINITY ? kSampleBins : whole_of(top - own_head.top);
+    shift[tid] = d < (uint32_t)kSampleBins ? (int)d : kSampleBins;
+    slice_listed[tid] = own_head.listed;
+    if (d < (uint32_t)kSampleBins && own_head.listed_bins < kSampleBins) atomicMin(&complete, (int)d + own_head.listed_bins);
+  }
+  if (tid < kSampleSlots) {
+    bin_top[tid] = kUnit * exp(((top - z_most) + (double)(1 - tid)) * 0.125);   // (of z of any size: the first difference is exact)
   }
   __syncthreads();
-  auto word_of = [&](int s, int b) -> uint64_t {      // bin b of the row in slice s
-    const int at = b - shift[s];
-    return at >= 0 && shift[s] < kSampleBins ? row_bins[(int64_t)s * kSampleBins + at] : 0;
+  // Bin b of the row in slice s, from what lies in its place, which need not be the slice's.
+  auto word = [&](uint64_t w, int s, int b) __attribute__((always_inline)) -> uint64_t {
+    return b < kSampleBins && (uint32_t)(b - shift[s]) < (uint32_t)kSampleBins ? w : 0;
   };
-  // its bins
+  // its bins: a thread adds up a slot of every other slice's and hands it over
   {
-    int32_t count = 0;
-    double mass = 0.0;
-    if (tid < kSampleBins) {
-      uint64_t units = 0;
-      for (int s = 0; s < slices; ++s) {
-        const uint64_t w = word_of(s, tid);
-        count += (int32_t)(w >> kCountShift);
-        units += w & kUnitsMask;
+    const int b = (top_slot - slot) & (kSampleSlots - 1);
+    uint32_t count = 0;
+    uint64_t units = 0;
+    for (int s0 = part; s0 < slices; s0 += kAhead * kParts) {
+      if (s0 != part) load_words(s0);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int s = s0 + i * kParts;
+        const uint64_t x = s < slices ? word(words[i], s, b) : 0;
+        count += (uint32_t)(x >> kCountShift);
+        units += x & kUnitsMask;
       }
-      const double scale = kUnit * exp((top * 0.125 - y_most) + (1 - tid) * 0.125);   // (of any size: the first difference is exact)
-      bin_top[tid] = scale;
-      mass = (double)(units + kFloorUnits * (uint64_t)count) * scale;
     }
-    int32_t count_all;
-    double mass_all;
-    count = row_scan(count, room_i, &count_all);
-    mass = row_scan(mass, room_d, &mass_all);
-    if (tid < kSampleBins) {
-      count_to[tid] = count;
-      mass_to[tid] = mass;
-    }
+    radix_units[part * kSampleSlots + b] = units + kFloorUnits * (uint64_t)count;
+    radix_count[part * kSampleSlots + b] = (int32_t)count;
   }
   __syncthreads();
-  const int32_t live = count_to[kSampleBins - 1];
-  const double mass_live = mass_to[kSampleBins - 1];
-
-  const int32_t k = top_k != nullptr ? top_k[row] : 0;
-  const float p = top_p != nullptr ? top_p[row] : 1.0f;
-  const float m = min_p != nullptr ? min_p[row] : 0.0f;
+  int32_t count_here = 0;
+  double mass = 0.0;
+  if (tid < kSampleSlots) {
+    count_here = radix_count[tid] + radix_count[kSampleSlots + tid];
+    mass = (double)(radix_units[tid] + radix_units[kSampleSlots + tid]) * bin_top[tid];
+  }
+  int32_t count = count_here;
+  row_scan2(count, rooms[0].count, mass, rooms[0].mass);
+  turn = 1;
+  if (tid < kSampleSlots) {
+    count_to[tid] = count;
+    mass_to[tid] = mass;
+  }
+  {
+    const uint64_t any = __builtin_amdgcn_ballot_w64(count_here > 0);
+    if (lane == 0 && any != 0) atomicMax(&found_last, wave * kWave + 63 - __builtin_clzll(any));       // the last bin with a token
+  }
+  if (k > 0 && count - count_here < k && count >= k) found_k = tid;      // (one thread's)
+  __syncthreads();
+  const int last_bin = found_last;
+  const int32_t live = count_to[last_bin];
+  const double mass_live = mass_to[last_bin];
   bool by_k = k > 0 && k < live, by_p = p < 1.0f;
   const bool by_m = m > 0.0f;
 
-  // The interval of logits, by order, that bins `from` to `to` have: the border of a bin is within a few floats of its place.
-  auto bounds = [&](int from, int to) {
+  // The first bin with a token by whose end the mass is `target`; the last with a token if none is.
+  auto bin_reaching = [&](double target) __attribute__((always_inline)) -> int {
     __syncthreads();
-    if (wave < 2) {
-      // wave 0: the lowest logit whose bin is at most `to`; wave 1: the lowest whose bin is below `from`
-      const double limit = top - (wave == 0 ? to : from - 1);        // its bin, counted from 0
-      const float guess = (float)__builtin_fmin(__builtin_fmax(limit * 0.125 * (double)t, -3.4028234663852886e38), 3.4028234663852886e38);
-      const int64_t o = (int64_t)order_of(guess + 0.0f) + lane - 32;
-      const uint32_t lowest = order_of(-3.4028234663852886e38f), highest = order_of(3.4028234663852886e38f);
-      const bool above = o > (int64_t)highest || (o >= (int64_t)lowest && bin_of(logit_of_order((uint32_t)o), inv_t) >= limit);
-      const uint64_t all = __builtin_amdgcn_ballot_w64(above);
-      const int first = all != 0 ? __builtin_ctzll(all) : 63;
-      if (lane == first) {
-        const uint32_t border = o < (int64_t)lowest ? lowest : (uint32_t)o;
-        if (wave == 0) {
-          bound_low = border;
-        } else {
-          bound_high = border - 1;
-        }
-      }
-    }
+    if (tid == 0) found_p = last_bin;
     __syncthreads();
-    if (from <= 0 && tid == 0) bound_high = order_of(most);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(count_here > 0 && mass >= target);
+    if (lane == 0 && past != 0) atomicMin(&found_p, wave * kWave + __builtin_ctzll(past));
     __syncthreads();
+    return found_p;
+  };
+  auto units_of_key = [&](uint64_t key) __attribute__((always_inline)) -> uint64_t {
+    return units_of(z_of(logit_of_key<TYPE>(key), z_per_x)) + kFloorUnits;
   };
 
-  // The tokens of bins [list_bins_from, list_bins_to], in their order; a wavefront takes a slice at a time.
-  int list_from = 0, list_to = -1, listed = 0;
-  auto gather = [&](int from, int to) {
-    if (list_from <= from && to <= list_to) return;
-    bounds(from, to);
-    const uint32_t low = bound_low, high = bound_high;
-    for (int s = wave; s < slices; s += kRowThreads / kWave) {
-      int32_t n = 0;
-      for (int b = from + lane; b <= to; b += kWave) n += (int32_t)(word_of(s, b) >> kCountShift);
-#pragma unroll
-      for (int off = 1; off < kWave; off <<= 1) n += __shfl_xor(n, off, kWave);
-      if (lane == 0) slice_ties[s] = n;
-    }
-    __syncthreads();
-    if (tid == 0) {
-      int32_t at = 0;
-      for (int s = 0; s < slices; ++s) {
-        slice_from[s] = at;
-        at += slice_ties[s];
-      }
-      slice_from[slices] = at;
-    }
-    __syncthreads();
-    for (int s = wave; s < slices; s += kRowThreads / kWave) {
-      int32_t at = slice_from[s];
-      if (slice_from[s + 1] == at) continue;
-      for (int v = 0; v < slice_vectors; v += kWave) {
-        const int64_t vec = (int64_t)s * slice_vectors + v + lane;
-        const bool there = v + lane < slice_vectors && vec < in.vectors;
-        const uint4_t raw = there ? *(const uint4_t *)(in.base + vec * 16) : uint4_t{0, 0, 0, 0};
-        float x[kPer];
-        const int64_t first = there ? vec * kPer - in.lead : -kPer;
-        logits_of<TYPE>(raw, first, vocab, x);
-        uint32_t mine = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const uint32_t o = order_of(x[i]);
-          mine |= (o >= low && o <= high ? 1u : 0u) << i;
-        }
-        if (__builtin_amdgcn_ballot_w64(mine != 0) == 0) continue;
-        const int32_t n = __builtin_popcount(mine);
-        const int32_t upto = wave_scan(n);
-        int32_t to_at = at + upto - n;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          if ((mine >> i & 1) && to_at < kSampleList) {
-            list_order[to_at] = order_of(x[i]);
-            list_at[to_at++] = (int32_t)(first + i);
-          }
-        }
-        at += __shfl(upto, kWave - 1, kWave);
-      }
-    }
-    __syncthreads();
-    list_from = from;
-    list_to = to;
-    listed = slice_from[slices] < kSampleList ? slice_from[slices] : kSampleList;
-  };
-  // Whether a bin's tokens fit the list; else they are read from the row each time.
-  auto fits = [&](int from, int to) { return count_to[to] - (from > 0 ? count_to[from - 1] : 0) <= kSampleList; };
-
-  // Every token of a bin: from the list, or from the row.
-  auto each_of_bin = [&](int bin, bool in_list, uint32_t low, uint32_t high, auto &&what) {
-    if (in_list) {
-      for (int i = tid; i < listed; i += kRowThreads) {
-        const uint32_t o = list_order[i];
-        if (o >= low && o <= high) what(o, list_at[i]);
-      }
-    } else {
-      for (int64_t v = tid; v < in.vectors; v += kRowThreads) {
-        float x[kPer];
-        const int64_t first = v * kPer - in.lead;
-        logits_of<TYPE>(*(const uint4_t *)(in.base + v * 16), first, vocab, x);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const uint32_t o = order_of(x[i]);
-          if (o >= low && o <= high) what(o, (int32_t)(first + i));
-        }
-      }
-    }
-  };
-  // Where a prefix ends in a bin: at the first token with which the bin's tokens are `count` (count > 0), or have `units` (a
-  // number above 0 of units). The bits of their orders are looked at ten at a time.
-  auto end_in_bin = [&](int bin, int32_t count, double units) -> Ending {
-    const bool in_list = fits(bin, bin);
-    if (in_list) gather(bin, bin);
-    bounds(bin, bin);
-    uint32_t low = bound_low, high = bound_high;
-    int32_t n_above = 0;
-    uint64_t u_above = 0;
-    while (true) {
-      int down = 0;
-      while (((high - low) >> down) >= (uint32_t)kRadix) ++down;
-      for (int i = tid; i < kRadix; i += kRowThreads) {
-        radix_units[i] = 0;
-        radix_count[i] = 0;
-      }
-      __syncthreads();
-      each_of_bin(bin, in_list, low, high, [&](uint32_t o, int32_t) {
-        const uint32_t r = (high - o) >> down;          // from the largest
-        atomicAdd(&radix_count[r], 1);
-        atomicAdd(&radix_units[r], (unsigned long long)(binned(logit_of_order(o), inv_t).units + kFloorUnits));
-      });
-      __syncthreads();
-      static_assert(kRadix == kRowThreads, "a thread has a digit");
-      int32_t n_all;
-      unsigned long long u_all;
-      const int32_t n = radix_count[tid];
-      const unsigned long long u = radix_units[tid];
-      const int32_t n_to = row_scan(n, room_i, &n_all);
-      const unsigned long long u_to = row_scan(u, room_u, &u_all);
-      if (tid == 0) found_at = kRadix;
-      __syncthreads();
-      const bool reached = count > 0 ? n_above + n_to >= count : (double)(u_above + u_to) >= units;
-      if (n > 0 && reached) atomicMin(&found_at, tid);
-      // (nowhere, by a rounding: the last that there is)
-      if (tid == 0) found_k = -1;
-      __syncthreads();
-      if (n > 0) atomicMax(&found_k, tid);
-      __syncthreads();
-      const int digit = found_at < kRadix ? found_at : found_k;
-      if (digit < 0) return Ending{low, 0x7fffffff, u_above};      // (no token: a bin that is asked for has one)
-      if (tid == digit) {
-        ending.ties = n_above + n_to - n;                 // tokens, units in front of the digit
-        ending.units = u_above + (u_to - u);
-        ending.order = (uint32_t)n;
-      }
-      __syncthreads();
-      n_above = ending.ties;
-      u_above = ending.units;
-      const int32_t here = (int32_t)ending.order;
-      const uint32_t new_high = high - ((uint32_t)digit << down);
-      const uint32_t width = (1u << down) - 1;
-      const uint32_t new_low = new_high - low > width ? new_high - width : low;
-      __syncthreads();
-      low = new_low;
-      high = new_high;
-      if (down == 0) {
-        const uint64_t each = binned(logit_of_order(high), inv_t).units + kFloorUnits;
-        int32_t ties = here;
-        if (count > 0) {
-          ties = count - n_above < here ? count - n_above : here;
-        } else {
-          const double more = __builtin_ceil((units - (double)u_above) / (double)each);
-          if (more < (double)here) ties = more < 1.0 ? 1 : (int32_t)more;
-        }
-        return Ending{high, ties, u_above + each * (uint64_t)ties};
-      }
-    }
-  };
-
-  // The filters, one after the other. `last`: the bin that the kept prefix ends in; `cut`: what of it is kept.
-  int last = kSampleBins - 1;
-  bool whole = true;                                    // all of bin `last`
-  Ending cut{0u, 0, 0};
-  double kept = mass_live;
-  // The first bin of those with a token that is reached; the last with a token if none is.
-  auto first_bin = [&](auto &&reached) -> int {
-    __syncthreads();
-    if (tid == 0) found_bin = kSampleBins;
-    if (tid == 1) found_k = 0;
-    __syncthreads();
-    if (tid < kSampleBins && count_to[tid] > (tid > 0 ? count_to[tid - 1] : 0)) {
-      if (reached(tid)) atomicMin(&found_bin, tid);
-      atomicMax(&found_k, tid);
-    }
-    __syncthreads();
-    return found_bin < kSampleBins ? found_bin : found_k;
-  };
-  // Where the prefixes end; one that ends behind min_p's (bin_m, or a bin more) says nothing, but top_k says what top_p is of.
-  int bin_k = kSampleBins - 1, bin_p = kSampleBins - 1, bin_m = kSampleBins - 1;
+  // Where the prefixes end; one that ends behind min_p's end (bin_m, or a bin more) says nothing, but top_k says what top_p is a
+  // share of.
+  const int bin_k = by_k ? found_k : last_bin;
+  int bin_p = last_bin, bin_m = last_bin;
   double log_m = 0.0;
   if (by_m) {
     log_m = log((double)(m < 1.0f ? m : 1.0f)) * (double)t;          // kept: x - most >= log_m
-    const double b = top - __builtin_floor((y_most + log_m * inv_t) * 8.0) + 1.0;
+    const double b = top - __builtin_floor(z_most + log_m * z_per_x) + 1.0;
     if (b < (double)bin_m) bin_m = (int)b;
   }
-  if (by_k) bin_k = first_bin([&](int b) { return count_to[b] >= k; });
   if (by_p && !by_k) {
-    const double target = (double)p * mass_live * kReached;
-    bin_p = first_bin([&](int b) { return mass_to[b] >= target; });
+    bin_p = bin_reaching((double)p * mass_live * kReached);
     by_p = bin_p <= bin_m;
   } else if (!by_p) {
     by_k = by_k && bin_k <= bin_m;
   }
-  // Where few tokens come into question they are listed at once, the draw's among them.
+  // Where the slices' lists have all tokens that come into question, those are the row's list, and the draw's; else it has a
+  // bin's tokens at a time, if they fit.
   const int most_bin = by_k ? bin_k : by_p ? bin_p : bin_m;
-  const bool few = fits(0, most_bin);
-  if (few) gather(0, most_bin);
-  if (by_k) {
-    last = bin_k;
-    const int32_t before = last > 0 ? count_to[last - 1] : 0;
-    if (count_to[last] > k) {
-      whole = false;
-      cut = end_in_bin(last, k - before, 0.0);
-      kept = (last > 0 ? mass_to[last - 1] : 0.0) + (double)cut.units * bin_top[last];
-    } else {
-      kept = mass_to[last];
+  const bool few = most_bin < complete && count_to[most_bin] <= kSampleList;
+  int listed = 0;
+  if (few) {
+    const uint64_t least = lowest_key<TYPE>(lowest_of_bin(top - most_bin, t, z_per_x));
+#pragma unroll 4
+    for (int i = tid; i < slices * kSliceList; i += kRowThreads) {
+      const uint64_t key = row_lists[i];
+      if (i % kSliceList < slice_listed[i / kSliceList] && key >= least) {
+        const int to = atomicAdd(&found_n, 1);
+        if (to < kSampleList) list[to] = key;
+      }
     }
+    __syncthreads();
+    listed = found_n < kSampleList ? found_n : kSampleList;
   }
-  if (by_p) {
-    const double target = (double)p * kept * kReached;
-    int bin = first_bin([&](int b) { return mass_to[b] >= target; });
-    if (bin > last) bin = last;
-    const double before = bin > 0 ? mass_to[bin - 1] : 0.0;
-    Ending e = end_in_bin(bin, 0, __builtin_fmax((target - before) / bin_top[bin], 1.0));
-    if (bin < last || whole || e.order > cut.order || (e.order == cut.order && e.ties < cut.ties)) {
+  int last = last_bin;                                  // the bin that the kept prefix ends in
+  bool whole = true;                                    // all of it; or its tokens from the key `cut` on
+  uint64_t cut = 0;
+  double kept = mass_live;
+  bool in_list = few;                                   // the bin's tokens are listed; else they are read from the row each time
+  int list_bin = -1;
+  // Every token of the row's list or, without it, of the row, whose key is in [from, to].
+  auto each_token = [&](uint64_t from, uint64_t to, auto &&what) __attribute__((always_inline)) {
+    if (in_list) {
+      for (int i = tid; i < listed; i += kRowThreads) {
+        const uint64_t key = list[i];
+        if (key >= from && key <= to) what(key);
+      }
+    } else {
+      for (int64_t v = tid; v < in.vectors; v += kRowThreads) {
+        float x[kPer];
+        logits_of<TYPE>(in, *(const uint4_t *)(in.base + v * 16), v, vocab, x);
+#pragma unroll 1
+        for (int i = 0; i < kPer; ++i) {
+          float e = x[0];
+#pragma unroll
+          for (int j = 1; j < kPer; ++j) e = i == j ? x[j] : e;
+          if (!(e > -INFINITY)) continue;
+          const uint64_t key = key_of<TYPE>(order_of(e), (int32_t)(v * kPer - in.lead + i));
+          if (key >= from && key <= to) what(key);
+        }
+      }
+    }
+  };
+
+  // Filter 0 is top_k, 1 top_p, 2 min_p and what the draw needs.
+  uint64_t low = 0, high = 0;                           // the keys of the bin's tokens
+#pragma unroll 1
+  for (int filter = 0; filter < 3; ++filter) {
+    int bin;
+    int32_t end_count = 0;         // the end is the first token with which the bin's are so many, if above 0,
+    double end_units = 0.0;        // or have so many units
+    if (filter == 0) {
+      if (!by_k) continue;
+      bin = last = bin_k;
+      kept = mass_to[last];
+      if (count_to[last] == k) continue;
+      end_count = k - (last > 0 ? count_to[last - 1] : 0);
+    } else if (filter == 1) {
+      if (!by_p) continue;
+      const double target = (double)p * kept * kReached;
+      if (by_k) {
+        bin_p = bin_reaching(target);
+        if (bin_p > last) bin_p = last;
+      }
+      bin = bin_p;
+      end_units = __builtin_fmax((target - (bin > 0 ? mass_to[bin - 1] : 0.0)) / bin_top[bin], 1.0);
+    } else {
+      if (by_m) {
+        const uint32_t order = border((double)most + log_m, [&](float x) { return x >= most || (double)x - (double)most >= log_m; });
+        const double d = top - __builtin_floor(z_of(logit_of_order(order), z_per_x));
+        const int b = d < (double)kSampleBins ? (int)d : kSampleBins;
+        const uint64_t least = lowest_key<TYPE>(order);
+        if (b < kSampleBins && (b < last || (b == last && (whole || least > cut)))) {
+          last = b;
+          whole = false;
+          cut = least;
+        }
+      }
+      if (few || whole) break;
+      bin = last;
+    }
+    const uint32_t low_order = lowest_of_bin(top - bin, t, z_per_x);
+    const uint32_t high_order = bin > 0 ? lowest_of_bin(top - bin + 1.0, t, z_per_x) - 1 : order_of(most);
+    low = lowest_key<TYPE>(low_order);
+    high = lowest_key<TYPE>(high_order + 1) - 1;
+    if (!few && list_bin != bin) {
+      in_list = count_to[bin] - (bin > 0 ? count_to[bin - 1] : 0) <= kSampleList;
+      list_bin = bin;
+      __syncthreads();
+      if (tid == 0) found_n = 0;
+      __syncthreads();
+      if (in_list) {
+        const float least_x = logit_of_order(low_order), most_x = logit_of_order(high_order);
+        constexpr int kVectors = 4;
+#pragma unroll 1
+        for (int64_t v0 = tid; v0 < in.vectors; v0 += kVectors * kRowThreads) {
+          uint4_t raw[kVectors];
+#pragma unroll
+          for (int j = 0; j < kVectors; ++j) {
+            const int64_t v = v0 + j * kRowThreads;
+            raw[j] = *(const uint4_t *)(in.base + (v < in.vectors ? v : in.vectors - 1) * 16);
+          }
+#pragma unroll
+          for (int j = 0; j < kVectors; ++j) {
+            const int64_t v = v0 + j * kRowThreads;
+            float x[kPer];
+            logits_of<TYPE>(in, raw[j], v, vocab, x);
+            uint32_t those = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) those |= (x[i] >= least_x && x[i] <= most_x ? 1u : 0u) << i;
+            while (those != 0) {
+              const int i = __builtin_ctz(those);
+              those &= those - 1;
+              float e = x[0];
+#pragma unroll
+              for (int n = 1; n < kPer; ++n) e = i == n ? x[n] : e;
+              const int to = atomicAdd(&found_n, 1);
+              if (to < kSampleList) list[to] = key_of<TYPE>(order_of(e), (int32_t)(v * kPer - in.lead + i));
+            }
+          }
+        }
+        __syncthreads();
+        listed = found_n < kSampleList ? found_n : kSampleList;
+      }
+    }
+    if (filter == 2) break;
+
+    // Where the prefix ends in the bin: while its tokens are many, by the next ten bits of their keys; then by ranking them.
+    int32_t n_above = 0, n_left = count_to[bin] - (bin > 0 ? count_to[bin - 1] : 0);
+    uint64_t u_above = 0, from = low, to = high;
+    while (true) {
+      __syncthreads();
+      if (tid == 0) {
+        found_n = 0;
+        found_at = -1;
+        found_key = from;
+        found_units = 0;
+      }
+      if (n_left > kRanked) {
+        int down = 0;
+        while (((to - from) >> down) >= (uint64_t)kRowThreads) ++down;
+        radix_units[tid] = 0;
+        radix_count[tid] = 0;
+        __syncthreads();
+        each_token(from, to, [&](uint64_t key) __attribute__((always_inline)) {
+          const uint32_t r = (uint32_t)((to - key) >> down);          // from the largest
+          atomicAdd(&radix_count[r], 1);
+          atomicAdd(&radix_units[r], (unsigned long long)units_of_key(key));
+        });
+        __syncthreads();
+        const int32_t n = radix_count[tid];
+        const unsigned long long units = radix_units[tid];
+        int32_t n_to = n;
+        unsigned long long u_to = units;
+        row_scan2(n_to, rooms[turn].count, u_to, rooms[turn].units);
+        turn ^= 1;
+        // the digit in which the end lies: not reached in front of it, and reached with it, or the last that there is
+        const bool open = end_count > 0 ? n_above + n_to - n < end_count : (double)(u_above + u_to - units) < end_units;
+        const uint64_t those = __builtin_amdgcn_ballot_w64(n > 0 && open);
+        if (lane == 0 && those != 0) atomicMax(&found_at, wave * kWave + 63 - __builtin_clzll(those));
+        __syncthreads();
+        const int digit = found_at;
+        if (digit < 0) break;                                // (no token: a bin that is asked for has one)
+        if (tid == digit) {
+          found_n = n;
+          found_key = (uint64_t)(uint32_t)(n_above + n_to - n);
+          found_units = u_above + (u_to - units);
+        }
+        __syncthreads();
+        n_left = found_n;                                    // tokens of the digit; tokens, units in front of it
+        n_above = (int32_t)found_key;
+        u_above = found_units;
+        to -= (uint64_t)digit << down;
+        const uint64_t width = (1ull << down) - 1;
+        from = to - from > width ? to - width : from;
+        continue;
+      }
+      __syncthreads();
+      each_token(from, to, [&](uint64_t key) __attribute__((always_inline)) {
+        const int i = atomicAdd(&found_n, 1);
+        if (i < kRanked) {
+          rank_key[i] = key;
+          rank_units[i] = units_of_key(key);
+        }
+      });
+      __syncthreads();
+      const int n = found_n < kRanked ? found_n : kRanked;
+      if (tid < n) {
+        const uint64_t mine = rank_key[tid];
+        int32_t before = n_above, ahead_of = 0;
+        uint64_t units_before = u_above;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+          const bool ahead = rank_key[i] > mine;
+          ahead_of += ahead;
+          units_before += ahead ? rank_units[i] : 0;
+        }
+        before += ahead_of;
+        const uint64_t with = units_before + rank_units[tid];
+        const bool is_last = ahead_of + 1 == n;             // (where a rounding keeps the end from being reached)
+        const bool ends = end_count > 0 ? before + 1 == end_count || (is_last && before + 1 < end_count)
+                                        : (double)units_before < end_units && ((double)with >= end_units || is_last);
+        if (ends) {
+          found_key = mine;
+          found_units = with;
+        }
+      }
+      __syncthreads();
+      break;
+    }
+    const uint64_t end = found_key;
+    if (filter == 0) {
+      whole = false;
+      cut = end;
+      kept = (last > 0 ? mass_to[last - 1] : 0.0) + (double)found_units * bin_top[last];
+    } else if (bin < last || whole || end > cut) {
       last = bin;
       whole = false;
-      cut = e;
+      cut = end;
     }
   }
-  if (by_m) {
-    // the lowest order that is kept: within a few floats of most + log_m
+
+  // Kept are the tokens from the key `cut` on, and above the cut of y.
+  const double x_cut = kCut * (double)t;
+  auto mass_of = [&](uint64_t key) __attribute__((always_inline)) -> double {
+    const float x = logit_of_key<TYPE>(key);
+    if (!((double)x - (double)most >= x_cut)) return 0.0;
+    const double z = z_of(x, z_per_x), d = top - __builtin_floor(z);
+    return d < (double)kSampleBins ? (double)(units_of(z) + kFloorUnits) * bin_top[(int)d] : 0.0;
+  };
+  uint64_t token = 0;
+  double all = 1.0;
+  if (few) {
+    // By the index: the run of indexes in which the target lies, then the token in it. Masses as whole numbers of 2^-43.
+    const int width = (vocab + kRowThreads - 1) / kRowThreads;
+    auto units_kept = [&](uint64_t key) __attribute__((always_inline)) -> uint64_t {
+      return __builtin_bit_cast(uint64_t, mass_of(key) * 0x1p43 + 0x1p52) - kMassOne;
+    };
+    __syncthreads();
+    radix_units[tid] = 0;
+    if (tid == 0) found_n = 0;
+    __syncthreads();
+    for (int i = tid; i < listed; i += kRowThreads) {
+      if (list[i] >= cut) atomicAdd(&radix_units[index_of_key(list[i]) / width], (unsigned long long)units_kept(list[i]));
+    }
+    __syncthreads();
+    const unsigned long long own = radix_units[tid];
+    unsigned long long sum;
+    const unsigned long long upto = row_scan(own, rooms[turn].units, &sum);
+    turn ^= 1;
+    const double target = u * (double)sum * (2.0 - kReached);
+    if ((double)upto > target && !((double)(upto - own) > target)) {
+      found_at = tid;
+      found_units = upto - own;
+    }
+    __syncthreads();
+    const int run = found_at;
+    const uint64_t before_run = found_units;
+    for (int i = tid; i < listed; i += kRowThreads) {
+      if (list[i] >= cut && index_of_key(list[i]) / width == run) {
+        const int to = atomicAdd(&found_n, 1);
+        rank_key[to] = list[i];                            // (of `width` indexes at most, no more than threads)
+        rank_units[to] = units_kept(list[i]);
+      }
+    }
+    __syncthreads();
+    if (tid >= found_n) return;
+    const uint64_t mine = rank_key[tid];
+    const int32_t at = index_of_key(mine);
+    uint64_t units_before = before_run;
+#pragma unroll 8
+    for (int i = 0; i < found_n; ++i) units_before += index_of_key(rank_key[i]) < at ? rank_units[i] : 0;
+    if (!((double)(units_before + rank_units[tid]) > target) || (double)units_before > target) return;
+    token = mine;
+    all = (double)sum * 0x1p-43;
+  } else {
+    // The kept mass of each slice: its bins in front of the last, and what it has of that one.
+    for (int s = tid; s < slices; s += kRowThreads) slice_units[s] = 0;
+    __syncthreads();
+    if (!whole) {
+      each_token(cut > low ? cut : low, high, [&](uint64_t key) __attribute__((always_inline)) {
+        atomicAdd(&slice_units[(index_of_key(key) + in.lead) / kPer / slice_vectors], (unsigned long long)units_of_key(key));
+      });
+    }
+    // (16 lanes a slice)
+    const int bins_kept = last + (whole ? 1 : 0);
+    for (int s0 = 0; s0 < slices; s0 += kRowThreads / 16) {
+      const int s = s0 + tid / 16 < slices ? s0 + tid / 16 : slices - 1;
+      double sum = 0.0;
+      for (int b0 = tid % 16; b0 < bins_kept; b0 += 16 * kAhead) {
+        uint64_t w[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          w[i] = row_bins[(int64_t)s * kSampleSlots + ((top_slot - (b0 + 16 * i)) & (kSampleSlots - 1))];
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int b = b0 + 16 * i;
+          const uint64_t x = b < bins_kept ? word(w[i], s, b) : 0;
+          sum += (double)((x & kUnitsMask) + kFloorUnits * (x >> kCountShift)) * bin_top[b & (kSampleSlots - 1)];
+        }
+      }
+      sum = over_row<16>(sum, [](double a, double b) { return a + b; });
+      if (s0 + tid / 16 < slices && tid % 16 == 0) slice_mass[s] = sum;
+    }
     __syncthreads();
     if (wave == 0) {
-      const float guess = (float)__builtin_fmax((double)most + log_m, -3.4028234663852886e38);
-      const int64_t o = (int64_t)order_of(guess + 0.0f) + lane - 32;
-      const int64_t lowest = order_of(-3.4028234663852886e38f);
-      const bool above = o >= (int64_t)order_of(most) ||
-                         (o >= lowest && (double)logit_of_order((uint32_t)o) - (double)most >= log_m);
-      const uint64_t all = __builtin_amdgcn_ballot_w64(above);
-      const int first = all != 0 ? __builtin_ctzll(all) : 63;
-      if (lane == first) bound_low = (uint32_t)(o < lowest ? lowest : o);
-    }
-    __syncthreads();
-    const uint32_t order = bound_low;
-    const double d = top - bin_of(logit_of_order(order), inv_t);
-    const int bin = d < (double)kSampleBins ? (int)d : kSampleBins;
-    if (bin < kSampleBins && (bin < last || (bin == last && (whole || order > cut.order)))) {
-      last = bin;
-      whole = false;
-      cut = Ending{order, 0x7fffffff, 0};
-    }
-  }
-  __syncthreads();
-
-  // Kept tokens: order above cut.order, or equal and among the first cut.ties; whole: all of them above the cut of y.
-  const uint32_t least = whole ? 0u : cut.order;
-  const int32_t most_ties = whole ? 0x7fffffff : cut.ties;
-  double u = (double)uniforms[row];
-  u = u > 0.0 ? (u < 1.0 - 0x1p-24 ? u : 1.0 - 0x1p-24) : 0.0;
-  const double x_cut = kCut * (double)t;
-  auto mass_of = [&](uint32_t o) -> double {
-    const float x = logit_of_order(o);
-    if ((double)x - (double)most < x_cut) return 0.0;
-    const Binned b = binned(x, inv_t);
-    const double d = top - b.bin;
-    return d < (double)kSampleBins ? (double)(b.units + kFloorUnits) * bin_top[(int)d] : 0.0;
-  };
-  auto finish = [&](int32_t token, uint32_t order, double all) {
-    tokens[row] = token;
-    if (logprobs != nullptr) {
-      logprobs[row] = (float)(((double)logit_of_order(order) - (double)most) * inv_t - log(all));
-    }
-  };
-  if (few) {
-    // the list has them all, in their order: a thread has a run of it
-    constexpr int kRun = kSampleList / kRowThreads;
-    const int each = (listed + kRowThreads - 1) / kRowThreads;
-    double mass[kRun];
-    int32_t ties = 0, ties_all;
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      const int at = tid * each + i;
-      if (i < each && at < listed && list_order[at] == least) ++ties;
-    }
-    int32_t tie = row_scan(ties, room_i, &ties_all) - ties;
-    double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      const int at = tid * each + i;
-      mass[i] = 0.0;
-      if (i < each && at < listed) {
-        const uint32_t o = list_order[at];
-        if (o > least || (o == least && tie++ < most_ties)) mass[i] = mass_of(o);
+      // 64 slices at a time: the sums of mass, then the first slice by whose end the target is passed; the last if none
+      const double above = whole ? 0.0 : bin_top[last];
+      double sum = 0.0;
+      for (int s0 = 0; s0 < slices; s0 += kWave) {
+        const int s = s0 + lane;
+        const double to = wave_scan(s < slices ? slice_mass[s] + (double)slice_units[s] * above : 0.0) + sum;
+        if (s < slices) slice_mass[s] = to;
+        sum = __shfl(to, kWave - 1, kWave);
       }
-      sum += mass[i];
-    }
-    double all;
-    double upto = row_scan(sum, room_d, &all) - sum;
-    const double target = u * all * (2.0 - kReached);
-    if (tid == 0) found_at = kSampleList;
-    __syncthreads();
-    int here = kSampleList;
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-      upto += mass[i];
-      if (here == kSampleList && mass[i] > 0.0 && upto > target) here = tid * each + i;
-    }
-    if (here < kSampleList) atomicMin(&found_at, here);
-    __syncthreads();
-    if (tid == 0) {
-      const int at = found_at < kSampleList ? found_at : listed - 1;
-      finish(list_at[at], list_order[at], all);
-    }
-    return;
-  }
-
-  // The kept mass of each slice: its bins in front of the last, and what it has of that one.
-  for (int s = tid; s < slices; s += kRowThreads) {
-    slice_units[s] = 0;
-    slice_ties[s] = 0;
-  }
-  __syncthreads();
-  if (!whole) {
-    const bool in_list = fits(last, last);
-    if (in_list) gather(last, last);
-    for (int s = tid; s < slices; s += kRowThreads) slice_ties[s] = 0;        // (the gather's)
-    bounds(last, last);
-    const uint32_t low = bound_low > least ? bound_low : least, high = bound_high;
-    each_of_bin(last, in_list, low, high, [&](uint32_t o, int32_t at) {
-      const int s = (int)((at + in.lead) / kPer / slice_vectors);
-      if (o == least) {
-        atomicAdd(&slice_ties[s], 1);
-      } else {
-        atomicAdd(&slice_units[s], (unsigned long long)(binned(logit_of_order(o), inv_t).units + kFloorUnits));
+      const double target = u * sum * (2.0 - kReached);
+      int slice = slices - 1;
+      for (int s0 = 0; s0 < slices; s0 += kWave) {
+        const int s = s0 + lane;
+        const uint64_t past = __builtin_amdgcn_ballot_w64(s < slices && slice_mass[s] > target);
+        if (past != 0) {
+          slice = s0 + __builtin_ctzll(past);
+          break;
+        }
       }
-    });
-    __syncthreads();
-  }
-  for (int s = wave; s < slices; s += kRowThreads / kWave) {
-    double sum = 0.0;
-    for (int b = lane; b < last + (whole ? 1 : 0); b += kWave) {
-      const uint64_t w = word_of(s, b);
-      sum += (double)((w & kUnitsMask) + kFloorUnits * (w >> kCountShift)) * bin_top[b];
-    }
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
-    if (lane == 0) slice_mass[s] = sum;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    const double each = whole ? 0.0 : mass_of(least);
-    int32_t left = most_ties;
-    double all = 0.0;
-    for (int s = 0; s < slices; ++s) {
-      const int32_t n = slice_ties[s] < left ? slice_ties[s] : left;
-      slice_from[s] = left;                              // ties that a slice may keep
-      left -= n;
-      slice_mass[s] += (double)slice_units[s] * (whole ? 0.0 : bin_top[last]) + (double)n * each;
-      all += slice_mass[s];
-    }
-    const double target = u * all * (2.0 - kReached);
-    double upto = 0.0;
-    int s = 0;
-    while (s + 1 < slices && !(upto + slice_mass[s] > target)) upto += slice_mass[s++];
-    found_slice = s;
-    room_d[0] = all;
-    room_d[1] = target - upto;
-  }
-  __syncthreads();
-  const double all = room_d[0];
-  double target = room_d[1];
-  for (int s = found_slice; s < slices; ++s) {
-    // a thread has neighbouring elements
-    constexpr int kVectors = kSampleSlice / kPer / kRowThreads;
-    uint32_t order[kVectors * kPer];
-    int32_t ties = 0, ties_all;
-    const int each = (slice_vectors + kRowThreads - 1) / kRowThreads;
-    const int64_t v0 = (int64_t)s * slice_vectors + (int64_t)tid * each;
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      const bool there = i < each && tid * each + i < slice_vectors && v0 + i < in.vectors;
-      float x[kPer];
-      logits_of<TYPE>(there ? *(const uint4_t *)(in.base + (v0 + i) * 16) : uint4_t{0, 0, 0, 0},
-                      there ? (v0 + i) * kPer - in.lead : -kPer, vocab, x);
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        order[i * kPer + j] = x[j] > -INFINITY ? order_of(x[j]) : 0u;
-        if (order[i * kPer + j] == least && !whole) ++ties;
+      if (lane == 0) {
+        found_slice = slice;
+        rooms[turn].mass[0] = sum;
+        rooms[turn].mass[1] = target - (slice > 0 ? slice_mass[slice - 1] : 0.0);
       }
     }
-    int32_t tie = row_scan(ties, room_i, &ties_all) - ties;
-    const int32_t may = slice_from[s];
-    double sum = 0.0;
-    double mass[kVectors * kPer];
-#pragma unroll
-    for (int i = 0; i < kVectors * kPer; ++i) {
-      const bool is = order[i] > least || (order[i] == least && !whole && tie++ < may);
-      mass[i] = is && order[i] != 0u ? mass_of(order[i]) : 0.0;
-      sum += mass[i];
-    }
-    double slice_all;
-    double upto = row_scan(sum, room_d, &slice_all) - sum;
-    if (tid == 0) found_at = 0x7fffffff;
     __syncthreads();
-    int here = 0x7fffffff;
-    uint32_t here_order = 0;
+    all = rooms[turn].mass[0];
+    double target = rooms[turn].mass[1];
+    turn ^= 1;
+#pragma unroll 1
+    for (int s = found_slice; s < slices; ++s) {
+      // a thread has neighbouring elements
+      constexpr int kVectors = kSampleSlice / kPer / kRowThreads;
+      float x[kVectors][kPer];
+      const int each = (slice_vectors + kRowThreads - 1) / kRowThreads;
+      const int64_t v0 = (int64_t)s * slice_vectors + (int64_t)tid * each;
+      uint4_t raw[kVectors];
 #pragma unroll
-    for (int i = 0; i < kVectors * kPer; ++i) {
-      upto += mass[i];
-      if (here == 0x7fffffff && mass[i] > 0.0 && upto > target) {
-        here = (int)(v0 * kPer + i - in.lead);
-        here_order = order[i];
+      for (int i = 0; i < kVectors; ++i) raw[i] = *(const uint4_t *)(in.base + (v0 + i < in.vectors ? v0 + i : in.vectors - 1) * 16);
+      double share[kVectors * kPer], sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) {
+        logits_of<TYPE>(in, raw[i], i < each && tid * each + i < slice_vectors ? v0 + i : in.vectors, vocab, x[i]);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const uint64_t key = key_of<TYPE>(order_of(x[i][j]), (int32_t)((v0 + i) * kPer - in.lead + j));
+          share[i * kPer + j] = x[i][j] > -INFINITY && key >= cut ? mass_of(key) : 0.0;
+          sum += share[i * kPer + j];
+        }
       }
+      if (tid == 0) found_at = 0x7fffffff;
+      double slice_all;
+      double upto = row_scan(sum, rooms[turn].mass, &slice_all) - sum;
+      turn ^= 1;
+      int here = 0x7fffffff;
+      uint64_t here_key = 0;
+#pragma unroll
+      for (int i = 0; i < kVectors * kPer; ++i) {
+        upto += share[i];
+        if (here == 0x7fffffff && share[i] > 0.0 && upto > target) {
+          here = (int)(v0 * kPer + i - in.lead);
+          here_key = key_of<TYPE>(order_of(x[i / kPer][i % kPer]), here);
+        }
+      }
+      if (here != 0x7fffffff) atomicMin(&found_at, here);
+      __syncthreads();
+      if (found_at != 0x7fffffff) {
+        if (here != found_at) return;
+        token = here_key;
+        break;
+      }
+      target = 0.0;                                        // (a rounding: the next that is kept)
+      __syncthreads();
     }
-    if (here != 0x7fffffff) atomicMin(&found_at, here);
-    __syncthreads();
-    if (found_at != 0x7fffffff) {
-      if (here == found_at) finish(here, here_order, all);
+    if (token == 0) {                                      // (never: u is below 1, so some slice passes the target)
+      if (tid == 0) tokens[row] = -1;
       return;
     }
-    target = 0.0;                                        // (a rounding: the next that is kept)
-    __syncthreads();
+  }
+  tokens[row] = index_of_key(token);
+  if (logprobs != nullptr) {
+    logprobs[row] = (float)(((double)logit_of_key<TYPE>(token) - (double)most) * z_per_x * 0.125 - log(all));
   }
 }
 
@@ -801,7 +987,7 @@ extern "C" size_t litekv_sample_tokens_workspace_bytes(int32_t logits_type, int3
   if (logits_type < kLogitsF16 || logits_type > kLogitsF32 || batch < 1 || batch > 65535 || vocab < 1 || vocab > kSampleMaxVocab) return 0;
   const int size = logit_size(logits_type), per = sample_slice_vectors(batch, vocab, size);
   const int64_t slices = (sample_vectors(vocab, size) + per - 1) / per;
-  return (size_t)batch * (size_t)slices * (sizeof(SampleSlice) + kSampleBins * sizeof(uint64_t));
+  return (size_t)batch * (size_t)slices * (sizeof(SampleSlice) + (kSampleSlots + kSliceList) * sizeof(uint64_t));
 }
 
 extern "C" int litekv_sample_tokens(const void *logits, int32_t logits_type, int64_t row_stride, const float *uniforms,
@@ -829,13 +1015,14 @@ extern "C" int litekv_sample_tokens(const void *logits, int32_t logits_type, int
   const int slices = (int)((sample_vectors(vocab, size) + per - 1) / per);
   SampleSlice *heads = static_cast<SampleSlice *>(workspace);
   uint64_t *bins = reinterpret_cast<uint64_t *>(heads + (int64_t)batch * slices);
+  uint64_t *lists = bins + (int64_t)batch * slices * kSampleSlots;
   auto launch = [&](auto slices_kernel, auto rows_kernel) {
     hipLaunchKernelGGL(slices_kernel, dim3((unsigned)slices, (unsigned)batch), dim3(kSampleThreads), 0,
-                       static_cast<hipStream_t>(stream), logits, row_stride, temperature, vocab, per, slices, heads, bins);
+                       static_cast<hipStream_t>(stream), logits, row_stride, temperature, vocab, per, slices, heads, bins, lists);
     const int rc = check_launch(what);
     if (rc != LITEKV_OK) return rc;
     hipLaunchKernelGGL(rows_kernel, dim3((unsigned)batch), dim3(kRowThreads), 0, static_cast<hipStream_t>(stream), logits,
-                       row_stride, uniforms, temperature, top_k, top_p, min_p, tokens, logprobs, vocab, per, slices, heads, bins);
+                       row_stride, uniforms, temperature, top_k, top_p, min_p, tokens, logprobs, vocab, per, slices, heads, bins, lists);
     return check_launch(what);
   };
   switch (logits_type) {
