@@ -29,12 +29,14 @@ constexpr int kSampleBins = 322;              // of 1/8: what is further than 40
 constexpr int kSampleSlots = 512;             // a slice's bins lie at their place on the grid modulo this
 constexpr int kSampleThreads = 256;           // of a slice's workgroup
 constexpr int kSampleSlice = 8192;            // tokens of a slice at most: their number has 14 bits of a bin's word
-constexpr int kSliceList = 128;               // tokens of a slice's list
-constexpr int kRowThreads = 1024;             // of a row's workgroup
+constexpr int kSliceList = 64;                // tokens of a slice's list
+constexpr int kRowThreads = 512;              // of a row's workgroup
 constexpr int kRowWaves = kRowThreads / kWave;
-constexpr int kSampleList = 8192;             // tokens that a row's workgroup holds
+constexpr int kOwnList = 16;                  // tokens that a thread of a row's workgroup holds for itself
+constexpr int kMoreList = 2048;               // and those of all that have more
+constexpr int kMostListed = 6144;             // tokens of a bin that are listed: 12 a thread on the average
 constexpr int kSampleMaxVocab = 1 << 20;
-constexpr int kMaxSlices = 520;
+constexpr int kMaxSlices = 512;
 constexpr int kRanked = 64;                   // tokens that are ranked against each other; more go by their digits
 constexpr int kCountShift = 50;
 constexpr uint64_t kUnitsMask = (1ull << kCountShift) - 1;
@@ -66,20 +68,37 @@ constexpr int logit_size(int type) { return type == kLogitsF32 ? 4 : 2; }
 // The largest finite logit of a type, which infinity counts as.
 template <int TYPE>
 constexpr float kMostLogit = TYPE == kLogitsF16 ? 65504.0f : TYPE == kLogitsBf16 ? 0x1.fep+127f : kMostFloat;
-// Element i of a vector as a float. NaN cannot be drawn and becomes -inf.
+// Element i of a vector as a float, as it is.
 template <int TYPE>
-__device__ __forceinline__ float logit_of(uint4_t raw, int i) {
-  float f;
+__device__ __forceinline__ float raw_logit(uint4_t raw, int i) {
   if constexpr (TYPE == kLogitsF32) {
     const uint32_t word = raw[i];        // (a bit cast of the element itself is one of the first)
-    f = __builtin_bit_cast(float, word);
+    return __builtin_bit_cast(float, word);
   } else if constexpr (TYPE == kLogitsBf16) {
     const uint32_t word = i & 1 ? raw[i >> 1] & 0xffff0000u : raw[i >> 1] << 16;
-    f = __builtin_bit_cast(float, word);
+    return __builtin_bit_cast(float, word);
   } else {
-    f = (float)__builtin_bit_cast(half_t, (uint16_t)(raw[i >> 1] >> (16 * (i & 1))));
+    return (float)__builtin_bit_cast(half_t, (uint16_t)(raw[i >> 1] >> (16 * (i & 1))));
   }
-  return __builtin_fminf(__builtin_fmaxf(f, -INFINITY), kMostLogit<TYPE>);
+}
+// NaN cannot be drawn and becomes -inf, infinity the largest finite logit.
+template <int TYPE>
+__device__ __forceinline__ float clean_logit(float x) {
+  return __builtin_fminf(__builtin_fmaxf(x, -INFINITY), kMostLogit<TYPE>);
+}
+// Whether a vector has an element that is not finite: two at a time by their bits without the signs.
+template <int TYPE>
+__device__ __forceinline__ bool has_special(uint4_t raw) {
+  static_assert(TYPE != kLogitsF32, "16-bit logits");
+  typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
+  ushort2_t top = __builtin_bit_cast(ushort2_t, raw[0] & 0x7fff7fffu);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    const uint32_t word = raw[i] & 0x7fff7fffu;
+    top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_t, word));
+  }
+  constexpr uint16_t kInfinity = TYPE == kLogitsF16 ? 0x7c00 : 0x7f80;
+  return top[0] >= kInfinity || top[1] >= kInfinity;
 }
 
 // Where the vector `at` of a row is; only those with an element of the row are read.
@@ -106,7 +125,7 @@ __device__ __forceinline__ void logits_of(const LogitsRow &in, uint4_t raw, int6
   const int64_t first = at * kPer - in.lead;
   const bool inside = first >= 0 && first + kPer <= vocab;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) x[i] = logit_of<TYPE>(raw, i);
+  for (int i = 0; i < kPer; ++i) x[i] = clean_logit<TYPE>(raw_logit<TYPE>(raw, i));
   if (!inside) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -115,22 +134,36 @@ __device__ __forceinline__ void logits_of(const LogitsRow &in, uint4_t raw, int6
   }
 }
 
-// z = 8 y; its bin is floor(z).
+// z = 8 y; its bin is floor(z). 8 / T: the hardware's approximation, twice improved (exact for powers of two).
+__device__ __forceinline__ double z_factor(float t) {
+  const double d = (double)t;
+  double r = __builtin_amdgcn_rcp(d);
+#pragma unroll
+  for (int step = 0; step < 2; ++step) r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+  return 8.0 * r;
+}
 __device__ __forceinline__ double z_of(float x, double z_per_x) { return (double)x * z_per_x; }
 // (1 - 2^-20) exp((f - 1) / 8) - 7/8 in units of 2^-40, f in [0, 1) the place in a bin: below 2^37, and above 0. By the polynomial of
-// degree 6 that agrees with it in seven Chebyshev points, within 0.02 of a unit. As the low 52 bits of a double: 2^52 is added.
-__device__ __forceinline__ uint64_t mass_bits(double f) {
-  double e = 0x1.56123fcc468c2p+12;
-  e = __builtin_fma(e, f, 0x1.e10f01fb822cdp+17);
-  e = __builtin_fma(e, f, 0x1.2d3c27a6b0e5fp+23);
-  e = __builtin_fma(e, f, 0x1.2d39a7c5007cap+28);
-  e = __builtin_fma(e, f, 0x1.c3d68623f9176p+32);
-  e = __builtin_fma(e, f, 0x1.c3d686115b6e3p+36);
-  e = __builtin_fma(e, f, 0x1.eb4308b7019d4p+32);
-  return __builtin_bit_cast(uint64_t, e + 0x1p52);
-}
+// degree 6 that agrees with it in seven Chebyshev points, within 0.02 of a unit but for c0, which with the 2^52 that is added to have the result in a double's low bits is a whole number, 0.01 from its own.
+// (The coefficients in scalar registers, where they stay: as literals each is moved in front of its step, two instructions a
+// coefficient and token.)
+struct MassPolynomial {
+  double c0 = 0x1.00001eb4308b7p+52, c1 = 0x1.c3d686115b6e3p+36, c2 = 0x1.c3d68623f9176p+32, c3 = 0x1.2d39a7c5007cap+28,
+         c4 = 0x1.2d3c27a6b0e5fp+23, c5 = 0x1.e10f01fb822cdp+17, c6 = 0x1.56123fcc468c2p+12;
+  __device__ __forceinline__ void keep() { asm("" : "+s"(c0), "+s"(c1), "+s"(c2), "+s"(c3), "+s"(c4), "+s"(c5)); }
+  __device__ __forceinline__ uint64_t bits(double f) const {
+    double e = __builtin_fma(c6, f, c5);
+    e = __builtin_fma(e, f, c4);
+    e = __builtin_fma(e, f, c3);
+    e = __builtin_fma(e, f, c2);
+    e = __builtin_fma(e, f, c1);
+    return __builtin_bit_cast(uint64_t, __builtin_fma(e, f, c0));
+  }
+};
 constexpr uint64_t kMassOne = 0x4330000000000000ull;      // 2^52's bits
-__device__ __forceinline__ uint64_t units_of(double z) { return mass_bits(z - __builtin_floor(z)) - kMassOne; }
+__device__ __forceinline__ uint64_t units_of(const MassPolynomial &mass, double z) {
+  return mass.bits(z - __builtin_floor(z)) - kMassOne;
+}
 // In whole numbers; out of their range the nearest, as the conversion does it, which C++ leaves open.
 __device__ __forceinline__ uint32_t whole_of(double x) {
   uint32_t n;
@@ -251,22 +284,40 @@ __global__ __launch_bounds__(kSampleThreads) void sample_slices_kernel(
     if (v < slice_vectors && v0 + v < in.vectors) raw[i] = *(const uint4_t *)(in.base + (v0 + v) * 16);
   }
   const float t = row_temperature(temperature, row);
-  const double z_per_x = 8.0 / (double)t;
+  const double z_per_x = z_factor(t);
 #pragma unroll
   for (int i = tid; i < kCopies * 2 * kSampleThreads; i += kSampleThreads) hist[0][i] = 0;
   if (tid == 0) {
     found_bins = 0;
     found_n = 0;
   }
+  const int first = (int)((v0 + tid) * kPer) - in.lead;        // this thread's first element, of the row's
   float x[kMostVectors][kPer];
-  float most = -INFINITY;
+  bool special = TYPE == kLogitsF32;
 #pragma unroll
   for (int i = 0; i < kMostVectors; ++i) {
-    const int v = i * kSampleThreads + tid;
-    logits_of<TYPE>(in, raw[i], v < slice_vectors ? v0 + v : in.vectors, vocab, x[i]);      // (behind the row: nothing of it)
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) most = __builtin_fmaxf(most, x[i][k]);
+    for (int k = 0; k < kPer; ++k) x[i][k] = raw_logit<TYPE>(raw[i], k);
+    if constexpr (TYPE != kLogitsF32) special |= has_special<TYPE>(raw[i]);
   }
+  if (__builtin_amdgcn_ballot_w64(special) != 0) {
+#pragma unroll
+    for (int i = 0; i < kMostVectors * kPer; ++i) x[i / kPer][i % kPer] = clean_logit<TYPE>(x[i / kPer][i % kPer]);
+  }
+  if (slice == 0 || v0 + kMostVectors * kSampleThreads >= in.vectors || slice_vectors < kMostVectors * kSampleThreads) {
+    // -inf in the places that are not the row's, or not the slice's
+#pragma unroll
+    for (int i = 0; i < kMostVectors; ++i) {
+      const bool there = i * kSampleThreads + tid < slice_vectors;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        if (!there || (uint32_t)(first + i * kSampleThreads * kPer + k) >= (uint32_t)vocab) x[i][k] = -INFINITY;
+      }
+    }
+  }
+  float most = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kMostVectors * kPer; ++i) most = __builtin_fmaxf(most, x[i / kPer][i % kPer]);
   most = wave_max(most);
   if (tid % kWave == 0) wave_most[wave] = most;
   __syncthreads();
@@ -283,7 +334,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_slices_kernel(
     for (int i = 0; i < kMostVectors; ++i) {
 #pragma unroll
       for (int k = 0; k < kPer; ++k) {
-        const int e = (int)((v0 + i * kSampleThreads + tid) * kPer - in.lead + k);
+        const int e = first + i * kSampleThreads * kPer + k;
         if (x[i][k] == most) at = e < at ? e : at;
       }
     }
@@ -301,14 +352,20 @@ __global__ __launch_bounds__(kSampleThreads) void sample_slices_kernel(
   }
   const double top = __builtin_floor(z_of(most, z_per_x));
   uint64_t *mine = hist[wave / (kWaves / kCopies)];
+  MassPolynomial mass;
+  mass.keep();
+  const uint32_t aside = kSampleBins + tid % kWave;        // (what is too far below goes to a place of the lane's, without a branch)
+  static_assert(kSampleBins + kWave <= 2 * kSampleThreads, "which is behind the bins");
 #pragma unroll
   for (int i = 0; i < kMostVectors; ++i) {
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       const double z = z_of(x[i][k], z_per_x), b = __builtin_floor(z);
-      const uint32_t d = whole_of(top - b);                      // (-inf: far below)
-      if (d < (uint32_t)kSampleBins) atomicAdd((unsigned long long *)&mine[d], (unsigned long long)mass_bits(z - b));
+      uint32_t d = whole_of(top - b);                            // (-inf: far below)
+      d = d < aside ? d : aside;
+      atomicAdd((unsigned long long *)&mine[d], (unsigned long long)mass.bits(z - b));
     }
+    __builtin_amdgcn_sched_barrier(0);                           // (more tokens at a time take more registers than there are)
   }
   __syncthreads();
   // Two bins a thread, to their places; and how many from the top on have no more tokens than a list takes.
@@ -328,8 +385,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_slices_kernel(
       n_all += n;
       units += u;
     }
-    if (b < kSampleBins) bins[place * kSampleSlots + ((top_slot - b) & (kSampleSlots - 1))] = units | n_all << kCountShift;
-    count += (int)n_all;
+    if (b < kSampleBins) {
+      bins[place * kSampleSlots + ((top_slot - b) & (kSampleSlots - 1))] = units | n_all << kCountShift;
+      count += (int)n_all;
+    }
     if (i == 0) count_first = count;
   }
   int upto = wave_scan(count);
@@ -342,23 +401,32 @@ __global__ __launch_bounds__(kSampleThreads) void sample_slices_kernel(
   __syncthreads();
   const int listed_bins = found_bins < kSampleBins ? found_bins : kSampleBins;
   if (listed_bins > 0) {
-    const float least = logit_of_order(lowest_of_bin(top - (listed_bins - 1), t, z_per_x));
+    if (wave == 0) {
+      const uint32_t order = lowest_of_bin(top - (listed_bins - 1), t, z_per_x);
+      if (tid == 0) wave_most[0] = logit_of_order(order);
+    }
+    __syncthreads();
+    const float least = wave_most[0];
+    uint64_t those[kMostVectors * kPer];
+    int n = 0;
 #pragma unroll
-    for (int i = 0; i < kMostVectors; ++i) {
-      uint32_t those = 0;
+    for (int i = 0; i < kMostVectors * kPer; ++i) {
+      those[i] = __builtin_amdgcn_ballot_w64(x[i / kPer][i % kPer] >= least);
+      n += __builtin_popcountll(those[i]);
+    }
+    int at = 0;
+    if (tid % kWave == 0 && n > 0) at = atomicAdd(&found_n, n);
+    at = __builtin_amdgcn_readfirstlane(at);
+    uint64_t *to = lists + place * kSliceList;
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) those |= (x[i][k] >= least ? 1u : 0u) << k;
-      while (those != 0) {
-        const int k = __builtin_ctz(those);
-        those &= those - 1;
-        float e = x[i][0];
-#pragma unroll
-        for (int j = 1; j < kPer; ++j) e = k == j ? x[i][j] : e;
-        const int slot = atomicAdd(&found_n, 1);
-        if (slot < kSliceList) {
-          lists[place * kSliceList + slot] = key_of<TYPE>(order_of(e), (int)((v0 + i * kSampleThreads + tid) * kPer - in.lead + k));
-        }
+    for (int i = 0; i < kMostVectors * kPer; ++i) {
+      if (those[i] == 0) continue;
+      const float e = x[i / kPer][i % kPer];
+      const int slot = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(those[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)those[i], 0));
+      if (e >= least && slot < kSliceList) {
+        to[slot] = (uint64_t)__builtin_bit_cast(uint32_t, e) << 32 | (uint32_t)(first + i / kPer * kSampleThreads * kPer + i % kPer);
       }
+      at += __builtin_popcountll(those[i]);
     }
     __syncthreads();
   }
@@ -409,6 +477,42 @@ __device__ __forceinline__ void row_scan2(T &x, T *room_x, U &y, U *room_y) {
   y += by;
 }
 
+// Whether a word of a vector may have a logit of [least, most]: 16-bit ones two at a time, by their bits in the order of whole numbers.
+template <int TYPE>
+struct RangeTest {
+  typedef int16_t short2_t __attribute__((ext_vector_type(2)));
+  typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
+  float least, most;
+  uint32_t low, beyond;      // twice: the lowest, and how far behind it the range has ended
+  __device__ __forceinline__ RangeTest(float least_x, float most_x) : least(least_x), most(most_x), low(0), beyond(0) {
+    if constexpr (TYPE != kLogitsF32) {
+      // (the zeros, infinity and, in fp16, those next to an end are looked at again)
+      const int from = least_x == 0.f ? -1 : in_order(bits_of(least_x));
+      const int to = most_x == kMostLogit<TYPE> ? 0x7fff : most_x == 0.f ? 0 : in_order(bits_of(most_x));
+      low = (uint16_t)from * 0x10001u;
+      beyond = (uint16_t)(to - from + 1) * 0x10001u;
+    } else if (most_x == kMostFloat) {
+      most = INFINITY;
+    }
+  }
+  static __device__ __forceinline__ int in_order(uint16_t bits) { return (int16_t)(bits ^ ((int16_t)bits >> 15 & 0x7fff)); }
+  static __device__ __forceinline__ uint16_t bits_of(float x) {
+    if constexpr (TYPE == kLogitsF16) return __builtin_bit_cast(uint16_t, (half_t)x);
+    return (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16);
+  }
+  __device__ __forceinline__ bool any(uint32_t word) const {
+    if constexpr (TYPE == kLogitsF32) {
+      const float x = __builtin_bit_cast(float, word);
+      return x >= least && x <= most;
+    } else {
+      const short2_t x = __builtin_bit_cast(short2_t, word);
+      const short2_t o = x ^ ((x >> 15) & (short2_t)0x7fff);
+      const ushort2_t from_low = __builtin_bit_cast(ushort2_t, o) - __builtin_bit_cast(ushort2_t, low);
+      return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(from_low, __builtin_bit_cast(ushort2_t, beyond))) != beyond;
+    }
+  }
+};
+
 // Bound by latency: one memory trip or one pass over the row after another, with barriers between them. So loads are made whatever
 // their place (clamped, and masked where they are used), each piece of code stands once, and what few threads can find, each
 // wavefront finds for itself.
@@ -420,8 +524,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     int32_t slice_vectors, int32_t slices, const SampleSlice *__restrict__ heads, const uint64_t *__restrict__ bins,
     const uint64_t *__restrict__ lists) {
   constexpr int kPer = 16 / logit_size(TYPE);
-  constexpr int kParts = kRowThreads / kSampleSlots;  // threads of a slot
-  static_assert(kParts == 2, "two threads a slot");
+  static_assert(kRowThreads == kSampleSlots, "a thread has a slot");
+  constexpr int kRun = (kSampleMaxVocab + kRowThreads - 1) / kRowThreads;    // indexes of a run, at most
   __shared__ double bin_top[kSampleSlots];            // exp(the bin's top - the row's largest y), in units
   __shared__ double mass_to[kSampleSlots];            // inclusive
   __shared__ int32_t count_to[kSampleSlots];
@@ -429,10 +533,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   __shared__ int32_t slice_listed[kMaxSlices];
   __shared__ double slice_mass[kMaxSlices];
   __shared__ unsigned long long slice_units[kMaxSlices];
-  __shared__ uint64_t list[kSampleList];              // keys, in any order
+  __shared__ uint64_t list[kOwnList][kRowThreads], more[kMoreList];   // keys, in any order
   __shared__ unsigned long long radix_units[kRowThreads];
   __shared__ int32_t radix_count[kRowThreads];
-  __shared__ unsigned long long rank_key[kRowThreads], rank_units[kRowThreads];
+  __shared__ unsigned long long rank_key[kRun], rank_units[kRun];
   __shared__ RowRoom rooms[2];
   __shared__ float room_f[kRowWaves];
   __shared__ int32_t found_k, found_p, found_last, found_at, found_slice, found_n, complete;
@@ -446,14 +550,12 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   int turn = 0;                                        // which room the next scan has
 
   // The words of the first slices are asked for before it is known what they mean.
-  constexpr int kAhead = 10;
-  const int slot = tid % kSampleSlots, part = tid / kSampleSlots;
+  constexpr int kAhead = 20;
   uint64_t words[kAhead];
   auto load_words = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int s = s0 + i * kParts;
-      words[i] = row_bins[(int64_t)(s < slices ? s : slices - 1) * kSampleSlots + slot];
+      words[i] = row_bins[(int64_t)(s0 + i < slices ? s0 + i : slices - 1) * kSampleSlots + tid];
     }
   };
   const SampleSlice own_head = head[tid < slices ? tid : slices - 1];
@@ -462,7 +564,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   const float p = top_p != nullptr ? top_p[row] : 1.0f;
   const float m = min_p != nullptr ? min_p[row] : 0.0f;
   double u = (double)uniforms[row];
-  load_words(part);
+  load_words(0);
   u = u > 0.0 ? (u < 1.0 - 0x1p-24 ? u : 1.0 - 0x1p-24) : 0.0;
 
   // the row's largest logit
@@ -493,7 +595,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     }
     return;
   }
-  const double z_per_x = 8.0 / (double)t;
+  const double z_per_x = z_factor(t);
   const double z_most = z_of(most, z_per_x), top = __builtin_floor(z_most);
   const int top_slot = slot_of(top);
   if (tid < slices) {
@@ -502,46 +604,38 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     slice_listed[tid] = own_head.listed;
     if (d < (uint32_t)kSampleBins && own_head.listed_bins < kSampleBins) atomicMin(&complete, (int)d + own_head.listed_bins);
   }
-  if (tid < kSampleSlots) {
-    bin_top[tid] = kUnit * exp(((top - z_most) + (double)(1 - tid)) * 0.125);   // (of z of any size: the first difference is exact)
-  }
+  bin_top[tid] = kUnit * exp(((top - z_most) + (double)(1 - tid)) * 0.125);     // (of z of any size: the first difference is exact)
   __syncthreads();
   // Bin b of the row in slice s, from what lies in its place, which need not be the slice's.
   auto word = [&](uint64_t w, int s, int b) __attribute__((always_inline)) -> uint64_t {
     return b < kSampleBins && (uint32_t)(b - shift[s]) < (uint32_t)kSampleBins ? w : 0;
   };
-  // its bins: a thread adds up a slot of every other slice's and hands it over
+  // its bins: a thread adds up a slot of the slices' and hands it over
   {
-    const int b = (top_slot - slot) & (kSampleSlots - 1);
+    const int b = (top_slot - tid) & (kSampleSlots - 1);
     uint32_t count = 0;
     uint64_t units = 0;
-    for (int s0 = part; s0 < slices; s0 += kAhead * kParts) {
-      if (s0 != part) load_words(s0);
+    for (int s0 = 0; s0 < slices; s0 += kAhead) {
+      if (s0 != 0) load_words(s0);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int s = s0 + i * kParts;
+        const int s = s0 + i;
         const uint64_t x = s < slices ? word(words[i], s, b) : 0;
         count += (uint32_t)(x >> kCountShift);
         units += x & kUnitsMask;
       }
     }
-    radix_units[part * kSampleSlots + b] = units + kFloorUnits * (uint64_t)count;
-    radix_count[part * kSampleSlots + b] = (int32_t)count;
+    radix_units[b] = units + kFloorUnits * (uint64_t)count;
+    radix_count[b] = (int32_t)count;
   }
   __syncthreads();
-  int32_t count_here = 0;
-  double mass = 0.0;
-  if (tid < kSampleSlots) {
-    count_here = radix_count[tid] + radix_count[kSampleSlots + tid];
-    mass = (double)(radix_units[tid] + radix_units[kSampleSlots + tid]) * bin_top[tid];
-  }
+  const int32_t count_here = radix_count[tid];
+  double mass = (double)radix_units[tid] * bin_top[tid];
   int32_t count = count_here;
   row_scan2(count, rooms[0].count, mass, rooms[0].mass);
   turn = 1;
-  if (tid < kSampleSlots) {
-    count_to[tid] = count;
-    mass_to[tid] = mass;
-  }
+  count_to[tid] = count;
+  mass_to[tid] = mass;
   {
     const uint64_t any = __builtin_amdgcn_ballot_w64(count_here > 0);
     if (lane == 0 && any != 0) atomicMax(&found_last, wave * kWave + 63 - __builtin_clzll(any));       // the last bin with a token
@@ -564,8 +658,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     __syncthreads();
     return found_p;
   };
+  MassPolynomial polynomial;
+  polynomial.keep();
   auto units_of_key = [&](uint64_t key) __attribute__((always_inline)) -> uint64_t {
-    return units_of(z_of(logit_of_key<TYPE>(key), z_per_x)) + kFloorUnits;
+    return units_of(polynomial, z_of(logit_of_key<TYPE>(key), z_per_x)) + kFloorUnits;
   };
 
   // Where the prefixes end; one that ends behind min_p's end (bin_m, or a bin more) says nothing, but top_k says what top_p is a
@@ -587,20 +683,29 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   // Where the slices' lists have all tokens that come into question, those are the row's list, and the draw's; else it has a
   // bin's tokens at a time, if they fit.
   const int most_bin = by_k ? bin_k : by_p ? bin_p : bin_m;
-  const bool few = most_bin < complete && count_to[most_bin] <= kSampleList;
-  int listed = 0;
+  const bool few = most_bin < complete && count_to[most_bin] <= kMoreList;
+  int own = 0;
+  const int own_room = few ? 0 : kOwnList;              // (few are spread evenly in the list of all)
+  auto enlist = [&](uint64_t key) __attribute__((always_inline)) {
+    if (own < own_room) {
+      list[own++][tid] = key;
+    } else {
+      const int to = atomicAdd(&found_n, 1);
+      if (to < kMoreList) more[to] = key;
+    }
+  };
+  int listed = 0;                                       // of `more`
   if (few) {
     const uint64_t least = lowest_key<TYPE>(lowest_of_bin(top - most_bin, t, z_per_x));
 #pragma unroll 4
     for (int i = tid; i < slices * kSliceList; i += kRowThreads) {
-      const uint64_t key = row_lists[i];
-      if (i % kSliceList < slice_listed[i / kSliceList] && key >= least) {
-        const int to = atomicAdd(&found_n, 1);
-        if (to < kSampleList) list[to] = key;
-      }
+      const uint64_t entry = row_lists[i];               // a logit's bits and its index
+      const uint32_t bits = (uint32_t)(entry >> 32);
+      const uint64_t key = key_of<TYPE>(order_of(__builtin_bit_cast(float, bits)), (int32_t)(uint32_t)entry);
+      if (i % kSliceList < slice_listed[i / kSliceList] && key >= least) enlist(key);
     }
     __syncthreads();
-    listed = found_n < kSampleList ? found_n : kSampleList;
+    listed = found_n < kMoreList ? found_n : kMoreList;
   }
   int last = last_bin;                                  // the bin that the kept prefix ends in
   bool whole = true;                                    // all of it; or its tokens from the key `cut` on
@@ -611,8 +716,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   // Every token of the row's list or, without it, of the row, whose key is in [from, to].
   auto each_token = [&](uint64_t from, uint64_t to, auto &&what) __attribute__((always_inline)) {
     if (in_list) {
-      for (int i = tid; i < listed; i += kRowThreads) {
-        const uint64_t key = list[i];
+      for (int i = 0, n = listed > tid ? own + (listed - tid + kRowThreads - 1) / kRowThreads : own; i < n; ++i) {
+        const uint64_t key = i < own ? list[i][tid] : more[tid + (i - own) * kRowThreads];
         if (key >= from && key <= to) what(key);
       }
     } else {
@@ -674,43 +779,54 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     low = lowest_key<TYPE>(low_order);
     high = lowest_key<TYPE>(high_order + 1) - 1;
     if (!few && list_bin != bin) {
-      in_list = count_to[bin] - (bin > 0 ? count_to[bin - 1] : 0) <= kSampleList;
+      in_list = count_to[bin] - (bin > 0 ? count_to[bin - 1] : 0) <= kMostListed;
       list_bin = bin;
+      own = listed = 0;
       __syncthreads();
       if (tid == 0) found_n = 0;
       __syncthreads();
       if (in_list) {
         const float least_x = logit_of_order(low_order), most_x = logit_of_order(high_order);
-        constexpr int kVectors = 4;
+        const RangeTest<TYPE> test(least_x, most_x);
+        constexpr int kVectors = 4, kPerWord = kPer / 4;
+        uint4_t raw[kVectors], next[kVectors];               // (the next ones on their way while these are looked at)
+        auto load = [&](int64_t v0, uint4_t (&to)[kVectors]) __attribute__((always_inline)) {
+#pragma unroll
+          for (int j = 0; j < kVectors; ++j) {
+            const int64_t v = v0 + j * kRowThreads;
+            to[j] = *(const uint4_t *)(in.base + (v < in.vectors ? v : in.vectors - 1) * 16);
+          }
+        };
+        load(tid, next);
 #pragma unroll 1
         for (int64_t v0 = tid; v0 < in.vectors; v0 += kVectors * kRowThreads) {
-          uint4_t raw[kVectors];
+#pragma unroll
+          for (int j = 0; j < kVectors; ++j) raw[j] = next[j];
+          load(v0 + kVectors * kRowThreads, next);
 #pragma unroll
           for (int j = 0; j < kVectors; ++j) {
             const int64_t v = v0 + j * kRowThreads;
-            raw[j] = *(const uint4_t *)(in.base + (v < in.vectors ? v : in.vectors - 1) * 16);
-          }
+            uint32_t those = 0;                            // words with an element in the range
 #pragma unroll
-          for (int j = 0; j < kVectors; ++j) {
-            const int64_t v = v0 + j * kRowThreads;
-            float x[kPer];
-            logits_of<TYPE>(in, raw[j], v, vocab, x);
-            uint32_t those = 0;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) those |= (x[i] >= least_x && x[i] <= most_x ? 1u : 0u) << i;
+            for (int i = 0; i < 4; ++i) those |= (test.any(raw[j][i]) ? 1u : 0u) << i;
             while (those != 0) {
               const int i = __builtin_ctz(those);
               those &= those - 1;
-              float e = x[0];
+              uint32_t one = raw[j][0];
 #pragma unroll
-              for (int n = 1; n < kPer; ++n) e = i == n ? x[n] : e;
-              const int to = atomicAdd(&found_n, 1);
-              if (to < kSampleList) list[to] = key_of<TYPE>(order_of(e), (int32_t)(v * kPer - in.lead + i));
+              for (int n = 1; n < 4; ++n) one = i == n ? raw[j][n] : one;
+#pragma unroll
+              for (int h = 0; h < kPerWord; ++h) {
+                const float e = clean_logit<TYPE>(raw_logit<TYPE>(uint4_t{one, one, one, one}, h));
+                const int32_t at = (int32_t)(v * kPer - in.lead) + i * kPerWord + h;
+                if (e >= least_x && e <= most_x && (uint32_t)at < (uint32_t)vocab) enlist(key_of<TYPE>(order_of(e), at));
+              }
             }
           }
         }
         __syncthreads();
-        listed = found_n < kSampleList ? found_n : kSampleList;
+        in_list = found_n <= kMoreList;                    // (else too many of them are too few threads')
+        listed = found_n;
       }
     }
     if (filter == 2) break;
@@ -816,7 +932,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     const float x = logit_of_key<TYPE>(key);
     if (!((double)x - (double)most >= x_cut)) return 0.0;
     const double z = z_of(x, z_per_x), d = top - __builtin_floor(z);
-    return d < (double)kSampleBins ? (double)(units_of(z) + kFloorUnits) * bin_top[(int)d] : 0.0;
+    return d < (double)kSampleBins ? (double)(units_of(polynomial, z) + kFloorUnits) * bin_top[(int)d] : 0.0;
   };
   uint64_t token = 0;
   double all = 1.0;
@@ -830,38 +946,39 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     radix_units[tid] = 0;
     if (tid == 0) found_n = 0;
     __syncthreads();
-    for (int i = tid; i < listed; i += kRowThreads) {
-      if (list[i] >= cut) atomicAdd(&radix_units[index_of_key(list[i]) / width], (unsigned long long)units_kept(list[i]));
-    }
+    each_token(cut, ~0ull, [&](uint64_t key) __attribute__((always_inline)) {
+      atomicAdd(&radix_units[index_of_key(key) / width], (unsigned long long)units_kept(key));
+    });
     __syncthreads();
-    const unsigned long long own = radix_units[tid];
+    const unsigned long long here = radix_units[tid];
     unsigned long long sum;
-    const unsigned long long upto = row_scan(own, rooms[turn].units, &sum);
+    const unsigned long long upto = row_scan(here, rooms[turn].units, &sum);
     turn ^= 1;
     const double target = u * (double)sum * (2.0 - kReached);
-    if ((double)upto > target && !((double)(upto - own) > target)) {
+    if ((double)upto > target && !((double)(upto - here) > target)) {
       found_at = tid;
-      found_units = upto - own;
+      found_units = upto - here;
     }
     __syncthreads();
     const int run = found_at;
     const uint64_t before_run = found_units;
-    for (int i = tid; i < listed; i += kRowThreads) {
-      if (list[i] >= cut && index_of_key(list[i]) / width == run) {
-        const int to = atomicAdd(&found_n, 1);
-        rank_key[to] = list[i];                            // (of `width` indexes at most, no more than threads)
-        rank_units[to] = units_kept(list[i]);
-      }
-    }
+    each_token(cut, ~0ull, [&](uint64_t key) __attribute__((always_inline)) {
+      if (index_of_key(key) / width != run) return;
+      const int to = atomicAdd(&found_n, 1);
+      rank_key[to] = key;                                  // (of `width` indexes, at most kRun)
+      rank_units[to] = units_kept(key);
+    });
     __syncthreads();
-    if (tid >= found_n) return;
-    const uint64_t mine = rank_key[tid];
-    const int32_t at = index_of_key(mine);
-    uint64_t units_before = before_run;
+    const int n = found_n;
+    for (int i = tid; i < n; i += kRowThreads) {
+      const uint64_t mine = rank_key[i];
+      const int32_t at = index_of_key(mine);
+      uint64_t units_before = before_run;
 #pragma unroll 8
-    for (int i = 0; i < found_n; ++i) units_before += index_of_key(rank_key[i]) < at ? rank_units[i] : 0;
-    if (!((double)(units_before + rank_units[tid]) > target) || (double)units_before > target) return;
-    token = mine;
+      for (int j = 0; j < n; ++j) units_before += index_of_key(rank_key[j]) < at ? rank_units[j] : 0;
+      if ((double)(units_before + rank_units[i]) > target && !((double)units_before > target)) token = mine;
+    }
+    if (token == 0) return;
     all = (double)sum * 0x1p-43;
   } else {
     // The kept mass of each slice: its bins in front of the last, and what it has of that one.
@@ -877,14 +994,15 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     for (int s0 = 0; s0 < slices; s0 += kRowThreads / 16) {
       const int s = s0 + tid / 16 < slices ? s0 + tid / 16 : slices - 1;
       double sum = 0.0;
-      for (int b0 = tid % 16; b0 < bins_kept; b0 += 16 * kAhead) {
-        uint64_t w[kAhead];
+      constexpr int kBinsAhead = 8;
+      for (int b0 = tid % 16; b0 < bins_kept; b0 += 16 * kBinsAhead) {
+        uint64_t w[kBinsAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
+        for (int i = 0; i < kBinsAhead; ++i) {
           w[i] = row_bins[(int64_t)s * kSampleSlots + ((top_slot - (b0 + 16 * i)) & (kSampleSlots - 1))];
         }
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
+        for (int i = 0; i < kBinsAhead; ++i) {
           const int b = b0 + 16 * i;
           const uint64_t x = b < bins_kept ? word(w[i], s, b) : 0;
           sum += (double)((x & kUnitsMask) + kFloorUnits * (x >> kCountShift)) * bin_top[b & (kSampleSlots - 1)];
