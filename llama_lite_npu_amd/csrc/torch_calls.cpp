@@ -432,12 +432,233 @@ PyObject *page_dequant(PyObject *, PyObject *const *a, Py_ssize_t n) {
   }
 }
 
+// Whether all tensors there are live on the current device, which a launch goes to.
+template <typename... Tensors>
+bool here(const Tensors *...all) {
+  const auto device = at::detail::getCUDAHooks().getCurrentDevice();
+  return ((all == nullptr || all->get_device() == device) && ...);
+}
+
+int32_t pool_format(Format f) {
+  return f == kF16 ? LITEKV_POOL_FP16 : f == kFp8 ? LITEKV_POOL_FP8 : f == kInt8 ? LITEKV_POOL_INT8 : LITEKV_POOL_INT4;
+}
+
+// (q, k, v, slot_mapping, kv_pool, positions, axes, cos_table, sin_table, q_norm_weight, k_norm_weight, eps, kv_scales,
+//  num_axes, stream): `axes` the bytes that ops.axis_of_pair made for the pool's head dim
+// -> True if launched, the library's status if that is not 0, or None
+PyObject *qk_norm_mrope_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (n != 15) Py_RETURN_NONE;
+  try {
+    const at::Tensor *q = half_tensor(a[0]), *k = half_tensor(a[1]), *v = half_tensor(a[2]);
+    if (q == nullptr || k == nullptr || v == nullptr || q->dim() != 3) Py_RETURN_NONE;
+    const Pool pool = pool_of(a[4], a[12]);
+    if (pool.format == kNone) Py_RETURN_NONE;
+    const int64_t t = q->size(0), hq = q->size(1), d = pool.d;
+    const int64_t qs = row_stride(*q, t, hq, d), ks = row_stride(*k, t, pool.hkv, d), vs = row_stride(*v, t, pool.hkv, d);
+    const at::Tensor *slots = index_tensor(a[3], t), *positions = gpu_tensor(a[5]);
+    const at::Tensor *cos = half_tensor(a[7]), *sin = half_tensor(a[8]), *qw = nullptr, *kw = nullptr;
+    if (qs < 0 || ks < 0 || vs < 0 || slots == nullptr || positions == nullptr || cos == nullptr || sin == nullptr) Py_RETURN_NONE;
+    const int64_t axes = PyLong_AsLongLong(a[13]);
+    const double eps = PyFloat_AsDouble(a[11]);
+    void *stream = PyLong_AsVoidPtr(a[14]);
+    if (PyErr_Occurred() || !PyBytes_CheckExact(a[6]) || PyBytes_GET_SIZE(a[6]) != d / 2) {
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    const bool wide = positions->scalar_type() == at::kLong;
+    if ((!wide && positions->scalar_type() != at::kInt) || positions->dim() != 2 || positions->size(0) != axes ||
+        positions->size(1) != t || cos->dim() != 2 || sin->dim() != 2 || cos->size(0) < 2 || cos->size(1) < d / 2 ||
+        cos->sizes() != sin->sizes() || cos->strides() != sin->strides() || cos->stride(1) != 1) {
+      Py_RETURN_NONE;
+    }
+    if (a[9] != Py_None || a[10] != Py_None) {
+      qw = half_tensor(a[9]);
+      kw = half_tensor(a[10]);
+      if (qw == nullptr || kw == nullptr || qw->numel() != d || kw->numel() != d || !qw->is_contiguous() || !kw->is_contiguous()) {
+        Py_RETURN_NONE;
+      }
+    }
+    const at::Tensor *scales = pool.scales != nullptr ? gpu_tensor(a[12]) : nullptr;
+    if (!here(q, k, v, slots, pool.t, positions, cos, sin, qw, kw, scales) || t > INT32_MAX || hq > INT32_MAX ||
+        pool.hkv > INT32_MAX || d > INT32_MAX) {
+      Py_RETURN_NONE;
+    }
+    void *qp = address(q), *kp = address(k), *vp = address(v), *qwp = address(qw), *kwp = address(kw), *cp = address(cos),
+         *sp = address(sin), *pp = address(pool.t), *at = address(positions);
+    const int32_t *slp = static_cast<const int32_t *>(address(slots));
+    const uint8_t *pairs = reinterpret_cast<const uint8_t *>(PyBytes_AS_STRING(a[6]));
+    const int64_t table_stride = cos->stride(0), table_rows = cos->size(0), as = positions->stride(0), ts = positions->stride(1);
+    const int rc = unlocked([&] {
+      return litekv_qk_norm_mrope_append(qp, qs, kp, ks, vp, vs, qwp, kwp, cp, sp, table_stride, table_rows, at, wide, as, ts,
+                                         (int32_t)axes, pairs, slp, pp, static_cast<const float *>(pool.scales),
+                                         pool_format(pool.format), (int32_t)t, (int32_t)hq, (int32_t)pool.hkv, (int32_t)d,
+                                         pool.slots, (float)eps, stream);
+    });
+    if (rc != 0) return PyLong_FromLong(rc);
+    Py_RETURN_TRUE;
+  } catch (...) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+}
+
+// (q, kv_pool, block_table, kv_lens, cu_q_lens or None, max_q_len, softmax_scale, page_size, kv_scales, max_kv_len or 0, splits,
+//  stream) -> the output, or the library's status if that is not 0, or None. Without cu_q_lens one row a sequence, on that many
+//  splits, or on the balanced schedule (0), its plan made here.
+PyObject *paged_cross_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (n != 12) Py_RETURN_NONE;
+  try {
+    const at::Tensor *q = half_tensor(a[0]);
+    if (q == nullptr || q->dim() != 3) Py_RETURN_NONE;
+    const Pool pool = pool_of(a[1], a[8]);
+    const bool rows = a[4] != Py_None;
+    if (pool.format == kNone || (pool.d != 64 && pool.d != 128) || (!rows && pool.format == kInt4)) Py_RETURN_NONE;
+    const int64_t t = q->size(0), hq = q->size(1), d = pool.d;
+    const int64_t qs = row_stride(*q, t, hq, d);
+    const at::Tensor *cu = rows ? index_tensor(a[4], -1) : nullptr;
+    if (qs < 0 || t < 1 || (rows && (cu == nullptr || cu->numel() < 2))) Py_RETURN_NONE;
+    const int64_t b = rows ? cu->numel() - 1 : t;
+    const at::Tensor *table = index_tensor(a[2], -1), *lens = index_tensor(a[3], b);
+    if (lens == nullptr || table == nullptr || table->dim() != 2 || table->size(0) != b || table->size(1) < 1) Py_RETURN_NONE;
+    const int64_t width = table->size(1);
+    const int64_t max_q = PyLong_AsLongLong(a[5]), page = PyLong_AsLongLong(a[7]), max_kv = PyLong_AsLongLong(a[9]);
+    const int64_t splits = PyLong_AsLongLong(a[10]);
+    const double scale = PyFloat_AsDouble(a[6]);
+    void *stream = PyLong_AsVoidPtr(a[11]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    const at::Tensor *scale_tensor = pool.scales != nullptr ? gpu_tensor(a[8]) : nullptr;
+    if (!here(q, pool.t, table, lens, cu, scale_tensor) || !(scale > 0.0) || page < 1 || page > 65536 || pool.slots % page != 0 ||
+        max_q < 0 || max_q > INT32_MAX || t > INT32_MAX || b > 65535 || hq > INT32_MAX || pool.hkv > INT32_MAX ||
+        hq % pool.hkv != 0 || width > INT32_MAX || splits < 0 || splits > 65535) {
+      Py_RETURN_NONE;
+    }
+    const int32_t b32 = (int32_t)b, hq32 = (int32_t)hq, hkv = (int32_t)pool.hkv, d32 = (int32_t)d, page32 = (int32_t)page;
+    const int64_t pages = pool.slots / page;
+    int32_t slices = 1, chunks = 0;
+    size_t room_bytes = 0, plan_bytes = 0;
+    if (rows) {
+      if (max_kv > 0 && t * hq <= 128 * 512) {
+        slices = litekv_paged_prefill_key_slices(b32, hq32, hkv, d32, (int32_t)max_q, max_kv);
+      }
+      room_bytes = slices > 1 ? litekv_paged_prefill_split_workspace_bytes(t, hq32, d32, slices) : 0;
+    } else if (splits > 0) {
+      room_bytes = litekv_paged_decode_workspace_bytes(b32, hq32, 128, (int32_t)splits);
+    } else {
+      chunks = litekv_paged_decode_balanced_chunks(hkv);
+      plan_bytes = litekv_decode_plan_bytes_paged(b32, (int32_t)width, hkv, chunks, page32);
+      room_bytes = litekv_paged_decode_balanced_workspace_bytes(b32, hq32, 128, chunks);
+      if (plan_bytes == 0) Py_RETURN_NONE;
+    }
+    at::Tensor out = at::empty({t, hq, d}, q->options()), room, plan;
+    if (room_bytes > 0) room = at::empty({(int64_t)(room_bytes / sizeof(float))}, q->options().dtype(at::kFloat));
+    if (plan_bytes > 0) plan = at::empty({(int64_t)((plan_bytes + 3) / 4)}, q->options().dtype(at::kInt));
+    const void *qp = address(q), *pp = address(pool.t);
+    const int32_t *tp = static_cast<const int32_t *>(address(table)), *lp = static_cast<const int32_t *>(address(lens));
+    const int32_t *cup = static_cast<const int32_t *>(address(cu));
+    const float *scales = static_cast<const float *>(pool.scales);
+    void *op = address(&out), *wp = room_bytes > 0 ? room.data_ptr() : nullptr, *plan_at = plan_bytes > 0 ? plan.data_ptr() : nullptr;
+    PyObject *result = THPVariable_Wrap(std::move(out));  // (before the launch: it may throw)
+    const int rc = unlocked([&]() -> int {
+      const float sc = (float)scale;
+      const int32_t w = (int32_t)width;
+      if (rows) {
+        return litekv_paged_cross_attention(qp, qs, pp, scales, pool_format(pool.format), tp, w, cup, lp, op, hq * d, b32, hq32, hkv,
+                                            d32, page32, pages, (int32_t)max_q, max_kv, t, slices > 1 ? slices : 1, wp, room_bytes, sc,
+                                            stream);
+      }
+      if (splits > 0) {
+        if (pool.format == kF16) {
+          return litekv_paged_decode(qp, qs, pp, tp, w, lp, op, wp, room_bytes, b32, hq32, hkv, d32, page32, pages, (int32_t)splits, 1,
+                                     sc, stream);
+        }
+        const auto call = pool.format == kInt8 ? litekv_paged_decode_int8 : litekv_paged_decode_fp8;
+        return call(qp, qs, pp, scales, tp, w, lp, op, wp, room_bytes, b32, hq32, hkv, d32, page32, pages, (int32_t)splits, 1, sc, stream);
+      }
+      const int made = litekv_decode_plan(tp, w, lp, b32, hkv, page32, pages, chunks, plan_at, plan_bytes, stream);
+      if (made != 0) return made;
+      void *kv = const_cast<void *>(pp);
+      if (pool.format == kF16) {
+        return litekv_paged_decode_balanced(qp, qs, kv, lp, plan_at, plan_bytes, nullptr, nullptr, 0, 0, op, wp, room_bytes, b32, hq32,
+                                            hkv, d32, page32, pages, w, chunks, sc, stream);
+      }
+      const auto call = pool.format == kInt8 ? litekv_paged_decode_balanced_int8 : litekv_paged_decode_balanced_fp8;
+      return call(qp, qs, kv, scales, lp, plan_at, plan_bytes, nullptr, nullptr, 0, 0, op, wp, room_bytes, b32, hq32, hkv, d32, page32,
+                  pages, w, chunks, sc, stream);
+    });
+    if (rc == 0) return result;
+    Py_DECREF(result);
+    return PyLong_FromLong(rc);
+  } catch (...) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+}
+
+// (logits, uniforms, temperature, top_k, top_p, min_p, whether the logprobs too, stream), the filters each a tensor or None
+// -> (tokens, logprobs or None), or the library's status if that is not 0, or None
+PyObject *sample_tokens(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  if (n != 8) Py_RETURN_NONE;
+  try {
+    const at::Tensor *x = gpu_tensor(a[0]);
+    if (x == nullptr || x->dim() != 2) Py_RETURN_NONE;
+    const int64_t b = x->size(0), vocab = x->size(1);
+    const auto type = x->scalar_type();
+    const int32_t kind = type == at::kHalf ? 0 : type == at::kBFloat16 ? 1 : type == at::kFloat ? 2 : -1;
+    if (kind < 0 || b < 1 || b > 65535 || vocab < 1 || vocab > INT32_MAX || (vocab > 1 && x->stride(1) != 1)) Py_RETURN_NONE;
+    const at::Tensor *per_row[5] = {};
+    for (int i = 0; i < 5; ++i) {
+      if (i > 0 && a[1 + i] == Py_None) continue;
+      const at::Tensor *y = gpu_tensor(a[1 + i]);
+      if (y == nullptr || y->scalar_type() != (i == 2 ? at::kInt : at::kFloat) || y->numel() != b || !y->is_contiguous()) Py_RETURN_NONE;
+      per_row[i] = y;
+    }
+    const int logprobs_too = PyObject_IsTrue(a[6]);
+    void *stream = PyLong_AsVoidPtr(a[7]);
+    if (PyErr_Occurred() || logprobs_too < 0) {
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    if (!here(x, per_row[0], per_row[1], per_row[2], per_row[3], per_row[4])) Py_RETURN_NONE;
+    const size_t bytes = litekv_sample_tokens_workspace_bytes(kind, (int32_t)b, (int32_t)vocab);
+    if (bytes == 0) Py_RETURN_NONE;
+    at::Tensor tokens = at::empty({b}, x->options().dtype(at::kLong));
+    at::Tensor room = at::empty({(int64_t)((bytes + 7) / 8)}, x->options().dtype(at::kLong)), logprobs;
+    if (logprobs_too) logprobs = at::empty({b}, x->options().dtype(at::kFloat));
+    const void *xp = address(x);
+    const float *up = static_cast<const float *>(address(per_row[0])), *tp = static_cast<const float *>(address(per_row[1]));
+    const float *pp = static_cast<const float *>(address(per_row[3])), *mp = static_cast<const float *>(address(per_row[4]));
+    const int32_t *kp = static_cast<const int32_t *>(address(per_row[2]));
+    int64_t *out = tokens.data_ptr<int64_t>();
+    float *lp = logprobs_too ? logprobs.data_ptr<float>() : nullptr;
+    void *wp = room.data_ptr();
+    const int64_t stride = b > 1 ? x->stride(0) : vocab;
+    PyObject *first = THPVariable_Wrap(std::move(tokens));  // (before the launch: they may throw)
+    PyObject *second = logprobs_too ? THPVariable_Wrap(std::move(logprobs)) : Py_NewRef(Py_None);
+    const int rc = unlocked([&] {
+      return litekv_sample_tokens(xp, kind, stride, up, tp, kp, pp, mp, out, lp, (int32_t)b, (int32_t)vocab, wp, bytes, stream);
+    });
+    if (rc == 0) return Py_BuildValue("(NN)", first, second);
+    Py_DECREF(first);
+    Py_DECREF(second);
+    return PyLong_FromLong(rc);
+  } catch (...) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+}
+
 PyMethodDef methods[] = {
     {"qk_norm_rope_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(qk_norm_rope_append)), METH_FASTCALL, nullptr},
     {"paged_prefill", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(paged_prefill)), METH_FASTCALL, nullptr},
     {"paged_decode_int4", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(paged_decode_int4)), METH_FASTCALL, nullptr},
     {"kv_append_quantised", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(kv_append_quantised)), METH_FASTCALL, nullptr},
     {"page_dequant", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(page_dequant)), METH_FASTCALL, nullptr},
+    {"qk_norm_mrope_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(qk_norm_mrope_append)), METH_FASTCALL, nullptr},
+    {"paged_cross_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(paged_cross_attention)), METH_FASTCALL, nullptr},
+    {"sample_tokens", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(sample_tokens)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1205,6 +1205,16 @@ def qk_norm_mrope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot
     ``positions[a, t]``, a the pair's axis (see ``axis_of_pair``). ``positions`` [A, T] is int32 or int64 with any strides (one
     row expanded to all axes: text); a position outside the tables reads the nearest row. Any pool format; fp32 from the
     inputs to the one rounding of q and to the pool's format. q [T, Hq, D] is updated in place and returned."""
+    if q.is_cuda:
+        width = kv_pool.shape[-1] if not is_int4_pool(kv_pool) else _INT4_HEAD_DIMS[kv_pool.shape[2]]
+        done = _lib.calls().qk_norm_mrope_append(q, k, v, slot_mapping, kv_pool, positions,
+                                                 axis_of_pair(tuple(sections), width, bool(interleaved)), cos_table, sin_table,
+                                                 q_norm_weight, k_norm_weight, rms_eps, kv_scales, len(sections), _stream())
+        if done is not None:
+            if done is not True:        # a status: q may have been written all the same, so never a second time
+                _lib.check(done)
+            return q
+    # (not a plain call)
     _dev_half("q", q), _dev_half("k", k), _dev_half("v", v)
     slots, hkv, d, _, _ = pool_geometry(kv_pool, 1)
     if is_int4_pool(kv_pool):
@@ -1259,6 +1269,16 @@ def paged_cross_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: t
     ``max_q_len``: the most rows of a sequence. ``max_kv_len``: the most keys, as the host knows it; launches of few rows
     are then cut along the keys as in ``paged_prefill``, and nothing but speed goes by it. Rows behind the last sequence are left as
     they are. ``key_slices`` and ``workspace`` as there."""
+    if q.is_cuda and out is None and key_slices is None and workspace is None and q.dim() == 3 and q.shape[2] in (64, 128):
+        splits = 0 if cu_q_lens is not None else _cross_splits(q, kv_pool, block_table, page_size, max_kv_len)
+        done = _lib.calls().paged_cross_attention(q, kv_pool, block_table, kv_lens, cu_q_lens, max_q_len,
+                                                  1.0 / math.sqrt(q.shape[2]) if softmax_scale is None else softmax_scale, page_size,
+                                                  kv_scales, max_kv_len or 0, splits, _stream())
+        if done is not None:
+            if type(done) is int:
+                _lib.check(done)
+            return done
+    # (not a plain call)
     _dev_half("q", q)
     int4, fp8 = is_int4_pool(kv_pool), is_quantised_pool(kv_pool)
     if q.dim() != 3:
@@ -1317,19 +1337,28 @@ def _cross_rows(q, kv_pool, block_table, kv_lens, softmax_scale, out, page_size,
     b, hq, d = q.shape
     if b == 0:
         return out
-    width = int(block_table.shape[1])
-    pages = width if max_kv_len is None else max(1, min(width, -(-int(max_kv_len) // page_size)))
     if is_int4_pool(kv_pool):
+        width = int(block_table.shape[1])
+        pages = width if max_kv_len is None else max(1, min(width, -(-int(max_kv_len) // page_size)))
         splits, least = int4_decode_splits(b, hkv, pages, page_size=page_size)
         return paged_decode(q, kv_pool, block_table, kv_lens, softmax_scale, max_splits=splits, min_pages_per_split=least, out=out,
                             page_size=page_size)
-    splits = _cross_schedule(b, hkv, pages, 2 * hkv * d * kv_pool.element_size(), page_size, hq // hkv, d)
+    splits = _cross_splits(q, kv_pool, block_table, page_size, max_kv_len)
     if splits > 0:
         return paged_decode(q, kv_pool, block_table, kv_lens, softmax_scale, max_splits=splits, min_pages_per_split=1, out=out,
                             page_size=page_size, kv_scales=kv_scales)
     plan = DecodePlan(block_table, kv_lens, hq, hkv, n_pages, page_size=page_size, kv_dtype=kv_pool.dtype,
                       token_bytes=2 * hkv * d * kv_pool.element_size())
     return decode_step(q, kv_pool, plan, None, None, softmax_scale, out, kv_scales)
+
+
+def _cross_splits(q, kv_pool, block_table, page_size: int, max_kv_len: Optional[int]) -> int:
+    """The schedule (``decode_schedule``) of one row a sequence, as if each had ``max_kv_len`` keys."""
+    if block_table.dim() != 2 or kv_pool.dim() != 3 or page_size < 1 or is_int4_pool(kv_pool):
+        return 0
+    (b, hq, d), hkv, width = q.shape, kv_pool.shape[1] // 2, block_table.shape[1]
+    pages = width if max_kv_len is None else max(1, min(width, -(-int(max_kv_len) // page_size)))
+    return _cross_schedule(b, max(1, hkv), pages, 2 * hkv * d * kv_pool.element_size(), page_size, max(1, hq // max(1, hkv)), d)
 
 
 @functools.lru_cache(maxsize=256)
@@ -1350,6 +1379,13 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Opt
     below 1, top_p of 1 or more and min_p of 0 or less are off. Temperature 0 (or less) takes the first largest logit.
     Tokens further than 40 * temperature below the largest are never drawn, nor are those of -inf or NaN; a row without any
     other gives token -1. With ``return_logprobs`` (tokens, logprobs): the token's logarithm of probability among the kept."""
+    if logits.is_cuda:
+        done = _lib.calls().sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p, return_logprobs, _stream())
+        if done is not None:
+            if type(done) is int:
+                _lib.check(done)
+            return done if return_logprobs else done[0]
+    # (not a plain call)
     if not logits.is_cuda or logits.dtype not in _LOGITS_TYPES:
         raise ValueError(f"logits must be float16, bfloat16 or float32 on the GPU, not {logits.dtype} on {logits.device}")
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
