@@ -8,6 +8,9 @@
 // From the fp16 inputs to the one rounding of q and to the pool's format everything is fp32, each product and sum rounded by
 // itself (no contraction), and the sum of squares fp64, where the order of its additions does not show: codes next to a
 // border are then the same however a row's lanes are laid out.
+//
+// Bound by memory: 10366 tokens of 64 + 16 heads of 128 over an fp16 pool in 82 to 84 us, 5.1 TB/s of what is read and written once,
+// which is what a large copy reaches; one token in 2.4 us, which is a launch.
 #include <type_traits>
 
 #include "common.h"
@@ -33,8 +36,9 @@ struct MropeArgs {
   int32_t num_q_heads, num_kv_heads, num_axes;
   int32_t wide_positions;     // int64
   int32_t mixed;              // some run of 8 pairs has several axes
+  int32_t each;               // rows of a lane
   float eps;
-  uint32_t axes[8];           // two bits a pair
+  uint64_t axes0, axes1, axes2, axes3;   // two bits a pair (by name: of an array indexed by the lane a copy is kept in memory)
 };
 
 // Sums and neighbours over the L lanes of a row (kv_int4.h has 8 and 16).
@@ -83,35 +87,54 @@ __device__ __forceinline__ uint2_t floats_to_codes(const float (&x)[8], float sc
   }
 }
 
-// Rows [0, num_q_heads) of a token are q's, the next num_kv_heads K's, then V's. Grid: x = token, y = run of ROWS * 256 / L rows; a
-// lane has ROWS of them, 256 / L apart.
-template <int KV, int L, int ROWS>
+// A lane's 8 elements of row r of a token (see below); the three pointers each count from row 0.
+template <int D>
+__device__ __forceinline__ half8_t head_row(int r, int kv0, int v0, const half_t *q, const half_t *k, const half_t *v) {
+  uint64_t at = (uint64_t)v;       // (numbers: of a choice among pointers the compiler keeps a table in memory)
+  at = r < v0 ? (uint64_t)k : at;
+  at = r < kv0 ? (uint64_t)q : at;
+  at += (uint64_t)((int64_t)r * D * 2);
+  return *(const __attribute__((address_space(1))) half8_t *)at;
+}
+
+// Rows [0, num_q_heads) of a token are q's, the next num_kv_heads K's, then V's. Grid: x = token, y = run of each * 256 / L rows; a
+// lane has `each` of them, 256 / L apart, the next one's load ahead of a row's work.
+template <int KV, int L>
 __global__ __launch_bounds__(256) void qk_norm_mrope_append_kernel(const MropeArgs a) {
 #pragma clang fp contract(off)
   constexpr int kDim = 8 * L, kApart = 256 / L;
   const int l = threadIdx.x & (L - 1);
   const int64_t token = blockIdx.x;
-  const int first = (int)blockIdx.y * (ROWS * kApart) + (int)(threadIdx.x / L);
   const int kv0 = a.num_q_heads, v0 = kv0 + a.num_kv_heads, rows = v0 + a.num_kv_heads;
-  half8_t x[ROWS];
-#pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int r = first + i * kApart < rows ? first + i * kApart : rows - 1;       // (repeats the last; nothing is stored)
-    const half_t *src = r < kv0  ? a.q + token * a.q_stride + (int64_t)r * kDim
-                        : r < v0 ? a.k + token * a.k_stride + (int64_t)(r - kv0) * kDim
-                                 : a.v + token * a.v_stride + (int64_t)(r - v0) * kDim;
-    x[i] = *(const half8_t *)(src + 8 * l);
-  }
+  int r = (int)blockIdx.y * (a.each * kApart) + (int)(threadIdx.x / L);
+  if (r >= rows) return;                                     // whole rows of lanes leave together
+  const int end = r + a.each * kApart < rows ? r + a.each * kApart : rows;
+  const half_t *q_row = a.q + token * a.q_stride + 8 * l, *k_row = a.k + token * a.k_stride + 8 * l - (int64_t)kv0 * kDim,
+               *v_row = a.v + token * a.v_stride + 8 * l - (int64_t)v0 * kDim;
+  half8_t next = head_row<kDim>(r, kv0, v0, q_row, k_row, v_row);
   const int64_t slot = a.slot_mapping[token];
+  // (what else a row needs is here, or comes with it: a load between a row and the next would be waited for with both)
+  half8_t q_weight = half8_t{0, 0, 0, 0, 0, 0, 0, 0}, k_weight = q_weight;
+  const bool norm = a.q_weight != nullptr;
+  if (norm) {
+    q_weight = *(const half8_t *)(a.q_weight + 8 * l);
+    k_weight = *(const half8_t *)(a.k_weight + 8 * l);
+  }
+  constexpr bool kScaled = KV == kKvFp8 || KV == kKvInt8;
+  float next_scale = 1.0f;
+  if constexpr (kScaled) next_scale = a.scales[r < kv0 ? 0 : r - kv0];
 
   // the entries of this lane's pairs
   const int run = l & (L / 2 - 1);
-  uint32_t mine = 0;                       // the axes of its eight pairs
-#pragma unroll
-  for (int i = 0; i < L / 2; ++i) mine = run == i ? (a.axes[i >> 1] >> (16 * (i & 1))) & 0xffffu : mine;
+  uint64_t near = run & 4 ? a.axes1 : a.axes0;
+  if constexpr (L == 32) near = run & 8 ? (run & 4 ? a.axes3 : a.axes2) : near;
+  const uint32_t mine = (uint32_t)(near >> (16 * (run & 3))) & 0xffffu;       // the axes of its eight pairs
+  // Where an axis' rows begin in the tables. (Both halves of a position are asked for at once, whatever its type.)
   auto row_of = [&](int axis) -> int64_t {
-    const int64_t at = axis * a.axis_stride + token * a.token_stride;
-    const int64_t p = a.wide_positions ? static_cast<const int64_t *>(a.positions)[at] : static_cast<const int32_t *>(a.positions)[at];
+    const int32_t *at = reinterpret_cast<const int32_t *>(static_cast<const char *>(a.positions) +
+                                                          (axis * a.axis_stride + token * a.token_stride) * (a.wide_positions ? 8 : 4));
+    const int32_t low = at[0], high = at[a.wide_positions];
+    const int64_t p = a.wide_positions ? (int64_t)high << 32 | (uint32_t)low : low;
     return (p < 0 ? 0 : p < a.table_rows ? p : a.table_rows - 1) * a.table_stride + 8 * run;
   };
   float c[8], s[8];
@@ -124,17 +147,13 @@ __global__ __launch_bounds__(256) void qk_norm_mrope_append_kernel(const MropeAr
       s[i] = (float)ss[i];
     }
   } else {
+    // (axes that there are not repeat the last)
     half8_t cc[kMaxAxes], ss[kMaxAxes];
 #pragma unroll
     for (int axis = 0; axis < kMaxAxes; ++axis) {
-      if (axis < a.num_axes) {
-        const int64_t at = row_of(axis);
-        cc[axis] = *(const half8_t *)(a.cos_table + at);
-        ss[axis] = *(const half8_t *)(a.sin_table + at);
-      } else {
-        cc[axis] = cc[0];
-        ss[axis] = ss[0];
-      }
+      const int64_t at = row_of(axis < a.num_axes ? axis : a.num_axes - 1);
+      cc[axis] = *(const half8_t *)(a.cos_table + at);
+      ss[axis] = *(const half8_t *)(a.sin_table + at);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -153,17 +172,19 @@ __global__ __launch_bounds__(256) void qk_norm_mrope_append_kernel(const MropeAr
 #pragma unroll
   for (int i = 0; i < 8; ++i) s[i] = l < L / 2 ? -s[i] : s[i];
 
-#pragma unroll
-  for (int n = 0; n < ROWS; ++n) {
-    const int r = first + n * kApart;
-    if (r >= rows) return;                                   // whole rows of lanes leave together
+  const bool there = slot >= 0 && slot < a.num_slots;
+#pragma unroll 1
+  for (; r < end; r += kApart) {
+    const half8_t x = next;
+    const float scale = next_scale;
+    if constexpr (kScaled) next_scale = a.scales[r + kApart < kv0 || r + kApart >= rows ? 0 : r + kApart - kv0];
+    if (r + kApart < end) next = head_row<kDim>(r + kApart, kv0, v0, q_row, k_row, v_row);
     const bool is_q = r < kv0, is_v = r >= v0;
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = (float)x[n][i];
-    const half_t *weight = is_q ? a.q_weight : a.k_weight;
-    if (weight != nullptr && !is_v) {
-      const half8_t w = *(const half8_t *)(weight + 8 * l);
+    for (int i = 0; i < 8; ++i) y[i] = (float)x[i];
+    if (norm && !is_v) {
+      const half8_t w = is_q ? q_weight : k_weight;
       double sum = 0.0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum = __builtin_fma((double)y[i], (double)y[i], sum);
@@ -196,7 +217,6 @@ __global__ __launch_bounds__(256) void qk_norm_mrope_append_kernel(const MropeAr
       *(half8_t *)(a.q + token * a.q_stride + (int64_t)r * kDim + 8 * l) = o;
       continue;
     }
-    const bool there = slot >= 0 && slot < a.num_slots;
     const int head = r - kv0;                                // as in the pool: K heads, then V heads
     if constexpr (KV == kKvInt4) {
       const Int4Row row = int4_row<L>(y);
@@ -210,7 +230,7 @@ __global__ __launch_bounds__(256) void qk_norm_mrope_append_kernel(const MropeAr
         for (int i = 0; i < 8; ++i) o[i] = (half_t)y[i];
         *(half8_t *)(static_cast<half_t *>(a.pool) + at) = o;
       } else {
-        *(uint2_t *)(static_cast<uint8_t *>(a.pool) + at) = floats_to_codes<KV>(y, a.scales[head]);
+        *(uint2_t *)(static_cast<uint8_t *>(a.pool) + at) = floats_to_codes<KV>(y, scale);
       }
     }
   }
@@ -241,7 +261,7 @@ extern "C" int litekv_qk_norm_mrope_append(void *q, int64_t q_token_stride, cons
   MropeArgs a{};
   for (int i = 0; i < head_dim / 2; ++i) {
     LITEKV_REQUIRE(axis_of_pair[i] < num_axes, "%s: pair %d has axis %d of %d", what, i, axis_of_pair[i], num_axes);
-    a.axes[i >> 4] |= (uint32_t)axis_of_pair[i] << (2 * (i & 15));
+    (i < 32 ? a.axes0 : i < 64 ? a.axes1 : i < 96 ? a.axes2 : a.axes3) |= (uint64_t)axis_of_pair[i] << (2 * (i & 31));
     a.mixed |= axis_of_pair[i] != axis_of_pair[i & ~7];
   }
   if (num_tokens == 0) {
@@ -292,19 +312,24 @@ extern "C" int litekv_qk_norm_mrope_append(void *q, int64_t q_token_stride, cons
   a.wide_positions = positions_int64 != 0;
   a.eps = rms_eps;
   const int rows = num_q_heads + 2 * num_kv_heads, apart = 256 / (head_dim / 8);
-  auto launch = [&](auto kernel, int each) {
-    const unsigned y = (unsigned)((rows + each * apart - 1) / (each * apart));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)num_tokens, y), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  // All rows of a token to a workgroup, the entries of its pairs gathered once for all, where that leaves every compute unit one; a
+  // pass of rows to one where there are fewer tokens. us, all rows / a pass, 64 / 8 heads of 128: 64 tokens 5.6 / 4.1, 256 6.2 / 6.1,
+  // 512 8.5 / 10.1, 2048 18.1 / 28.3, 8192 67 / 114; 32 / 8 heads of 64: 64 tokens 4.0 / 3.6, 256 4.2 / 4.1, 2048 11.0 / 13.2.
+  const int passes = (rows + apart - 1) / apart;
+  a.each = num_tokens >= 256 ? passes : 1;
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)num_tokens, (unsigned)((passes + a.each - 1) / a.each)), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), a);
   };
   LITEKV_REQUIRE((rows + apart - 1) / apart <= 65535, "%s: too many heads", what);
   auto by_format = [&](auto lanes) {
     constexpr int L = decltype(lanes)::value;
     if constexpr (L == 8 || L == 16) {
-      if (pool_format == kKvInt4) return launch(qk_norm_mrope_append_kernel<kKvInt4, L, 1>, 1);
+      if (pool_format == kKvInt4) return launch(qk_norm_mrope_append_kernel<kKvInt4, L>);
     }
-    if (pool_format == kKvFp8) return launch(qk_norm_mrope_append_kernel<kKvFp8, L, 1>, 1);
-    if (pool_format == kKvInt8) return launch(qk_norm_mrope_append_kernel<kKvInt8, L, 1>, 1);
-    launch(qk_norm_mrope_append_kernel<kKvF16, L, 1>, 1);
+    if (pool_format == kKvFp8) return launch(qk_norm_mrope_append_kernel<kKvFp8, L>);
+    if (pool_format == kKvInt8) return launch(qk_norm_mrope_append_kernel<kKvInt8, L>);
+    launch(qk_norm_mrope_append_kernel<kKvF16, L>);
   };
   switch (head_dim) {
     case 32: by_format(std::integral_constant<int, 4>{}); break;
