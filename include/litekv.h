@@ -911,11 +911,15 @@ int litekv_qk_norm_mrope_append(void *q, int64_t q_token_stride, const void *k,
  * and softmax_scale (above 0) as in litekv_paged_prefill; head dims 64 and 128. max_q_len is the most rows of a
  * sequence and has to be true; max_kv_len the most keys as the host knows it, 0 if it does
  * not, and only a choice of form goes by it. key_slices above 1 cuts the keys, for launches of
- * few rows: litekv_paged_prefill_key_slices says into how many, and
+ * few rows: litekv_paged_cross_key_slices says into how many, and
  * litekv_paged_prefill_split_workspace_bytes what workspace that takes (num_tokens rows,
  * those behind the last sequence among them). One row a sequence: litekv_paged_decode and its
  * like, with kv_lens for seq_lens, stream the keys without a tile.
  */
+int32_t litekv_paged_cross_key_slices(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                      int32_t head_dim, int32_t max_q_len, int64_t max_kv_len,
+                                      int64_t num_tokens);
+
 int litekv_paged_cross_attention(const void *q, int64_t q_token_stride, const void *kv_pool,
                                  const float *kv_scales, int32_t pool_format,
                                  const int32_t *block_table, int32_t block_table_stride,

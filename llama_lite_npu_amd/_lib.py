@@ -270,6 +270,7 @@ SIGNATURES = {
          c_int64, c_int64, c_void_p, c_int32, c_int64, c_int64, c_int32, c_char_p, c_void_p, c_void_p, c_void_p,
          c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_float, c_void_p],
     ),
+    "litekv_paged_cross_key_slices": (c_int32, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64]),
     "litekv_paged_cross_attention": (
         c_int32,
         [c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p,

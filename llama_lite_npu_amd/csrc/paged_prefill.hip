@@ -1,5 +1,8 @@
 // Host side of the varlen causal prefill and of the shared-prefix pass of a decode step: argument
 // checks, launch shapes and the C ABI. The kernel is in prefill_tile.h.
+#include <algorithm>
+#include <cmath>
+
 #include "prefill_tile.h"
 
 namespace litekv {
@@ -522,6 +525,31 @@ const PrefillBuild &hd256_prefill() {
 }  // namespace litekv
 
 #if LITEKV_CROSS && LITEKV_HD == 128
+// Slices of the keys for a launch of few rows over an encoder's states: as many as balance the chain of tiles that a workgroup walks
+// (0.8 us a tile, 0.4 of 64-wide heads) against the partial rows written and read back (6 MB/us), up to four workgroups a compute unit, since lengths
+// are seldom even; none where that comes to fewer than four, or a launch that has a workgroup on every other compute unit
+// walks fewer than 48 tiles. us, uncut / by this rule / in the best of 1, 2, 3, 4, 6 and 8: 32 sequences of 5 rows over up to 6400 states,
+// 64 / 8 heads 124 / 112 / 112 (int8 111 / 83 / 83), 16 / 8 125 / 101 / 101 (112 / 81 / 79); 12 of up to 9 over up to 3000 41 / 25 / 24,
+// 32 / 8 heads of 64, int8, 38 / 18 / 18; 4 of 40 over 1000, 16 / 8, 15.8 / 12.9 / 12.3; 2 of 300 over 6400, 32 / 4, 82 / 58 / 58; 8 of 64 over
+// 1600, 64 / 8, 28 / 28 / 28 (in four slices 37). Over 88 shapes (1 to 64 sequences of 2 to 300 rows over 500 to 6400 states, the
+// layouts 64 / 8, 16 / 8, 32 / 4 and 32 / 8 of 64, fp16 and int8) it takes 1.04 times as long as the best count, uncut launches 1.49.
+extern "C" int32_t litekv_paged_cross_key_slices(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                                 int32_t max_q_len, int64_t max_kv_len, int64_t num_tokens) {
+  using namespace litekv;
+  if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || max_q_len <= 0 ||
+      max_kv_len <= 0 || num_tokens <= 0 || num_q_heads / num_kv_heads > kMaxGroup || (head_dim != 64 && head_dim != 128)) {
+    return 1;
+  }
+  const PrefillShape s = prefill_shape(num_q_heads / num_kv_heads, max_q_len);
+  const int64_t wgs = (int64_t)num_kv_heads * s.head_splits * s.row_blocks * batch, cus = device_cus();
+  const int64_t tiles = (max_kv_len + kKvTile - 1) / kKvTile;
+  if (wgs > cus || (2 * wgs >= cus && tiles < 48)) return 1;
+  const double chain_us = (head_dim == 64 ? 0.4 : 0.8) * (double)tiles;
+  const double partial_us = (double)num_tokens * num_q_heads * (head_dim + 1) * 2.0 * sizeof(float) / 6.0e6;
+  const int64_t n = std::min<int64_t>(std::min<int64_t>(kMaxPrefillKeySlices, 4 * cus / wgs), (int64_t)(std::sqrt(chain_us / partial_us) + 0.5));
+  return n < 4 ? 1 : (int32_t)n;
+}
+
 extern "C" int litekv_paged_cross_attention(const void *q, int64_t q_token_stride, const void *kv_pool,
                                             const float *kv_scales, int32_t pool_format,
                                             const int32_t *block_table, int32_t block_table_stride,

@@ -540,9 +540,7 @@ PyObject *paged_cross_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     int32_t slices = 1, chunks = 0;
     size_t room_bytes = 0, plan_bytes = 0;
     if (rows) {
-      if (max_kv > 0 && t * hq <= 128 * 512) {
-        slices = litekv_paged_prefill_key_slices(b32, hq32, hkv, d32, (int32_t)max_q, max_kv);
-      }
+      slices = litekv_paged_cross_key_slices(b32, hq32, hkv, d32, (int32_t)max_q, max_kv, t);
       room_bytes = slices > 1 ? litekv_paged_prefill_split_workspace_bytes(t, hq32, d32, slices) : 0;
     } else if (splits > 0) {
       room_bytes = litekv_paged_decode_workspace_bytes(b32, hq32, 128, (int32_t)splits);

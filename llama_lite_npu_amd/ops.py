@@ -1316,8 +1316,7 @@ def paged_cross_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: t
     lib = _lib.load()
     most = 0 if max_kv_len is None else int(max_kv_len)
     if key_slices is None:
-        # (as in paged_prefill)
-        key_slices = int(lib.litekv_paged_prefill_key_slices(b, hq, hkv, d, int(max_q_len), most)) if most > 0 and 0 < t * hq <= 128 * 512 else 1
+        key_slices = int(lib.litekv_paged_cross_key_slices(b, hq, hkv, d, int(max_q_len), most, t))
     key_slices = max(1, int(key_slices))
     if key_slices > 1:
         need = paged_prefill_workspace_floats(t, hq, d, key_slices)
