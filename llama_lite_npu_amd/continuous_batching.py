@@ -48,7 +48,8 @@ class BatchRequest:
     def __init__(self, request_id: str, prompt_tokens: Sequence[int], max_new_tokens: int,
                  temperature: float, top_p: float, control_id: Optional[int] = None, top_k: int = 0,
                  min_p: float = 0.0, seed: Optional[int] = None) -> None:
-        """``top_k`` (0: off), ``min_p`` (0: off) and ``seed`` are beside the reference's: see ``draw_tokens``."""
+        """``top_k`` (0: off), ``min_p`` (0: off) and ``seed`` are beside the reference's: see ``draw_tokens``. A sampler of the
+        backend's owner is not given them, and sharded logits refuse them."""
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens must be positive")
         self.top_k, self.min_p, self.seed = int(top_k), float(min_p), seed
@@ -109,16 +110,19 @@ def sample_next_token(logits: torch.Tensor, temperature: Sequence[float], top_p:
     return torch.where(is_greedy, greedy, drawn)
 
 
-def draw_tokens(logits: torch.Tensor, requests: Sequence) -> torch.Tensor:
+def draw_tokens(logits: torch.Tensor, requests: Sequence, generated: Optional[Sequence[int]] = None) -> torch.Tensor:
     """One token per row of ``logits`` [n, vocab] (or [n, seq, vocab]: last position), by each request's temperature, top_k, top_p
     and min_p (``ops.sample_tokens``; one small upload, two launches). The uniform number of a request with a ``seed`` depends
-    on that and on the number of tokens it has generated, so its answer is the same in any batch; the others' come
-    from Python's generator."""
+    on that and on the number of tokens it has generated (``generated``, or what its list says), in any batch and after any
+    preemption; the others' come from Python's generator."""
     rows = logits[:, -1, :] if logits.dim() == 3 else logits
     numbers = []
-    for r in requests:
+    for i, r in enumerate(requests):
         seed = getattr(r, "seed", None)
-        source = random if seed is None else random.Random(f"{seed}/{len(r.generated_token_ids)}")
+        if seed is None:
+            source = random
+        else:
+            source = random.Random(f"{seed}/{len(r.generated_token_ids) if generated is None else int(generated[i])}")
         numbers.append(int(source.random() * 2 ** 24) / 2 ** 24)          # a float32 below 1
     # top_k as the bits of an int32 in a float32's place
     top_k = [min(int(getattr(r, "top_k", 0)), 2 ** 31 - 1) for r in requests]
@@ -199,11 +203,16 @@ class ContinuousBatchModelBackend:
     def _tensor(self, values) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.long, device=self.executor.device)
 
-    def _sample(self, logits, requests: Sequence[BatchRequest]) -> torch.Tensor:
-        if self._sampler is sample_next_token and not getattr(self.executor, "logits_are_sharded", False) and any(
+    def _sample(self, logits, requests: Sequence[BatchRequest], decoding: bool = False) -> torch.Tensor:
+        if self._sampler is sample_next_token and any(
                 getattr(r, "top_k", 0) > 0 or getattr(r, "min_p", 0.0) > 0.0 or getattr(r, "seed", None) is not None
                 for r in requests):
-            return draw_tokens(logits, requests)
+            if getattr(self.executor, "logits_are_sharded", False):
+                raise ValueError("top_k, min_p and seed take whole rows of logits, not a vocabulary's shards")
+            generated = None
+            if decoding:            # (a request's list may lag behind, or stay empty where tokens stay on the device)
+                generated = [self._positions[int(r.model_request_id)] + 1 - len(r.prompt_tokens) for r in requests]
+            return draw_tokens(logits, requests, generated)
         return self._sampler(logits, temperature=[r.temperature for r in requests],
                              top_p=[r.top_p for r in requests],
                              vocab_parallel=bool(getattr(self.executor, "logits_are_sharded", False)))
@@ -580,7 +589,7 @@ class ContinuousBatchModelBackend:
             ex.activate_paged_decode_batch(ids)
             position_ids = self._tensor([[self._positions[i]] for i in ids])
             logits = ex.forward(input_ids, position_ids)
-        sampled = self._sample(logits, requests)
+        sampled = self._sample(logits, requests, decoding=True)
         self._remember(requests, sampled)
         self._step_ids, self._step_tokens = ids, sampled
         for req_idx in ids:

@@ -111,7 +111,7 @@ def test_tensors_on_the_cpu_are_refused(call):
 def test_requests_carry_their_filters_and_plain_ones_go_the_old_way(monkeypatch):
     """A batch without top_k, min_p or a seed is sampled as before; one request with any of them sends it to the kernel."""
     seen = []
-    monkeypatch.setattr(continuous_batching, "draw_tokens", lambda logits, requests: seen.append(len(requests)) or "drawn")
+    monkeypatch.setattr(continuous_batching, "draw_tokens", lambda logits, requests, generated: seen.append(len(requests)) or "drawn")
     backend = object.__new__(continuous_batching.ContinuousBatchModelBackend)
     backend.executor, backend._sampler = SimpleNamespace(), continuous_batching.sample_next_token
     plain = [continuous_batching.BatchRequest("a", [1], 4, 0.0, 1.0), SimpleNamespace(temperature=0.0, top_p=1.0)]
@@ -138,3 +138,18 @@ def test_a_seeded_request_draws_the_same_numbers_in_any_batch(monkeypatch):
     (u, t, k, p, m), second, third = calls
     assert u[0] == second[0][1] != third[0][0] and u[0] != u[1] and all(0 <= x < 1 for x in u)
     assert t == [0.5, 0.5] and k == [5, 0] and p == [0.75, 0.75] and m == [0.0, 0.25]
+
+
+def test_sharded_logits_refuse_filters_and_a_decode_step_counts_by_positions(monkeypatch):
+    seen = []
+    monkeypatch.setattr(continuous_batching, "draw_tokens", lambda logits, requests, generated: seen.append(generated) or "drawn")
+    backend = object.__new__(continuous_batching.ContinuousBatchModelBackend)
+    backend.executor, backend._sampler = SimpleNamespace(logits_are_sharded=False), continuous_batching.sample_next_token
+    backend._positions = {9: 6}
+    request = continuous_batching.BatchRequest("a", [1, 2, 3], 8, 0.7, 1.0, seed=1)
+    request.model_request_id = 9                     # its list is empty, its last token's position 6: 4 have been drawn
+    assert backend._sample(None, [request], decoding=True) == "drawn" and backend._sample(None, [request]) == "drawn"
+    assert seen == [[4], None]
+    backend.executor.logits_are_sharded = True
+    with pytest.raises(ValueError, match="shards"):
+        backend._sample(None, [request])
