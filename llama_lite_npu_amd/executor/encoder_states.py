@@ -54,11 +54,15 @@ class EncoderStates:
             ops.kv_append_quantised(xk, xv, self.slot_mapping, pool, self.kv_scales[layer_index])
 
     def decode_plan(self, num_q_heads: int) -> ops.DecodePlan:
-        """How a step of one row a sequence reads the states: made at its first call, and the same for every layer and step."""
-        plan = self._plans.get(num_q_heads)
+        """How a step of one row a sequence reads the states: made at its first call, and the same for every layer and step. Steps
+        share its workspace, so they run one after the other (one stream). In the capture of a graph, where nothing has run
+        yet, the graph gets a plan of its own, made at each of its replays."""
+        captured = torch.cuda.is_current_stream_capturing()
+        plan = None if captured else self._plans.get(num_q_heads)
         if plan is None:
             row = 2 * self.num_kv_heads * (self.kv_buffer[0].shape[2] * self.kv_buffer[0].element_size())
             plan = ops.DecodePlan(self.block_table, self.kv_lens, num_q_heads, self.num_kv_heads, self._pages,
                                   page_size=self.page_size, host_seq_lens=self.lengths, token_bytes=row, kv_dtype=self._dtype)
-            self._plans[num_q_heads] = plan
+            if not captured:
+                self._plans[num_q_heads] = plan
         return plan

@@ -1265,7 +1265,8 @@ def paged_cross_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: t
     name), whatever their own number; a sequence without keys gets rows of zeros. Head dims 64 and 128, any pool format, a
     softmax scale above 0.
 
-    ``cu_q_lens`` None: one row a sequence (a decode step), q [B, Hq, D], which streams the keys like ``paged_decode``.
+    ``cu_q_lens`` None: one row a sequence (a decode step), q [B, Hq, D], which streams the keys like ``paged_decode``, whose
+    lengths have to be ones that the block table can name.
     ``max_q_len``: the most rows of a sequence. ``max_kv_len``: the most keys, as the host knows it; launches of few rows
     are then cut along the keys as in ``paged_prefill``, and nothing but speed goes by it. Rows behind the last sequence are left as
     they are. ``key_slices`` and ``workspace`` as there."""
