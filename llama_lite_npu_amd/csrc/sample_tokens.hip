@@ -711,29 +711,56 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   bool whole = true;                                    // all of it; or its tokens from the key `cut` on
   uint64_t cut = 0;
   double kept = mass_live;
-  bool in_list = few;                                   // the bin's tokens are listed; else they are read from the row each time
-  int list_bin = -1;
-  // Every token of the row's list or, without it, of the row, whose key is in [from, to].
+  uint64_t list_from = few ? 0 : 1, list_to = few ? ~0ull : 0;        // the keys whose tokens are listed; others are read from the row
+  // Every token of the row whose key is in [from, to].
+  auto over_the_row = [&](uint64_t from, uint64_t to, auto &&what) __attribute__((always_inline)) {
+    const RangeTest<TYPE> test(logit_of_key<TYPE>(from), logit_of_key<TYPE>(to));
+    constexpr int kVectors = 4, kPerWord = kPer / 4;
+    uint4_t raw[kVectors], next[kVectors];                   // (the next ones on their way while these are looked at)
+    auto load = [&](int64_t v0, uint4_t (&into)[kVectors]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j) {
+        const int64_t v = v0 + j * kRowThreads;
+        into[j] = *(const uint4_t *)(in.base + (v < in.vectors ? v : in.vectors - 1) * 16);
+      }
+    };
+    load(tid, next);
+#pragma unroll 1
+    for (int64_t v0 = tid; v0 < in.vectors; v0 += kVectors * kRowThreads) {
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j) raw[j] = next[j];
+      load(v0 + kVectors * kRowThreads, next);
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j) {
+        const int64_t v = v0 + j * kRowThreads;
+        uint32_t those = 0;                                  // words with an element in the range
+#pragma unroll
+        for (int i = 0; i < 4; ++i) those |= (test.any(raw[j][i]) ? 1u : 0u) << i;
+        while (those != 0) {
+          const int i = __builtin_ctz(those);
+          those &= those - 1;
+          uint32_t one = raw[j][0];
+#pragma unroll
+          for (int n = 1; n < 4; ++n) one = i == n ? raw[j][n] : one;
+#pragma unroll
+          for (int h = 0; h < kPerWord; ++h) {
+            const float e = clean_logit<TYPE>(raw_logit<TYPE>(uint4_t{one, one, one, one}, h));
+            const int32_t at = (int32_t)(v * kPer - in.lead) + i * kPerWord + h;
+            const uint64_t key = key_of<TYPE>(order_of(e), at);
+            if (key >= from && key <= to && (uint32_t)at < (uint32_t)vocab) what(key);
+          }
+        }
+      }
+    }
+  };
   auto each_token = [&](uint64_t from, uint64_t to, auto &&what) __attribute__((always_inline)) {
-    if (in_list) {
+    if (from >= list_from && to <= list_to) {
       for (int i = 0, n = listed > tid ? own + (listed - tid + kRowThreads - 1) / kRowThreads : own; i < n; ++i) {
         const uint64_t key = i < own ? list[i][tid] : more[tid + (i - own) * kRowThreads];
         if (key >= from && key <= to) what(key);
       }
     } else {
-      for (int64_t v = tid; v < in.vectors; v += kRowThreads) {
-        float x[kPer];
-        logits_of<TYPE>(in, *(const uint4_t *)(in.base + v * 16), v, vocab, x);
-#pragma unroll 1
-        for (int i = 0; i < kPer; ++i) {
-          float e = x[0];
-#pragma unroll
-          for (int j = 1; j < kPer; ++j) e = i == j ? x[j] : e;
-          if (!(e > -INFINITY)) continue;
-          const uint64_t key = key_of<TYPE>(order_of(e), (int32_t)(v * kPer - in.lead + i));
-          if (key >= from && key <= to) what(key);
-        }
-      }
+      over_the_row(from, to, what);
     }
   };
 
@@ -778,63 +805,23 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     const uint32_t high_order = bin > 0 ? lowest_of_bin(top - bin + 1.0, t, z_per_x) - 1 : order_of(most);
     low = lowest_key<TYPE>(low_order);
     high = lowest_key<TYPE>(high_order + 1) - 1;
-    if (!few && list_bin != bin) {
-      in_list = count_to[bin] - (bin > 0 ? count_to[bin - 1] : 0) <= kMostListed;
-      list_bin = bin;
-      own = listed = 0;
-      __syncthreads();
-      if (tid == 0) found_n = 0;
-      __syncthreads();
-      if (in_list) {
-        const float least_x = logit_of_order(low_order), most_x = logit_of_order(high_order);
-        const RangeTest<TYPE> test(least_x, most_x);
-        constexpr int kVectors = 4, kPerWord = kPer / 4;
-        uint4_t raw[kVectors], next[kVectors];               // (the next ones on their way while these are looked at)
-        auto load = [&](int64_t v0, uint4_t (&to)[kVectors]) __attribute__((always_inline)) {
-#pragma unroll
-          for (int j = 0; j < kVectors; ++j) {
-            const int64_t v = v0 + j * kRowThreads;
-            to[j] = *(const uint4_t *)(in.base + (v < in.vectors ? v : in.vectors - 1) * 16);
-          }
-        };
-        load(tid, next);
-#pragma unroll 1
-        for (int64_t v0 = tid; v0 < in.vectors; v0 += kVectors * kRowThreads) {
-#pragma unroll
-          for (int j = 0; j < kVectors; ++j) raw[j] = next[j];
-          load(v0 + kVectors * kRowThreads, next);
-#pragma unroll
-          for (int j = 0; j < kVectors; ++j) {
-            const int64_t v = v0 + j * kRowThreads;
-            uint32_t those = 0;                            // words with an element in the range
-#pragma unroll
-            for (int i = 0; i < 4; ++i) those |= (test.any(raw[j][i]) ? 1u : 0u) << i;
-            while (those != 0) {
-              const int i = __builtin_ctz(those);
-              those &= those - 1;
-              uint32_t one = raw[j][0];
-#pragma unroll
-              for (int n = 1; n < 4; ++n) one = i == n ? raw[j][n] : one;
-#pragma unroll
-              for (int h = 0; h < kPerWord; ++h) {
-                const float e = clean_logit<TYPE>(raw_logit<TYPE>(uint4_t{one, one, one, one}, h));
-                const int32_t at = (int32_t)(v * kPer - in.lead) + i * kPerWord + h;
-                if (e >= least_x && e <= most_x && (uint32_t)at < (uint32_t)vocab) enlist(key_of<TYPE>(order_of(e), at));
-              }
-            }
-          }
-        }
-        __syncthreads();
-        in_list = found_n <= kMoreList;                    // (else too many of them are too few threads')
-        listed = found_n;
-      }
-    }
     if (filter == 2) break;
 
     // Where the prefix ends in the bin: while its tokens are many, by the next ten bits of their keys; then by ranking them.
     int32_t n_above = 0, n_left = count_to[bin] - (bin > 0 ? count_to[bin - 1] : 0);
     uint64_t u_above = 0, from = low, to = high;
     while (true) {
+      if (n_left <= kMostListed && !(from >= list_from && to <= list_to)) {
+        __syncthreads();
+        own = 0;
+        if (tid == 0) found_n = 0;
+        __syncthreads();
+        over_the_row(from, to, enlist);
+        __syncthreads();
+        listed = found_n;
+        list_from = listed <= kMoreList ? from : 1;            // (else too many of them are too few threads')
+        list_to = listed <= kMoreList ? to : 0;
+      }
       __syncthreads();
       if (tid == 0) {
         found_n = 0;
