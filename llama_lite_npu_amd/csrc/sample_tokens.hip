@@ -32,9 +32,9 @@ constexpr int kSampleSlice = 8192;            // tokens of a slice at most: thei
 constexpr int kSliceList = 64;                // tokens of a slice's list
 constexpr int kRowThreads = 512;              // of a row's workgroup
 constexpr int kRowWaves = kRowThreads / kWave;
-constexpr int kOwnList = 16;                  // tokens that a thread of a row's workgroup holds for itself
-constexpr int kMoreList = 2048;               // and those of all that have more
+constexpr int kMostFew = 2048;                // tokens that are taken from the slices' lists
 constexpr int kMostListed = 6144;             // tokens of a bin that are listed: 12 a thread on the average
+constexpr int kOwnPlaces = 30;                // places that a thread has for them at first
 constexpr int kSampleMaxVocab = 1 << 20;
 constexpr int kMaxSlices = 512;
 constexpr int kRanked = 64;                   // tokens that are ranked against each other; more go by their digits
@@ -151,13 +151,14 @@ struct MassPolynomial {
   double c0 = 0x1.00001eb4308b7p+52, c1 = 0x1.c3d686115b6e3p+36, c2 = 0x1.c3d68623f9176p+32, c3 = 0x1.2d39a7c5007cap+28,
          c4 = 0x1.2d3c27a6b0e5fp+23, c5 = 0x1.e10f01fb822cdp+17, c6 = 0x1.56123fcc468c2p+12;
   __device__ __forceinline__ void keep() { asm("" : "+s"(c0), "+s"(c1), "+s"(c2), "+s"(c3), "+s"(c4), "+s"(c5)); }
-  __device__ __forceinline__ uint64_t bits(double f) const {
+  __device__ __forceinline__ uint64_t bits(double f) const { return __builtin_bit_cast(uint64_t, raised(f)); }
+  __device__ __forceinline__ double raised(double f) const {       // ... and 2^52
     double e = __builtin_fma(c6, f, c5);
     e = __builtin_fma(e, f, c4);
     e = __builtin_fma(e, f, c3);
     e = __builtin_fma(e, f, c2);
     e = __builtin_fma(e, f, c1);
-    return __builtin_bit_cast(uint64_t, __builtin_fma(e, f, c0));
+    return __builtin_fma(e, f, c0);
   }
 };
 constexpr uint64_t kMassOne = 0x4330000000000000ull;      // 2^52's bits
@@ -180,28 +181,28 @@ __device__ __forceinline__ float logit_of_order(uint32_t k) {
 }
 
 // Tokens are told apart, and ordered like p and the index, by a key: the order of the logit without the bits that its type leaves
-// alike, then the index from the last down.
+// alike, then the index from the last down, in as many bits as the vocabulary takes (with more, the keys' digits would be few).
 template <int TYPE>
 constexpr int kAlike = TYPE == kLogitsF16 ? 13 : TYPE == kLogitsBf16 ? 16 : 0;
-constexpr int kIndexBits = 20;
 template <int TYPE>
-__device__ __forceinline__ uint64_t key_of(uint32_t order, int32_t at) {
-  return (uint64_t)(order >> kAlike<TYPE>) << kIndexBits | (uint64_t)(kSampleMaxVocab - 1 - at);
-}
-__device__ __forceinline__ int32_t index_of_key(uint64_t key) {
-  return kSampleMaxVocab - 1 - (int32_t)(key & (uint64_t)(kSampleMaxVocab - 1));
-}
-template <int TYPE>
-__device__ __forceinline__ float logit_of_key(uint64_t key) {
-  const uint32_t o = (uint32_t)(key >> kIndexBits) << kAlike<TYPE>;
-  return logit_of_order(o & 0x80000000u ? o : o | ((1u << kAlike<TYPE>) - 1u));
-}
-// The lowest key of a token whose order is at least `order`.
-template <int TYPE>
-__device__ __forceinline__ uint64_t lowest_key(uint32_t order) {
-  const uint32_t up = order & 0x80000000u ? (1u << kAlike<TYPE>) - 1u : 0u;      // (a negative token's alike bits are ones)
-  return (((uint64_t)order + up) >> kAlike<TYPE>) << kIndexBits;
-}
+struct Keys {
+  int bits;
+  uint32_t most;
+  __device__ __forceinline__ explicit Keys(int32_t vocab) : bits(32 - __builtin_clz((uint32_t)vocab | 1u)), most((1u << bits) - 1u) {}
+  __device__ __forceinline__ uint64_t of(uint32_t order, int32_t at) const {
+    return (uint64_t)(order >> kAlike<TYPE>) << bits | (uint64_t)(most - (uint32_t)at);
+  }
+  __device__ __forceinline__ int32_t index(uint64_t key) const { return (int32_t)(most - ((uint32_t)key & most)); }
+  __device__ __forceinline__ float logit(uint64_t key) const {
+    const uint32_t o = (uint32_t)(key >> bits) << kAlike<TYPE>;
+    return logit_of_order(o & 0x80000000u ? o : o | ((1u << kAlike<TYPE>) - 1u));
+  }
+  // The lowest key of a token whose order is at least `order`.
+  __device__ __forceinline__ uint64_t lowest(uint32_t order) const {
+    const uint32_t up = order & 0x80000000u ? (1u << kAlike<TYPE>) - 1u : 0u;    // (a negative token's alike bits are ones)
+    return (((uint64_t)order + up) >> kAlike<TYPE>) << bits;
+  }
+};
 
 __device__ __forceinline__ float row_temperature(const float *temperature, int row) {
   const float t = temperature != nullptr ? temperature[row] : 1.0f;
@@ -500,15 +501,21 @@ struct RangeTest {
     if constexpr (TYPE == kLogitsF16) return __builtin_bit_cast(uint16_t, (half_t)x);
     return (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16);
   }
+  // How far the two logits of a word are from the lowest.
+  __device__ __forceinline__ uint32_t from_low(uint32_t word) const {
+    const short2_t x = __builtin_bit_cast(short2_t, word);
+    const short2_t o = x ^ ((x >> 15) & (short2_t)0x7fff);
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(ushort2_t, o) - __builtin_bit_cast(ushort2_t, low));
+  }
+  static __device__ __forceinline__ bool any_nearer(uint32_t from_low, uint32_t end) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(ushort2_t, from_low), __builtin_bit_cast(ushort2_t, end))) != end;
+  }
   __device__ __forceinline__ bool any(uint32_t word) const {
     if constexpr (TYPE == kLogitsF32) {
       const float x = __builtin_bit_cast(float, word);
       return x >= least && x <= most;
     } else {
-      const short2_t x = __builtin_bit_cast(short2_t, word);
-      const short2_t o = x ^ ((x >> 15) & (short2_t)0x7fff);
-      const ushort2_t from_low = __builtin_bit_cast(ushort2_t, o) - __builtin_bit_cast(ushort2_t, low);
-      return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(from_low, __builtin_bit_cast(ushort2_t, beyond))) != beyond;
+      return any_nearer(from_low(word), beyond);
     }
   }
 };
@@ -533,10 +540,16 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   __shared__ int32_t slice_listed[kMaxSlices];
   __shared__ double slice_mass[kMaxSlices];
   __shared__ unsigned long long slice_units[kMaxSlices];
-  __shared__ uint64_t list[kOwnList][kRowThreads], more[kMoreList];   // keys, in any order
+  __shared__ uint64_t list[kMostListed];              // keys, in any order
   __shared__ unsigned long long radix_units[kRowThreads];
   __shared__ int32_t radix_count[kRowThreads];
-  __shared__ unsigned long long rank_key[kRun], rank_units[kRun];
+  __shared__ union {
+    struct {
+      unsigned long long key[kRun], units[kRun];
+    } rank;
+    uint32_t own[kOwnPlaces + 2][kRowThreads];        // (two places more are written to and never read)
+  } room;
+  auto &rank_key = room.rank.key, &rank_units = room.rank.units;
   __shared__ RowRoom rooms[2];
   __shared__ float room_f[kRowWaves];
   __shared__ int32_t found_k, found_p, found_last, found_at, found_slice, found_n, complete;
@@ -544,6 +557,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   const int tid = threadIdx.x, row = blockIdx.x, lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const LogitsRow in = logits_row<TYPE>(logits, row_stride, row, vocab);
+  const Keys<TYPE> keys(vocab);
   const SampleSlice *head = heads + (int64_t)row * slices;
   const uint64_t *row_bins = bins + (int64_t)row * slices * kSampleSlots;
   const uint64_t *row_lists = lists + (int64_t)row * slices * kSliceList;
@@ -661,7 +675,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   MassPolynomial polynomial;
   polynomial.keep();
   auto units_of_key = [&](uint64_t key) __attribute__((always_inline)) -> uint64_t {
-    return units_of(polynomial, z_of(logit_of_key<TYPE>(key), z_per_x)) + kFloorUnits;
+    return units_of(polynomial, z_of(keys.logit(key), z_per_x)) + kFloorUnits;
   };
 
   // Where the prefixes end; one that ends behind min_p's end (bin_m, or a bin more) says nothing, but top_k says what top_p is a
@@ -683,38 +697,119 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   // Where the slices' lists have all tokens that come into question, those are the row's list, and the draw's; else it has a
   // bin's tokens at a time, if they fit.
   const int most_bin = by_k ? bin_k : by_p ? bin_p : bin_m;
-  const bool few = most_bin < complete && count_to[most_bin] <= kMoreList;
-  int own = 0;
-  const int own_room = few ? 0 : kOwnList;              // (few are spread evenly in the list of all)
+  const bool few = most_bin < complete && count_to[most_bin] <= kMostFew;
   auto enlist = [&](uint64_t key) __attribute__((always_inline)) {
-    if (own < own_room) {
-      list[own++][tid] = key;
-    } else {
-      const int to = atomicAdd(&found_n, 1);
-      if (to < kMoreList) more[to] = key;
-    }
+    const int to = atomicAdd(&found_n, 1);
+    if (to < kMostListed) list[to] = key;
   };
-  int listed = 0;                                       // of `more`
+  int listed = 0;
   if (few) {
-    const uint64_t least = lowest_key<TYPE>(lowest_of_bin(top - most_bin, t, z_per_x));
+    const uint64_t least = keys.lowest(lowest_of_bin(top - most_bin, t, z_per_x));
 #pragma unroll 4
     for (int i = tid; i < slices * kSliceList; i += kRowThreads) {
       const uint64_t entry = row_lists[i];               // a logit's bits and its index
       const uint32_t bits = (uint32_t)(entry >> 32);
-      const uint64_t key = key_of<TYPE>(order_of(__builtin_bit_cast(float, bits)), (int32_t)(uint32_t)entry);
+      const uint64_t key = keys.of(order_of(__builtin_bit_cast(float, bits)), (int32_t)(uint32_t)entry);
       if (i % kSliceList < slice_listed[i / kSliceList] && key >= least) enlist(key);
     }
     __syncthreads();
-    listed = found_n < kMoreList ? found_n : kMoreList;
+    listed = found_n < kMostListed ? found_n : kMostListed;
   }
   int last = last_bin;                                  // the bin that the kept prefix ends in
   bool whole = true;                                    // all of it; or its tokens from the key `cut` on
   uint64_t cut = 0;
   double kept = mass_live;
   uint64_t list_from = few ? 0 : 1, list_to = few ? ~0ull : 0;        // the keys whose tokens are listed; others are read from the row
+  // All tokens with the logits of [from, to], which are whole ones. First each thread's, its elements by their numbers (16-bit logits
+  // with how far they are from the lowest): every element is written to the next place, which is moved on behind one of the range,
+  // without a branch. Then as keys, side by side.
+  static_assert(kSampleMaxVocab / kRowThreads + 8 * kPer <= 1 << 16, "an element's number has 16 bits");
+  auto list_logits = [&](uint64_t from, uint64_t to) __attribute__((always_inline)) {
+    const RangeTest<TYPE> test(keys.logit(from), keys.logit(to));
+    uint32_t *const places = &room.own[0][tid];
+    uint32_t *const last_place = places + kOwnPlaces * kRowThreads;
+    uint32_t *place = places;
+    constexpr int kVectors = 4;
+    uint4_t raw[kVectors], next[kVectors];                   // (the next ones on their way while these are looked at)
+    auto load = [&](int64_t v0, uint4_t (&into)[kVectors]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j) {
+        const int64_t v = v0 + j * kRowThreads;
+        into[j] = *(const uint4_t *)(in.base + (v < in.vectors ? v : in.vectors - 1) * 16);
+      }
+    };
+    load(tid, next);
+    uint32_t number = 0;
+#pragma unroll 1
+    for (int64_t v0 = tid; v0 < in.vectors; v0 += kVectors * kRowThreads) {
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j) raw[j] = next[j];
+      load(v0 + kVectors * kRowThreads, next);
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j) {
+        const bool there = v0 + j * kRowThreads < in.vectors;
+        if constexpr (TYPE == kLogitsF32) {
+          bool hit[4], any = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            hit[i] = there && test.any(raw[j][i]);
+            any |= hit[i];
+          }
+          if (__builtin_amdgcn_ballot_w64(any) == 0) continue;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            *place = number + (uint32_t)(kPer * j + i);
+            place += hit[i] ? kRowThreads : 0;
+            if (i & 1) place = place < last_place ? place : last_place;
+          }
+        } else {
+          const uint32_t end = there ? test.beyond : 0;
+          uint32_t far[4];
+          bool any = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            far[i] = test.from_low(raw[j][i]);
+            any |= RangeTest<TYPE>::any_nearer(far[i], end);
+          }
+          if (__builtin_amdgcn_ballot_w64(any) == 0) continue;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t at = number + (uint32_t)(kPer * j + 2 * i);
+            *place = far[i] << 16 | at;
+            place += (uint16_t)far[i] < (uint16_t)end ? kRowThreads : 0;
+            *place = (far[i] & 0xffff0000u) | (at + 1);
+            place += far[i] < (end & 0xffff0000u) ? kRowThreads : 0;
+            place = place < last_place ? place : last_place;
+          }
+        }
+      }
+      number += kPer * kVectors;
+    }
+    const int own = (int)(place - places) / kRowThreads;
+    int all;
+    const int before = row_scan(own < kOwnPlaces ? own : kMostListed + 1, rooms[turn].count, &all) - own;
+    turn ^= 1;
+    listed = all;
+    if (all > kMostListed) return;                           // (too many of them are some thread's)
+#pragma unroll 4
+    for (int i = 0; i < own; ++i) {
+      const uint32_t word = places[i * kRowThreads], n = word & 0xffffu;
+      const int32_t at = (int32_t)((n / kPer * kRowThreads + tid) * kPer + n % kPer) - in.lead;
+      uint32_t bits;
+      if constexpr (TYPE == kLogitsF32) {
+        bits = *(const uint32_t *)(in.base + (int64_t)(at + in.lead) * 4);
+      } else {
+        const int32_t o = (int16_t)(uint16_t)((word >> 16) + test.low);
+        bits = (uint16_t)(o ^ ((o >> 31) & 0x7fff));
+      }
+      const float e = clean_logit<TYPE>(raw_logit<TYPE>(uint4_t{bits, bits, bits, bits}, 0));
+      list[before + i] = (uint32_t)at < (uint32_t)vocab ? keys.of(order_of(e), at) : 0;      // (no token's key)
+    }
+    __syncthreads();
+  };
   // Every token of the row whose key is in [from, to].
   auto over_the_row = [&](uint64_t from, uint64_t to, auto &&what) __attribute__((always_inline)) {
-    const RangeTest<TYPE> test(logit_of_key<TYPE>(from), logit_of_key<TYPE>(to));
+    const RangeTest<TYPE> test(keys.logit(from), keys.logit(to));
     constexpr int kVectors = 4, kPerWord = kPer / 4;
     uint4_t raw[kVectors], next[kVectors];                   // (the next ones on their way while these are looked at)
     auto load = [&](int64_t v0, uint4_t (&into)[kVectors]) __attribute__((always_inline)) {
@@ -746,8 +841,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
           for (int h = 0; h < kPerWord; ++h) {
             const float e = clean_logit<TYPE>(raw_logit<TYPE>(uint4_t{one, one, one, one}, h));
             const int32_t at = (int32_t)(v * kPer - in.lead) + i * kPerWord + h;
-            const uint64_t key = key_of<TYPE>(order_of(e), at);
-            if (key >= from && key <= to && (uint32_t)at < (uint32_t)vocab) what(key);
+            const uint64_t key = keys.of(order_of(e), at);
+            if (key >= from && key <= to && (uint32_t)at < (uint32_t)vocab) what(key, true);
           }
         }
       }
@@ -755,9 +850,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   };
   auto each_token = [&](uint64_t from, uint64_t to, auto &&what) __attribute__((always_inline)) {
     if (from >= list_from && to <= list_to) {
-      for (int i = 0, n = listed > tid ? own + (listed - tid + kRowThreads - 1) / kRowThreads : own; i < n; ++i) {
-        const uint64_t key = i < own ? list[i][tid] : more[tid + (i - own) * kRowThreads];
-        if (key >= from && key <= to) what(key);
+#pragma unroll 4
+      for (int i = tid; i < listed; i += kRowThreads) {
+        const uint64_t key = list[i];
+        what(key, key >= from && key <= to);
       }
     } else {
       over_the_row(from, to, what);
@@ -791,7 +887,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
         const uint32_t order = border((double)most + log_m, [&](float x) { return x >= most || (double)x - (double)most >= log_m; });
         const double d = top - __builtin_floor(z_of(logit_of_order(order), z_per_x));
         const int b = d < (double)kSampleBins ? (int)d : kSampleBins;
-        const uint64_t least = lowest_key<TYPE>(order);
+        const uint64_t least = keys.lowest(order);
         if (b < kSampleBins && (b < last || (b == last && (whole || least > cut)))) {
           last = b;
           whole = false;
@@ -803,24 +899,28 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     }
     const uint32_t low_order = lowest_of_bin(top - bin, t, z_per_x);
     const uint32_t high_order = bin > 0 ? lowest_of_bin(top - bin + 1.0, t, z_per_x) - 1 : order_of(most);
-    low = lowest_key<TYPE>(low_order);
-    high = lowest_key<TYPE>(high_order + 1) - 1;
+    low = keys.lowest(low_order);
+    high = keys.lowest(high_order + 1) - 1;
     if (filter == 2) break;
 
     // Where the prefix ends in the bin: while its tokens are many, by the next ten bits of their keys; then by ranking them.
     int32_t n_above = 0, n_left = count_to[bin] - (bin > 0 ? count_to[bin - 1] : 0);
     uint64_t u_above = 0, from = low, to = high;
     while (true) {
-      if (n_left <= kMostListed && !(from >= list_from && to <= list_to)) {
+      const bool whole_logits = from == low && to == high;
+      if (n_left <= (whole_logits ? kMostListed : kMostFew) && !(from >= list_from && to <= list_to)) {
         __syncthreads();
-        own = 0;
-        if (tid == 0) found_n = 0;
-        __syncthreads();
-        over_the_row(from, to, enlist);
-        __syncthreads();
-        listed = found_n;
-        list_from = listed <= kMoreList ? from : 1;            // (else too many of them are too few threads')
-        list_to = listed <= kMoreList ? to : 0;
+        if (whole_logits) {
+          list_logits(from, to);
+        } else {
+          if (tid == 0) found_n = 0;
+          __syncthreads();
+          over_the_row(from, to, [&](uint64_t key, bool) __attribute__((always_inline)) { enlist(key); });
+          __syncthreads();
+          listed = found_n;
+        }
+        list_from = listed <= kMostListed ? from : 1;
+        list_to = listed <= kMostListed ? to : 0;
       }
       __syncthreads();
       if (tid == 0) {
@@ -835,10 +935,12 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
         radix_units[tid] = 0;
         radix_count[tid] = 0;
         __syncthreads();
-        each_token(from, to, [&](uint64_t key) __attribute__((always_inline)) {
-          const uint32_t r = (uint32_t)((to - key) >> down);          // from the largest
-          atomicAdd(&radix_count[r], 1);
-          atomicAdd(&radix_units[r], (unsigned long long)units_of_key(key));
+        // (one outside adds nothing somewhere: without branches several are on their way at once)
+        each_token(from, to, [&](uint64_t key, bool inside) __attribute__((always_inline)) {
+          const uint32_t r = inside ? (uint32_t)((to - key) >> down) : (uint32_t)tid;          // from the largest
+          const uint64_t units = units_of_key(key);
+          atomicAdd(&radix_count[r], inside ? 1 : 0);
+          atomicAdd(&radix_units[r], (unsigned long long)(inside ? units : 0));
         });
         __syncthreads();
         const int32_t n = radix_count[tid];
@@ -869,7 +971,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
         continue;
       }
       __syncthreads();
-      each_token(from, to, [&](uint64_t key) __attribute__((always_inline)) {
+      each_token(from, to, [&](uint64_t key, bool inside) __attribute__((always_inline)) {
+        if (!inside) return;
         const int i = atomicAdd(&found_n, 1);
         if (i < kRanked) {
           rank_key[i] = key;
@@ -916,10 +1019,12 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   // Kept are the tokens from the key `cut` on, and above the cut of y.
   const double x_cut = kCut * (double)t;
   auto mass_of = [&](uint64_t key) __attribute__((always_inline)) -> double {
-    const float x = logit_of_key<TYPE>(key);
-    if (!((double)x - (double)most >= x_cut)) return 0.0;
-    const double z = z_of(x, z_per_x), d = top - __builtin_floor(z);
-    return d < (double)kSampleBins ? (double)(units_of(polynomial, z) + kFloorUnits) * bin_top[(int)d] : 0.0;
+    const float x = keys.logit(key);
+    const double z = z_of(x, z_per_x), b = __builtin_floor(z);
+    const uint32_t d = whole_of(top - b);
+    const double units = polynomial.raised(z - b) - (0x1p52 - (double)kFloorUnits);
+    const bool kept_x = (double)x - (double)most >= x_cut && d < (uint32_t)kSampleBins;
+    return kept_x ? units * bin_top[d < (uint32_t)kSampleBins ? d : 0u] : 0.0;
   };
   uint64_t token = 0;
   double all = 1.0;
@@ -933,8 +1038,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     radix_units[tid] = 0;
     if (tid == 0) found_n = 0;
     __syncthreads();
-    each_token(cut, ~0ull, [&](uint64_t key) __attribute__((always_inline)) {
-      atomicAdd(&radix_units[index_of_key(key) / width], (unsigned long long)units_kept(key));
+    each_token(cut, ~0ull, [&](uint64_t key, bool inside) __attribute__((always_inline)) {
+      if (inside) atomicAdd(&radix_units[keys.index(key) / width], (unsigned long long)units_kept(key));
     });
     __syncthreads();
     const unsigned long long here = radix_units[tid];
@@ -949,8 +1054,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     __syncthreads();
     const int run = found_at;
     const uint64_t before_run = found_units;
-    each_token(cut, ~0ull, [&](uint64_t key) __attribute__((always_inline)) {
-      if (index_of_key(key) / width != run) return;
+    each_token(cut, ~0ull, [&](uint64_t key, bool inside) __attribute__((always_inline)) {
+      if (!inside || keys.index(key) / width != run) return;
       const int to = atomicAdd(&found_n, 1);
       rank_key[to] = key;                                  // (of `width` indexes, at most kRun)
       rank_units[to] = units_kept(key);
@@ -959,10 +1064,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     const int n = found_n;
     for (int i = tid; i < n; i += kRowThreads) {
       const uint64_t mine = rank_key[i];
-      const int32_t at = index_of_key(mine);
+      const int32_t at = keys.index(mine);
       uint64_t units_before = before_run;
 #pragma unroll 8
-      for (int j = 0; j < n; ++j) units_before += index_of_key(rank_key[j]) < at ? rank_units[j] : 0;
+      for (int j = 0; j < n; ++j) units_before += keys.index(rank_key[j]) < at ? rank_units[j] : 0;
       if ((double)(units_before + rank_units[i]) > target && !((double)units_before > target)) token = mine;
     }
     if (token == 0) return;
@@ -972,8 +1077,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     for (int s = tid; s < slices; s += kRowThreads) slice_units[s] = 0;
     __syncthreads();
     if (!whole) {
-      each_token(cut > low ? cut : low, high, [&](uint64_t key) __attribute__((always_inline)) {
-        atomicAdd(&slice_units[(index_of_key(key) + in.lead) / kPer / slice_vectors], (unsigned long long)units_of_key(key));
+      each_token(cut > low ? cut : low, high, [&](uint64_t key, bool inside) __attribute__((always_inline)) {
+        const int s = inside ? (keys.index(key) + in.lead) / kPer / slice_vectors : 0;
+        const uint64_t units = units_of_key(key);
+        atomicAdd(&slice_units[s], (unsigned long long)(inside ? units : 0));
       });
     }
     // (16 lanes a slice)
@@ -1045,8 +1152,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
         logits_of<TYPE>(in, raw[i], i < each && tid * each + i < slice_vectors ? v0 + i : in.vectors, vocab, x[i]);
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-          const uint64_t key = key_of<TYPE>(order_of(x[i][j]), (int32_t)((v0 + i) * kPer - in.lead + j));
-          share[i * kPer + j] = x[i][j] > -INFINITY && key >= cut ? mass_of(key) : 0.0;
+          const uint64_t key = keys.of(order_of(x[i][j]), (int32_t)((v0 + i) * kPer - in.lead + j));
+          const double of_it = mass_of(key);                 // (of any: without branches several are on their way at once)
+          share[i * kPer + j] = x[i][j] > -INFINITY && key >= cut ? of_it : 0.0;
           sum += share[i * kPer + j];
         }
       }
@@ -1061,7 +1169,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
         upto += share[i];
         if (here == 0x7fffffff && share[i] > 0.0 && upto > target) {
           here = (int)(v0 * kPer + i - in.lead);
-          here_key = key_of<TYPE>(order_of(x[i / kPer][i % kPer]), here);
+          here_key = keys.of(order_of(x[i / kPer][i % kPer]), here);
         }
       }
       if (here != 0x7fffffff) atomicMin(&found_at, here);
@@ -1079,9 +1187,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
       return;
     }
   }
-  tokens[row] = index_of_key(token);
+  tokens[row] = keys.index(token);
   if (logprobs != nullptr) {
-    logprobs[row] = (float)(((double)logit_of_key<TYPE>(token) - (double)most) * z_per_x * 0.125 - log(all));
+    logprobs[row] = (float)(((double)keys.logit(token) - (double)most) * z_per_x * 0.125 - log(all));
   }
 }
 
