@@ -848,13 +848,16 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
       }
     }
   };
+  auto each_listed = [&](uint64_t from, uint64_t to, auto &&what) __attribute__((always_inline)) {
+#pragma unroll 4
+    for (int i = tid; i < listed; i += kRowThreads) {
+      const uint64_t key = list[i];
+      what(key, key >= from && key <= to);
+    }
+  };
   auto each_token = [&](uint64_t from, uint64_t to, auto &&what) __attribute__((always_inline)) {
     if (from >= list_from && to <= list_to) {
-#pragma unroll 4
-      for (int i = tid; i < listed; i += kRowThreads) {
-        const uint64_t key = list[i];
-        what(key, key >= from && key <= to);
-      }
+      each_listed(from, to, what);
     } else {
       over_the_row(from, to, what);
     }
@@ -1038,7 +1041,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     radix_units[tid] = 0;
     if (tid == 0) found_n = 0;
     __syncthreads();
-    each_token(cut, ~0ull, [&](uint64_t key, bool inside) __attribute__((always_inline)) {
+    each_listed(cut, ~0ull, [&](uint64_t key, bool inside) __attribute__((always_inline)) {
       if (inside) atomicAdd(&radix_units[keys.index(key) / width], (unsigned long long)units_kept(key));
     });
     __syncthreads();
@@ -1054,7 +1057,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     __syncthreads();
     const int run = found_at;
     const uint64_t before_run = found_units;
-    each_token(cut, ~0ull, [&](uint64_t key, bool inside) __attribute__((always_inline)) {
+    each_listed(cut, ~0ull, [&](uint64_t key, bool inside) __attribute__((always_inline)) {
       if (!inside || keys.index(key) / width != run) return;
       const int to = atomicAdd(&found_n, 1);
       rank_key[to] = key;                                  // (of `width` indexes, at most kRun)
