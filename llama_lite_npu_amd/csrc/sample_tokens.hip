@@ -1030,7 +1030,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     return kept_x ? units * bin_top[d < (uint32_t)kSampleBins ? d : 0u] : 0.0;
   };
   uint64_t token = 0;
-  double all = 1.0;
+  const uint64_t most_key = keys.of(order_of(most), 0);
+  double all = 1.0;                                      // of the largest's mass: exactly 1 where it is all that is kept
   if (few) {
     // By the index: the run of indexes in which the target lies, then the token in it. Masses as whole numbers of 2^-43.
     const int width = (vocab + kRowThreads - 1) / kRowThreads;
@@ -1074,7 +1075,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
       if ((double)(units_before + rank_units[i]) > target && !((double)units_before > target)) token = mine;
     }
     if (token == 0) return;
-    all = (double)sum * 0x1p-43;
+    all = (double)sum / (double)units_kept(most_key);
   } else {
     // The kept mass of each slice: its bins in front of the last, and what it has of that one.
     for (int s = tid; s < slices; s += kRowThreads) slice_units[s] = 0;
@@ -1185,6 +1186,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
       target = 0.0;                                        // (a rounding: the next that is kept)
       __syncthreads();
     }
+    all /= mass_of(most_key);
     if (token == 0) {                                      // (never: u is below 1, so some slice passes the target)
       if (tid == 0) tokens[row] = -1;
       return;

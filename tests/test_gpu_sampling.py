@@ -90,6 +90,19 @@ def test_flat_and_steep_rows(spread, t):
             _check(logits.to(dtype), torch.rand(4, generator=g, device=DEV), t, k, p, m)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("spread", [0.01, 2.0])
+def test_one_kept_token_has_probability_1(dtype, spread):
+    """Its logarithm is 0 and nothing beside it, by each filter, from the lists and from the row."""
+    print(f"sample: one kept {dtype} {spread}", flush=True)
+    x, u = _logits(80, 40, 50000, dtype, spread)
+    x[:, 77] = x.max(1).values + x.abs().max() * 2.0 ** -6
+    t, full = torch.linspace(0.3, 2.0, 40, device=DEV), lambda v, d=torch.float32: torch.full((40,), v, device=DEV, dtype=d)  # noqa: E731
+    for filters in (dict(top_k=full(1, torch.int32)), dict(top_p=full(1e-6)), dict(min_p=full(1.0))):
+        tokens, logprobs = ops.sample_tokens(x, u, t, **filters, return_logprobs=True)
+        assert (tokens == 77).all() and (logprobs == 0).all(), (filters, logprobs)
+
+
 def test_ties_go_to_the_lowest_index():
     print("sample: ties", flush=True)
     for v in (1000, 20000):
