@@ -1078,6 +1078,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     all = (double)sum / (double)units_kept(most_key);
   } else {
     // The kept mass of each slice: its bins in front of the last, and what it has of that one.
+    if (whole) cut = keys.lowest(lowest_of_bin(top - last, t, z_per_x));      // (top_k may end with a bin)
     for (int s = tid; s < slices; s += kRowThreads) slice_units[s] = 0;
     __syncthreads();
     if (!whole) {

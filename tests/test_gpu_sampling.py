@@ -91,6 +91,20 @@ def test_flat_and_steep_rows(spread, t):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("first", [3, 100, 7000])
+def test_top_k_that_ends_between_two_distant_logits(dtype, first):
+    """The first top_k are apart from all others: what lies below them is not drawn, whether a slice's list holds them or not."""
+    print(f"sample: top_k ends with a bin, {dtype} {first}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(90)
+    x = 3 + 3 * torch.rand(64, 9001, generator=g, device=DEV)
+    x[:, torch.randperm(9001, generator=g, device=DEV)[:first]] = 7.0
+    u = (torch.arange(64, device=DEV) + 0.5) / 64
+    for k in (first, first - 1, first + 1):
+        _check(x.to(dtype), u, k=k)
+        _check(x.to(dtype), u, k=k, p=0.99, m=0.2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("spread", [0.01, 2.0])
 def test_one_kept_token_has_probability_1(dtype, spread):
     """Its logarithm is 0 and nothing beside it, by each filter, from the lists and from the row."""
