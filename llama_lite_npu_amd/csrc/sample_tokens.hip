@@ -13,7 +13,15 @@
 // Sums of mass are sums of whole numbers: the mass of a token is rounded to 2^-40 of its bin's top (y enters in fp64, and exp by a
 // polynomial over the width of a bin), so no order of additions shows in a token, and a bin's top is a factor applied once. A
 // cumulative mass is then within 2^-40 of itself wherever it is compared, which in a row of 150 000 tokens moves one draw in some
-// millions to a neighbour of the token that exact arithmetic gives.
+// millions to a neighbour of the token that exact arithmetic gives. (Of 380 000 rows of every type and filter none did.)
+//
+// Measured, us of the slices' and of the rows' kernel: 1 x 32000 fp16 with top-k and top-p 6 to 8 and 14, 32 x 151936 fp16 with all
+// filters 11 and 17, 33 x 49999 fp32 11 and 12, 256 x 128000 bf16 with top-p 37 and 45 (65 MB: a copy takes 13). The first is bound
+// by its instructions, 17 a token, 12 of them fp64, and by its atomics in LDS (two thirds of the cycles issue vector instructions
+// there, the LDS is busy in a third). The second by latency, some twenty steps of about 0.7 us (a memory trip, a scan, a barrier), and
+// where a bin has to be listed from the row (half the rows of the last case) by the pass over it: 12 us, 5.4 TB/s over the device. A
+// row whose end lies in a bin of more tokens than a list takes (151936 logits of standard deviation 1: 7500) takes 110 us, and one of
+// nothing but equal logits up to 600, whichever their number: one compute unit goes over it several times.
 #include <cmath>
 
 #include "common.h"
@@ -29,7 +37,9 @@ constexpr int kSampleBins = 322;              // of 1/8: what is further than 40
 constexpr int kSampleSlots = 512;             // a slice's bins lie at their place on the grid modulo this
 constexpr int kSampleThreads = 256;           // of a slice's workgroup
 constexpr int kSampleSlice = 8192;            // tokens of a slice at most: their number has 14 bits of a bin's word
-constexpr int kSliceList = 64;                // tokens of a slice's list
+// Tokens of a slice's list. (us of the whole call with 32 / 64 / 128: 32 x 151936 26.3 / 27.0 / 28.4; 33 x 49999, few slices, 29.1 / 23.1
+// / 23.9; 64 x 32000 36 / 24.5 / 25.0)
+constexpr int kSliceList = 64;
 constexpr int kRowThreads = 512;              // of a row's workgroup
 constexpr int kRowWaves = kRowThreads / kWave;
 constexpr int kMostFew = 2048;                // tokens that are taken from the slices' lists
@@ -37,11 +47,11 @@ constexpr int kMostListed = 6144;             // tokens of a bin that are listed
 constexpr int kOwnPlaces = 30;                // places that a thread has for them at first
 constexpr int kSampleMaxVocab = 1 << 20;
 constexpr int kMaxSlices = 512;
-constexpr int kRanked = 64;                   // tokens that are ranked against each other; more go by their digits
+constexpr int kRanked = 64;                   // tokens that are ranked against each other; more go by their digits (with 192 no faster)
 constexpr int kCountShift = 50;
 constexpr uint64_t kUnitsMask = (1ull << kCountShift) - 1;
 constexpr uint64_t kFloorUnits = 7ull << 37;  // 7/8, below exp(-1/8): a bin's word has the sum of what is above it
-constexpr double kUnit = 0x1p-40 / (1.0 - 0x1p-20);   // of a bin's top (see mass_bits)
+constexpr double kUnit = 0x1p-40 / (1.0 - 0x1p-20);   // of a bin's top (see MassPolynomial)
 constexpr double kCut = -40.0;
 constexpr double kReached = 1.0 - 0x1p-40;    // a border that rounding alone keeps from being reached is
 constexpr float kMostFloat = 3.4028234663852886e38f;
@@ -56,6 +66,8 @@ struct SampleSlice {      // of the workspace, in front of the histograms and th
 
 // The vectors of 16 bytes that a row's slices are counted in: of V elements, the first of them anywhere in its vector.
 __host__ __device__ constexpr int64_t sample_vectors(int64_t vocab, int size) { return (vocab * size + 30) / 16; }
+// Slices of 8192 tokens, or of half and a quarter of that where there are fewer than compute units: us of the whole call: 33 x 49999
+// 29.4 in 231 slices of 8192, 23.1 in 429; 8 x 128000 43 in 128, 46 in 256; 1 x 32000 22.9 in slices of 2048, 26.3 in slices of 1024.
 static int sample_slice_vectors(int32_t batch, int32_t vocab, int size) {
   int tokens = kSampleSlice;
   while (tokens > 2048 && (int64_t)batch * ((vocab + tokens - 1) / tokens) < 256) tokens /= 2;
@@ -521,7 +533,7 @@ struct RangeTest {
 };
 
 // Bound by latency: one memory trip or one pass over the row after another, with barriers between them. So loads are made whatever
-// their place (clamped, and masked where they are used), each piece of code stands once, and what few threads can find, each
+// their place (clamped, and masked where they are used), loops over a list have no branches, and what few threads can find, each
 // wavefront finds for itself.
 template <int TYPE>
 __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
