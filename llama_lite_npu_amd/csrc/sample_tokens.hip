@@ -15,10 +15,10 @@
 // cumulative mass is then within 2^-40 of itself wherever it is compared, which in a row of 150 000 tokens moves one draw in some
 // millions to a neighbour of the token that exact arithmetic gives. (Of 380 000 rows of every type and filter none did.)
 //
-// Measured, us of the slices' and of the rows' kernel: 1 x 32000 fp16 with top-k and top-p 6 to 8 and 14, 32 x 151936 fp16 with all
-// filters 11 and 17, 33 x 49999 fp32 11 and 12, 256 x 128000 bf16 with top-p 37 and 45 (65 MB: a copy takes 13). The first is bound
+// Measured, us of the slices' and of the rows' kernel: 1 x 32000 fp16 with top-k and top-p 7 and 10, 32 x 151936 fp16 with all
+// filters 11 and 11.5, 33 x 49999 fp32 11 and 10, 256 x 128000 bf16 with top-p 37 and 45 (65 MB: a copy takes 13). The first is bound
 // by its instructions, 17 a token, 12 of them fp64, and by its atomics in LDS (two thirds of the cycles issue vector instructions
-// there, the LDS is busy in a third). The second by latency, some twenty steps of about 0.7 us (a memory trip, a scan, a barrier), and
+// there, the LDS is busy in a third). The second by latency, some twelve to twenty steps of about 0.7 us (a memory trip, a scan, a barrier), and
 // where a bin has to be listed from the row (half the rows of the last case) by the pass over it: 12 us, 5.4 TB/s over the device. A
 // row whose end lies in a bin of more tokens than a list takes (151936 logits of standard deviation 1: 7500) takes 110 us, and one of
 // nothing but equal logits up to 600, whichever their number: one compute unit goes over it several times.
@@ -43,6 +43,7 @@ constexpr int kSliceList = 64;
 constexpr int kRowThreads = 512;              // of a row's workgroup
 constexpr int kRowWaves = kRowThreads / kWave;
 constexpr int kMostFew = 2048;                // tokens that are taken from the slices' lists
+constexpr int kOneGo = 256;                   // and of these, which are all ranked against each other (rows 17 -> 11.5 us at 32 x 151936)
 constexpr int kMostListed = 6144;             // tokens of a bin that are listed: 12 a thread on the average
 constexpr int kOwnPlaces = 30;                // places that a thread has for them at first
 constexpr int kSampleMaxVocab = 1 << 20;
@@ -673,6 +674,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   const double mass_live = mass_to[last_bin];
   bool by_k = k > 0 && k < live, by_p = p < 1.0f;
   const bool by_m = m > 0.0f;
+  double log_m = 0.0;
 
   // The first bin with a token by whose end the mass is `target`; the last with a token if none is.
   auto bin_reaching = [&](double target) __attribute__((always_inline)) -> int {
@@ -690,11 +692,35 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     return units_of(polynomial, z_of(keys.logit(key), z_per_x)) + kFloorUnits;
   };
 
+  // Of y's that are not cut off. In the few tokens' case as whole numbers of 2^-43.
+  const double x_cut = kCut * (double)t;
+  auto mass_of = [&](uint64_t key) __attribute__((always_inline)) -> double {
+    const float x = keys.logit(key);
+    const double z = z_of(x, z_per_x), b = __builtin_floor(z);
+    const uint32_t d = whole_of(top - b);
+    const double units = polynomial.raised(z - b) - (0x1p52 - (double)kFloorUnits);
+    const bool kept_x = (double)x - (double)most >= x_cut && d < (uint32_t)kSampleBins;
+    return kept_x ? units * bin_top[d < (uint32_t)kSampleBins ? d : 0u] : 0.0;
+  };
+  auto units_kept = [&](uint64_t key) __attribute__((always_inline)) -> uint64_t {
+    return __builtin_bit_cast(uint64_t, mass_of(key) * 0x1p43 + 0x1p52) - kMassOne;
+  };
+  const uint64_t most_key = keys.of(order_of(most), 0);
+  auto answer = [&](uint64_t token, double all) __attribute__((always_inline)) {
+    tokens[row] = keys.index(token);
+    if (logprobs != nullptr) {
+      logprobs[row] = (float)(((double)keys.logit(token) - (double)most) * z_per_x * 0.125 - log(all));
+    }
+  };
+  // min_p's lowest key.
+  auto least_kept = [&]() __attribute__((always_inline)) -> uint32_t {
+    return border((double)most + log_m, [&](float x) { return x >= most || (double)x - (double)most >= log_m; });
+  };
+
   // Where the prefixes end; one that ends behind min_p's end (bin_m, or a bin more) says nothing, but top_k says what top_p is a
   // share of.
   const int bin_k = by_k ? found_k : last_bin;
   int bin_p = last_bin, bin_m = last_bin;
-  double log_m = 0.0;
   if (by_m) {
     log_m = log((double)(m < 1.0f ? m : 1.0f)) * (double)t;          // kept: x - most >= log_m
     const double b = top - __builtin_floor(z_most + log_m * z_per_x) + 1.0;
@@ -726,6 +752,59 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     }
     __syncthreads();
     listed = found_n < kMostListed ? found_n : kMostListed;
+  }
+  if (few && listed <= kOneGo) {
+    // All at once: ranked against each other, the sums of their masses in that order, the first that is not kept, and of the kept ones
+    // the sums in the order of the index. Against each other by several threads a token, each a share of the others.
+    const int n = listed;
+    const int threads = n <= kWave ? kWave : n <= 2 * kWave ? 2 * kWave : kOneGo;     // of a share
+    const int one = tid & (threads - 1), each = (n + kRowThreads / threads - 1) / (kRowThreads / threads);
+    const int from = __builtin_amdgcn_readfirstlane(tid / threads) * each, to = from + each < n ? from + each : n;
+    radix_count[tid] = 0;
+    slice_units[tid] = 0;
+    __syncthreads();
+    uint64_t mine = one < n ? list[one] : 0;
+    int before = 0;
+#pragma unroll 8
+    for (int i = from; i < to; ++i) before += list[i] > mine;
+    atomicAdd(&radix_count[one], before);
+    const uint64_t units = units_kept(mine);
+    __syncthreads();
+    if (tid < n) {
+      rank_key[radix_count[tid]] = mine;
+      rank_units[radix_count[tid]] = units;
+    }
+    __syncthreads();
+    mine = tid < n ? rank_key[tid] : 0;
+    const unsigned long long here = tid < n ? rank_units[tid] : 0;
+    unsigned long long all_units;
+    const unsigned long long upto = row_scan(here, rooms[turn].units, &all_units);
+    radix_units[tid] = upto;
+    const uint64_t least = by_m ? keys.lowest(least_kept()) : 0;
+    __syncthreads();
+    const double p_target = (double)p * (by_k ? (double)radix_units[k - 1] : mass_live * 0x1p43) * kReached;
+    const bool out = tid > 0 && (tid >= n || (by_k && tid >= k) || mine < least || (by_p && (double)(upto - here) >= p_target));
+    const uint64_t those = __builtin_amdgcn_ballot_w64(out);
+    if (lane == 0 && those != 0) atomicMin(&found_at, wave * kWave + __builtin_ctzll(those));
+    __syncthreads();
+    const int kept_n = found_at < n ? found_at : n;
+    const unsigned long long sum = radix_units[kept_n - 1];
+    const double target = u * (double)sum * (2.0 - kReached);
+    const uint64_t at = rank_key[one < n ? one : 0] & keys.most;
+    const int kept_each = (kept_n + kRowThreads / threads - 1) / (kRowThreads / threads);
+    const int kept_from = __builtin_amdgcn_readfirstlane(tid / threads) * kept_each;
+    const int kept_to = kept_from + kept_each < kept_n ? kept_from + kept_each : kept_n;
+    unsigned long long part = 0;
+#pragma unroll 8
+    for (int i = kept_from; i < kept_to; ++i) part += (rank_key[i] & keys.most) > at ? rank_units[i] : 0;
+    atomicAdd(&slice_units[one], part);
+    __syncthreads();
+    if (tid >= kept_n) return;
+    const unsigned long long units_before = slice_units[tid];
+    if ((double)(units_before + here) > target && !((double)units_before > target)) {
+      answer(mine, (double)sum / (double)units_kept(most_key));
+    }
+    return;
   }
   int last = last_bin;                                  // the bin that the kept prefix ends in
   bool whole = true;                                    // all of it; or its tokens from the key `cut` on
@@ -899,7 +978,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
       end_units = __builtin_fmax((target - (bin > 0 ? mass_to[bin - 1] : 0.0)) / bin_top[bin], 1.0);
     } else {
       if (by_m) {
-        const uint32_t order = border((double)most + log_m, [&](float x) { return x >= most || (double)x - (double)most >= log_m; });
+        const uint32_t order = least_kept();
         const double d = top - __builtin_floor(z_of(logit_of_order(order), z_per_x));
         const int b = d < (double)kSampleBins ? (int)d : kSampleBins;
         const uint64_t least = keys.lowest(order);
@@ -1032,24 +1111,11 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
   }
 
   // Kept are the tokens from the key `cut` on, and above the cut of y.
-  const double x_cut = kCut * (double)t;
-  auto mass_of = [&](uint64_t key) __attribute__((always_inline)) -> double {
-    const float x = keys.logit(key);
-    const double z = z_of(x, z_per_x), b = __builtin_floor(z);
-    const uint32_t d = whole_of(top - b);
-    const double units = polynomial.raised(z - b) - (0x1p52 - (double)kFloorUnits);
-    const bool kept_x = (double)x - (double)most >= x_cut && d < (uint32_t)kSampleBins;
-    return kept_x ? units * bin_top[d < (uint32_t)kSampleBins ? d : 0u] : 0.0;
-  };
   uint64_t token = 0;
-  const uint64_t most_key = keys.of(order_of(most), 0);
   double all = 1.0;                                      // of the largest's mass: exactly 1 where it is all that is kept
   if (few) {
-    // By the index: the run of indexes in which the target lies, then the token in it. Masses as whole numbers of 2^-43.
+    // By the index: the run of indexes in which the target lies, then the token in it.
     const int width = (vocab + kRowThreads - 1) / kRowThreads;
-    auto units_kept = [&](uint64_t key) __attribute__((always_inline)) -> uint64_t {
-      return __builtin_bit_cast(uint64_t, mass_of(key) * 0x1p43 + 0x1p52) - kMassOne;
-    };
     __syncthreads();
     radix_units[tid] = 0;
     if (tid == 0) found_n = 0;
@@ -1205,10 +1271,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
       return;
     }
   }
-  tokens[row] = keys.index(token);
-  if (logprobs != nullptr) {
-    logprobs[row] = (float)(((double)keys.logit(token) - (double)most) * z_per_x * 0.125 - log(all));
-  }
+  answer(token, all);
 }
 
 }  // namespace litekv
