@@ -411,16 +411,14 @@ __global__ __launch_bounds__(kSampleThreads) void sample_slices_kernel(
 #pragma unroll
   for (int w = 0; w < kWaves - 1; ++w) upto += w < wave ? wave_at[w] : 0;
   const int first_upto = upto - count + count_first;
-  if (first_upto <= kSliceList) atomicMax(&found_bins, upto <= kSliceList ? 2 * tid + 2 : 2 * tid + 1);
+  // (both grow with the bin: as many as hold are the bins from the top on)
+  const int fit = __builtin_popcountll(__builtin_amdgcn_ballot_w64(first_upto <= kSliceList)) +
+                  __builtin_popcountll(__builtin_amdgcn_ballot_w64(upto <= kSliceList));
+  if (tid % kWave == 0 && fit > 0) atomicAdd(&found_bins, fit);
   __syncthreads();
   const int listed_bins = found_bins < kSampleBins ? found_bins : kSampleBins;
   if (listed_bins > 0) {
-    if (wave == 0) {
-      const uint32_t order = lowest_of_bin(top - (listed_bins - 1), t, z_per_x);
-      if (tid == 0) wave_most[0] = logit_of_order(order);
-    }
-    __syncthreads();
-    const float least = wave_most[0];
+    const float least = logit_of_order(lowest_of_bin(top - (listed_bins - 1), t, z_per_x));
     uint64_t those[kMostVectors * kPer];
     int n = 0;
 #pragma unroll
@@ -433,14 +431,21 @@ __global__ __launch_bounds__(kSampleThreads) void sample_slices_kernel(
     at = __builtin_amdgcn_readfirstlane(at);
     uint64_t *to = lists + place * kSliceList;
 #pragma unroll
-    for (int i = 0; i < kMostVectors * kPer; ++i) {
-      if (those[i] == 0) continue;
-      const float e = x[i / kPer][i % kPer];
-      const int slot = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(those[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)those[i], 0));
-      if (e >= least && slot < kSliceList) {
-        to[slot] = (uint64_t)__builtin_bit_cast(uint32_t, e) << 32 | (uint32_t)(first + i / kPer * kSampleThreads * kPer + i % kPer);
+    for (int i0 = 0; i0 < kMostVectors * kPer; i0 += kPer) {
+      uint64_t any = 0;
+#pragma unroll
+      for (int i = i0; i < i0 + kPer; ++i) any |= those[i];
+      if (any == 0) continue;
+#pragma unroll
+      for (int i = i0; i < i0 + kPer; ++i) {
+        if (those[i] == 0) continue;
+        const float e = x[i / kPer][i % kPer];
+        const int slot = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(those[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)those[i], 0));
+        if (e >= least && slot < kSliceList) {
+          to[slot] = (uint64_t)__builtin_bit_cast(uint32_t, e) << 32 | (uint32_t)(first + i / kPer * kSampleThreads * kPer + i % kPer);
+        }
+        at += __builtin_popcountll(those[i]);
       }
-      at += __builtin_popcountll(those[i]);
     }
     __syncthreads();
   }
