@@ -119,6 +119,10 @@ struct LogitsRow {
   const char *base;        // the row's first vector
   int lead;                // elements in front of the row in it
   int64_t vectors;
+  // Its vector v, the last for those behind it.
+  __device__ __forceinline__ uint4_t vector(int64_t v) const {
+    return *(const __attribute__((address_space(1))) uint4_t *)(uint64_t)(base + (v < vectors ? v : vectors - 1) * 16);
+  }
 };
 template <int TYPE>
 __device__ __forceinline__ LogitsRow logits_row(const void *logits, int64_t row_stride, int row, int32_t vocab) {
@@ -294,8 +298,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_slices_kernel(
 #pragma unroll
   for (int i = 0; i < kMostVectors; ++i) {
     const int v = i * kSampleThreads + tid;
-    raw[i] = uint4_t{0, 0, 0, 0};
-    if (v < slice_vectors && v0 + v < in.vectors) raw[i] = *(const uint4_t *)(in.base + (v0 + v) * 16);
+    raw[i] = in.vector(v0 + v);                                // (what is not the slice's is masked; a condition would have each load waited for)
   }
   const float t = row_temperature(temperature, row);
   const double z_per_x = z_factor(t);
@@ -831,7 +834,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
 #pragma unroll
       for (int j = 0; j < kVectors; ++j) {
         const int64_t v = v0 + j * kRowThreads;
-        into[j] = *(const uint4_t *)(in.base + (v < in.vectors ? v : in.vectors - 1) * 16);
+        into[j] = in.vector(v);
       }
     };
     load(tid, next);
@@ -893,7 +896,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
       const int32_t at = (int32_t)((n / kPer * kRowThreads + tid) * kPer + n % kPer) - in.lead;
       uint32_t bits;
       if constexpr (TYPE == kLogitsF32) {
-        bits = *(const uint32_t *)(in.base + (int64_t)(at + in.lead) * 4);
+        bits = *(const __attribute__((address_space(1))) uint32_t *)(uint64_t)(in.base + (int64_t)(at + in.lead) * 4);
       } else {
         const int32_t o = (int16_t)(uint16_t)((word >> 16) + test.low);
         bits = (uint16_t)(o ^ ((o >> 31) & 0x7fff));
@@ -912,7 +915,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
 #pragma unroll
       for (int j = 0; j < kVectors; ++j) {
         const int64_t v = v0 + j * kRowThreads;
-        into[j] = *(const uint4_t *)(in.base + (v < in.vectors ? v : in.vectors - 1) * 16);
+        into[j] = in.vector(v);
       }
     };
     load(tid, next);
@@ -1233,7 +1236,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
       const int64_t v0 = (int64_t)s * slice_vectors + (int64_t)tid * each;
       uint4_t raw[kVectors];
 #pragma unroll
-      for (int i = 0; i < kVectors; ++i) raw[i] = *(const uint4_t *)(in.base + (v0 + i < in.vectors ? v0 + i : in.vectors - 1) * 16);
+      for (int i = 0; i < kVectors; ++i) raw[i] = in.vector(v0 + i);
       double share[kVectors * kPer], sum = 0.0;
 #pragma unroll
       for (int i = 0; i < kVectors; ++i) {
