@@ -13,11 +13,11 @@
 // Sums of mass are sums of whole numbers: the mass of a token is rounded to 2^-40 of its bin's top (y enters in fp64, and exp by a
 // polynomial over the width of a bin), so no order of additions shows in a token, and a bin's top is a factor applied once. A
 // cumulative mass is then within 2^-40 of itself wherever it is compared, which in a row of 150 000 tokens moves one draw in some
-// millions to a neighbour of the token that exact arithmetic gives. (Of 380 000 rows of every type and filter none did.)
+// millions to a neighbour of the token that exact arithmetic gives. (Of 760 000 rows of every type and filter none did.)
 //
-// Measured, us of the slices' and of the rows' kernel: 1 x 32000 fp16 with top-k and top-p 7 and 10, 32 x 151936 fp16 with all
-// filters 11 and 11.5, 33 x 49999 fp32 11 and 10, 256 x 128000 bf16 with top-p 37 and 45 (65 MB: a copy takes 13). The first is bound
-// by its instructions, 17 a token, 12 of them fp64, and by its atomics in LDS (two thirds of the cycles issue vector instructions
+// Measured, us of the slices' and of the rows' kernel: 1 x 32000 fp16 with top-k and top-p 6 and 10, 32 x 151936 fp16 with all
+// filters 10 and 12, 33 x 49999 fp32 9 and 12, 256 x 128000 bf16 with top-p 34 and 43 (65 MB: a copy takes 13). The first is bound
+// by its instructions, 17 a token, 12 of them fp64, and by its atomics in LDS (three quarters of the cycles issue vector instructions
 // there, the LDS is busy in a third). The second by latency, some twelve to twenty steps of about 0.7 us (a memory trip, a scan, a barrier), and
 // where a bin has to be listed from the row (half the rows of the last case) by the pass over it: 12 us, 5.4 TB/s over the device. A
 // row whose end lies in a bin of more tokens than a list takes (151936 logits of standard deviation 1: 7500) takes 110 us, and one of
@@ -43,7 +43,7 @@ constexpr int kSliceList = 64;
 constexpr int kRowThreads = 512;              // of a row's workgroup
 constexpr int kRowWaves = kRowThreads / kWave;
 constexpr int kMostFew = 2048;                // tokens that are taken from the slices' lists
-constexpr int kOneGo = 256;                   // and of these, which are all ranked against each other (rows 17 -> 11.5 us at 32 x 151936)
+constexpr int kOneGo = 256;                   // and of these, which are all ranked against each other (rows 17 -> 12 us at 32 x 151936)
 constexpr int kMostListed = 6144;             // tokens of a bin that are listed: 12 a thread on the average
 constexpr int kOwnPlaces = 30;                // places that a thread has for them at first
 constexpr int kSampleMaxVocab = 1 << 20;
