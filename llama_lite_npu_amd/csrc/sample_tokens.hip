@@ -37,18 +37,20 @@ constexpr int kSampleBins = 322;              // of 1/8: what is further than 40
 constexpr int kSampleSlots = 512;             // a slice's bins lie at their place on the grid modulo this
 constexpr int kSampleThreads = 256;           // of a slice's workgroup
 constexpr int kSampleSlice = 8192;            // tokens of a slice at most: their number has 14 bits of a bin's word
-// Tokens of a slice's list. (us of the whole call with 32 / 64 / 128: 32 x 151936 26.3 / 27.0 / 28.4; 33 x 49999, few slices, 29.1 / 23.1
-// / 23.9; 64 x 32000 36 / 24.5 / 25.0)
+// Tokens of a slice's list. (us of the whole call with 32 / 64 / 128: 32 x 151936 19.9 / 20.8 / 22.4; 33 x 49999, few slices, 26.5 / 18.6
+// / 19.5; 64 x 32000 33.5 / 17.3 / 17.7)
 constexpr int kSliceList = 64;
 constexpr int kRowThreads = 512;              // of a row's workgroup
 constexpr int kRowWaves = kRowThreads / kWave;
 constexpr int kMostFew = 2048;                // tokens that are taken from the slices' lists
-constexpr int kOneGo = 256;                   // and of these, which are all ranked against each other (rows 17 -> 12 us at 32 x 151936)
+// And of these, which are ranked against each other all at once, 256 where two filters end among them, 128 for one. (us of the whole call so /
+// filter by filter: 32 x 151936 20.7 / 25.9, 1 x 32000 17.3 / 21.4, top-k and top-p up to 200; 16 x 151936 with top-k alone up to 200 23.1 / 21.0.)
+constexpr int kOneGo = 256;
 constexpr int kMostListed = 6144;             // tokens of a bin that are listed: 12 a thread on the average
 constexpr int kOwnPlaces = 30;                // places that a thread has for them at first
 constexpr int kSampleMaxVocab = 1 << 20;
 constexpr int kMaxSlices = 512;
-constexpr int kRanked = 64;                   // tokens that are ranked against each other; more go by their digits (with 192 no faster)
+constexpr int kRanked = 64;                   // tokens that are ranked against each other; more go by their digits (with 128 no faster)
 constexpr int kCountShift = 50;
 constexpr uint64_t kUnitsMask = (1ull << kCountShift) - 1;
 constexpr uint64_t kFloorUnits = 7ull << 37;  // 7/8, below exp(-1/8): a bin's word has the sum of what is above it
@@ -68,7 +70,7 @@ struct SampleSlice {      // of the workspace, in front of the histograms and th
 // The vectors of 16 bytes that a row's slices are counted in: of V elements, the first of them anywhere in its vector.
 __host__ __device__ constexpr int64_t sample_vectors(int64_t vocab, int size) { return (vocab * size + 30) / 16; }
 // Slices of 8192 tokens, or of half and a quarter of that where there are fewer than compute units: us of the whole call: 33 x 49999
-// 29.4 in 231 slices of 8192, 23.1 in 429; 8 x 128000 43 in 128, 46 in 256; 1 x 32000 22.9 in slices of 2048, 26.3 in slices of 1024.
+// 25.4 in 231 slices of 8192, 18.6 in 429; 8 x 128000 42 in 128, 44 in 256; 1 x 32000 17.3 in slices of 2048, 20.9 in slices of 1024.
 static int sample_slice_vectors(int32_t batch, int32_t vocab, int size) {
   int tokens = kSampleSlice;
   while (tokens > 2048 && (int64_t)batch * ((vocab + tokens - 1) / tokens) < 256) tokens /= 2;
@@ -761,7 +763,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     __syncthreads();
     listed = found_n < kMostListed ? found_n : kMostListed;
   }
-  if (few && listed <= kOneGo) {
+  if (few && listed <= (by_k && by_p ? kOneGo : kOneGo / 2)) {
     // All at once: ranked against each other, the sums of their masses in that order, the first that is not kept, and of the kept ones
     // the sums in the order of the index. Against each other by several threads a token, each a share of the others.
     const int n = listed;
