@@ -249,3 +249,44 @@ def test_prompts_then_captured_steps():
         order = p.sort(descending=True, stable=True)
         kept = torch.zeros_like(p).scatter_(1, order.indices, ((order.values.cumsum(-1) - order.values) < 0.9).double())
         assert (kept.gather(1, tokens[:, None]) == 1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.uint4])
+def test_a_batch_without_states(dtype):
+    """No sequence has any: nothing to store, rows of zeros in both forms."""
+    print(f"image requests: no states {dtype}", flush=True)
+    states, layer = EncoderStates([0, 0], 1, HKV, D, PAGE, dtype, DEV), Attention(HQ, HKV, D)
+    none = torch.empty(0, HKV, D, device=DEV, dtype=torch.float16)
+    states.store(0, none, none)
+    q = torch.randn(5, HQ, D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).half()
+    cu = torch.tensor([0, 2, 5], device=DEV, dtype=torch.int32)
+    assert (layer.cross_forward(q, states, 0, cu, 3) == 0).all() and (layer.cross_forward(q[:2], states, 0) == 0).all()
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on two streams have workspaces of their own: each is what it is alone."""
+    print("image requests: two streams", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    sides = []
+    for n in (2000, 900):
+        pool = torch.randn(2048 + 16 * n % 512, 2 * HKV, D, generator=g, device=DEV).half()
+        table = torch.randperm(pool.shape[0] // PAGE, generator=g, device=DEV).to(torch.int32)[None, :128].contiguous()
+        q, x = torch.randn(4, HQ, D, generator=g, device=DEV).half(), torch.randn(7, 30000, generator=g, device=DEV)
+        lens, cu = torch.tensor([n], device=DEV, dtype=torch.int32), torch.tensor([0, 4], device=DEV, dtype=torch.int32)
+        u, p = torch.rand(7, generator=g, device=DEV), torch.full((7,), 0.9, device=DEV)
+
+        def call(q=q, pool=pool, table=table, lens=lens, cu=cu, x=x, u=u, p=p, n=n):
+            return (ops.paged_cross_attention(q, pool, table, lens, cu, 4, page_size=PAGE, max_kv_len=n),
+                    ops.paged_cross_attention(q[:1], pool, table, lens, page_size=PAGE, max_kv_len=n), ops.sample_tokens(x, u, top_p=p))
+
+        sides.append((call, call(), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for (call, _, stream), kept in zip(sides, got):
+            with torch.cuda.stream(stream):
+                kept.append(call())
+    torch.cuda.synchronize()
+    for (_, want, _), kept in zip(sides, got):
+        for one in kept:
+            assert all(torch.equal(a, b) for a, b in zip(one, want))
