@@ -937,8 +937,9 @@ int litekv_paged_cross_attention(const void *q, int64_t q_token_stride, const vo
  * them the shortest run whose mass reaches top_p of theirs; of them those with
  * p_i >= min_p; always the first. tokens[r] is the first token, by index, at which the kept
  * mass exceeds uniforms[r] times all of it, logprobs[r] its logarithm of probability among the
- * kept. Masses are exact to 2^-41 of themselves. T <= 0 (or NaN) takes the first
- * largest logit, with logprob 0.
+ * kept. T <= 0 (or NaN) takes the first largest logit, with logprob 0. Sums of mass are
+ * exact to 2^-40 of the whole that they are a part of, and no kept token counts as nothing:
+ * with 0 for a number the first of them, by index, is drawn.
  *   logits       [batch][row_stride], logits_type 0 fp16, 1 bf16, 2 fp32; aligned to an
  *                element. NaN and -inf are never drawn, +inf counts as the type's largest finite
  *                number. A row without any other: token -1, logprob -inf

@@ -702,7 +702,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     return units_of(polynomial, z_of(keys.logit(key), z_per_x)) + kFloorUnits;
   };
 
-  // Of y's that are not cut off. In the few tokens' case as whole numbers of 2^-43.
+  // Of y's that are not cut off. In the few tokens' case as whole numbers of 2^-51, so that 2^11 of them are within 2^-40 of what they
+  // sum up to and their sums within 63 bits; a token that is kept has one at least, as the smallest numbers take the first that is.
   const double x_cut = kCut * (double)t;
   auto mass_of = [&](uint64_t key) __attribute__((always_inline)) -> double {
     const float x = keys.logit(key);
@@ -713,7 +714,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     return kept_x ? units * bin_top[d < (uint32_t)kSampleBins ? d : 0u] : 0.0;
   };
   auto units_kept = [&](uint64_t key) __attribute__((always_inline)) -> uint64_t {
-    return __builtin_bit_cast(uint64_t, mass_of(key) * 0x1p43 + 0x1p52) - kMassOne;
+    const double mass_here = mass_of(key);
+    const double units = __builtin_fmax(mass_here * 0x1p51, mass_here > 0.0 ? 1.0 : 0.0);
+    return __builtin_bit_cast(uint64_t, units + 0x1p52) - kMassOne;
   };
   const uint64_t most_key = keys.of(order_of(most), 0);
   auto answer = [&](uint64_t token, double all) __attribute__((always_inline)) {
@@ -792,7 +795,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
     radix_units[tid] = upto;
     const uint64_t least = by_m ? keys.lowest(least_kept()) : 0;
     __syncthreads();
-    const double p_target = (double)p * (by_k ? (double)radix_units[k - 1] : mass_live * 0x1p43) * kReached;
+    const double p_target = (double)p * (by_k ? (double)radix_units[k - 1] : mass_live * 0x1p51) * kReached;
     const bool out = tid > 0 && (tid >= n || (by_k && tid >= k) || mine < least || (by_p && (double)(upto - here) >= p_target));
     const uint64_t those = __builtin_amdgcn_ballot_w64(out);
     if (lane == 0 && those != 0) atomicMin(&found_at, wave * kWave + __builtin_ctzll(those));
