@@ -941,8 +941,9 @@ int litekv_paged_cross_attention(const void *q, int64_t q_token_stride, const vo
  * exact to 2^-40 of the whole that they are a part of, and no kept token counts as nothing:
  * with 0 for a number the first of them, by index, is drawn.
  *   logits       [batch][row_stride], logits_type 0 fp16, 1 bf16, 2 fp32; aligned to an
- *                element. NaN and -inf are never drawn, +inf counts as the type's largest finite
- *                number. A row without any other: token -1, logprob -inf
+ *                element. NaN and -inf are never drawn, +inf counts as the largest finite fp32
+ *                number, which is above all others of 16 bits. A row without any: token -1,
+ *                logprob -inf
  *   uniforms     [batch], in [0, 1) (what is outside counts as the nearest inside, NaN as 0)
  *   temperature  [batch], NULL: 1
  *   top_k        [batch], below 1: off. NULL: off

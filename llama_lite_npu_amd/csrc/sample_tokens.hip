@@ -80,7 +80,7 @@ static int sample_slice_vectors(int32_t batch, int32_t vocab, int size) {
 enum { kLogitsF16 = 0, kLogitsBf16 = 1, kLogitsF32 = 2 };
 constexpr int logit_size(int type) { return type == kLogitsF32 ? 4 : 2; }
 
-// The largest finite logit of a type, which infinity counts as.
+// The largest finite logit of a type.
 template <int TYPE>
 constexpr float kMostLogit = TYPE == kLogitsF16 ? 65504.0f : TYPE == kLogitsBf16 ? 0x1.fep+127f : kMostFloat;
 // Element i of a vector as a float, as it is.
@@ -96,11 +96,8 @@ __device__ __forceinline__ float raw_logit(uint4_t raw, int i) {
     return (float)__builtin_bit_cast(half_t, (uint16_t)(raw[i >> 1] >> (16 * (i & 1))));
   }
 }
-// NaN cannot be drawn and becomes -inf, infinity the largest finite logit.
-template <int TYPE>
-__device__ __forceinline__ float clean_logit(float x) {
-  return __builtin_fminf(__builtin_fmaxf(x, -INFINITY), kMostLogit<TYPE>);
-}
+// NaN cannot be drawn and becomes -inf, infinity the largest finite float, which among 16-bit logits is above all others.
+__device__ __forceinline__ float clean_logit(float x) { return __builtin_fminf(__builtin_fmaxf(x, -INFINITY), kMostFloat); }
 // Whether a vector has an element that is not finite: two at a time by their bits without the signs.
 template <int TYPE>
 __device__ __forceinline__ bool has_special(uint4_t raw) {
@@ -144,7 +141,7 @@ __device__ __forceinline__ void logits_of(const LogitsRow &in, uint4_t raw, int6
   const int64_t first = at * kPer - in.lead;
   const bool inside = first >= 0 && first + kPer <= vocab;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) x[i] = clean_logit<TYPE>(raw_logit<TYPE>(raw, i));
+  for (int i = 0; i < kPer; ++i) x[i] = clean_logit(raw_logit<TYPE>(raw, i));
   if (!inside) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -201,6 +198,7 @@ __device__ __forceinline__ float logit_of_order(uint32_t k) {
 
 // Tokens are told apart, and ordered like p and the index, by a key: the order of the logit without the bits that its type leaves
 // alike, then the index from the last down, in as many bits as the vocabulary takes (with more, the keys' digits would be few).
+// Infinity, which has become the largest float, has the order of infinity there: what is left of its own is bf16's largest finite one.
 template <int TYPE>
 constexpr int kAlike = TYPE == kLogitsF16 ? 13 : TYPE == kLogitsBf16 ? 16 : 0;
 template <int TYPE>
@@ -209,17 +207,19 @@ struct Keys {
   uint32_t most;
   __device__ __forceinline__ explicit Keys(int32_t vocab) : bits(32 - __builtin_clz((uint32_t)vocab | 1u)), most((1u << bits) - 1u) {}
   __device__ __forceinline__ uint64_t of(uint32_t order, int32_t at) const {
-    return (uint64_t)(order >> kAlike<TYPE>) << bits | (uint64_t)(most - (uint32_t)at);
+    return (uint64_t)(upwards(order) >> kAlike<TYPE>) << bits | (uint64_t)(most - (uint32_t)at);
   }
   __device__ __forceinline__ int32_t index(uint64_t key) const { return (int32_t)(most - ((uint32_t)key & most)); }
   __device__ __forceinline__ float logit(uint64_t key) const {
     const uint32_t o = (uint32_t)(key >> bits) << kAlike<TYPE>;
-    return logit_of_order(o & 0x80000000u ? o : o | ((1u << kAlike<TYPE>) - 1u));
+    const float x = logit_of_order(o & 0x80000000u ? o : o | ((1u << kAlike<TYPE>) - 1u));
+    return TYPE == kLogitsF32 ? x : __builtin_fminf(x, kMostFloat);
   }
   // The lowest key of a token whose order is at least `order`.
-  __device__ __forceinline__ uint64_t lowest(uint32_t order) const {
-    const uint32_t up = order & 0x80000000u ? (1u << kAlike<TYPE>) - 1u : 0u;    // (a negative token's alike bits are ones)
-    return (((uint64_t)order + up) >> kAlike<TYPE>) << bits;
+  __device__ __forceinline__ uint64_t lowest(uint32_t order) const { return (uint64_t)(upwards(order) >> kAlike<TYPE>) << bits; }
+  // The order itself, or the next that a logit of the type has, in the bits that are not alike. (Orders end with infinity's, 0xff800000.)
+  static __device__ __forceinline__ uint32_t upwards(uint32_t order) {
+    return order + ((uint32_t)((int32_t)order >> 31) & ((1u << kAlike<TYPE>) - 1u));      // (a negative token's alike bits are ones)
   }
 };
 
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_slices_kernel(
   }
   if (__builtin_amdgcn_ballot_w64(special) != 0) {
 #pragma unroll
-    for (int i = 0; i < kMostVectors * kPer; ++i) x[i / kPer][i % kPer] = clean_logit<TYPE>(x[i / kPer][i % kPer]);
+    for (int i = 0; i < kMostVectors * kPer; ++i) x[i / kPer][i % kPer] = clean_logit(x[i / kPer][i % kPer]);
   }
   if (slice == 0 || v0 + kMostVectors * kSampleThreads >= in.vectors || slice_vectors < kMostVectors * kSampleThreads) {
     // -inf in the places that are not the row's, or not the slice's
@@ -510,9 +510,9 @@ struct RangeTest {
   uint32_t low, beyond;      // twice: the lowest, and how far behind it the range has ended
   __device__ __forceinline__ RangeTest(float least_x, float most_x) : least(least_x), most(most_x), low(0), beyond(0) {
     if constexpr (TYPE != kLogitsF32) {
-      // (the zeros, infinity and, in fp16, those next to an end are looked at again)
+      // (the zeros and, in fp16, those next to an end are looked at again)
       const int from = least_x == 0.f ? -1 : in_order(bits_of(least_x));
-      const int to = most_x == kMostLogit<TYPE> ? 0x7fff : most_x == 0.f ? 0 : in_order(bits_of(most_x));
+      const int to = most_x == 0.f ? 0 : in_order(bits_of(most_x));
       low = (uint16_t)from * 0x10001u;
       beyond = (uint16_t)(to - from + 1) * 0x10001u;
     } else if (most_x == kMostFloat) {
@@ -521,6 +521,7 @@ struct RangeTest {
   }
   static __device__ __forceinline__ int in_order(uint16_t bits) { return (int16_t)(bits ^ ((int16_t)bits >> 15 & 0x7fff)); }
   static __device__ __forceinline__ uint16_t bits_of(float x) {
+    if (x > kMostLogit<TYPE>) return TYPE == kLogitsF16 ? 0x7c00 : 0x7f80;          // infinity's
     if constexpr (TYPE == kLogitsF16) return __builtin_bit_cast(uint16_t, (half_t)x);
     return (uint16_t)(__builtin_bit_cast(uint32_t, x) >> 16);
   }
@@ -906,7 +907,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
         const int32_t o = (int16_t)(uint16_t)((word >> 16) + test.low);
         bits = (uint16_t)(o ^ ((o >> 31) & 0x7fff));
       }
-      const float e = clean_logit<TYPE>(raw_logit<TYPE>(uint4_t{bits, bits, bits, bits}, 0));
+      const float e = clean_logit(raw_logit<TYPE>(uint4_t{bits, bits, bits, bits}, 0));
       list[before + i] = (uint32_t)at < (uint32_t)vocab ? keys.of(order_of(e), at) : 0;      // (no token's key)
     }
     __syncthreads();
@@ -943,7 +944,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
           for (int n = 1; n < 4; ++n) one = i == n ? raw[j][n] : one;
 #pragma unroll
           for (int h = 0; h < kPerWord; ++h) {
-            const float e = clean_logit<TYPE>(raw_logit<TYPE>(uint4_t{one, one, one, one}, h));
+            const float e = clean_logit(raw_logit<TYPE>(uint4_t{one, one, one, one}, h));
             const int32_t at = (int32_t)(v * kPer - in.lead) + i * kPerWord + h;
             const uint64_t key = keys.of(order_of(e), at);
             if (key >= from && key <= to && (uint32_t)at < (uint32_t)vocab) what(key, true);
@@ -1005,9 +1006,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(
       bin = last;
     }
     const uint32_t low_order = lowest_of_bin(top - bin, t, z_per_x);
-    const uint32_t high_order = bin > 0 ? lowest_of_bin(top - bin + 1.0, t, z_per_x) - 1 : order_of(most);
     low = keys.lowest(low_order);
-    high = keys.lowest(high_order + 1) - 1;
+    high = bin > 0 ? keys.lowest(lowest_of_bin(top - bin + 1.0, t, z_per_x)) - 1 : most_key;
     if (filter == 2) break;
 
     // Where the prefix ends in the bin: while its tokens are many, by the next ten bits of their keys; then by ranking them.

@@ -1377,8 +1377,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Opt
     probability (ties: the lowest index first), of them the shortest run that reaches ``top_p`` of their mass, of them those of at
     least ``min_p`` times the largest probability; always the first. Each filter is a tensor of the batch or None; a row's top_k
     below 1, top_p of 1 or more and min_p of 0 or less are off. Temperature 0 (or less) takes the first largest logit.
-    Tokens further than 40 * temperature below the largest are never drawn, nor are those of -inf or NaN; a row without any
-    other gives token -1. With ``return_logprobs`` (tokens, logprobs): the token's logarithm of probability among the kept."""
+    Tokens further than 40 * temperature below the largest are never drawn, nor are those of -inf or NaN; +inf counts as the largest
+    finite float32. A row without a token that can be drawn gives -1. With ``return_logprobs`` (tokens, logprobs): the token's logarithm of probability among the kept."""
     if logits.is_cuda:
         done = _lib.calls().sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p, return_logprobs, _stream())
         if done is not None:
