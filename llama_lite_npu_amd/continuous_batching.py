@@ -49,7 +49,8 @@ class BatchRequest:
                  temperature: float, top_p: float, control_id: Optional[int] = None, top_k: int = 0,
                  min_p: float = 0.0, seed: Optional[int] = None) -> None:
         """``top_k`` (0: off), ``min_p`` (0: off) and ``seed`` are beside the reference's: see ``draw_tokens``. A sampler of the
-        backend's owner is not given them, and sharded logits refuse them."""
+        backend's owner is not given them, and sharded logits refuse them. ``failed``: its logits had no token that can be drawn
+        (all NaN or -inf), and the backend ended its answer."""
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens must be positive")
         self.top_k, self.min_p, self.seed = int(top_k), float(min_p), seed
@@ -65,6 +66,7 @@ class BatchRequest:
         self.model_request_id: Optional[int] = None
         self.finished = False
         self.cancelled = False
+        self.failed = False
 
     @property
     def last_token_id(self) -> int:
@@ -112,7 +114,7 @@ def sample_next_token(logits: torch.Tensor, temperature: Sequence[float], top_p:
 
 def draw_tokens(logits: torch.Tensor, requests: Sequence, generated: Optional[Sequence[int]] = None) -> torch.Tensor:
     """One token per row of ``logits`` [n, vocab] (or [n, seq, vocab]: last position), by each request's temperature, top_k, top_p
-    and min_p (``ops.sample_tokens``; one small upload, two launches). The uniform number of a request with a ``seed`` depends
+    and min_p (``ops.sample_tokens``; one small upload, two launches), -1 where none can be drawn. The uniform number of a request with a ``seed`` depends
     on that and on the number of tokens it has generated (``generated``, or what its list says), in any batch and after any
     preemption; the others' come from Python's generator."""
     rows = logits[:, -1, :] if logits.dim() == 3 else logits
@@ -203,10 +205,13 @@ class ContinuousBatchModelBackend:
     def _tensor(self, values) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.long, device=self.executor.device)
 
+    def _filtered(self, requests: Sequence[BatchRequest]) -> bool:
+        """Whether the batch's tokens are drawn by ``draw_tokens``."""
+        return self._sampler is sample_next_token and any(
+            getattr(r, "top_k", 0) > 0 or getattr(r, "min_p", 0.0) > 0.0 or getattr(r, "seed", None) is not None for r in requests)
+
     def _sample(self, logits, requests: Sequence[BatchRequest], decoding: bool = False) -> torch.Tensor:
-        if self._sampler is sample_next_token and any(
-                getattr(r, "top_k", 0) > 0 or getattr(r, "min_p", 0.0) > 0.0 or getattr(r, "seed", None) is not None
-                for r in requests):
+        if self._filtered(requests):
             if getattr(self.executor, "logits_are_sharded", False):
                 raise ValueError("top_k, min_p and seed take whole rows of logits, not a vocabulary's shards")
             generated = None
@@ -216,6 +221,21 @@ class ContinuousBatchModelBackend:
         return self._sampler(logits, temperature=[r.temperature for r in requests],
                              top_p=[r.top_p for r in requests],
                              vocab_parallel=bool(getattr(self.executor, "logits_are_sharded", False)))
+
+    def _in_range(self, sampled: torch.Tensor, requests: Sequence[BatchRequest]) -> torch.Tensor:
+        """What the next forward is given: the end token where a row had none that can be drawn."""
+        return sampled.masked_fill(sampled < 0, self.eos_token_id) if self._filtered(requests) else sampled
+
+    def _read_back(self, sampled: torch.Tensor, requests: Sequence[BatchRequest]) -> list[int]:
+        """The sampled tokens on the host. A request without one gets the end token, which ends it, and is marked as failed; the
+        rest of its batch goes on."""
+        tokens = [int(t) for t in sampled.detach().cpu().tolist()]
+        if self._filtered(requests):
+            for row, request in enumerate(requests):
+                if tokens[row] < 0:
+                    logger.error("request %r: its logits are all NaN or -inf, no token can be drawn; its answer ends", request.request_id)
+                    request.failed, tokens[row] = True, self.eos_token_id
+        return tokens
 
     def _remember(self, requests: Sequence[BatchRequest], sampled: torch.Tensor,
                   positions: Optional[Sequence[int]] = None) -> None:
@@ -229,15 +249,16 @@ class ContinuousBatchModelBackend:
         """The prompts of ``requests`` are cached and ``logits`` holds one row per request for the
         last prompt token: sample the first generated token, book its slot, store the prefix."""
         sampled = self._sample(logits, requests)
-        self._remember(requests, sampled, [len(r.model_context_tokens) for r in requests])
+        self._remember(requests, self._in_range(sampled, requests), [len(r.model_context_tokens) for r in requests])
         ids = tuple(int(r.model_request_id) for r in requests)
         self.executor.extend_paged_requests(ids)
         if not self.return_host_tokens:
             return [None] * len(requests)
-        tokens = [int(t) for t in sampled.detach().cpu().tolist()]
+        tokens = self._read_back(sampled, requests)
         if hasattr(self.executor, "store_paged_request_prefix"):
             for request, token in zip(requests, tokens):
-                if request.temperature == 0:        # only greedy continuations are reusable
+                # only greedy continuations are reusable, and those that there are
+                if request.temperature == 0 and not getattr(request, "failed", False):
                     self.executor.store_paged_request_prefix(request.model_context_tokens,
                                                              int(request.model_request_id), token)
         return tokens
@@ -590,14 +611,15 @@ class ContinuousBatchModelBackend:
             position_ids = self._tensor([[self._positions[i]] for i in ids])
             logits = ex.forward(input_ids, position_ids)
         sampled = self._sample(logits, requests, decoding=True)
-        self._remember(requests, sampled)
-        self._step_ids, self._step_tokens = ids, sampled
+        given = self._in_range(sampled, requests)
+        self._remember(requests, given)
+        self._step_ids, self._step_tokens = ids, given
         for req_idx in ids:
             self._positions[req_idx] += 1
         ex.extend_paged_requests(ids)
         if not self.return_host_tokens:
             return []
-        tokens = [int(t) for t in sampled.detach().cpu().tolist()]
+        tokens = self._read_back(sampled, requests)
         # the readback above has waited for the step: the device batch's refusal flag is current
         batch = getattr(ex, "_device_batch", None) if self.device_decode else None
         if batch is not None and int(batch.overflow.item()) != 0:
