@@ -114,24 +114,27 @@ def sample_next_token(logits: torch.Tensor, temperature: Sequence[float], top_p:
 
 def draw_tokens(logits: torch.Tensor, requests: Sequence, generated: Optional[Sequence[int]] = None) -> torch.Tensor:
     """One token per row of ``logits`` [n, vocab] (or [n, seq, vocab]: last position), by each request's temperature, top_k, top_p
-    and min_p (``ops.sample_tokens``; one small upload, two launches), -1 where none can be drawn. The uniform number of a request with a ``seed`` depends
-    on that and on the number of tokens it has generated (``generated``, or what its list says), in any batch and after any
-    preemption; the others' come from Python's generator."""
+    and min_p (``ops.sample_tokens``; one small upload, two launches), -1 where none can be drawn. The uniform number of a request
+    with a ``seed`` depends on that and on the number of tokens it has generated (``generated``, or what its list says), in any
+    batch and after any preemption; the others' come from PyTorch's generator of the logits' device, as ``sample_next_token``'s do."""
     rows = logits[:, -1, :] if logits.dim() == 3 else logits
     numbers = []
     for i, r in enumerate(requests):
         seed = getattr(r, "seed", None)
         if seed is None:
-            source = random
+            numbers.append(-1.0)
         else:
             source = random.Random(f"{seed}/{len(r.generated_token_ids) if generated is None else int(generated[i])}")
-        numbers.append(int(source.random() * 2 ** 24) / 2 ** 24)          # a float32 below 1
+            numbers.append(int(source.random() * 2 ** 24) / 2 ** 24)      # a float32 below 1
     # top_k as the bits of an int32 in a float32's place
     top_k = [min(int(getattr(r, "top_k", 0)), 2 ** 31 - 1) for r in requests]
     floats = [numbers, [float(r.temperature) for r in requests], [float(r.top_p) for r in requests],
               [float(getattr(r, "min_p", 0.0)) for r in requests]]
     packed = torch.cat((torch.tensor(floats, dtype=torch.float32), torch.tensor([top_k], dtype=torch.int32).view(torch.float32)))
     uniforms, temperature, top_p, min_p, bits = packed.to(rows.device).unbind(0)
+    if any(x < 0 for x in numbers):
+        drawn = torch.rand(len(numbers), device=rows.device)
+        uniforms = torch.where(uniforms < 0, drawn, uniforms)
     return ops.sample_tokens(rows, uniforms, temperature, bits.view(torch.int32), top_p, min_p)
 
 
