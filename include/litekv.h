@@ -50,13 +50,19 @@ extern "C" {
 #define LITEKV_ERR_INVALID_ARGUMENT 1
 #define LITEKV_ERR_LAUNCH 2
 
-#define LITEKV_ABI_VERSION 6
+#define LITEKV_ABI_VERSION 7
 
 /* ABI version of the loaded library (LITEKV_ABI_VERSION at build time). */
 int litekv_abi_version(void);
 
 /* Message of the last failing call made by this thread ("" if none). */
 const char *litekv_last_error(void);
+
+/*
+ * *id: which capture `stream` is in, a number that no other capture of the process has; 0 where
+ * it is in none. For what a graph has of its own, made once however many of its calls need it.
+ */
+int litekv_stream_capture_id(void *stream, uint64_t *id);
 
 /*
  * KV append. Replaces `update_kv_buffer(KV_Values, Select_Index, KV_Buffer)`

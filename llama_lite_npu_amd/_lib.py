@@ -19,12 +19,13 @@ import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "csrc" / "liblitekv.so"
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 # name -> (restype, argtypes); mirrors include/litekv.h declaration by declaration.
 SIGNATURES = {
     "litekv_abi_version": (c_int32, []),
     "litekv_last_error": (c_char_p, []),
+    "litekv_stream_capture_id": (c_int32, [c_void_p, c_void_p]),
     "litekv_kv_append": (
         c_int32,
         [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int32, c_int32,

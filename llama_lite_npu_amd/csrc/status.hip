@@ -32,3 +32,18 @@ int check_launch(const char *what) {
 extern "C" int litekv_abi_version(void) { return LITEKV_ABI_VERSION; }
 
 extern "C" const char *litekv_last_error(void) { return litekv::g_last_error; }
+
+extern "C" int litekv_stream_capture_id(void *stream, uint64_t *id) {
+  using namespace litekv;
+  LITEKV_REQUIRE(id != nullptr, "%s: null pointer", "stream_capture_id");
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long number = 0;
+  const hipError_t err = hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &number);
+  if (err != hipSuccess) {
+    (void)hipGetLastError();
+    return fail(LITEKV_ERR_LAUNCH, "stream_capture_id: %s", hipGetErrorString(err));
+  }
+  *id = status == hipStreamCaptureStatusActive ? number + 1 : 0;
+  clear_error();
+  return LITEKV_OK;
+}

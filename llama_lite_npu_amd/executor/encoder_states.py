@@ -44,6 +44,7 @@ class EncoderStates:
             raise ValueError("kv_scales, one a layer, belong to pools of 8-bit codes")
         self.kv_scales = list(kv_scales) if coded else [None] * num_layers
         self._dtype, self._pages, self._plans = dtype, pages, {}
+        self._graph_plans: dict = {}          # head count -> (capture, its plan), of the last capture
 
     def store(self, layer_index: int, xk: torch.Tensor, xv: torch.Tensor) -> None:
         """K and V [sum of the lengths, Hkv, D] of all sequences' states, one sequence after another."""
@@ -55,14 +56,20 @@ class EncoderStates:
 
     def decode_plan(self, num_q_heads: int) -> ops.DecodePlan:
         """How a step of one row a sequence reads the states: made at its first call, and the same for every layer and step. Steps
-        share its workspace, so they run one after the other (one stream). In the capture of a graph, where nothing has run
-        yet, the graph gets a plan of its own, made at each of its replays."""
-        captured = torch.cuda.is_current_stream_capturing()
-        plan = None if captured else self._plans.get(num_q_heads)
+        share its workspace, so they run one after the other (one stream). A graph gets a plan of its own, shared by its layers
+        and made once at each of its replays: nothing has run while it is captured, and it may run beside other steps."""
+        captured = ops.capture_id()
+        if captured is None:
+            plan = self._plans.get(num_q_heads)
+        else:
+            known, plan = self._graph_plans.get(num_q_heads, (None, None))
+            plan = plan if known == captured else None
         if plan is None:
             row = 2 * self.num_kv_heads * (self.kv_buffer[0].shape[2] * self.kv_buffer[0].element_size())
             plan = ops.DecodePlan(self.block_table, self.kv_lens, num_q_heads, self.num_kv_heads, self._pages,
                                   page_size=self.page_size, host_seq_lens=self.lengths, token_bytes=row, kv_dtype=self._dtype)
-            if not captured:
+            if captured is None:
                 self._plans[num_q_heads] = plan
+            else:
+                self._graph_plans[num_q_heads] = captured, plan
         return plan

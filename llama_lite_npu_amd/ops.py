@@ -30,6 +30,15 @@ def _stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def capture_id() -> Optional[int]:
+    """Which capture of a graph the current stream is in, a number of its own for each; None if it is in none."""
+    if not torch.cuda.is_current_stream_capturing():
+        return None
+    number = ctypes.c_uint64()
+    _lib.check(_lib.load().litekv_stream_capture_id(_stream(), ctypes.byref(number)))
+    return number.value
+
+
 # The wrappers run once per layer and step: checks on their path are plain conditions, and the message
 # of one is only put together when it fails.
 def _need(cond: bool, msg: str) -> None:
