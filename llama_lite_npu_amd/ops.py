@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import numbers
 from typing import Optional, Sequence
 
 import torch
@@ -1196,9 +1197,10 @@ def axis_of_pair(sections: tuple, head_dim: int, interleaved: bool = False) -> b
     """Which axis' position each of a row's head_dim / 2 pairs takes, a byte each. ``sections``: pairs of each axis, together
     head_dim / 2. In runs, axis after axis; or ``interleaved``: pair i that of axis i mod A where i < A * sections[axis], all
     others axis 0's (whose own number then does not matter)."""
-    if not (1 <= len(sections) <= 4 and all(type(s) is int and s >= 0 for s in sections) and 2 * sum(sections) == head_dim):
+    whole = all(isinstance(s, numbers.Integral) and not isinstance(s, bool) and s >= 0 for s in sections)
+    if not (1 <= len(sections) <= 4 and whole and 2 * sum(map(int, sections)) == head_dim):
         raise ValueError(f"sections {sections} must be 1 to 4 whole numbers that add up to head_dim / 2 = {head_dim // 2}")
-    axes = len(sections)
+    axes, sections = len(sections), [int(s) for s in sections]      # (numpy's, too)
     if not interleaved:
         return bytes(a for a, n in enumerate(sections) for _ in range(n))
     return bytes(i % axes if i < axes * sections[i % axes] else 0 for i in range(head_dim // 2))
