@@ -305,7 +305,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_slices_kernel(
   const float t = row_temperature(temperature, row);
   const double z_per_x = z_factor(t);
 #pragma unroll
-  for (int i = tid; i < kCopies * 2 * kSampleThreads; i += kSampleThreads) hist[0][i] = 0;
+  for (int i = 0; i < kCopies * 2; ++i) hist[i / 2][i % 2 * kSampleThreads + tid] = 0;
   if (tid == 0) {
     found_bins = 0;
     found_n = 0;
