@@ -173,6 +173,7 @@ class ContinuousBatchModelBackend:
         self._positions: dict[int, int] = {}                  # position of that token
         self._step_ids: tuple[int, ...] = ()                  # requests of the last decode step ...
         self._step_tokens: Optional[torch.Tensor] = None      # ... and what it sampled, [B]
+        self._drawn = False                                   # whether draw_tokens has sampled the last batch
         self._announced_paths = False
         self._warned_replay = False
         if not self.executor.use_paged_attn:
@@ -208,13 +209,10 @@ class ContinuousBatchModelBackend:
     def _tensor(self, values) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.long, device=self.executor.device)
 
-    def _filtered(self, requests: Sequence[BatchRequest]) -> bool:
-        """Whether the batch's tokens are drawn by ``draw_tokens``."""
-        return self._sampler is sample_next_token and any(
-            getattr(r, "top_k", 0) > 0 or getattr(r, "min_p", 0.0) > 0.0 or getattr(r, "seed", None) is not None for r in requests)
-
     def _sample(self, logits, requests: Sequence[BatchRequest], decoding: bool = False) -> torch.Tensor:
-        if self._filtered(requests):
+        self._drawn = self._sampler is sample_next_token and any(
+            getattr(r, "top_k", 0) > 0 or getattr(r, "min_p", 0.0) > 0.0 or getattr(r, "seed", None) is not None for r in requests)
+        if self._drawn:
             if getattr(self.executor, "logits_are_sharded", False):
                 raise ValueError("top_k, min_p and seed take whole rows of logits, not a vocabulary's shards")
             generated = None
@@ -225,15 +223,15 @@ class ContinuousBatchModelBackend:
                              top_p=[r.top_p for r in requests],
                              vocab_parallel=bool(getattr(self.executor, "logits_are_sharded", False)))
 
-    def _in_range(self, sampled: torch.Tensor, requests: Sequence[BatchRequest]) -> torch.Tensor:
+    def _in_range(self, sampled: torch.Tensor) -> torch.Tensor:
         """What the next forward is given: the end token where a row had none that can be drawn."""
-        return sampled.masked_fill(sampled < 0, self.eos_token_id) if self._filtered(requests) else sampled
+        return sampled.masked_fill(sampled < 0, self.eos_token_id) if self._drawn else sampled
 
     def _read_back(self, sampled: torch.Tensor, requests: Sequence[BatchRequest]) -> list[int]:
         """The sampled tokens on the host. A request without one gets the end token, which ends it, and is marked as failed; the
         rest of its batch goes on."""
         tokens = [int(t) for t in sampled.detach().cpu().tolist()]
-        if self._filtered(requests):
+        if self._drawn:
             for row, request in enumerate(requests):
                 if tokens[row] < 0:
                     logger.error("request %r: its logits are all NaN or -inf, no token can be drawn; its answer ends", request.request_id)
@@ -252,7 +250,7 @@ class ContinuousBatchModelBackend:
         """The prompts of ``requests`` are cached and ``logits`` holds one row per request for the
         last prompt token: sample the first generated token, book its slot, store the prefix."""
         sampled = self._sample(logits, requests)
-        self._remember(requests, self._in_range(sampled, requests), [len(r.model_context_tokens) for r in requests])
+        self._remember(requests, self._in_range(sampled), [len(r.model_context_tokens) for r in requests])
         ids = tuple(int(r.model_request_id) for r in requests)
         self.executor.extend_paged_requests(ids)
         if not self.return_host_tokens:
@@ -614,7 +612,7 @@ class ContinuousBatchModelBackend:
             position_ids = self._tensor([[self._positions[i]] for i in ids])
             logits = ex.forward(input_ids, position_ids)
         sampled = self._sample(logits, requests, decoding=True)
-        given = self._in_range(sampled, requests)
+        given = self._in_range(sampled)
         self._remember(requests, given)
         self._step_ids, self._step_tokens = ids, given
         for req_idx in ids:
