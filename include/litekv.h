@@ -944,8 +944,9 @@ int litekv_paged_cross_attention(const void *q, int64_t q_token_stride, const vo
  * p_i >= min_p; always the first. tokens[r] is the first token, by index, at which the kept
  * mass exceeds uniforms[r] times all of it, logprobs[r] its logarithm of probability among the
  * kept. T <= 0 (or NaN) takes the first largest logit, with logprob 0. Sums of mass are
- * exact to 2^-40 of the whole that they are a part of, and no kept token counts as nothing:
- * with 0 for a number the first of them, by index, is drawn.
+ * exact to 2^-40 of the whole that they are a part of, and to 2^-51 |x| / T more (x / T is
+ * rounded to 64 bits before the largest is subtracted). No kept token counts as nothing: with
+ * 0 for a number the first of them, by index, is drawn.
  *   logits       [batch][row_stride], logits_type 0 fp16, 1 bf16, 2 fp32; aligned to an
  *                element. NaN and -inf are never drawn, +inf counts as the largest finite fp32
  *                number, which is above all others of 16 bits. A row without any: token -1,

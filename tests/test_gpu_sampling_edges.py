@@ -1,5 +1,5 @@
 """Draws at the ends of what counts: tokens far below the largest that are still kept, infinity beside the largest finite logit of a
-type. Against the definition in 64 bits, as in test_gpu_sampling.py."""
+type, logits far from zero. Against the definition in 64 bits, as in test_gpu_sampling.py."""
 
 import math
 
@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from llama_lite_npu_amd import ops
-from tests.test_gpu_sampling import DEV, MOST, _check
+from tests.test_gpu_sampling import DEV, MOST, _check, _want
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,22 @@ def test_many_infinities(dtype, many):
         if k is None or k <= many:
             assert (got % 4 == 1).all()
     _check_by_logit(x, u, 3e37, 2 * many)
+
+
+@pytest.mark.parametrize("offset", [-3e7, 1e6, 2e5])
+def test_logits_far_from_zero(offset):
+    """x / T is rounded to 64 bits before the row's largest is subtracted: 2^-53 |x| / T of it for each, twice where a token is set
+    against the rest, beside what draws near zero are good to."""
+    print(f"sample: offset {offset}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(17)
+    x = 4 * torch.randn(40, 30000, generator=g, device=DEV) + offset
+    u = torch.rand(40, generator=g, device=DEV)
+    for k, p, m in ((None, None, None), (50, 0.9, None), (None, 0.95, None), (None, None, 0.05)):
+        per = lambda v, d=torch.float32: None if v is None else torch.full((40,), v, device=DEV, dtype=d)  # noqa: E731
+        tokens, logprobs = ops.sample_tokens(x, u, None, per(k, torch.int32), per(p), per(m), return_logprobs=True)
+        for r in range(40):
+            p32 = 1.0 if p is None else per(p)[r].item()
+            m32 = 0.0 if m is None else per(m)[r].item()
+            want, lp = _want(x[r].cpu().numpy(), u[r].item(), 1.0, k or 0, p32, m32)
+            assert tokens[r].item() == want
+            assert abs(logprobs[r].item() - lp) <= abs(lp) * 2.0 ** -24 + 2.0 ** -39 + abs(offset) * 1.01 * 2.0 ** -51
