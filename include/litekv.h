@@ -955,7 +955,7 @@ int litekv_paged_cross_attention(const void *q, int64_t q_token_stride, const vo
  *   temperature  [batch], NULL: 1
  *   top_k        [batch], below 1: off. NULL: off
  *   top_p        [batch], 1 and above (or NaN): off. NULL: off
- *   min_p        [batch], 0 and below (or NaN): off. NULL: off
+ *   min_p        [batch], 0 and below (or NaN): off; above 1 it counts as 1. NULL: off
  *   logprobs     [batch] or NULL
  * vocab at most 2^20. Reads the 16-byte blocks that hold an element of a row. The same inputs give the same
  * outputs, whatever the order the device works in.

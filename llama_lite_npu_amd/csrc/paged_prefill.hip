@@ -62,7 +62,7 @@ static PrefillShape prefill_shape(int group, int max_q_len, int wg_col_tiles = k
 
 // Folds the key slices of a split prefill: the lanes of a (query row, head), four elements each, read the row's
 // `slices` log-sum-exps and partial rows (fp32, normalised per slice) and write the fp16 row. A slice without keys has
-// log-sum-exp -inf and weight 0; the last slice always has keys. Rows behind the last sequence, which no slice wrote, are left as they
+// log-sum-exp -inf and weight 0; a causal row's last slice always has keys, a row that sees another sequence's keys may have none. Rows behind the last sequence, which no slice wrote, are left as they
 // are in `out` (their cells are read, and only the store waits for the number of rows). Bound by memory trips, then by memory: no lane needs another's
 // numbers, and all loads are ahead of the arithmetic (64 rows of 16 heads of 128 in 8 slices 3.8 us, 1224 rows of 32 heads
 // of 64 in 2 7.7; with a wavefront a row that gathers them by shuffles 5.5 and 15).

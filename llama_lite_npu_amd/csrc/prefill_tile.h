@@ -191,7 +191,8 @@ constexpr int kPagedPrefill = 0, kPackedPrefill = 1, kSharedPrefix = 2, kPagedPr
 // context_lens), which are another sequence's than its own, an encoder's states say. All tiles but the last are then plain
 // ones, and the last is masked behind the last key. A sequence without keys has rows of zeros. (At most the keys that a row
 // of the block table can name.) Without a diagonal a block's rows all take every tile: 8 sequences of up to 1024 rows over 1000 to 6400 states,
-// 64 / 8 heads of 128, 0.59 TFLOP, in 548 us, 1.08 PFLOP/s (a large fp16 product 1.25).
+// 64 / 8 heads of 128, 0.59 TFLOP, in 548 to 580 us, with the clock, 1.02 to 1.08 PFLOP/s (a large fp16 product 1.25; by itself
+// under a profiler 563 to 624 us).
 constexpr int kCross = 16;
 
 // Column tiles per wavefront and wavefronts per workgroup of a prefill of 128 columns. Head dim 256 leaves one

@@ -1277,7 +1277,7 @@ def paged_cross_attention(q: torch.Tensor, kv_pool: torch.Tensor, block_table: t
     softmax scale above 0.
 
     ``cu_q_lens`` None: one row a sequence (a decode step), q [B, Hq, D], which streams the keys like ``paged_decode``, whose
-    lengths have to be ones that the block table can name.
+    lengths have to be ones that the block table can name (a longer one attends the row's last page again, or not, by schedule).
     ``max_q_len``: the most rows of a sequence. ``max_kv_len``: the most keys, as the host knows it; launches of few rows
     are then cut along the keys as in ``paged_prefill``, and nothing but speed goes by it. Rows behind the last sequence are left as
     they are. ``key_slices`` and ``workspace`` as there."""
@@ -1386,8 +1386,8 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Opt
     """One token (int64) per row of ``logits`` [B, vocab] (fp16, bf16 or fp32, rows with any stride), drawn with ``uniforms`` [B]
     in [0, 1): the first token, by index, at which the kept mass exceeds u times all of it. Kept are the first ``top_k`` tokens by
     probability (ties: the lowest index first), of them the shortest run that reaches ``top_p`` of their mass, of them those of at
-    least ``min_p`` times the largest probability; always the first. Each filter is a tensor of the batch or None; a row's top_k
-    below 1, top_p of 1 or more and min_p of 0 or less are off. Temperature 0 (or less) takes the first largest logit.
+    least ``min_p`` (at most 1) times the largest probability; always the first. Each filter is a tensor of the batch or None; a
+    row's top_k below 1, top_p of 1 or more and min_p of 0 or less are off. Temperature 0 (or less) takes the first largest logit.
     Tokens further than 40 * temperature below the largest are never drawn, nor are those of -inf or NaN; +inf counts as the largest
     finite float32. A row without a token that can be drawn gives -1. With ``return_logprobs`` (tokens, logprobs): the token's logarithm of probability among the kept."""
     if logits.is_cuda:
