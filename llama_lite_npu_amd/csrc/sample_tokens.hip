@@ -19,7 +19,7 @@
 // Measured, us of the slices' and of the rows' kernel: 1 x 32000 fp16 with top-k and top-p 6 and 10, 32 x 151936 fp16 with all
 // filters 10 and 12, 33 x 49999 fp32 9 and 12, 256 x 128000 bf16 with top-p 34 and 43 (65 MB: a copy takes 13). The first is bound
 // by its instructions, 17 a token for the histogram, 12 of them fp64, and 11 for the rest (conversion, maximum, list), and by its atomics
-// in LDS (vector instructions issue in 89 % of the cycles there, the LDS is busy in 44 %, three fifths of that with bank conflicts). The second by latency, some twelve to twenty steps of about 0.7 us (a memory trip, a scan, a barrier), and
+// in LDS (vector instructions issue in 90 % of the cycles there, the LDS is busy in 45 %, three fifths of that with bank conflicts). The second by latency, some twelve to twenty steps of about 0.7 us (a memory trip, a scan, a barrier), and
 // where a bin has to be listed from the row (half the rows of the last case) by the pass over it: 12 us, 5.4 TB/s over the device. A
 // row whose end lies in a bin of more tokens than a list takes (151936 logits of standard deviation 1: 7500) takes 110 us, and one of
 // nothing but equal logits up to 600, whichever their number: one compute unit goes over it several times.
